@@ -560,6 +560,64 @@ int saber_iu8_moe_combine(saber_iu8_ctx *ctx, const void *y_bf16, const saber_iu
  * parity suite compares it with the host formula for all 65,536 inputs. */
 int saber_iu8_silu_table(saber_iu8_ctx *ctx, void *out_u16, void *stream);
 
+/* ------------------------------------------------------------------ paged key/value cache, attention */
+
+/* What stands between a decoder layer's qkv linear and its output gate (saber_iu8_attn_gate_quant_had): new tokens into a
+ * paged cache, and the attention that reads it. Rows are bf16; no counterpart among the reference's interfaces for this path.
+ *
+ * The cache in the gfx950 order, E = the elements of 16 bytes (8 bf16, 16 e4m3): K [pages][kv_heads][page_tokens / 16][head_dim / E]
+ * [16 tokens][E], V [pages][kv_heads][page_tokens][head_dim] (saber_iu8_kv_k_offset, _v_offset). head_dim 64, 128 or 256; page_tokens a
+ * power of two from 16 to 256. An e4m3 cache holds value / scale, a scale a kv head, rounded to nearest even and saturated at 448;
+ * the attention multiplies by it. Entry [s * table_stride + p] of the page table is the page that holds tokens p * page_tokens ... of
+ * sequence s; an entry outside 0 .. pages - 1 is a hole: nothing is written there and its keys take no part. kv_len[s] counts
+ * the sequence's tokens, the call's new ones included (both operators of a step read the same number); counts above
+ * table_stride * page_tokens are taken as that, below 0 as 0. The counts and the table are read on the device, so a captured launch
+ * follows them. */
+#define SABER_IU8_KV_BF16 0
+#define SABER_IU8_KV_E4M3 1
+typedef struct {
+  void *k, *v;                   /* saber_iu8_kv_bytes each */
+  const float *k_scale, *v_scale; /* [kv_heads], e4m3 only */
+  const int32_t *page_table;     /* [sequences * table_stride] */
+  const int32_t *kv_len;         /* [sequences] */
+  uint32_t kind, kv_heads, head_dim, page_tokens, pages, table_stride;
+} saber_iu8_kv_cache;
+uint64_t saber_iu8_kv_bytes(uint32_t pages, uint32_t kv_heads, uint32_t head_dim, uint32_t page_tokens, uint32_t kind);
+/* Byte offset of (page, kv head, token of the page, channel) in k / in v. */
+uint64_t saber_iu8_kv_k_offset(uint32_t page, uint32_t kv_head, uint32_t token, uint32_t channel, uint32_t kv_heads, uint32_t head_dim,
+                               uint32_t page_tokens, uint32_t kind);
+uint64_t saber_iu8_kv_v_offset(uint32_t page, uint32_t kv_head, uint32_t token, uint32_t channel, uint32_t kv_heads, uint32_t head_dim,
+                               uint32_t page_tokens, uint32_t kind);
+
+/* The new tokens of `seqs` sequences into the cache. Rows cu_q[s] .. cu_q[s + 1] - 1 (device, [seqs + 1]) are sequence s's newest
+ * tokens, at positions kv_len[s] - n .. kv_len[s] - 1; cu_q NULL: one row a sequence. Rows behind the last sequence (of `tokens`),
+ * and rows whose position would be negative, are left as they were, in q_out as in the cache.
+ *   q [tokens] rows `q_row` elements apart, head h at h * q_head (q_head = 2 * head_dim reads a gated projection's [q | gate] heads
+ *   in place); k, v rows `kv_row` apart, heads head_dim apart; q_out [tokens, heads, head_dim].
+ *   q_norm, k_norm (bf16 [head_dim], may be NULL): x * 1/sqrt(mean(x^2) + eps) * (1 + w) over the head's channels.
+ *   inv_freq (f64 [rot_dim / 2], device): channels i and i + rot_dim / 2 (interleaved: 2i and 2i + 1) of q and k turn by
+ *   position * inv_freq[i]; the other channels stay. rot_dim a multiple of 16, 0 for none.
+ * All in f32 (the angle in f64), rounded once. q, k, v and q_out must not overlap one another's rows unless q_out is q itself
+ * with q_row = heads * head_dim. Pointers on 16 bytes, strides multiples of 8. Asynchronous. */
+int saber_iu8_kv_append(saber_iu8_ctx *ctx, const void *q, const void *k, const void *v, void *q_out, const saber_iu8_kv_cache *cache,
+                        const int32_t *cu_q, uint32_t tokens, uint32_t seqs, uint32_t heads, uint32_t q_row, uint32_t q_head, uint32_t kv_row,
+                        const double *inv_freq, uint32_t rot_dim, int interleaved, const void *q_norm, const void *k_norm, float eps, void *stream);
+
+/* The new rows' attention over the cache, causal: row i of sequence s's n new ones sees positions 0 .. kv_len[s] - n + i.
+ *   out[t, h] = sum_j softmax_j(scale * q[t, h] . k_j) v_j, heads in groups of heads / kv_heads a kv head
+ * q rows `q_row` elements apart, heads head_dim apart; out bf16 [tokens, heads, head_dim]. A row that sees no key gives zeros; rows behind
+ * the last sequence are left as they were. max_q: the most new rows of a sequence (rows past it are not computed); max_kv: what
+ * kv_len is expected to reach, for the split of the cache's length alone (a longer one is right, and slower).
+ * Up to 32 rows a kv head (new rows x group) run on the few-row kernels, which stream the cache; more on the many-row kernels,
+ * 128 a workgroup. Both share the cache's length among workgroups where the grid would leave the card idle, with
+ * the workspaces of saber_iu8_attn_workspace: `partial` (scratch) and `counter` (zeroed once, left zero); either NULL: in one piece.
+ * Calls that share them must not overlap in time. Scores and sums in f32, the softmax's weights rounded to bf16 for the
+ * second product, the output rounded once; the same bytes on every run of one plan. Asynchronous. */
+int saber_iu8_attn_workspace(uint32_t seqs, uint32_t max_q, uint32_t max_kv, uint32_t heads, uint32_t kv_heads, uint32_t head_dim,
+                             uint64_t *partial_bytes, uint64_t *counter_bytes);
+int saber_iu8_attn(saber_iu8_ctx *ctx, const void *q, uint32_t q_row, const saber_iu8_kv_cache *cache, const int32_t *cu_q, void *out, uint32_t tokens,
+                   uint32_t seqs, uint32_t max_q, uint32_t max_kv, uint32_t heads, float scale, void *partial, void *counter, void *stream);
+
 /* ---- tier packs ("SBRPACK1"): reading the iu8 records of a built pack ------------------------------
  * The byte layout of include/saber_abi.h:541-944 and the open-time rules of
  * crates/saber-mem/src/pack/{format,reader}.rs (PackReader::open_with / open_expecting): magic,

@@ -1,0 +1,234 @@
+// The paged key/value cache and the attention that reads it (include/saber_iu8.h): checks of arguments, the launch law and the
+// launches. No counterpart among the reference's interfaces for this path.
+#include <algorithm>
+#include <cmath>
+
+#include "../../../include/saber_iu8.h"
+#include "rules.h"
+#include "util.h"
+
+using namespace iu8;
+
+namespace {
+
+constexpr uint32_t FEW_ROWS = 32;    // rows a kv head and sequence up to which the few-row kernels run (16 or 32 a workgroup)
+constexpr uint32_t MANY_ROWS = 128;  // rows a workgroup of the many-row kernels
+constexpr uint32_t I32_MAX = 0x7FFFFFFFu;
+constexpr uint32_t WHOLE = 0x7FFFFF00u;  // a part that holds any sequence: the positions a table's row may reach
+
+void set_f32(saber_iu8_desc *d, const char *name, float v) {
+  for (uint32_t i = 0; i < d->n_args; ++i)
+    if (!strcmp(d->args[i].name, name)) d->args[i].kind = SABER_IU8_ARG_F32, d->args[i].fval = v;
+}
+
+int log2_of(uint32_t x) {
+  int s = 0;
+  while ((1u << s) < x) ++s;
+  return s;
+}
+
+int cache_check(const char *op, const saber_iu8_kv_cache *c, uint32_t heads, uint32_t seqs, uint32_t tokens, const int32_t *cu_q) {
+  if (!c) return fail(SABER_IU8_E_ARG, fmt("%s: null cache", op));
+  if (!c->k || !c->v || !c->page_table || !c->kv_len) return fail(SABER_IU8_E_ARG, fmt("%s: the cache's k, v, page_table and kv_len must be given", op));
+  if (c->kind != SABER_IU8_KV_BF16 && c->kind != SABER_IU8_KV_E4M3) return fail(SABER_IU8_E_ARG, fmt("%s: unknown cache kind %u", op, c->kind));
+  if (c->kind == SABER_IU8_KV_E4M3 && (!c->k_scale || !c->v_scale))
+    return fail(SABER_IU8_E_ARG, fmt("%s: an e4m3 cache has a k_scale and a v_scale a kv head", op));
+  if (((uintptr_t)c->k | (uintptr_t)c->v) % 16) return fail(SABER_IU8_E_ARG, fmt("%s: the cache's k and v must lie on 16 bytes", op));
+  if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256)
+    return fail(SABER_IU8_E_RULE, fmt("%s: head width %u; the kernels hold 64, 128 and 256", op, c->head_dim));
+  if (c->page_tokens < 16 || c->page_tokens > 256 || (c->page_tokens & (c->page_tokens - 1)))
+    return fail(SABER_IU8_E_RULE, fmt("%s: pages of %u tokens; a power of two from 16 to 256", op, c->page_tokens));
+  if (!heads || !c->kv_heads || heads % c->kv_heads || heads > 0xFFFF || c->kv_heads > 0x7FFF)
+    return fail(SABER_IU8_E_RULE, fmt("%s: %u heads over %u kv heads: whole groups, at most 65535 and 32767", op, heads, c->kv_heads));
+  if (!c->pages || c->pages > I32_MAX || !c->table_stride || (uint64_t)c->table_stride * c->page_tokens > WHOLE)
+    return fail(SABER_IU8_E_RULE, fmt("%s: %u pages, %u of %u tokens a sequence: at least one, positions below 2^31 - 256", op, c->pages, c->table_stride, c->page_tokens));
+  if (!seqs || !tokens || seqs >= I32_MAX || tokens > I32_MAX) return fail(SABER_IU8_E_RULE, fmt("%s: %u rows of %u sequences has nothing to do", op, tokens, seqs));
+  if (!cu_q && tokens != seqs) return fail(SABER_IU8_E_RULE, fmt("%s: %u rows of %u sequences without cu_q (one row a sequence)", op, tokens, seqs));
+  return 0;
+}
+
+struct Plan {
+  uint32_t rows;  // a workgroup's (16, 32, 128)
+  uint64_t qtiles, items;
+  uint32_t chunk, splits;
+  bool few() const { return rows <= FEW_ROWS; }
+};
+
+// The split of the cache's length. The grid wants a few workgroups a CU; a part is at least 128 tokens (few rows: a 32-token tile
+// for each of the four waves) or 512 (many rows).
+Plan plan(uint32_t seqs, uint32_t max_q, uint32_t max_kv, uint32_t heads, uint32_t kv_heads) {
+  Plan p;
+  const uint64_t rows = (uint64_t)max_q * (heads / kv_heads);
+  p.rows = rows <= 16 ? 16 : rows <= FEW_ROWS ? FEW_ROWS : MANY_ROWS;
+  p.qtiles = p.few() ? 1 : (rows + MANY_ROWS - 1) / MANY_ROWS;
+  p.items = (uint64_t)seqs * kv_heads * p.qtiles;
+  const uint64_t target = p.few() ? 1024 : 512, unit = p.few() ? 128 : 512;
+  uint64_t parts = std::max<uint64_t>(1, target / std::max<uint64_t>(p.items, 1));
+  const uint64_t most = std::max<uint64_t>(1, (max_kv + unit - 1) / unit);
+  parts = std::min(parts, most);
+  uint64_t chunk = (max_kv + parts - 1) / parts;
+  chunk = std::max<uint64_t>(unit, (chunk + 127) / 128 * 128);
+  p.splits = (uint32_t)std::max<uint64_t>(1, (max_kv + chunk - 1) / chunk);
+  p.chunk = p.splits == 1 ? WHOLE : (uint32_t)chunk;
+  return p;
+}
+
+int attn_args(const char *op, uint32_t seqs, uint32_t max_q, uint32_t max_kv, uint32_t heads, uint32_t kv_heads, Plan *p) {
+  if (!max_q || max_kv > I32_MAX) return fail(SABER_IU8_E_RULE, fmt("%s: at most %u new rows and %u keys a sequence: from 1 and below 2^31", op, max_q, max_kv));
+  *p = plan(seqs, max_q, max_kv, heads, kv_heads);
+  if ((uint64_t)max_q * (heads / kv_heads) > I32_MAX || p->items * p->splits > I32_MAX)
+    return fail(SABER_IU8_E_RULE, fmt("%s: %u sequences of up to %u new rows and %u heads pass a launch's 32-bit sizes", op, seqs, max_q, heads));
+  return 0;
+}
+
+const saber_iu8_slot *slot(const saber_iu8_desc *d, const char *name) {
+  for (uint32_t i = 0; i < d->n_args; ++i)
+    if (!strcmp(d->args[i].name, name)) return &d->args[i];
+  return nullptr;
+}
+
+}  // namespace
+
+// What a hand-edited descriptor could get wrong for these kernels, whose walk over the cache follows their scalars.
+int iu8::attn_guard(const saber_iu8_desc *d) {
+  auto num = [&](const char *name) -> int64_t {
+    const saber_iu8_slot *s = slot(d, name);
+    return s && s->kind == SABER_IU8_ARG_I32 ? s->ival : -1;
+  };
+  const int64_t shape = num("shape"), heads = shape & 0xFFFF, kv_heads = shape >> 16, pages = num("pages"), stride = num("table_stride");
+  const bool append = !strncmp(d->kernel, "kv_append_", 10);
+  const int64_t form = append ? num("form") : num("page_shift"), shift = form & 0xFF, rot = append ? form >> 16 : 0;
+  const char *w = strstr(d->kernel, "_d");
+  const int64_t dim = w ? atoi(w + 2) : 0;
+  bool ok = shape > 0 && kv_heads > 0 && heads > 0 && heads % kv_heads == 0 && form >= 0 && shift >= 4 && shift <= 8 && pages > 0 && stride > 0 &&
+            (stride << shift) <= (int64_t)WHOLE && num("tokens") > 0 && d->grid[1] == 1 && d->grid[2] == 1;
+  if (append) ok = ok && rot % 16 == 0 && rot <= dim && num("seqs") > 0;
+  else ok = ok && num("chunk") >= 64 && num("chunk") % 64 == 0 && num("splits") > 0 && num("qtiles") > 0 && d->grid[0] % (uint64_t)num("splits") == 0;
+  return ok ? 0 : fail(SABER_IU8_E_RULE, fmt("%s: scalars that the kernel's walk over the cache does not hold", d->kernel));
+}
+
+extern "C" {
+
+uint64_t saber_iu8_kv_bytes(uint32_t pages, uint32_t kv_heads, uint32_t head_dim, uint32_t page_tokens, uint32_t kind) {
+  return (uint64_t)pages * kv_heads * head_dim * page_tokens * (kind == SABER_IU8_KV_E4M3 ? 1 : 2);
+}
+
+uint64_t saber_iu8_kv_k_offset(uint32_t page, uint32_t kv_head, uint32_t token, uint32_t channel, uint32_t kv_heads, uint32_t head_dim,
+                               uint32_t page_tokens, uint32_t kind) {
+  const uint64_t size = kind == SABER_IU8_KV_E4M3 ? 1 : 2, e = 16 / size;
+  const uint64_t block = ((uint64_t)page * kv_heads + kv_head) * page_tokens * head_dim + (uint64_t)(token / 16) * 16 * head_dim;
+  return (block + ((channel / e) * 16 + token % 16) * e + channel % e) * size;
+}
+
+uint64_t saber_iu8_kv_v_offset(uint32_t page, uint32_t kv_head, uint32_t token, uint32_t channel, uint32_t kv_heads, uint32_t head_dim,
+                               uint32_t page_tokens, uint32_t kind) {
+  return ((((uint64_t)page * kv_heads + kv_head) * page_tokens + token) * head_dim + channel) * (kind == SABER_IU8_KV_E4M3 ? 1 : 2);
+}
+
+int saber_iu8_kv_append(saber_iu8_ctx *ctx, const void *q, const void *k, const void *v, void *q_out, const saber_iu8_kv_cache *cache,
+                        const int32_t *cu_q, uint32_t tokens, uint32_t seqs, uint32_t heads, uint32_t q_row, uint32_t q_head, uint32_t kv_row,
+                        const double *inv_freq, uint32_t rot_dim, int interleaved, const void *q_norm, const void *k_norm, float eps, void *stream) {
+  const char *op = "kv_append";
+  if (int rc = cache_check(op, cache, heads, seqs, tokens, cu_q)) return rc;
+  const uint32_t D = cache->head_dim;
+  if (!q || !k || !v || !q_out) return fail(SABER_IU8_E_ARG, "kv_append: null rows");
+  if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q_out | (uintptr_t)q_norm | (uintptr_t)k_norm) % 16)
+    return fail(SABER_IU8_E_ARG, "kv_append: rows and norm weights must lie on 16 bytes");
+  if (q_row % 8 || q_head % 8 || kv_row % 8 || q_head < D || q_row > I32_MAX || kv_row > I32_MAX || (uint64_t)(heads - 1) * q_head + D > q_row ||
+      (uint64_t)cache->kv_heads * D > kv_row)
+    return fail(SABER_IU8_E_RULE, fmt("kv_append: rows of %u (q, heads %u apart) and %u (k, v) elements: whole 16-byte pieces that cover %u and %u heads of %u",
+                                      q_row, q_head, kv_row, heads, cache->kv_heads, D));
+  if (rot_dim % 16 || rot_dim > D) return fail(SABER_IU8_E_RULE, fmt("kv_append: %u rotated channels; a multiple of 16 up to the head's %u", rot_dim, D));
+  if (rot_dim && !inv_freq) return fail(SABER_IU8_E_ARG, "kv_append: a rotation without inv_freq");
+  if ((q_norm || k_norm) && !(eps >= 0.f && std::isfinite(eps))) return fail(SABER_IU8_E_RULE, "kv_append: eps must be a number from 0");
+  const uint32_t heads_a_wave = 64 / (D / 16), waves = (heads + 2 * cache->kv_heads + heads_a_wave - 1) / heads_a_wave;
+  const uint64_t all = (uint64_t)tokens * waves;
+  if (all > I32_MAX) return fail(SABER_IU8_E_RULE, fmt("kv_append: %u rows of %u heads pass a launch's 32-bit sizes", tokens, heads));
+  const bool f8 = cache->kind == SABER_IU8_KV_E4M3;
+  saber_iu8_desc d;
+  const uint32_t grid[3] = {(uint32_t)((all + 3) / 4), 1, 1};
+  if (int rc = saber_iu8_describe_raw(fmt("kv_append_%s_d%u", f8 ? "e4m3" : "bf16", D).c_str(), "attn_paged", grid, 256, &d)) return rc;
+  copy_name(d.op, sizeof d.op, op);
+  set_i32(&d, "q_row", q_row), set_i32(&d, "q_head", q_head), set_i32(&d, "kv_row", kv_row);
+  set_i32(&d, "tokens", tokens), set_i32(&d, "seqs", seqs);
+  set_i32(&d, "shape", heads | cache->kv_heads << 16);
+  set_i32(&d, "form", log2_of(cache->page_tokens) | (interleaved ? 0x100 : 0) | rot_dim << 16);
+  set_i32(&d, "pages", cache->pages), set_i32(&d, "table_stride", cache->table_stride);
+  set_f32(&d, "eps", eps);
+  if (!f8) set_null(&d, "k_scale"), set_null(&d, "v_scale");
+  if (!cu_q) set_null(&d, "cu_q");
+  if (!q_norm) set_null(&d, "q_norm");
+  if (!k_norm) set_null(&d, "k_norm");
+  if (!rot_dim) set_null(&d, "inv_freq");
+  const saber_iu8_binding b[] = {{"q", (void *)q},
+                                 {"k", (void *)k},
+                                 {"v", (void *)v},
+                                 {"q_out", q_out},
+                                 {"kc", cache->k},
+                                 {"vc", cache->v},
+                                 {"k_scale", (void *)cache->k_scale},
+                                 {"v_scale", (void *)cache->v_scale},
+                                 {"table", (void *)cache->page_table},
+                                 {"kv_len", (void *)cache->kv_len},
+                                 {"cu_q", (void *)cu_q},
+                                 {"q_norm", (void *)q_norm},
+                                 {"k_norm", (void *)k_norm},
+                                 {"inv_freq", (void *)inv_freq}};
+  return saber_iu8_launch(ctx, &d, b, 14, stream);
+}
+
+int saber_iu8_attn_workspace(uint32_t seqs, uint32_t max_q, uint32_t max_kv, uint32_t heads, uint32_t kv_heads, uint32_t head_dim,
+                             uint64_t *partial_bytes, uint64_t *counter_bytes) {
+  if (!seqs || !heads || !kv_heads || heads % kv_heads || (head_dim != 64 && head_dim != 128 && head_dim != 256))
+    return fail(SABER_IU8_E_RULE, fmt("attn_workspace: %u sequences of %u heads over %u kv heads of %u", seqs, heads, kv_heads, head_dim));
+  Plan p;
+  if (int rc = attn_args("attn_workspace", seqs, max_q, max_kv, heads, kv_heads, &p)) return rc;
+  const bool split = p.splits > 1;
+  if (partial_bytes) *partial_bytes = split ? p.items * p.splits * p.rows * (head_dim + 4) * 4 : 0;
+  if (counter_bytes) *counter_bytes = split ? p.items * 4 : 0;
+  return 0;
+}
+
+int saber_iu8_attn(saber_iu8_ctx *ctx, const void *q, uint32_t q_row, const saber_iu8_kv_cache *cache, const int32_t *cu_q, void *out, uint32_t tokens,
+                   uint32_t seqs, uint32_t max_q, uint32_t max_kv, uint32_t heads, float scale, void *partial, void *counter, void *stream) {
+  const char *op = "attn";
+  if (int rc = cache_check(op, cache, heads, seqs, tokens, cu_q)) return rc;
+  const uint32_t D = cache->head_dim;
+  if (!q || !out) return fail(SABER_IU8_E_ARG, "attn: null rows");
+  if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)partial) % 16 || (uintptr_t)counter % 4) return fail(SABER_IU8_E_ARG, "attn: rows and partials must lie on 16 bytes");
+  if (q_row % 8 || q_row > I32_MAX || q_row < (uint64_t)heads * D)
+    return fail(SABER_IU8_E_RULE, fmt("attn: rows of %u elements: whole 16-byte pieces that cover %u heads of %u", q_row, heads, D));
+  if (!std::isfinite(scale)) return fail(SABER_IU8_E_RULE, "attn: the scale must be a number");
+  if (!cu_q) max_q = 1;
+  Plan p;
+  if (int rc = attn_args(op, seqs, max_q, max_kv, heads, cache->kv_heads, &p)) return rc;
+  if (!partial || !counter) p.splits = 1, p.chunk = WHOLE;  // in one piece
+  const bool f8 = cache->kind == SABER_IU8_KV_E4M3;
+  const char *kind = f8 ? "e4m3" : "bf16";
+  saber_iu8_desc d;
+  const uint32_t grid[3] = {(uint32_t)(p.items * p.splits), 1, 1};
+  const std::string name = p.few() ? fmt("attn_few_%s_d%u_r%u", kind, D, p.rows) : fmt("attn_many_%s_d%u", kind, D);
+  if (int rc = saber_iu8_describe_raw(name.c_str(), "attn_paged", grid, 256, &d)) return rc;
+  copy_name(d.op, sizeof d.op, op);
+  set_i32(&d, "q_row", q_row), set_i32(&d, "tokens", tokens), set_i32(&d, "shape", heads | cache->kv_heads << 16);
+  set_i32(&d, "page_shift", log2_of(cache->page_tokens)), set_i32(&d, "pages", cache->pages), set_i32(&d, "table_stride", cache->table_stride);
+  set_i32(&d, "chunk", p.chunk), set_i32(&d, "splits", p.splits), set_i32(&d, "qtiles", p.qtiles);
+  set_f32(&d, "scale", scale);
+  if (!f8) set_null(&d, "k_scale"), set_null(&d, "v_scale");
+  if (!cu_q) set_null(&d, "cu_q");
+  if (p.splits == 1) set_null(&d, "partial"), set_null(&d, "counter");
+  const saber_iu8_binding b[] = {{"q", (void *)q},
+                                 {"kc", cache->k},
+                                 {"vc", cache->v},
+                                 {"k_scale", (void *)cache->k_scale},
+                                 {"v_scale", (void *)cache->v_scale},
+                                 {"table", (void *)cache->page_table},
+                                 {"kv_len", (void *)cache->kv_len},
+                                 {"cu_q", (void *)cu_q},
+                                 {"out", out},
+                                 {"partial", partial},
+                                 {"counter", counter}};
+  return saber_iu8_launch(ctx, &d, b, 11, stream);
+}
+
+}  // extern "C"

@@ -122,6 +122,9 @@ int ref_symbol_by_law(const std::string &kernel, int *w8, const char **note);
 std::string band_toml();
 std::string device_profile_toml();
 
+// The scalars of a descriptor of the paged cache's kernels (attn.cpp).
+int attn_guard(const saber_iu8_desc *d);
+
 // Fills name/offset/size of every slot from the kernel's signature; kinds default to BUFFER.
 int fill_slots(const std::string &kernel, saber_iu8_desc *d);
 void set_i32(saber_iu8_desc *d, const char *name, int64_t v);

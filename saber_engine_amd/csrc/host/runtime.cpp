@@ -396,6 +396,7 @@ static int counters_guard(const saber_iu8_desc *d) {
 static int launch_guard(const LoadedKernel &lk, const saber_iu8_desc *d) {
   if (int rc = counters_guard(d)) return rc;
   if (strncmp(d->kernel, "macaq_iu8f_mlp_", 15) == 0) return chain_guard(lk, d);
+  if (!strncmp(d->kernel, "kv_append_", 10) || !strncmp(d->kernel, "attn_few_", 9) || !strncmp(d->kernel, "attn_many_", 10)) return attn_guard(d);
   if (strncmp(d->kernel, "macaq_iu8f_gateup_act_", 22) == 0) {
     const int64_t m = i32_arg(d, "m"), n = i32_arg(d, "n"), k = i32_arg(d, "k");
     if (m <= 0 || n <= 0 || k <= 0 || !gate_up_act_holds((uint32_t)m, (uint32_t)k, (uint32_t)n))

@@ -1,0 +1,67 @@
+// Shared device helpers of the paged key/value cache and the attention that reads it.
+//
+// CACHE ORDER (gfx950 device-final; E = the elements of 16 bytes: 8 bf16 or 16 e4m3). A page holds `page_tokens` tokens (a
+// power of two, 16 to 256) of every kv head; page p, head h start at element (p * kv_heads + h) * page_tokens * D in both arrays.
+//   K   blocks of 16 tokens, [D / E][16 tokens][E]: 64 lanes x 16 bytes in a row are 16 tokens x 4 pieces, which is the operand
+//       of a 16x16x32 MFMA (bf16; two of them for e4m3), and 32 tokens x 2 pieces the one of a 32x32x16 MFMA: both kinds of kernel
+//       read whole lines and no lane exchanges anything.
+//   V   [token][D]. Its operand wants several tokens of one channel a lane; the few-row kernel pairs them with byte permutes
+//       on the way from the load (a sixteenth of its time budget), the many-row kernel with the LDS's transposing read.
+// A block of 16 tokens is the same 16 * D elements in both arrays, contiguous.
+//
+// A sequence's tokens lie in the pages of its row of the page table. An entry outside 0 .. pages - 1 is a hole: its keys take no
+// part and nothing is written through it. Lengths are bounded by the table's row, so no length makes a kernel read past either.
+#pragma once
+#include "iu8_common.h"
+
+typedef __bf16 at_v8bf __attribute__((ext_vector_type(8)));
+typedef __bf16 at_v2bf __attribute__((ext_vector_type(2)));
+typedef float at_v16f __attribute__((ext_vector_type(16)));
+typedef short at_v4s __attribute__((ext_vector_type(4)));
+
+struct AtCache {
+  const unsigned char *k, *v;
+  const int *table, *kv_len;
+  int kv_heads, page_shift, pages, table_stride;
+};
+
+static __device__ __forceinline__ int at_uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// Tokens of sequence s, bounded by what its row of the page table can hold.
+static __device__ __forceinline__ int at_len(const int *kv_len, int s, int table_stride, int page_shift) {
+  const long long most = (long long)table_stride << page_shift;
+  const int n = kv_len[s];
+  return n < 0 ? 0 : (long long)n > most ? (int)most : n;
+}
+
+// The sequence that row t belongs to when rows are packed (cu[s] .. cu[s + 1] - 1), by one wave: the number of ends at or before
+// t. `seqs` when t lies behind the last sequence.
+static __device__ __forceinline__ int at_find(const int *__restrict__ cu, int seqs, int t) {
+  int s = 0;
+  for (int base = 0; base < seqs; base += 64) {
+    const int i = base + (int)(threadIdx.x & 63);
+    const bool before = i < seqs && cu[i + 1] <= t;
+    s += __popcll(__ballot(before));
+  }
+  return s;
+}
+
+static __device__ __forceinline__ at_v8bf at_bf(iu8_v4u x) { return __builtin_bit_cast(at_v8bf, x); }
+static __device__ __forceinline__ at_v8bf at_bf(unsigned a, unsigned b, unsigned c, unsigned d) { return at_bf(iu8_v4u{a, b, c, d}); }
+
+// Two e4m3 values (bytes 0, 1 or 2, 3 of x) as packed bf16: exact, every e4m3 value is a bf16 value.
+template <bool HI>
+static __device__ __forceinline__ unsigned at_e4m3_bf16(unsigned x) {
+  return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)x, 1.f, HI));
+}
+// Eight e4m3 values -> eight bf16.
+static __device__ __forceinline__ iu8_v4u at_e4m3x8(unsigned lo, unsigned hi) {
+  return iu8_v4u{at_e4m3_bf16<false>(lo), at_e4m3_bf16<true>(lo), at_e4m3_bf16<false>(hi), at_e4m3_bf16<true>(hi)};
+}
+
+// A packed pair of bf16 holds an infinity or a NaN.
+static __device__ __forceinline__ bool at_nonfinite2(unsigned x) { return (x & 0x7F80u) == 0x7F80u || (x & 0x7F800000u) == 0x7F800000u; }
+
+// f32 partials of a split: 16 bytes a store / load that are coherent across the XCDs' L2s by themselves (iu8_common.h).
+static __device__ __forceinline__ void at_store_through(float *p, iu8_v4f v) { iu8_store_through((int *)p, __builtin_bit_cast(iu8_v4i, v)); }
+static __device__ __forceinline__ iu8_v4f at_load_through(const float *p) { return __builtin_bit_cast(iu8_v4f, iu8_load_through((const int *)p)); }

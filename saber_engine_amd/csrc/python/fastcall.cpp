@@ -6,7 +6,7 @@
 // share, util.h: a one-row linear of 5120 x 5120 in a loop of calls 7.5-8.1 -> 6.5-7.2 us, its kernel 5; 16 rows, quantiser and
 // GEMM, 11.6-12.7 -> 9.7-11.0.) The conversions are ctypes' own for what a caller
 // passes: a pointer is an int or None, a number an int, a float a float, each taken modulo its width; the routed operators'
-// tables are the structure itself (an address in their place is refused, as ctypes refuses it). Anything else in an argument's
+// tables and the key/value cache are the structure itself (an address in their place is refused, as ctypes refuses it). Anything else in an argument's
 // place (a ctypes object, a bool, another count of arguments) sends the whole call, its arguments as they came, to the ctypes
 // function of the same name, which converts or refuses them. The interpreter lock is released around the call, as ctypes does.
 #define PY_SSIZE_T_CLEAN
@@ -21,11 +21,12 @@
 namespace {
 
 PyObject *tables_type = nullptr;  // the binding's saber_iu8_moe_tables
+PyObject *cache_type = nullptr;   // ... and saber_iu8_kv_cache
 
 template <class T>
 bool take(PyObject *o, T &v) {
-  if constexpr (std::is_same_v<T, const saber_iu8_moe_tables *>) {
-    if ((PyObject *)Py_TYPE(o) != tables_type) return false;
+  if constexpr (std::is_same_v<T, const saber_iu8_moe_tables *> || std::is_same_v<T, const saber_iu8_kv_cache *>) {
+    if ((PyObject *)Py_TYPE(o) != (std::is_same_v<T, const saber_iu8_moe_tables *> ? tables_type : cache_type)) return false;
     Py_buffer b;
     if (PyObject_GetBuffer(o, &b, PyBUF_SIMPLE)) return false;
     const bool whole = b.len == (Py_ssize_t)sizeof *v;
@@ -80,12 +81,15 @@ struct Entry<F> {
   X(quant) X(quant_rowmajor) X(gemm) X(rowscale) X(linear_prefill_fused) X(gemm_static) X(gemm_pair) X(linear_fused) X(mlp_chain)  \
   X(gate_up_act) X(quant_had) X(silu_mul_quant_had) X(silu_mul_quant_had_lut) X(add_rms_quant_had) X(gdn_norm_quant_had)          \
   X(attn_gate_quant_had) X(attn_gate_quant_had_lut) X(moe_route) X(moe_route_quant) X(moe_grouped) X(moe_quant_rows)              \
-  X(moe_silu_mul_quant) X(moe_gate_up_act) X(moe_down_rows) X(moe_combine)
+  X(moe_silu_mul_quant) X(moe_gate_up_act) X(moe_down_rows) X(moe_combine) X(kv_append) X(attn)
 
-// bind(functions, tables): {name: ctypes function}, the ctypes structure of the routed operators' tables
+// bind(functions, tables, cache): {name: ctypes function}, the ctypes structures of the routed operators' tables and of the
+// key/value cache
 PyObject *bind(PyObject *, PyObject *args) {
-  PyObject *functions, *tables;
-  if (!PyArg_ParseTuple(args, "O!O!", &PyDict_Type, &functions, &PyType_Type, &tables)) return nullptr;
+  PyObject *functions, *tables, *cache;
+  if (!PyArg_ParseTuple(args, "O!O!O!", &PyDict_Type, &functions, &PyType_Type, &tables, &PyType_Type, &cache)) return nullptr;
+  Py_INCREF(cache);
+  Py_XSETREF(cache_type, cache);
   Py_INCREF(tables);
   Py_XSETREF(tables_type, tables);
 #define BIND(name)                                                  \

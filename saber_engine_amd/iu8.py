@@ -78,6 +78,19 @@ class MoeTables(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in MOE_TABLE_FIELDS]
 
 
+KV_BF16, KV_E4M3 = 0, 1
+
+
+class KvCache(C.Structure):
+    """A paged key/value cache (saber_iu8_kv_cache): device addresses, the caller's."""
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "k_scale", "v_scale", "page_table", "kv_len")] + [
+        (n, C.c_uint32) for n in ("kind", "kv_heads", "head_dim", "page_tokens", "pages", "table_stride")]
+
+    @classmethod
+    def of(cls, k, v, page_table, kv_len, *, kv_heads, head_dim, page_tokens, pages, table_stride, kind=KV_BF16, k_scale=None, v_scale=None):
+        return cls(k, v, k_scale, v_scale, page_table, kv_len, kind, kv_heads, head_dim, page_tokens, pages, table_stride)
+
+
 class IU8Error(RuntimeError):
     def __init__(self, code, msg):
         super().__init__(f"[{code}] {msg}")
@@ -162,6 +175,16 @@ def lib():
         L.saber_iu8_moe_down_rows.argtypes = [C.c_void_p] * 4 + [C.c_uint32] * 6 + [C.POINTER(MoeTables), C.c_void_p]
         L.saber_iu8_moe_silu_mul_quant.argtypes = [C.c_void_p] * 4 + [C.c_uint32, C.c_uint32, C.POINTER(MoeTables), C.c_void_p]
         L.saber_iu8_moe_combine.argtypes = [C.c_void_p, C.c_void_p, C.POINTER(MoeTables), C.c_void_p] + [C.c_uint32] * 3 + [C.c_void_p]
+        L.saber_iu8_kv_bytes.restype = C.c_uint64
+        L.saber_iu8_kv_bytes.argtypes = [C.c_uint32] * 5
+        for fn in ("saber_iu8_kv_k_offset", "saber_iu8_kv_v_offset"):
+            getattr(L, fn).restype = C.c_uint64
+            getattr(L, fn).argtypes = [C.c_uint32] * 8
+        L.saber_iu8_kv_append.argtypes = ([C.c_void_p] * 5 + [C.POINTER(KvCache), C.c_void_p] + [C.c_uint32] * 6 +
+                                          [C.c_void_p, C.c_uint32, C.c_int, C.c_void_p, C.c_void_p, C.c_float, C.c_void_p])
+        L.saber_iu8_attn_workspace.argtypes = [C.c_uint32] * 6 + [C.POINTER(C.c_uint64)] * 2
+        L.saber_iu8_attn.argtypes = ([C.c_void_p, C.c_void_p, C.c_uint32, C.POINTER(KvCache), C.c_void_p, C.c_void_p] + [C.c_uint32] * 5 +
+                                     [C.c_float] + [C.c_void_p] * 3)
         L.saber_iu8_silu_table.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p]
         _lib = L
     return _lib
@@ -389,14 +412,15 @@ def operators():
         except ImportError:
             _ops = _CtypesOperators()
             return _ops
-        _fastcall.bind({n: getattr(L, "saber_iu8_" + n) for n in dir(_fastcall) if not n.startswith("_") and n != "bind"}, MoeTables)
+        _fastcall.bind({n: getattr(L, "saber_iu8_" + n) for n in dir(_fastcall) if not n.startswith("_") and n != "bind"}, MoeTables, KvCache)
         _ops = _fastcall
     return _ops
 
 
 def _tables(t):
-    """The routed operators' tables as both kinds of entry points take them (never as an address, which ctypes refuses)."""
-    return t if type(t) is MoeTables else C.byref(t)
+    """The routed operators' tables, or a key/value cache, as both kinds of entry points take them (never as an address, which
+    ctypes refuses)."""
+    return t if type(t) in (MoeTables, KvCache) else C.byref(t)
 
 
 class Context:
@@ -535,6 +559,19 @@ class Context:
     def silu_table(self, out, stream=0):
         _check(lib().saber_iu8_silu_table(self._h, out, stream))
 
+    # ---- paged key/value cache, attention
+    def kv_append(self, q, k, v, q_out, cache, cu_q, tokens, seqs, heads, q_row, q_head, kv_row, inv_freq=None, rot_dim=0, interleaved=False,
+                  q_norm=None, k_norm=None, eps=1e-6, stream=0):
+        """New tokens into the cache, q and k normed (optional) and rotated by their positions on the way; q_out bf16 [tokens, heads,
+        head_dim]. cu_q None: one row a sequence."""
+        _check(self._op.kv_append(self._addr, q, k, v, q_out, _tables(cache), cu_q, tokens, seqs, heads, q_row, q_head, kv_row, inv_freq, rot_dim,
+                                  int(interleaved), q_norm, k_norm, eps, stream))
+
+    def attn(self, q, q_row, cache, cu_q, out, tokens, seqs, max_q, max_kv, heads, scale, partial=None, counter=None, stream=0):
+        """The new rows' causal attention over the cache: out bf16 [tokens, heads, head_dim]. The workspaces of attn_workspace, or
+        neither: in one piece."""
+        _check(self._op.attn(self._addr, q, q_row, _tables(cache), cu_q, out, tokens, seqs, max_q, max_kv, heads, scale, partial, counter, stream))
+
 
 def moe_rows_cap(tokens, topk, experts, shared=False):
     return (lib().saber_iu8_moe_rows_cap_shared if shared else lib().saber_iu8_moe_rows_cap)(tokens, topk, experts)
@@ -562,3 +599,15 @@ def gemm_workspace(wkind, m, n, k):
     p, c = C.c_uint64(), C.c_uint64()
     _check(lib().saber_iu8_gemm_workspace(wkind, m, n, k, C.byref(p), C.byref(c)))
     return p.value, c.value
+
+
+def attn_workspace(seqs, max_q, max_kv, heads, kv_heads, head_dim):
+    """Bytes of attn()'s (partial, counter); both 0 where it runs in one piece."""
+    p, c = C.c_uint64(), C.c_uint64()
+    _check(lib().saber_iu8_attn_workspace(seqs, max_q, max_kv, heads, kv_heads, head_dim, C.byref(p), C.byref(c)))
+    return p.value, c.value
+
+
+def kv_bytes(pages, kv_heads, head_dim, page_tokens, kind=KV_BF16):
+    """Bytes of a cache's k (and of its v)."""
+    return lib().saber_iu8_kv_bytes(pages, kv_heads, head_dim, page_tokens, kind)
