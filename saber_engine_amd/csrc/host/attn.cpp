@@ -54,15 +54,17 @@ struct Plan {
   bool few() const { return rows <= FEW_ROWS; }
 };
 
-// The split of the cache's length. The grid wants a few workgroups a CU; a part is at least 128 tokens (few rows: a 32-token tile
-// for each of the four waves) or 512 (many rows).
-Plan plan(uint32_t seqs, uint32_t max_q, uint32_t max_kv, uint32_t heads, uint32_t kv_heads) {
+// The split of the cache's length. Few rows: a part is at least 128 tokens (a 32-token tile for each of the four waves); one
+// sequence is cut into as many equal parts as the card holds workgroups (by their LDS), several into four times as many, since
+// their lengths differ and a short one's workgroups leave at once. Many rows: parts of at least 512 tokens, two workgroups a CU.
+Plan plan(uint32_t seqs, uint32_t max_q, uint32_t max_kv, uint32_t heads, uint32_t kv_heads, uint32_t dim, bool f8) {
   Plan p;
   const uint64_t rows = (uint64_t)max_q * (heads / kv_heads);
   p.rows = rows <= 16 ? 16 : rows <= FEW_ROWS ? FEW_ROWS : MANY_ROWS;
   p.qtiles = p.few() ? 1 : (rows + MANY_ROWS - 1) / MANY_ROWS;
   p.items = (uint64_t)seqs * kv_heads * p.qtiles;
-  const uint64_t target = p.few() ? 1024 : 512, unit = p.few() ? 128 : 512;
+  const uint32_t held = p.rows == 16 && (f8 || dim < 256) ? 2 : 1;
+  const uint64_t target = p.few() ? (uint64_t)CU_COUNT * held * (seqs == 1 ? 1 : 4) : 2 * CU_COUNT, unit = p.few() ? 128 : 512;
   uint64_t parts = std::max<uint64_t>(1, target / std::max<uint64_t>(p.items, 1));
   const uint64_t most = std::max<uint64_t>(1, (max_kv + unit - 1) / unit);
   parts = std::min(parts, most);
@@ -73,9 +75,9 @@ Plan plan(uint32_t seqs, uint32_t max_q, uint32_t max_kv, uint32_t heads, uint32
   return p;
 }
 
-int attn_args(const char *op, uint32_t seqs, uint32_t max_q, uint32_t max_kv, uint32_t heads, uint32_t kv_heads, Plan *p) {
+int attn_args(const char *op, uint32_t seqs, uint32_t max_q, uint32_t max_kv, uint32_t heads, uint32_t kv_heads, uint32_t dim, bool f8, Plan *p) {
   if (!max_q || max_kv > I32_MAX) return fail(SABER_IU8_E_RULE, fmt("%s: at most %u new rows and %u keys a sequence: from 1 and below 2^31", op, max_q, max_kv));
-  *p = plan(seqs, max_q, max_kv, heads, kv_heads);
+  *p = plan(seqs, max_q, max_kv, heads, kv_heads, dim, f8);
   if ((uint64_t)max_q * (heads / kv_heads) > I32_MAX || p->items * p->splits > I32_MAX)
     return fail(SABER_IU8_E_RULE, fmt("%s: %u sequences of up to %u new rows and %u heads pass a launch's 32-bit sizes", op, seqs, max_q, heads));
   return 0;
@@ -181,11 +183,16 @@ int saber_iu8_attn_workspace(uint32_t seqs, uint32_t max_q, uint32_t max_kv, uin
                              uint64_t *partial_bytes, uint64_t *counter_bytes) {
   if (!seqs || !heads || !kv_heads || heads % kv_heads || (head_dim != 64 && head_dim != 128 && head_dim != 256))
     return fail(SABER_IU8_E_RULE, fmt("attn_workspace: %u sequences of %u heads over %u kv heads of %u", seqs, heads, kv_heads, head_dim));
-  Plan p;
-  if (int rc = attn_args("attn_workspace", seqs, max_q, max_kv, heads, kv_heads, &p)) return rc;
-  const bool split = p.splits > 1;
-  if (partial_bytes) *partial_bytes = split ? p.items * p.splits * p.rows * (head_dim + 4) * 4 : 0;
-  if (counter_bytes) *counter_bytes = split ? p.items * 4 : 0;
+  uint64_t partial = 0, counter = 0;
+  for (bool f8 : {false, true}) {  // enough for a cache of either kind
+    Plan p;
+    if (int rc = attn_args("attn_workspace", seqs, max_q, max_kv, heads, kv_heads, head_dim, f8, &p)) return rc;
+    if (p.splits == 1) continue;
+    partial = std::max(partial, p.items * p.splits * p.rows * (head_dim + 4) * 4);
+    counter = std::max(counter, p.items * 4);
+  }
+  if (partial_bytes) *partial_bytes = partial;
+  if (counter_bytes) *counter_bytes = counter;
   return 0;
 }
 
@@ -201,9 +208,9 @@ int saber_iu8_attn(saber_iu8_ctx *ctx, const void *q, uint32_t q_row, const sabe
   if (!std::isfinite(scale)) return fail(SABER_IU8_E_RULE, "attn: the scale must be a number");
   if (!cu_q) max_q = 1;
   Plan p;
-  if (int rc = attn_args(op, seqs, max_q, max_kv, heads, cache->kv_heads, &p)) return rc;
-  if (!partial || !counter) p.splits = 1, p.chunk = WHOLE;  // in one piece
   const bool f8 = cache->kind == SABER_IU8_KV_E4M3;
+  if (int rc = attn_args(op, seqs, max_q, max_kv, heads, cache->kv_heads, D, f8, &p)) return rc;
+  if (!partial || !counter) p.splits = 1, p.chunk = WHOLE;  // in one piece
   const char *kind = f8 ? "e4m3" : "bf16";
   saber_iu8_desc d;
   const uint32_t grid[3] = {(uint32_t)(p.items * p.splits), 1, 1};

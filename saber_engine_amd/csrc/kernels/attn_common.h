@@ -5,8 +5,7 @@
 //   K   blocks of 16 tokens, [D / E][16 tokens][E]: 64 lanes x 16 bytes in a row are 16 tokens x 4 pieces, which is the operand
 //       of a 16x16x32 MFMA (bf16; two of them for e4m3), and 32 tokens x 2 pieces the one of a 32x32x16 MFMA: both kinds of kernel
 //       read whole lines and no lane exchanges anything.
-//   V   [token][D]. Its operand wants several tokens of one channel a lane; the few-row kernel pairs them with byte permutes
-//       on the way from the load (a sixteenth of its time budget), the many-row kernel with the LDS's transposing read.
+//   V   [token][D]. Its operand wants several tokens of one channel a lane, which the LDS's transposing reads give.
 // A block of 16 tokens is the same 16 * D elements in both arrays, contiguous.
 //
 // A sequence's tokens lie in the pages of its row of the page table. An entry outside 0 .. pages - 1 is a hole: its keys take no
@@ -61,6 +60,22 @@ static __device__ __forceinline__ iu8_v4u at_e4m3x8(unsigned lo, unsigned hi) {
 
 // A packed pair of bf16 holds an infinity or a NaN.
 static __device__ __forceinline__ bool at_nonfinite2(unsigned x) { return (x & 0x7F80u) == 0x7F80u || (x & 0x7F800000u) == 0x7F800000u; }
+
+// A packed quadruple of e4m3 holds a NaN (it has no infinities).
+static __device__ __forceinline__ bool at_e4m3_nan4(unsigned x) { return (((x & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) != 0; }
+// Four neighbouring values of an LDS row as f32.
+template <bool F8>
+static __device__ __forceinline__ void at_four(const unsigned char *p, float (&v)[4]) {
+  iu8_v2u x;
+  if constexpr (F8) {
+    const unsigned y = *(const unsigned *)p;
+    x = iu8_v2u{at_e4m3_bf16<false>(y), at_e4m3_bf16<true>(y)};
+  } else {
+    x = *(const iu8_v2u *)p;
+  }
+  v[0] = __uint_as_float(x[0] << 16), v[1] = __uint_as_float(x[0] & 0xFFFF0000u);
+  v[2] = __uint_as_float(x[1] << 16), v[3] = __uint_as_float(x[1] & 0xFFFF0000u);
+}
 
 // f32 partials of a split: 16 bytes a store / load that are coherent across the XCDs' L2s by themselves (iu8_common.h).
 static __device__ __forceinline__ void at_store_through(float *p, iu8_v4f v) { iu8_store_through((int *)p, __builtin_bit_cast(iu8_v4i, v)); }

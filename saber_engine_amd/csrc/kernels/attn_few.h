@@ -6,12 +6,21 @@
 //   M = max m_i, L = sum exp(m_i - M) l_i, o = sum exp(m_i - M) o_i / L.
 // A row that sees no key gives zeros.
 //
-// One workgroup: one kv head of one sequence, a run of `chunk` tokens; its four waves take the run's 32-token tiles in turn and
-// every wave streams K and V from memory to registers, no LDS between: the rows of the whole group of query heads (and of all new
-// tokens: row r is new token r / G, head r % G) share each byte. Bound by the bytes of the cache. Both products have the
-// row as the MFMA's column (S^T = K Q^T, O^T = V^T P^T), so a lane keeps one row: its maximum, sum and rescale are plain lane
-// arithmetic but for two exchanges a tile, and P goes from the first product's result to the second's operand where it is (the
-// second's token order is whatever the first left: 4 g + r of the two blocks of 16).
+// One workgroup: one kv head of one sequence, a run of `chunk` tokens; its four waves take the run's 32-token tiles in turn. The
+// rows of the whole group of query heads (and of all new tokens: row r is new token r / G, head r % G) share each byte. Bound by
+// the bytes of the cache, so what matters is bytes in flight: every wave has a tile of K and a tile of V in LDS of its own, filled
+// straight from memory, and asks for the next K as soon as its scores are made, for the next V as soon as its product is: up to
+// 128 KiB a compute unit on the way, with no register held for it and no barrier between the waves.
+//
+// Both products have the row as the MFMA's column (S^T = K Q^T, O^T = V^T P^T), so a lane keeps one row: its maximum, sum and
+// rescale are plain lane arithmetic but for two exchanges a tile, and P goes from the first product's result to the second's
+// operand where it is (the second's token order is whatever the first left: 4 g + r of the two blocks of 16). V's operand has
+// eight tokens of one channel a lane: the LDS's transposing reads give it from V's rows, whose 16-byte pieces are exchanged
+// within a row on the way into LDS so that a read's rows lie in all banks.
+//
+// A weight of zero would keep an infinity or a NaN of V (0 * inf), so what a row does not see must not reach its product: V's
+// rows behind the end and in holes are zeroed in LDS; a value that is not finite among the new tokens themselves, which some
+// rows see and others do not, takes the product's slow form (lane arithmetic, only for the rows that see it).
 //
 // Rounding: scores, statistics and sums in f32; P is rounded to bf16 for the second product (each weight off by at most 2^-8 of
 // itself, the sum of weights taken of the unrounded ones), the output once to bf16.
@@ -25,47 +34,102 @@ static __device__ __forceinline__ int at_chunk(int len, int chunk, int splits) {
   return (long long)chunk * splits >= len ? chunk : (((len - 1) / splits + 1) + 127) / 128 * 128;
 }
 
-// Joins `ns` parts of one item: part i's rows at part + i * R * D, their (m, l) at ml + i * 2 R; rows r < live go out.
-template <int D, int R, int T>
+// Joins `ns` parts of one item: part i's rows at part + i * R * D, their (m, l) -- four floats a row, one 16-byte store -- at
+// ml + i * 4 R; rows r < live go out. The parts come from memory (other XCDs wrote them), so as many loads as registers allow are
+// in flight: U items x K parts a thread. `s_f`: LDS for the rows' (m, l) of PARTS parts at a time.
+template <int D, int R, int T, int PARTS, int U, int K>
 static __device__ __forceinline__ void at_join(const float *__restrict__ part, const float *__restrict__ ml, int ns, int live, float vs, int tid,
-                                               unsigned short *__restrict__ out, const long long *s_dst, float *s_m, float *s_il) {
-  // the rows' joint maximum and sum, a row a thread
-  for (int r = tid; r < live; r += T) {
-    float m = -__builtin_inff(), l = 0.f;
-    for (int i = 0; i < ns; ++i) {
-      const iu8_v4f x = at_load_through(ml + ((size_t)i * R + r) * 4);
-      const float mn = fmaxf(m, x[0]), base = mn == -__builtin_inff() ? 0.f : mn;
-      l = l * __builtin_amdgcn_exp2f(m - base) + x[1] * __builtin_amdgcn_exp2f(x[0] - base);
-      m = mn;
-    }
-    s_m[r] = m == -__builtin_inff() ? 0.f : m;
-    s_il[r] = l == 0.f ? 0.f : vs / l;
-  }
+                                               unsigned short *__restrict__ out, const long long *s_dst, float *s_m, float *s_il, float *s_f) {
+  constexpr int NI = (R * (D / 4) + T - 1) / T;
+  // the rows' joint maxima and sums
+  for (int r = tid; r < R; r += T) s_m[r] = -__builtin_inff(), s_il[r] = 0.f;
   __syncthreads();
-  for (int e = tid; e < live * (D / 4); e += T) {
-    const int r = e / (D / 4), d = (e % (D / 4)) * 4;
-    iu8_v4f o = {0.f, 0.f, 0.f, 0.f};
-    for (int i = 0; i < ns; ++i) {
-      const float m = at_load_through(ml + ((size_t)i * R + r) * 4)[0], f = __builtin_amdgcn_exp2f(m - s_m[r]);
-      const iu8_v4f x = at_load_through(part + ((size_t)i * R + r) * D + d);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) o[c] = fmaf(f, x[c], o[c]);
+  for (int i0 = 0; i0 < ns; i0 += PARTS) {
+    const int np = min(PARTS, ns - i0);
+    for (int e = tid; e < np * live; e += T) {
+      const iu8_v4f x = at_load_through(ml + ((size_t)(i0 + e / live) * R + e % live) * 4);
+      s_f[2 * e] = x[0], s_f[2 * e + 1] = x[1];
     }
-    const float il = s_il[r];
-    *(iu8_v2u *)(out + s_dst[r] + d) = iu8_v2u{iu8_bf16_pack(o[0] * il, o[1] * il), iu8_bf16_pack(o[2] * il, o[3] * il)};
+    __syncthreads();
+    for (int r = tid; r < live; r += T) {
+      float m = s_m[r], l = s_il[r];
+      for (int i = 0; i < np; ++i) {
+        const float mi = s_f[2 * (i * live + r)], mn = fmaxf(m, mi), base = mn == -__builtin_inff() ? 0.f : mn;
+        l = l * __builtin_amdgcn_exp2f(m - base) + s_f[2 * (i * live + r) + 1] * __builtin_amdgcn_exp2f(mi - base);
+        m = mn;
+      }
+      s_m[r] = m, s_il[r] = l;
+    }
+    __syncthreads();
+  }
+  for (int it = 0; it < NI; it += U) {
+    if (it * T >= live * (D / 4)) break;  // (the same for every thread)
+    iu8_v4f o[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) o[u] = iu8_v4f{0.f, 0.f, 0.f, 0.f};
+    for (int i0 = 0; i0 < ns; i0 += PARTS) {
+      const int np = min(PARTS, ns - i0);
+      if (ns > PARTS || it == 0) {  // the parts' factors
+        __syncthreads();
+        for (int e = tid; e < np * live; e += T) {
+          const int r = e % live;
+          const float m = at_load_through(ml + ((size_t)(i0 + e / live) * R + r) * 4)[0], top = s_m[r];
+          s_f[e] = top == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - top);
+        }
+        __syncthreads();
+      }
+      for (int i = 0; i < np; i += K) {
+        iu8_v4f x[U][K];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int k = 0; k < K; ++k) {
+            const int e = min((it + u) * T + tid, live * (D / 4) - 1), ii = min(i + k, np - 1);
+            x[u][k] = at_load_through(part + ((size_t)(i0 + ii) * R + e / (D / 4)) * D + e % (D / 4) * 4);
+          }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int k = 0; k < K; ++k) {
+            const int e = min((it + u) * T + tid, live * (D / 4) - 1);
+            const float f = i + k < np ? s_f[(i + k) * live + e / (D / 4)] : 0.f;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) o[u][c] = i + k < np ? fmaf(f, x[u][k][c], o[u][c]) : o[u][c];
+          }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int e = (it + u) * T + tid;
+      if (it + u < NI && e < live * (D / 4)) {
+        const int r = e / (D / 4);
+        const float il = s_il[r] == 0.f ? 0.f : vs / s_il[r];
+        *(iu8_v2u *)(out + s_dst[r] + e % (D / 4) * 4) = iu8_v2u{iu8_bf16_pack(o[u][0] * il, o[u][1] * il), iu8_bf16_pack(o[u][2] * il, o[u][3] * il)};
+      }
+    }
   }
 }
 
-// The rows' (m, l) in a partial take four floats a row, so that a row's pair is one 16-byte store.
+template <int D, bool F8>
+struct AtFew {
+  static constexpr int ES = F8 ? 1 : 2, ROWB = D * ES, TILE = 32 * ROWB, NL = TILE / 1024;  // wave-loads of 1 KiB a tile
+  // where V's piece lies in its row: piece ^ swz(token), so that the rows that one transposing read takes together (16 of
+  // 32 bytes for bf16, 32 of 16 bytes for e4m3) lie in all banks
+  static __device__ __forceinline__ int swz(int t) {
+    if constexpr (F8) return D == 256 ? t & 15 : D == 128 ? t & 7 : (t >> 1) & 3;
+    else return 2 * (D == 256 ? t & 15 : D == 128 ? t & 7 : t & 3);
+  }
+};
+
 template <int D, bool F8, int RT>
 static __device__ __forceinline__ void attn_few_body(
     const unsigned short *__restrict__ q, const unsigned char *__restrict__ kc, const unsigned char *__restrict__ vc,
     const float *__restrict__ k_scale, const float *__restrict__ v_scale, const int *__restrict__ table, const int *__restrict__ kv_len,
     const int *__restrict__ cu_q, unsigned short *__restrict__ out, float *__restrict__ partial, int *__restrict__ counter, int q_row,
     int tokens, int shape, int page_shift, int pages, int table_stride, int chunk, int splits, float scale) {
-  constexpr int ES = F8 ? 1 : 2, R = 16 * RT, KS = D / 32, DL = D / 16, W = 4;
-  constexpr int NV = DL * ES >= 16 ? DL * ES / 16 : 1;  // 16-byte loads (one shorter load) a token and lane of V
-  constexpr int VD = DL * ES >= 16 ? 4 : DL * ES / 4;   // dwords of each
+  using A = AtFew<D, F8>;
+  constexpr int ES = A::ES, ROWB = A::ROWB, TILE = A::TILE, NL = A::NL, R = 16 * RT, KS = D / 32, DT = D / 16, W = 4;
+  constexpr int REGION = 2 * TILE > R * (D + 4) * 4 ? 2 * TILE : R * (D + 4) * 4;  // a wave's LDS: its tiles, then its part of the sum
   const int heads = shape & 0xFFFF, kv_heads = shape >> 16, G = heads / kv_heads;
   const int split = blockIdx.x % splits, item = blockIdx.x / splits, h = item % kv_heads, s = item / kv_heads;
   const int tid = threadIdx.x, lane = tid & 63, wave = at_uniform(tid >> 6), n = lane & 15, g = lane >> 4;
@@ -79,13 +143,65 @@ static __device__ __forceinline__ void attn_few_body(
   const int ns = len > chunk ? (len + chunk - 1) / chunk : 1;
   if (split >= ns) return;
 
-  __shared__ __attribute__((aligned(16))) float s_o[W][R][D + 4];
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[W * REGION];
   __shared__ float s_ml[2][W][R];
   __shared__ float s_m[R], s_il[R];
   __shared__ long long s_dst[R];
   __shared__ int s_last;
+  const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) unsigned char *)smem;
+  unsigned char *sk = smem + wave * REGION, *sv = sk + TILE;
 
-  // query fragments and the last position that each row sees
+  const int begin = split * chunk, end = len - begin > chunk ? begin + chunk : len;
+  const int free_end = len - nq + 1;  // tokens below it are seen by every row
+  const int *row = table + (size_t)s * table_stride;
+  const size_t head_elems = (size_t)D << page_shift;
+  const int mask = (1 << page_shift) - 1;
+
+  // where a tile's two blocks of 16 tokens lie; a block past the end or in a hole is read at page 0 and masked
+  struct Tile {
+    size_t at[2];
+    unsigned holes;
+  };
+  auto locate = [&](int tile) {
+    Tile t;
+    t.holes = 0;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int tok = tile + 16 * b, p = tok < end ? row[tok >> page_shift] : -1;
+      const bool hole = (unsigned)p >= (unsigned)pages;
+      t.holes |= hole ? 1u << b : 0u;
+      t.at[b] = hole ? 0 : (((size_t)p * kv_heads + h) * head_elems + (size_t)(tok & mask) * D) * ES;
+    }
+    return t;
+  };
+  auto dma = [&](const unsigned char *base, unsigned off, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(off), "s"(base) : "memory", "m0");
+  };
+  const unsigned lk = lds0 + wave * REGION, lv = lk + TILE;
+  auto issue_k = [&](const Tile &t) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) dma(kc + t.at[i / (NL / 2)], (i % (NL / 2)) * 1024 + lane * 16, lk + i * 1024);
+  };
+  auto issue_v = [&](const Tile &t) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const unsigned slot = i * 1024 + lane * 16, tok = slot / ROWB, p = slot % ROWB / 16;
+      dma(vc + t.at[i / (NL / 2)], (tok % 16) * ROWB + ((p ^ A::swz(tok)) * 16), lv + i * 1024);
+    }
+  };
+
+  int tile = begin + wave * 32;
+  Tile cur;
+  if (tile < end) {
+    cur = locate(tile);
+    issue_k(cur);
+    issue_v(cur);
+  }
+  // query fragments and the last position that each row sees; with a negative scale the rows change sign (exact), so that the
+  // factor of the scores is positive and their order the weights'
+  const float ks_ = F8 ? k_scale[h] : 1.f, vs = F8 ? v_scale[h] : 1.f, cs = scale * AT_LOG2E * ks_;
+  const unsigned flip = cs < 0.f ? 0x80008000u : 0u;
+  const float c = fmaxf(fabsf(cs), 1e-37f);  // (of a zero scale: every weight rounds to one)
   iu8_v4u qf[RT][KS];
   int limit[RT];
 #pragma unroll
@@ -97,93 +213,83 @@ static __device__ __forceinline__ void attn_few_body(
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       const int d = F8 ? 64 * (ks >> 1) + 16 * g + 8 * (ks & 1) : 32 * ks + 8 * g;
-      qf[rt][ks] = real ? *(const iu8_v4u *)(src + d) : iu8_v4u{0, 0, 0, 0};
+      const iu8_v4u x = *(const iu8_v4u *)(src + d);
+      qf[rt][ks] = real ? x ^ flip : iu8_v4u{0, 0, 0, 0};
     }
   }
   if (tid < R) {
     const int i = tid / G;
     s_dst[tid] = tid < live ? ((long long)(t0 + i) * heads + h * G + (tid - i * G)) * D : 0;
   }
-  const float ks_ = F8 ? k_scale[h] : 1.f, vs = F8 ? v_scale[h] : 1.f, c = scale * AT_LOG2E * ks_;
-  const int free_end = len - nq + 1;  // tokens below it are seen by every row
-  const int begin = split * chunk, end = len - begin > chunk ? begin + chunk : len;
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[rt][ks]));  // here, not in the loop, is what waits for them
 
-  iu8_v4f o[RT][DL];
-  float m[RT], l[RT];
+  iu8_v4f o[RT][DT];
+  float m[RT], l[RT];  // m of the scores as they come, in units of 1 / c of log2
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     m[rt] = -__builtin_inff(), l[rt] = 0.f;
 #pragma unroll
-    for (int i = 0; i < DL; ++i) o[rt][i] = iu8_v4f{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < DT; ++i) o[rt][i] = iu8_v4f{0.f, 0.f, 0.f, 0.f};
   }
-  const int *row = table + (size_t)s * table_stride;
-  const size_t head_elems = (size_t)D << page_shift;
-  const int mask = (1 << page_shift) - 1;
 
-  for (int tile = begin + wave * 32; tile < end; tile += W * 32) {
-    // the two blocks of 16 tokens; a block past the end or in a hole is read at page 0 and masked
-    size_t at[2];
-    bool hole[2];
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const int tok = tile + 16 * b, p = tok < end ? at_uniform(row[tok >> page_shift]) : -1;
-      hole[b] = (unsigned)p >= (unsigned)pages;
-      at[b] = hole[b] ? 0 : (((size_t)p * kv_heads + h) * head_elems + (size_t)(tok & mask) * D) * ES;
-    }
-    iu8_v4u kf[2][KS * ES / 2];
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int i = 0; i < KS * ES / 2; ++i) kf[b][i] = *(const iu8_v4u *)(kc + at[b] + i * 1024 + lane * 16);
-    unsigned vf[8][NV][VD];
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const unsigned char *p = vc + at[j >> 2] + (4 * g + (j & 3)) * (D * ES) + i * 256 + n * (VD * 4);
-        if constexpr (VD == 4) {
-          const iu8_v4u x = *(const iu8_v4u *)p;
-#pragma unroll
-          for (int w = 0; w < 4; ++w) vf[j][i][w] = x[w];
-        } else if constexpr (VD == 2) {
-          const iu8_v2u x = *(const iu8_v2u *)p;
-          vf[j][i][0] = x[0], vf[j][i][1] = x[1];
-        } else {
-          vf[j][i][0] = *(const unsigned *)p;
-        }
-      }
-    // scores of the tile's tokens 16 b + 4 g + r, in units of log2
+  for (; tile < end; tile += W * 32) {
+    const bool more = tile + W * 32 < end;
+    Tile next;
+    if (more) next = locate(tile + W * 32);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");  // K is in (its loads are older than V's)
+    // scores of the tile's tokens 16 b + 4 g + r
     float sc[RT][8];
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
+      iu8_v4f acc[RT];
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        iu8_v4f acc = {0.f, 0.f, 0.f, 0.f};
+      for (int rt = 0; rt < RT; ++rt) acc[rt] = iu8_v4f{0.f, 0.f, 0.f, 0.f};
+      if constexpr (F8) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ks += 2) {
+          const iu8_v4u x = *(const iu8_v4u *)(sk + b * 16 * ROWB + ks * 512 + lane * 16);
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) {
+            acc[rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(at_bf(at_e4m3x8(x[0], x[1])), at_bf(qf[rt][ks]), acc[rt], 0, 0, 0);
+            acc[rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(at_bf(at_e4m3x8(x[2], x[3])), at_bf(qf[rt][ks + 1]), acc[rt], 0, 0, 0);
+          }
+        }
+      } else {
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-          iu8_v4u a;
-          if constexpr (F8) a = ks & 1 ? at_e4m3x8(kf[b][ks >> 1][2], kf[b][ks >> 1][3]) : at_e4m3x8(kf[b][ks >> 1][0], kf[b][ks >> 1][1]);
-          else a = kf[b][ks];
-          acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(at_bf(a), at_bf(qf[rt][ks]), acc, 0, 0, 0);
-        }
+          const iu8_v4u x = *(const iu8_v4u *)(sk + b * 16 * ROWB + ks * 1024 + lane * 16);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) sc[rt][4 * b + r] = acc[r] * c;
+          for (int rt = 0; rt < RT; ++rt) acc[rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(at_bf(x), at_bf(qf[rt][ks]), acc[rt], 0, 0, 0);
+        }
       }
+      // (read in the block that makes them: behind a branch this compiler leaves too few wait states between a matrix
+      // instruction and the first read of its result, seen as wrong scores)
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float x = acc[rt][r];
+          asm volatile("" : "+v"(x));
+          sc[rt][4 * b + r] = x;
+        }
     }
-    if (tile + 32 > min(end, free_end) || hole[0] || hole[1]) {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (more) issue_k(next);
+    const bool special = tile + 32 > min(end, free_end) || cur.holes;
+    if (special) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int tok = tile + 16 * (j >> 2) + 4 * g + (j & 3);
-        const bool gone = hole[j >> 2] || tok >= end;
+        const bool gone = (cur.holes >> (j >> 2) & 1) || tok >= end;
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
           if (gone || tok > limit[rt]) sc[rt][j] = -__builtin_inff();
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-          for (int w = 0; w < VD; ++w) vf[j][i][w] = gone ? 0u : vf[j][i][w];
       }
     }
+    float p[RT][8];
     unsigned pf[RT][4];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
@@ -194,89 +300,120 @@ static __device__ __forceinline__ void attn_few_body(
       top = fmaxf(top, __shfl_xor(top, 32));
       const float mn = fmaxf(m[rt], top), base = mn == -__builtin_inff() ? 0.f : mn;
       if (__any(mn > m[rt])) {
-        const float f = __builtin_amdgcn_exp2f(m[rt] - base);
+        const float f = __builtin_amdgcn_exp2f((m[rt] - base) * c);
         l[rt] *= f;
 #pragma unroll
-        for (int i = 0; i < DL; ++i)
+        for (int i = 0; i < DT; ++i)
 #pragma unroll
           for (int r = 0; r < 4; ++r) o[rt][i][r] *= f;
         m[rt] = mn;
       }
-      float p[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(sc[rt][j] - base), l[rt] += p[j];
+      for (int j = 0; j < 8; ++j) p[rt][j] = __builtin_amdgcn_exp2f((sc[rt][j] - base) * c), l[rt] += p[rt][j];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) pf[rt][j] = iu8_bf16_pack(p[2 * j], p[2 * j + 1]);
+      for (int j = 0; j < 4; ++j) pf[rt][j] = iu8_bf16_pack(p[rt][2 * j], p[rt][2 * j + 1]);
     }
-    // V's operand, channel after channel: eight tokens of one channel a lane
+    if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");  // V is in (the next K's loads are younger)
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (special) {
+      auto piece = [&](int t, int x) -> unsigned char * { return sv + t * ROWB + ((x ^ A::swz(t)) * 16); };
+      bool odd = false;  // a value that is not finite among tokens that some rows see and others do not
+      for (int x = lane; x < TILE / 16; x += 64) {
+        const int t = x / (ROWB / 16), tok = tile + t;
+        iu8_v4u *at = (iu8_v4u *)piece(t, x % (ROWB / 16));
+        if (tok >= end || (cur.holes >> (t >> 4) & 1)) {
+          *at = iu8_v4u{0, 0, 0, 0};
+        } else if (tok >= free_end) {
+          const iu8_v4u v = *at;
 #pragma unroll
-    for (int i = 0; i < DL; i += 2) {
-      unsigned lo[4], hi[4];
-#pragma unroll
-      for (int jj = 0; jj < 4; ++jj) {
-        unsigned x, y;  // channels i, i + 1 of tokens 2 jj and 2 jj + 1
-        if constexpr (F8) {
-          const unsigned dx = vf[2 * jj][i / 16][i / 4 % 4 % VD], dy = vf[2 * jj + 1][i / 16][i / 4 % 4 % VD];
-          x = i & 2 ? at_e4m3_bf16<true>(dx) : at_e4m3_bf16<false>(dx);
-          y = i & 2 ? at_e4m3_bf16<true>(dy) : at_e4m3_bf16<false>(dy);
-        } else {
-          x = vf[2 * jj][i / 8][i / 2 % 4 % VD], y = vf[2 * jj + 1][i / 8][i / 2 % 4 % VD];
+          for (int w = 0; w < 4; ++w) odd |= F8 ? at_e4m3_nan4(v[w]) : at_nonfinite2(v[w]);
         }
-        lo[jj] = __builtin_amdgcn_perm(y, x, 0x05040100u);
-        hi[jj] = __builtin_amdgcn_perm(y, x, 0x07060302u);
       }
+      if (__any(odd)) {
+#pragma unroll 1
+        for (int t = max(free_end - tile, 0); t < min(end - tile, 32); ++t) {
+          if (cur.holes >> (t >> 4) & 1) continue;
+          const int j = 4 * (t >> 4) + (t & 3);
+          float v[DT][4];
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        const at_v8bf p = at_bf(pf[rt][0], pf[rt][1], pf[rt][2], pf[rt][3]);
-        o[rt][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(at_bf(lo[0], lo[1], lo[2], lo[3]), p, o[rt][i], 0, 0, 0);
-        o[rt][i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(at_bf(hi[0], hi[1], hi[2], hi[3]), p, o[rt][i + 1], 0, 0, 0);
+          for (int dt = 0; dt < DT; ++dt) at_four<F8>(piece(t, (16 * dt + 4 * g) * ES / 16) + (16 * dt + 4 * g) * ES % 16, v[dt]);
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) {
+            float pj = p[rt][0];
+#pragma unroll
+            for (int x = 1; x < 8; ++x) pj = j == x ? p[rt][x] : pj;
+            pj = __shfl(pj, n + 16 * ((t >> 2) & 3));
+            if (tile + t <= limit[rt]) {
+#pragma unroll
+              for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[rt][dt][r] = fmaf(pj, v[dt][r], o[rt][dt][r]);
+            }
+          }
+          for (int x = lane; x < ROWB / 16; x += 64) *(iu8_v4u *)(sv + t * ROWB + x * 16) = iu8_v4u{0, 0, 0, 0};
+        }
       }
     }
+    // V's operand: eight tokens of channel 16 dt + n a lane
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      iu8_v4u a;
+      if constexpr (F8) {
+        const int e = n >> 1, t = (e & 4) * 4 + 4 * g + (e & 3);
+        typedef int v2i __attribute__((ext_vector_type(2)));
+        const v2i x = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+            (__attribute__((address_space(3))) v2i *)(sv + t * ROWB + ((dt ^ A::swz(t)) * 16) + (n & 1) * 8));
+        a = at_e4m3x8((unsigned)x[0], (unsigned)x[1]);
+      } else {
+        const int t = 4 * g + (n >> 2), p16 = 2 * dt + ((n >> 1) & 1);
+        const unsigned char *at = sv + t * ROWB + (n & 1) * 8;
+        const at_v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) at_v4s *)(at + (p16 ^ A::swz(t)) * 16));
+        const at_v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) at_v4s *)(at + 16 * ROWB + (p16 ^ A::swz(t)) * 16));
+        const iu8_v2u x = __builtin_bit_cast(iu8_v2u, lo), y = __builtin_bit_cast(iu8_v2u, hi);
+        a = iu8_v4u{x[0], x[1], y[0], y[1]};
+      }
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+        o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(at_bf(a), at_bf(pf[rt][0], pf[rt][1], pf[rt][2], pf[rt][3]), o[rt][dt], 0, 0, 0);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (more) issue_v(next);
+    cur = next;
   }
 
   // the waves' parts: maxima and sums first, then each wave's rows on the joint maximum
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
+    m[rt] *= c;
     l[rt] += __shfl_xor(l[rt], 16);
     l[rt] += __shfl_xor(l[rt], 32);
     if (g == 0) s_ml[0][wave][rt * 16 + n] = m[rt], s_ml[1][wave][rt * 16 + n] = l[rt];
   }
   __syncthreads();
-  float top[RT], sum[RT];
+  float *so = (float *)(smem + wave * REGION);
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const int r = rt * 16 + n;
-    top[rt] = -__builtin_inff();
+    float top = -__builtin_inff(), sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < W; ++w) top[rt] = fmaxf(top[rt], s_ml[0][w][r]);
-    const float base = top[rt] == -__builtin_inff() ? 0.f : top[rt];
-    sum[rt] = 0.f;
+    for (int w = 0; w < W; ++w) top = fmaxf(top, s_ml[0][w][r]);
+    const float base = top == -__builtin_inff() ? 0.f : top;
 #pragma unroll
-    for (int w = 0; w < W; ++w) sum[rt] += s_ml[1][w][r] * __builtin_amdgcn_exp2f(s_ml[0][w][r] - base);
+    for (int w = 0; w < W; ++w) sum += s_ml[1][w][r] * __builtin_amdgcn_exp2f(s_ml[0][w][r] - base);
     const float f = __builtin_amdgcn_exp2f(m[rt] - base);
-    // lane (n, g) holds row n: channel index 4 g + r of each of the DL products
-    constexpr int RUN = F8 ? DL : DL < 8 ? DL : 8;  // channels in a row: DL of an e4m3 row, up to 8 of a bf16 one
 #pragma unroll
-    for (int x = 0; x < 4; ++x)
-#pragma unroll
-      for (int i = 0; i < DL; i += 4) {
-        const int d = (i / RUN) * 16 * RUN + (4 * g + x) * RUN + i % RUN;
-        *(iu8_v4f *)&s_o[wave][r][d] = iu8_v4f{o[rt][i][x] * f, o[rt][i + 1][x] * f, o[rt][i + 2][x] * f, o[rt][i + 3][x] * f};
-      }
-    if (wave == 0 && g == 0) s_m[r] = top[rt], s_il[r] = sum[rt];
+    for (int dt = 0; dt < DT; ++dt) *(iu8_v4f *)(so + r * (D + 4) + 16 * dt + 4 * g) = o[rt][dt] * f;
+    if (wave == 0 && g == 0) s_m[r] = top, s_il[r] = sum;
   }
   __syncthreads();
-  float *part = nullptr, *ml = nullptr;
-  if (ns > 1) {
-    const size_t per = (size_t)R * (D + 4);
-    part = partial + (size_t)item * splits * per;
-    ml = part + (size_t)splits * R * D;
-  }
+  const size_t per = (size_t)R * (D + 4);
+  float *part = partial + (size_t)item * splits * per, *ml = part + (size_t)splits * R * D;  // (not looked at in one piece)
   for (int e = tid; e < live * (D / 4); e += 256) {
     const int r = e / (D / 4), d = (e % (D / 4)) * 4;
-    iu8_v4f x = *(const iu8_v4f *)&s_o[0][r][d];
+    const float *x0 = (const float *)smem + r * (D + 4) + d;
+    iu8_v4f x = *(const iu8_v4f *)x0;
 #pragma unroll
-    for (int w = 1; w < W; ++w) x += *(const iu8_v4f *)&s_o[w][r][d];
+    for (int w = 1; w < W; ++w) x += *(const iu8_v4f *)(x0 + w * (REGION / 4));
     if (ns > 1) {
       at_store_through(part + ((size_t)split * R + r) * D + d, x);
     } else {
@@ -295,5 +432,6 @@ static __device__ __forceinline__ void attn_few_body(
   }
   __syncthreads();
   if (!s_last) return;
-  at_join<D, R, 256>(part, ml, ns, live, vs, tid, out, s_dst, s_m, s_il);
+  constexpr int PARTS = W * REGION / (R * 8) < 512 ? W * REGION / (R * 8) : 512;
+  at_join<D, R, 256, PARTS, 2, 16>(part, ml, ns, live, vs, tid, out, s_dst, s_m, s_il, (float *)smem);
 }

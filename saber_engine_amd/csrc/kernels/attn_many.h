@@ -256,5 +256,5 @@ static __device__ __forceinline__ void attn_many_body(
   }
   __syncthreads();
   if (!s_last) return;
-  at_join<D, R, 256>(part, ml, ns, live, vs, tid, out, s_dst, s_m, s_il);
+  at_join<D, R, 256, 4 * TILE / (R * 8), 4, 8>(part, ml, ns, live, vs, tid, out, s_dst, s_m, s_il, (float *)smem);
 }

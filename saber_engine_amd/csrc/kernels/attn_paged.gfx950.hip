@@ -20,7 +20,7 @@
                           kv_row, tokens, seqs, shape, form, pages, table_stride, eps);                                           \
   }
 #define ATTN_FEW(name, D, F8, RT, R)                                                                                              \
-  extern "C" __global__ __launch_bounds__(256) void attn_few_##name##_d##D##_r##R(                                                \
+  extern "C" __global__ __launch_bounds__(256, RT == 1 && (D < 256 || F8) ? 2 : 1) void attn_few_##name##_d##D##_r##R(                                                \
       const unsigned short *__restrict__ q, const unsigned char *__restrict__ kc, const unsigned char *__restrict__ vc,           \
       const float *__restrict__ k_scale, const float *__restrict__ v_scale, const int *__restrict__ table,                        \
       const int *__restrict__ kv_len, const int *__restrict__ cu_q, unsigned short *__restrict__ out, float *__restrict__ partial, \

@@ -259,3 +259,34 @@ def test_attn_sharp_flat_and_turned_scores(ctx, news):
 def test_attn_on_a_side_stream(ctx):
     say("attn on another stream")
     attn_case(ctx, 128, 8, 2, [900, 40], [1, 1], stream=torch.cuda.Stream())
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("dim,heads,kvh,news", [(64, 4, 2, [8]), (128, 3, 1, [5]), (256, 6, 2, [10]), (128, 1, 1, [2])])
+def test_attn_values_that_are_not_finite_where_a_row_does_not_look(ctx, dim, heads, kvh, news, e4m3):
+    """The last new tokens' keys and values are NaN (and infinite): the rows before them give what they give without, the last
+    ones, which see them, NaN."""
+    say(f"attn, NaN ahead {dim} {heads} {kvh} {news} {e4m3}")
+    n, total = news[0], 75
+    last = n - 1
+
+    def spoil(c):
+        bad = torch.full((1, kvh, dim), float("nan")).cuda()
+        if not e4m3:
+            bad[:, :, ::2] = float("inf")
+        c.put(0, total - 1, bad.to(c.kind), bad.to(c.kind))
+
+    clean = attn_case(ctx, dim, heads, kvh, [total], news, page=16, e4m3=e4m3)[2]
+    c = Paged(1, kvh, dim, 16, total, e4m3, 2)
+    g = torch.Generator().manual_seed(2)
+    c.kv_len[0] = total
+    c.put(0, 0, random_rows(g, total, kvh, dim, e4m3=e4m3), random_rows(g, total, kvh, dim, e4m3=e4m3))
+    spoil(c)
+    q = random_rows(g, n, heads * dim)
+    out = torch.zeros_like(clean)
+    ctx.attn(q.data_ptr(), heads * dim, c.desc(), ends(news).data_ptr(), out.data_ptr(), n, 1, n, total, heads, 1 / math.sqrt(dim))
+    torch.cuda.synchronize()
+    k, v, there = c.rows(0, total - 1)
+    want, tol = attention(f64(q[:last].float()).reshape(last, heads, dim), k, v, there, 1 / math.sqrt(dim))
+    check(f64(out[:last].float()), want, tol, "rows before the NaN")
+    assert torch.isnan(out[last]).all()
