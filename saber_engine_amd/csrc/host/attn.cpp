@@ -13,6 +13,7 @@ namespace {
 
 constexpr uint32_t FEW_ROWS = 32;    // rows a kv head and sequence up to which the few-row kernels run (16 or 32 a workgroup)
 constexpr uint32_t MANY_ROWS = 128;  // rows a workgroup of the many-row kernels
+constexpr uint32_t FEW_PARTS = 128, MANY_PARTS = 32;  // parts at most: their maxima and sums lie in a workgroup's LDS where they are joined
 constexpr uint32_t I32_MAX = 0x7FFFFFFFu;
 constexpr uint32_t WHOLE = 0x7FFFFF00u;  // a part that holds any sequence: the positions a table's row may reach
 
@@ -66,7 +67,7 @@ Plan plan(uint32_t seqs, uint32_t max_q, uint32_t max_kv, uint32_t heads, uint32
   const uint32_t held = p.rows == 16 && (f8 || dim < 256) ? 2 : 1;
   const uint64_t target = p.few() ? (uint64_t)CU_COUNT * held * (seqs == 1 ? 1 : 4) : 2 * CU_COUNT, unit = p.few() ? 128 : 512;
   uint64_t parts = std::max<uint64_t>(1, target / std::max<uint64_t>(p.items, 1));
-  const uint64_t most = std::max<uint64_t>(1, (max_kv + unit - 1) / unit);
+  const uint64_t most = std::min<uint64_t>(p.few() ? FEW_PARTS : MANY_PARTS, std::max<uint64_t>(1, (max_kv + unit - 1) / unit));
   parts = std::min(parts, most);
   uint64_t chunk = (max_kv + parts - 1) / parts;
   chunk = std::max<uint64_t>(unit, (chunk + 127) / 128 * 128);
@@ -105,7 +106,8 @@ int iu8::attn_guard(const saber_iu8_desc *d) {
   bool ok = shape > 0 && kv_heads > 0 && heads > 0 && heads % kv_heads == 0 && form >= 0 && shift >= 4 && shift <= 8 && pages > 0 && stride > 0 &&
             (stride << shift) <= (int64_t)WHOLE && num("tokens") > 0 && d->grid[1] == 1 && d->grid[2] == 1;
   if (append) ok = ok && rot % 16 == 0 && rot <= dim && num("seqs") > 0;
-  else ok = ok && num("chunk") >= 64 && num("chunk") % 64 == 0 && num("splits") > 0 && num("qtiles") > 0 && d->grid[0] % (uint64_t)num("splits") == 0;
+  else ok = ok && num("chunk") >= 64 && num("chunk") % 64 == 0 && num("qtiles") > 0 && num("splits") > 0 &&
+                 num("splits") <= (strncmp(d->kernel, "attn_few_", 9) ? MANY_PARTS : FEW_PARTS) && d->grid[0] % (uint64_t)(num("splits") * num("qtiles") * kv_heads) == 0;
   return ok ? 0 : fail(SABER_IU8_E_RULE, fmt("%s: scalars that the kernel's walk over the cache does not hold", d->kernel));
 }
 

@@ -36,75 +36,76 @@ static __device__ __forceinline__ int at_chunk(int len, int chunk, int splits) {
 
 // Joins `ns` parts of one item: part i's rows at part + i * R * D, their (m, l) -- four floats a row, one 16-byte store -- at
 // ml + i * 4 R; rows r < live go out. The parts come from memory (other XCDs wrote them), so as many loads as registers allow are
-// in flight: U items x K parts a thread. `s_f`: LDS for the rows' (m, l) of PARTS parts at a time.
-template <int D, int R, int T, int PARTS, int U, int K>
+// in flight, U items x K parts a thread, the first of them beside the (m, l). `s_f`: ns * live floats of LDS; ns at most 128 (R = 128: 32).
+template <int D, int R, int T, int U, int K>
 static __device__ __forceinline__ void at_join(const float *__restrict__ part, const float *__restrict__ ml, int ns, int live, float vs, int tid,
-                                               unsigned short *__restrict__ out, const long long *s_dst, float *s_m, float *s_il, float *s_f) {
-  constexpr int NI = (R * (D / 4) + T - 1) / T;
-  // the rows' joint maxima and sums
-  for (int r = tid; r < R; r += T) s_m[r] = -__builtin_inff(), s_il[r] = 0.f;
-  __syncthreads();
-  for (int i0 = 0; i0 < ns; i0 += PARTS) {
-    const int np = min(PARTS, ns - i0);
-    for (int e = tid; e < np * live; e += T) {
-      const iu8_v4f x = at_load_through(ml + ((size_t)(i0 + e / live) * R + e % live) * 4);
-      s_f[2 * e] = x[0], s_f[2 * e + 1] = x[1];
-    }
-    __syncthreads();
-    for (int r = tid; r < live; r += T) {
-      float m = s_m[r], l = s_il[r];
-      for (int i = 0; i < np; ++i) {
-        const float mi = s_f[2 * (i * live + r)], mn = fmaxf(m, mi), base = mn == -__builtin_inff() ? 0.f : mn;
-        l = l * __builtin_amdgcn_exp2f(m - base) + s_f[2 * (i * live + r) + 1] * __builtin_amdgcn_exp2f(mi - base);
-        m = mn;
+                                               unsigned short *__restrict__ out, const long long *s_dst, float *s_il, float *s_f) {
+  constexpr int D4 = D / 4, NI = (R * D4 + T - 1) / T;
+  const int all = live * D4;
+  iu8_v4f x[U][K];
+  auto load = [&](int it, int i) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int e = min((it + u) * T + tid, all - 1);
+        x[u][k] = at_load_through(part + ((size_t)min(i + k, ns - 1) * R + e / D4) * D + e % D4 * 4);
       }
-      s_m[r] = m, s_il[r] = l;
+  };
+  load(0, 0);
+  {  // a row's joint maximum, its parts' factors, its sum: LPR lanes a row, up to PL parts a lane
+    constexpr int LPR = T / R, PL = 128 / LPR < 16 ? 128 / LPR : 16;
+    const int r = tid / LPR, j = tid % LPR;
+    float m[PL], l[PL], top = -__builtin_inff(), sum = 0.f;
+#pragma unroll
+    for (int x = 0; x < PL; ++x) {
+      const int i = x * LPR + j;
+      iu8_v4f y = {-__builtin_inff(), 0.f, 0.f, 0.f};
+      if (i < ns && r < live) y = at_load_through(ml + ((size_t)i * R + r) * 4);
+      m[x] = y[0], l[x] = y[1];
     }
-    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < PL; ++x) top = fmaxf(top, m[x]);
+#pragma unroll
+    for (int x = 1; x < LPR; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
+    const float base = top == -__builtin_inff() ? 0.f : top;
+#pragma unroll
+    for (int x = 0; x < PL; ++x) {
+      const int i = x * LPR + j;
+      const float f = __builtin_amdgcn_exp2f(m[x] - base);
+      sum = fmaf(f, l[x], sum);
+      if (i < ns && r < live) s_f[i * live + r] = f;
+    }
+#pragma unroll
+    for (int x = 1; x < LPR; x *= 2) sum += __shfl_xor(sum, x);
+    if (j == 0 && r < live) s_il[r] = sum == 0.f ? 0.f : vs / sum;
   }
+  __syncthreads();
   for (int it = 0; it < NI; it += U) {
-    if (it * T >= live * (D / 4)) break;  // (the same for every thread)
+    if (it * T >= all) break;  // (the same for every thread)
     iu8_v4f o[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) o[u] = iu8_v4f{0.f, 0.f, 0.f, 0.f};
-    for (int i0 = 0; i0 < ns; i0 += PARTS) {
-      const int np = min(PARTS, ns - i0);
-      if (ns > PARTS || it == 0) {  // the parts' factors
-        __syncthreads();
-        for (int e = tid; e < np * live; e += T) {
-          const int r = e % live;
-          const float m = at_load_through(ml + ((size_t)(i0 + e / live) * R + r) * 4)[0], top = s_m[r];
-          s_f[e] = top == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - top);
+    for (int i = 0; i < ns; i += K) {
+      if (it || i) load(it, i);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int r = min((it + u) * T + tid, all - 1) / D4;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          const float f = s_f[min(i + k, ns - 1) * live + r];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) o[u][c] = i + k < ns ? fmaf(f, x[u][k][c], o[u][c]) : o[u][c];
         }
-        __syncthreads();
-      }
-      for (int i = 0; i < np; i += K) {
-        iu8_v4f x[U][K];
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-          for (int k = 0; k < K; ++k) {
-            const int e = min((it + u) * T + tid, live * (D / 4) - 1), ii = min(i + k, np - 1);
-            x[u][k] = at_load_through(part + ((size_t)(i0 + ii) * R + e / (D / 4)) * D + e % (D / 4) * 4);
-          }
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-          for (int k = 0; k < K; ++k) {
-            const int e = min((it + u) * T + tid, live * (D / 4) - 1);
-            const float f = i + k < np ? s_f[(i + k) * live + e / (D / 4)] : 0.f;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) o[u][c] = i + k < np ? fmaf(f, x[u][k][c], o[u][c]) : o[u][c];
-          }
       }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int e = (it + u) * T + tid;
-      if (it + u < NI && e < live * (D / 4)) {
-        const int r = e / (D / 4);
-        const float il = s_il[r] == 0.f ? 0.f : vs / s_il[r];
-        *(iu8_v2u *)(out + s_dst[r] + e % (D / 4) * 4) = iu8_v2u{iu8_bf16_pack(o[u][0] * il, o[u][1] * il), iu8_bf16_pack(o[u][2] * il, o[u][3] * il)};
+      if (it + u < NI && e < all) {
+        const int r = e / D4;
+        const float il = s_il[r];
+        *(iu8_v2u *)(out + s_dst[r] + e % D4 * 4) = iu8_v2u{iu8_bf16_pack(o[u][0] * il, o[u][1] * il), iu8_bf16_pack(o[u][2] * il, o[u][3] * il)};
       }
     }
   }
@@ -131,9 +132,20 @@ static __device__ __forceinline__ void attn_few_body(
   constexpr int ES = A::ES, ROWB = A::ROWB, TILE = A::TILE, NL = A::NL, R = 16 * RT, KS = D / 32, DT = D / 16, W = 4;
   constexpr int REGION = 2 * TILE > R * (D + 4) * 4 ? 2 * TILE : R * (D + 4) * 4;  // a wave's LDS: its tiles, then its part of the sum
   const int heads = shape & 0xFFFF, kv_heads = shape >> 16, G = heads / kv_heads;
-  const int split = blockIdx.x % splits, item = blockIdx.x / splits, h = item % kv_heads, s = item / kv_heads;
+  // the parts of one item lie a launch's items apart, so that they spread over the XCDs (workgroups are dealt to them in turn) and
+  // the parts that short sequences do not have come last
+  const int items = gridDim.x / splits, split = blockIdx.x / items, item = blockIdx.x % items, h = item % kv_heads, s = item / kv_heads;
   const int tid = threadIdx.x, lane = tid & 63, wave = at_uniform(tid >> 6), n = lane & 15, g = lane >> 4;
 
+  // the first tile's pages are asked for beside the length, at the place that the launch law gives this part
+  const int *row = table + (size_t)s * table_stride;
+  auto fetch = [&](int tile, int (&p)[2]) {
+#pragma unroll
+    for (int b = 0; b < 2; ++b) p[b] = row[min((unsigned)(tile + 16 * b) >> page_shift, (unsigned)table_stride - 1u)];
+  };
+  int p_cur[2], p_next[2];
+  const int told = chunk;
+  fetch(split * told + wave * 32, p_cur);
   const int t0 = cu_q ? cu_q[s] : s;
   const int nq = min((cu_q ? cu_q[s + 1] : s + 1), tokens) - t0;
   const int len = at_len(kv_len, s, table_stride, page_shift);
@@ -153,7 +165,6 @@ static __device__ __forceinline__ void attn_few_body(
 
   const int begin = split * chunk, end = len - begin > chunk ? begin + chunk : len;
   const int free_end = len - nq + 1;  // tokens below it are seen by every row
-  const int *row = table + (size_t)s * table_stride;
   const size_t head_elems = (size_t)D << page_shift;
   const int mask = (1 << page_shift) - 1;
 
@@ -162,20 +173,20 @@ static __device__ __forceinline__ void attn_few_body(
     size_t at[2];
     unsigned holes;
   };
-  auto locate = [&](int tile) {
+  auto locate = [&](int tile, const int (&p)[2]) {
     Tile t;
     t.holes = 0;
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-      const int tok = tile + 16 * b, p = tok < end ? row[tok >> page_shift] : -1;
-      const bool hole = (unsigned)p >= (unsigned)pages;
+      const int tok = tile + 16 * b;
+      const bool hole = tok >= end || (unsigned)p[b] >= (unsigned)pages;
       t.holes |= hole ? 1u << b : 0u;
-      t.at[b] = hole ? 0 : (((size_t)p * kv_heads + h) * head_elems + (size_t)(tok & mask) * D) * ES;
+      t.at[b] = hole ? 0 : (((size_t)p[b] * kv_heads + h) * head_elems + (size_t)(tok & mask) * D) * ES;
     }
     return t;
   };
   auto dma = [&](const unsigned char *base, unsigned off, unsigned lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(off), "s"(base) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" : : "s"(lds), "v"(off), "s"(base) : "memory", "m0");
   };
   const unsigned lk = lds0 + wave * REGION, lv = lk + TILE;
   auto issue_k = [&](const Tile &t) {
@@ -192,8 +203,9 @@ static __device__ __forceinline__ void attn_few_body(
 
   int tile = begin + wave * 32;
   Tile cur;
+  if (chunk != told) fetch(tile, p_cur);
   if (tile < end) {
-    cur = locate(tile);
+    cur = locate(tile, p_cur);
     issue_k(cur);
     issue_v(cur);
   }
@@ -238,7 +250,7 @@ static __device__ __forceinline__ void attn_few_body(
   for (; tile < end; tile += W * 32) {
     const bool more = tile + W * 32 < end;
     Tile next;
-    if (more) next = locate(tile + W * 32);
+    if (more) fetch(tile + W * 32, p_next);
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");  // K is in (its loads are older than V's)
     // scores of the tile's tokens 16 b + 4 g + r
     float sc[RT][8];
@@ -277,7 +289,10 @@ static __device__ __forceinline__ void attn_few_body(
         }
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    if (more) issue_k(next);
+    if (more) {
+      next = locate(tile + W * 32, p_next);
+      issue_k(next);
+    }
     const bool special = tile + 32 > min(end, free_end) || cur.holes;
     if (special) {
 #pragma unroll
@@ -432,6 +447,5 @@ static __device__ __forceinline__ void attn_few_body(
   }
   __syncthreads();
   if (!s_last) return;
-  constexpr int PARTS = W * REGION / (R * 8) < 512 ? W * REGION / (R * 8) : 512;
-  at_join<D, R, 256, PARTS, 2, 16>(part, ml, ns, live, vs, tid, out, s_dst, s_m, s_il, (float *)smem);
+  at_join<D, R, 256, 2, 16>(part, ml, ns, live, vs, tid, out, s_dst, s_il, (float *)smem);
 }

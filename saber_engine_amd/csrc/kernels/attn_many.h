@@ -26,8 +26,10 @@ static __device__ __forceinline__ void attn_many_body(
     int tokens, int shape, int page_shift, int pages, int table_stride, int chunk, int splits, int qtiles, float scale) {
   constexpr int ES = F8 ? 1 : 2, R = 128, BK = at_many_bk<D>(), HB = BK / 32, KS = D / 16, MT = D / 32, ROWB = D * 2, TILE = BK * ROWB;
   const int heads = shape & 0xFFFF, kv_heads = shape >> 16, G = heads / kv_heads;
-  const int split = blockIdx.x % splits, item = blockIdx.x / splits;
-  const int qt = qtiles - 1 - item % qtiles, h = item / qtiles % kv_heads, s = item / qtiles / kv_heads;  // the longest rows first
+  // the longest rows first; a head's tiles lie a launch's heads apart, so that few XCDs (to which workgroups are dealt in turn)
+  // hold its keys
+  const int items = gridDim.x / splits, split = blockIdx.x / items, item = blockIdx.x % items;
+  const int heads_all = items / qtiles, qt = qtiles - 1 - item / heads_all, h = item % heads_all % kv_heads, s = item % heads_all / kv_heads;
   const int tid = threadIdx.x, lane = tid & 63, wave = at_uniform(tid >> 6), n = lane & 31, hf = lane >> 5;
 
   const int t0 = cu_q ? cu_q[s] : s;
@@ -43,22 +45,24 @@ static __device__ __forceinline__ void attn_many_body(
   if (split >= ns) return;
 
   __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * TILE];  // K, V of stage 0; K, V of stage 1
-  __shared__ float s_m[R], s_il[R];
+  __shared__ float s_il[R];
   __shared__ long long s_dst[R];
   __shared__ int s_last;
 
   const int r = qt * R + wave * 32 + n, i = r / G;
   const bool real = wave * 32 + n < live;
   const int limit = real ? len - nq + i : len - 1;
+  const float ks_ = F8 ? k_scale[h] : 1.f, vs = F8 ? v_scale[h] : 1.f, cs = scale * AT_LOG2E * ks_;
+  const unsigned flip = cs < 0.f ? 0x80008000u : 0u;  // attn_few.h
+  const float c = fmaxf(fabsf(cs), 1e-37f);
   iu8_v4u qf[KS];
   {
     const unsigned short *src = q + (size_t)(t0 + (real ? i : 0)) * q_row + (size_t)(h * G + (real ? r - i * G : 0)) * D;
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) qf[ks] = real ? *(const iu8_v4u *)(src + 16 * ks + 8 * hf) : iu8_v4u{0, 0, 0, 0};
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = real ? *(const iu8_v4u *)(src + 16 * ks + 8 * hf) ^ flip : iu8_v4u{0, 0, 0, 0};
   }
   const long long dst = ((long long)(t0 + i) * heads + h * G + (r - i * G)) * D;
   if (hf == 0) s_dst[wave * 32 + n] = dst;
-  const float ks_ = F8 ? k_scale[h] : 1.f, vs = F8 ? v_scale[h] : 1.f, c = scale * AT_LOG2E * ks_;
   const int begin = split * chunk, end = kv_end - begin > chunk ? begin + chunk : kv_end;
 
   const int *row = table + (size_t)s * table_stride;
@@ -75,19 +79,18 @@ static __device__ __forceinline__ void attn_many_body(
   auto swz = [](int t) { return D == 256 ? t & 7 : D == 128 ? t & 3 : t & 1; };
 
   constexpr int RAW = F8 ? BK * D / 256 / 16 : 1;  // 16-byte pieces of K (and of V) a thread, e4m3
-  iu8_v4u rk[RAW], rv[RAW];
-  auto issue = [&](int tile, int stage) {
-    if constexpr (F8) {
+  iu8_v4u raw[RAW];
+  auto fetch = [&](int tile, const unsigned char *src) {  // e4m3: a tile of K or of V into registers
 #pragma unroll
-      for (int x = 0; x < RAW; ++x) {
-        // a block is D pieces, and 256 threads take whole blocks or a whole number of threads share one: uniform a wave
-        const int piece = x * 256 + tid, blk = at_uniform((x * 256 + wave * 64) / D);
-        bool hole;
-        const size_t at = block_at(tile + 16 * blk, hole);
-        rk[x] = *(const iu8_v4u *)(kc + at + (size_t)(piece % D) * 16);
-        rv[x] = *(const iu8_v4u *)(vc + at + (size_t)(piece % D) * 16);
-      }
-    } else {
+    for (int x = 0; x < RAW; ++x) {
+      // (a block is D pieces: a wave's 64 lie in one)
+      bool hole;
+      const size_t at = block_at(tile + 16 * at_uniform((x * 256 + wave * 64) / D), hole);
+      raw[x] = *(const iu8_v4u *)(src + at + (size_t)((x * 256 + tid) % D) * 16);
+    }
+  };
+  auto issue = [&](int tile, int stage) {  // bf16: a tile of both straight into a stage
+    if constexpr (!F8) {
       constexpr int BLK = 16 * ROWB / 1024, LOADS = BK / 16 * BLK;  // wave-loads of 1 KiB a block, a tile
 #pragma unroll
       for (int x = 0; x < LOADS / 4; ++x) {
@@ -103,20 +106,22 @@ static __device__ __forceinline__ void attn_many_body(
       }
     }
   };
-  auto commit = [&](int stage) {  // e4m3: widen into the stage
-    if constexpr (F8) {
-      unsigned char *sk = smem + stage * 2 * TILE, *sv = sk + TILE;
+  auto widen_k = [&](int stage) {
 #pragma unroll
-      for (int x = 0; x < RAW; ++x) {
-        const int piece = x * 256 + tid, blk = piece / D, in = piece % D;
-        unsigned char *pk = sk + blk * 16 * ROWB + ((in / 16) * 32 + in % 16) * 16;
-        *(iu8_v4u *)pk = at_e4m3x8(rk[x][0], rk[x][1]);
-        *(iu8_v4u *)(pk + 256) = at_e4m3x8(rk[x][2], rk[x][3]);
-        const int t = blk * 16 + in / (D / 16), p = in % (D / 16) * 2;
-        unsigned char *pv = sv + t * ROWB + ((p ^ (4 * swz(t))) * 16);
-        *(iu8_v4u *)pv = at_e4m3x8(rv[x][0], rv[x][1]);
-        *(iu8_v4u *)(pv + 16) = at_e4m3x8(rv[x][2], rv[x][3]);
-      }
+    for (int x = 0; x < RAW; ++x) {
+      const int piece = x * 256 + tid, blk = piece / D, in = piece % D;
+      unsigned char *to = smem + stage * 2 * TILE + blk * 16 * ROWB + ((in / 16) * 32 + in % 16) * 16;
+      *(iu8_v4u *)to = at_e4m3x8(raw[x][0], raw[x][1]);
+      *(iu8_v4u *)(to + 256) = at_e4m3x8(raw[x][2], raw[x][3]);
+    }
+  };
+  auto widen_v = [&](int stage) {
+#pragma unroll
+    for (int x = 0; x < RAW; ++x) {
+      const int piece = x * 256 + tid, t = piece / (D / 16), p = piece % (D / 16) * 2;
+      unsigned char *to = smem + (stage * 2 + 1) * TILE + t * ROWB + ((p ^ (4 * swz(t))) * 16);
+      *(iu8_v4u *)to = at_e4m3x8(raw[x][0], raw[x][1]);
+      *(iu8_v4u *)(to + 16) = at_e4m3x8(raw[x][2], raw[x][3]);
     }
   };
   auto arrived = [&]() {
@@ -133,14 +138,23 @@ static __device__ __forceinline__ void attn_many_body(
   const unsigned v_lane = vrow * ROWB + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
 
   if (begin < end) {
-    issue(begin, 0);
-    commit(0);
+    if constexpr (F8) {
+      fetch(begin, kc);
+      widen_k(0);
+      fetch(begin, vc);
+      widen_v(0);
+    } else {
+      issue(begin, 0);
+    }
   }
   arrived();
   int stage = 0;
   for (int tile = begin; tile < end; tile += BK, stage ^= 1) {
     const bool more = tile + BK < end;
-    if (more) issue(tile + BK, stage ^ 1);
+    if (more) {
+      if constexpr (F8) fetch(tile + BK, kc);
+      else issue(tile + BK, stage ^ 1);
+    }
     unsigned char *sk = smem + stage * 2 * TILE, *sv = sk + TILE;
     unsigned holes = 0;
 #pragma unroll
@@ -150,30 +164,46 @@ static __device__ __forceinline__ void attn_many_body(
       holes |= (hole ? 1u : 0u) << b;
     }
     const bool special = holes || tile + BK > min(end, free_end);
-    if (holes || tile + BK > end) {  // rows of V that take no part: a weight of zero would keep their NaNs
+    auto piece = [&](int t, int x) -> unsigned char * { return sv + t * ROWB + ((x ^ (4 * swz(t))) * 16); };
+    int odd = 0;  // a value that is not finite among tokens that some rows see and others do not
+    if (special) {
       for (int x = tid; x < BK * (ROWB / 16); x += 256) {
         const int t = x / (ROWB / 16);
-        if (tile + t >= end || (holes >> (t >> 4) & 1)) *(iu8_v4u *)(sv + x * 16) = iu8_v4u{0, 0, 0, 0};
+        iu8_v4u *at = (iu8_v4u *)(sv + x * 16);
+        if (tile + t >= end || (holes >> (t >> 4) & 1)) {  // takes no part: a weight of zero would keep its NaNs
+          *at = iu8_v4u{0, 0, 0, 0};
+        } else if (tile + t >= free_end) {
+          const iu8_v4u v = *at;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) odd |= at_nonfinite2(v[w]);
+        }
       }
-      __syncthreads();
+      odd = __syncthreads_or(odd);
     }
-    at_v16f sc[HB];
+    // scores. (The products are read in the block that makes them: behind a branch this compiler leaves too few wait states
+    // between a matrix instruction and the first read of its result, seen as wrong scores.)
+    float st[HB][16];
 #pragma unroll
     for (int hb = 0; hb < HB; ++hb) {
-      sc[hb] = at_v16f{};
+      at_v16f sc = at_v16f{};
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         const iu8_v4u a = *(const iu8_v4u *)(sk + k_lane + hb * 32 * ROWB + ks * 512);
-        sc[hb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at_bf(a), at_bf(qf[ks]), sc[hb], 0, 0, 0);
+        sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at_bf(a), at_bf(qf[ks]), sc, 0, 0, 0);
+      }
+#pragma unroll
+      for (int x = 0; x < 16; ++x) {
+        float y = sc[x];
+        asm volatile("" : "+v"(y));
+        st[hb][x] = y;
       }
     }
-    // (the products are read here, in the block that makes them: behind a branch this compiler leaves too few wait states between
-    // a matrix instruction and the first read of its result, seen as wrong scores)
-    float st[HB][16];
-#pragma unroll
-    for (int hb = 0; hb < HB; ++hb)
-#pragma unroll
-      for (int x = 0; x < 16; ++x) st[hb][x] = sc[hb][x] * c;
+    if constexpr (F8) {
+      if (more) {
+        widen_k(stage ^ 1);
+        fetch(tile + BK, vc);
+      }
+    }
     if (special) {
 #pragma unroll
       for (int hb = 0; hb < HB; ++hb)
@@ -189,23 +219,54 @@ static __device__ __forceinline__ void attn_many_body(
 #pragma unroll
       for (int x = 0; x < 16; ++x) top = fmaxf(top, st[hb][x]);
     top = fmaxf(top, __shfl_xor(top, 32));
-    const float mn = fmaxf(m, top), base = mn == -__builtin_inff() ? 0.f : mn;
-    if (__any(mn > m)) {
-      const float f = __builtin_amdgcn_exp2f(m - base);
+    // The maximum that the weights are taken against moves only when a score passes it by 2^8 or more (and at the first key): until
+    // then weights of up to 256 are as exact, and the sums' rescale is saved.
+    if (__any((top - m) * c > 8.f)) {
+      const float mn = fmaxf(m, top), f = __builtin_amdgcn_exp2f((m - (mn == -__builtin_inff() ? 0.f : mn)) * c);
       l *= f;
 #pragma unroll
       for (int x = 0; x < MT; ++x) o[x] *= f;
       m = mn;
     }
+    const float mc = m == -__builtin_inff() ? 0.f : m * c;
     unsigned pf[HB][8];
 #pragma unroll
     for (int hb = 0; hb < HB; ++hb)
 #pragma unroll
       for (int x = 0; x < 16; x += 2) {
-        const float p0 = __builtin_amdgcn_exp2f(st[hb][x] - base), p1 = __builtin_amdgcn_exp2f(st[hb][x + 1] - base);
-        l += p0 + p1;
-        pf[hb][x / 2] = iu8_bf16_pack(p0, p1);
+        st[hb][x] = __builtin_amdgcn_exp2f(fmaf(st[hb][x], c, -mc));
+        st[hb][x + 1] = __builtin_amdgcn_exp2f(fmaf(st[hb][x + 1], c, -mc));
+        l += st[hb][x] + st[hb][x + 1];
+        pf[hb][x / 2] = iu8_bf16_pack(st[hb][x], st[hb][x + 1]);
       }
+    if (odd) {  // these tokens' values by lane arithmetic, for the rows that see them; the product then finds zeros
+      const int from = max(free_end - tile, 0), to = min(end - tile, BK);
+#pragma unroll
+      for (int hb = 0; hb < HB; ++hb)
+#pragma unroll 1
+        for (int t = max(from - 32 * hb, 0); t < min(to - 32 * hb, 32); ++t) {
+          float pj = st[hb][0];
+#pragma unroll
+          for (int x = 1; x < 16; ++x) pj = (t >> 3) * 4 + (t & 3) == x ? st[hb][x] : pj;
+          pj = __shfl(pj, n + 32 * ((t >> 2) & 1));
+          const int tt = t + 32 * hb;
+          if (tile + tt <= limit && !(holes >> (tt >> 4) & 1)) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+              for (int x = 0; x < 16; x += 4) {
+                float v[4];
+                at_four<false>(piece(tt, 4 * mt + x / 4) + 8 * hf, v);
+#pragma unroll
+                for (int r2 = 0; r2 < 4; ++r2) o[mt][x + r2] = fmaf(pj, v[r2], o[mt][x + r2]);
+              }
+          }
+        }
+      __syncthreads();
+      for (int x = tid; x < BK * (ROWB / 16); x += 256)
+        if (x / (ROWB / 16) >= from) *(iu8_v4u *)(sv + x * 16) = iu8_v4u{0, 0, 0, 0};
+      __syncthreads();
+    }
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       const unsigned char *pv = sv + v_lane + ((mt ^ swz(vrow)) * 64);
@@ -220,7 +281,9 @@ static __device__ __forceinline__ void attn_many_body(
                                                           o[mt], 0, 0, 0);
         }
     }
-    if (more) commit(stage ^ 1);
+    if constexpr (F8) {
+      if (more) widen_v(stage ^ 1);
+    }
     arrived();
   }
   l += __shfl_xor(l, 32);
@@ -245,7 +308,7 @@ static __device__ __forceinline__ void attn_many_body(
 #pragma unroll
       for (int x = 0; x < 16; x += 4)
         at_store_through(p + 32 * mt + 2 * x + 4 * hf, iu8_v4f{o[mt][x], o[mt][x + 1], o[mt][x + 2], o[mt][x + 3]});
-    if (hf == 0) at_store_through(ml + ((size_t)split * R + wave * 32 + n) * 4, iu8_v4f{m, l, 0.f, 0.f});
+    if (hf == 0) at_store_through(ml + ((size_t)split * R + wave * 32 + n) * 4, iu8_v4f{m * c, l, 0.f, 0.f});
   }
   iu8_stores_done();
   __syncthreads();
@@ -256,5 +319,5 @@ static __device__ __forceinline__ void attn_many_body(
   }
   __syncthreads();
   if (!s_last) return;
-  at_join<D, R, 256, 4 * TILE / (R * 8), 4, 8>(part, ml, ns, live, vs, tid, out, s_dst, s_m, s_il, (float *)smem);
+  at_join<D, R, 256, 2, 8>(part, ml, ns, live, vs, tid, out, s_dst, s_il, (float *)smem);
 }

@@ -30,7 +30,7 @@
                              page_shift, pages, table_stride, chunk, splits, scale);                                              \
   }
 #define ATTN_MANY(name, D, F8)                                                                                                    \
-  extern "C" __global__ __launch_bounds__(256) void attn_many_##name##_d##D(                                                      \
+  extern "C" __global__ __launch_bounds__(256, 2) void attn_many_##name##_d##D(                                                      \
       const unsigned short *__restrict__ q, const unsigned char *__restrict__ kc, const unsigned char *__restrict__ vc,           \
       const float *__restrict__ k_scale, const float *__restrict__ v_scale, const int *__restrict__ table,                        \
       const int *__restrict__ kv_len, const int *__restrict__ cu_q, unsigned short *__restrict__ out, float *__restrict__ partial, \
