@@ -87,7 +87,12 @@ static const Signature SIG_KV_APPEND = {
     {"k_scale", K::Buffer}, {"v_scale", K::Buffer}, {"table", K::Buffer}, {"kv_len", K::Buffer}, {"cu_q", K::Buffer},  {"q_norm", K::Buffer},
     {"k_norm", K::Buffer},  {"inv_freq", K::Buffer}, {"q_row", K::I32},   {"q_head", K::I32},   {"kv_row", K::I32},    {"tokens", K::I32},
     {"seqs", K::I32},       {"shape", K::I32},     {"form", K::I32},      {"pages", K::I32},    {"table_stride", K::I32}, {"eps", K::F32}};
-static const Signature SIG_ATTN = {
+static const Signature SIG_ATTN_FEW = {
+    {"q", K::Buffer},      {"kc", K::Buffer},    {"vc", K::Buffer},  {"k_scale", K::Buffer}, {"v_scale", K::Buffer}, {"table", K::Buffer},
+    {"kv_len", K::Buffer}, {"cu_q", K::Buffer},  {"out", K::Buffer}, {"partial", K::Buffer}, {"counter", K::Buffer}, {"q_row", K::I32},
+    {"tokens", K::I32},    {"seqs", K::I32},     {"shape", K::I32},  {"page_shift", K::I32}, {"pages", K::I32},      {"table_stride", K::I32},
+    {"unit_shift", K::I32}, {"qtiles", K::I32},   {"scale", K::F32}};
+static const Signature SIG_ATTN_MANY = {
     {"q", K::Buffer},      {"kc", K::Buffer},    {"vc", K::Buffer},  {"k_scale", K::Buffer}, {"v_scale", K::Buffer}, {"table", K::Buffer},
     {"kv_len", K::Buffer}, {"cu_q", K::Buffer},  {"out", K::Buffer}, {"partial", K::Buffer}, {"counter", K::Buffer}, {"q_row", K::I32},
     {"tokens", K::I32},    {"shape", K::I32},    {"page_shift", K::I32}, {"pages", K::I32},  {"table_stride", K::I32}, {"chunk", K::I32},
@@ -128,7 +133,8 @@ const Signature *signature_for(const std::string &k) {
   if (starts(k, "moe_iu8_grouped_")) return &SIG_MOE_GROUPED;
   if (starts(k, "moe_iu8_combine_")) return &SIG_MOE_COMBINE;
   if (starts(k, "kv_append_")) return &SIG_KV_APPEND;
-  if (starts(k, "attn_few_") || starts(k, "attn_many_")) return &SIG_ATTN;
+  if (starts(k, "attn_few_")) return &SIG_ATTN_FEW;
+  if (starts(k, "attn_many_")) return &SIG_ATTN_MANY;
   return nullptr;
 }
 

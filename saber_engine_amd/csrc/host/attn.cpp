@@ -13,7 +13,8 @@ namespace {
 
 constexpr uint32_t FEW_ROWS = 32;    // rows a kv head and sequence up to which the few-row kernels run (16 or 32 a workgroup)
 constexpr uint32_t MANY_ROWS = 128;  // rows a workgroup of the many-row kernels
-constexpr uint32_t FEW_PARTS = 128, MANY_PARTS = 32;  // parts at most: their maxima and sums lie in a workgroup's LDS where they are joined
+constexpr int FEW_UNIT_SHIFT = 7, WHOLE_SHIFT = 31;  // log2 of the tokens a unit of the few-row kernels' deal (attn_few.h)
+constexpr uint32_t MANY_PARTS = 32;  // parts of an item at most: their maxima and sums lie in one workgroup's LDS when they are joined
 constexpr uint32_t I32_MAX = 0x7FFFFFFFu;
 constexpr uint32_t WHOLE = 0x7FFFFF00u;  // a part that holds any sequence: the positions a table's row may reach
 
@@ -49,37 +50,57 @@ int cache_check(const char *op, const saber_iu8_kv_cache *c, uint32_t heads, uin
 }
 
 struct Plan {
-  uint32_t rows;  // a workgroup's (16, 32, 128)
-  uint64_t qtiles, items;
-  uint32_t chunk, splits;
+  uint32_t rows;        // a workgroup's: 16 or 32 (few), 128 (many)
+  uint64_t qtiles, items, grid;
+  int unit_shift;       // few: log2 of the tokens a unit, WHOLE_SHIFT for whole items
+  uint32_t chunk, splits;  // many: tokens a part, parts
+  uint64_t partial, counter;  // bytes
   bool few() const { return rows <= FEW_ROWS; }
 };
 
-// The split of the cache's length. Few rows: a part is at least 128 tokens (a 32-token tile for each of the four waves); one
-// sequence is cut into as many equal parts as the card holds workgroups (by their LDS), several into four times as many, since
-// their lengths differ and a short one's workgroups leave at once. Many rows: parts of at least 512 tokens, two workgroups a CU.
-Plan plan(uint32_t seqs, uint32_t max_q, uint32_t max_kv, uint32_t heads, uint32_t kv_heads, uint32_t dim, bool f8) {
-  Plan p;
-  const uint64_t rows = (uint64_t)max_q * (heads / kv_heads);
-  p.rows = rows <= 16 ? 16 : rows <= FEW_ROWS ? FEW_ROWS : MANY_ROWS;
-  p.qtiles = p.few() ? 1 : (rows + MANY_ROWS - 1) / MANY_ROWS;
+// Which kernels, and the grid. Few rows (attn_few.h) up to 32 a kv head and sequence; above, still where a long cache meets so
+// few rows that its tiles of 32 make at most five units a CU -- 40 new tokens of group 6 on 4,000 keys, head width 256, 30 us
+// against 51 of the many-row kernel; 100 on 8,000 (19 units a CU) 119 against 71; 40 of group 5 on 4,000, width 128 (7) 32.5 / 32.3.
+// Their grid: the workgroups that the card holds at once (by their LDS: two a CU, or one), which deal the units level; three
+// quarters of the CUs where each then has 16 units and more (131,072 keys, 4 kv heads of 256: 192 workgroups 93 us, 256 96; 64
+// sequences of up to 8,192, 8 heads of 128: 199 against 203 of 512).
+// Many rows: parts of at least 512 tokens where the row tiles alone are fewer than two workgroups a CU (512 rows of group 6
+// on 16,896 keys: one part 1,140 us, five 281).
+// `whole`: no workspaces, every item in one piece; `held`: the tokens that a sequence's row of the page table can hold.
+Plan plan(uint32_t seqs, uint32_t max_q, uint32_t max_kv, uint32_t heads, uint32_t kv_heads, uint32_t dim, bool f8, bool whole, uint64_t held) {
+  Plan p{};
+  const uint64_t rows = (uint64_t)max_q * (heads / kv_heads), units = max_kv ? ((max_kv - 1) >> FEW_UNIT_SHIFT) + 1 : 1;
+  const uint64_t all32 = (uint64_t)seqs * kv_heads * ((rows + FEW_ROWS - 1) / FEW_ROWS) * units;
+  p.rows = rows <= 16 ? 16 : rows <= FEW_ROWS || (!whole && units >= 8 && all32 <= 5 * CU_COUNT) ? FEW_ROWS : MANY_ROWS;
+  p.qtiles = (rows + p.rows - 1) / p.rows;
   p.items = (uint64_t)seqs * kv_heads * p.qtiles;
-  const uint32_t held = p.rows == 16 && (f8 || dim < 256) ? 2 : 1;
-  const uint64_t target = p.few() ? (uint64_t)CU_COUNT * held * (seqs == 1 ? 1 : 4) : 2 * CU_COUNT, unit = p.few() ? 128 : 512;
-  uint64_t parts = std::max<uint64_t>(1, target / std::max<uint64_t>(p.items, 1));
-  const uint64_t most = std::min<uint64_t>(p.few() ? FEW_PARTS : MANY_PARTS, std::max<uint64_t>(1, (max_kv + unit - 1) / unit));
-  parts = std::min(parts, most);
-  uint64_t chunk = (max_kv + parts - 1) / parts;
-  chunk = std::max<uint64_t>(unit, (chunk + 127) / 128 * 128);
-  p.splits = (uint32_t)std::max<uint64_t>(1, (max_kv + chunk - 1) / chunk);
-  p.chunk = p.splits == 1 ? WHOLE : (uint32_t)chunk;
+  p.splits = 1, p.chunk = WHOLE, p.unit_shift = WHOLE_SHIFT;
+  if (p.few()) {
+    const uint64_t slots = p.items * units >= 16 * CU_COUNT ? CU_COUNT * 3 / 4 : CU_COUNT * (p.rows == 16 && (f8 || dim < 256) ? 2 : 1);
+    if (!whole && units > 1) {
+      p.unit_shift = FEW_UNIT_SHIFT;
+      while (p.unit_shift < WHOLE_SHIFT && p.items * ((held >> p.unit_shift) + 1) > I32_MAX) ++p.unit_shift;  // the kernel counts them in 32 bits
+    }
+    const bool split = p.unit_shift != WHOLE_SHIFT;
+    p.grid = std::min(split ? slots : std::max<uint64_t>(slots, 2 * CU_COUNT), p.items * (split ? units : 1));
+    if (split) p.partial = p.grid * 2 * p.rows * (dim + 4) * 4, p.counter = p.items * 4;
+    return p;
+  }
+  const uint64_t target = 2 * CU_COUNT, least = 512;
+  const uint64_t parts = std::min<uint64_t>({std::max<uint64_t>(1, target / p.items), MANY_PARTS, std::max<uint64_t>(1, (max_kv + least - 1) / least)});
+  if (!whole && parts > 1) {
+    p.chunk = (uint32_t)(((max_kv + parts - 1) / parts + 127) / 128 * 128);
+    p.splits = (max_kv + p.chunk - 1) / p.chunk;
+  }
+  p.grid = p.items * p.splits;
+  if (p.splits > 1) p.partial = p.grid * p.rows * (dim + 4) * 4, p.counter = p.items * 4;
   return p;
 }
 
-int attn_args(const char *op, uint32_t seqs, uint32_t max_q, uint32_t max_kv, uint32_t heads, uint32_t kv_heads, uint32_t dim, bool f8, Plan *p) {
+int attn_plan(const char *op, uint32_t seqs, uint32_t max_q, uint32_t max_kv, uint32_t heads, uint32_t kv_heads, uint32_t dim, bool f8, bool whole, uint64_t held, Plan *p) {
   if (!max_q || max_kv > I32_MAX) return fail(SABER_IU8_E_RULE, fmt("%s: at most %u new rows and %u keys a sequence: from 1 and below 2^31", op, max_q, max_kv));
-  *p = plan(seqs, max_q, max_kv, heads, kv_heads, dim, f8);
-  if ((uint64_t)max_q * (heads / kv_heads) > I32_MAX || p->items * p->splits > I32_MAX)
+  *p = plan(seqs, max_q, max_kv, heads, kv_heads, dim, f8, whole, held);
+  if ((uint64_t)max_q * (heads / kv_heads) > I32_MAX || p->items > I32_MAX || p->grid > I32_MAX)
     return fail(SABER_IU8_E_RULE, fmt("%s: %u sequences of up to %u new rows and %u heads pass a launch's 32-bit sizes", op, seqs, max_q, heads));
   return 0;
 }
@@ -99,15 +120,28 @@ int iu8::attn_guard(const saber_iu8_desc *d) {
     return s && s->kind == SABER_IU8_ARG_I32 ? s->ival : -1;
   };
   const int64_t shape = num("shape"), heads = shape & 0xFFFF, kv_heads = shape >> 16, pages = num("pages"), stride = num("table_stride");
-  const bool append = !strncmp(d->kernel, "kv_append_", 10);
+  const bool append = !strncmp(d->kernel, "kv_append_", 10), few = !strncmp(d->kernel, "attn_few_", 9);
   const int64_t form = append ? num("form") : num("page_shift"), shift = form & 0xFF, rot = append ? form >> 16 : 0;
   const char *w = strstr(d->kernel, "_d");
   const int64_t dim = w ? atoi(w + 2) : 0;
   bool ok = shape > 0 && kv_heads > 0 && heads > 0 && heads % kv_heads == 0 && form >= 0 && shift >= 4 && shift <= 8 && pages > 0 && stride > 0 &&
             (stride << shift) <= (int64_t)WHOLE && num("tokens") > 0 && d->grid[1] == 1 && d->grid[2] == 1;
-  if (append) ok = ok && rot % 16 == 0 && rot <= dim && num("seqs") > 0;
-  else ok = ok && num("chunk") >= 64 && num("chunk") % 64 == 0 && num("qtiles") > 0 && num("splits") > 0 &&
-                 num("splits") <= (strncmp(d->kernel, "attn_few_", 9) ? MANY_PARTS : FEW_PARTS) && d->grid[0] % (uint64_t)(num("splits") * num("qtiles") * kv_heads) == 0;
+  if (append) {
+    ok = ok && rot % 16 == 0 && rot <= dim && num("seqs") > 0;
+  } else {
+    const saber_iu8_slot *part = slot(d, "partial"), *count = slot(d, "counter");
+    const bool bound = part && count && part->kind == SABER_IU8_ARG_BUFFER && count->kind == SABER_IU8_ARG_BUFFER;
+    const int64_t qtiles = num("qtiles");
+    if (few) {
+      const int64_t unit = num("unit_shift"), seqs = num("seqs");
+      ok = ok && qtiles > 0 && seqs > 0 && unit >= FEW_UNIT_SHIFT && unit <= WHOLE_SHIFT && (bound || unit == WHOLE_SHIFT) &&
+           (__int128)seqs * kv_heads * qtiles * (((stride << shift) >> unit) + 1) <= (int64_t)I32_MAX;
+    } else {
+      const int64_t chunk = num("chunk"), splits = num("splits");
+      ok = ok && qtiles > 0 && splits > 0 && splits <= MANY_PARTS && chunk >= 128 && chunk <= (int64_t)WHOLE && chunk % 128 == 0 && (bound || splits == 1) &&
+           d->grid[0] % (uint64_t)(splits * qtiles * kv_heads) == 0;
+    }
+  }
   return ok ? 0 : fail(SABER_IU8_E_RULE, fmt("%s: scalars that the kernel's walk over the cache does not hold", d->kernel));
 }
 
@@ -188,10 +222,8 @@ int saber_iu8_attn_workspace(uint32_t seqs, uint32_t max_q, uint32_t max_kv, uin
   uint64_t partial = 0, counter = 0;
   for (bool f8 : {false, true}) {  // enough for a cache of either kind
     Plan p;
-    if (int rc = attn_args("attn_workspace", seqs, max_q, max_kv, heads, kv_heads, head_dim, f8, &p)) return rc;
-    if (p.splits == 1) continue;
-    partial = std::max(partial, p.items * p.splits * p.rows * (head_dim + 4) * 4);
-    counter = std::max(counter, p.items * 4);
+    if (int rc = attn_plan("attn_workspace", seqs, max_q, max_kv, heads, kv_heads, head_dim, f8, false, max_kv, &p)) return rc;
+    partial = std::max(partial, p.partial), counter = std::max(counter, p.counter);
   }
   if (partial_bytes) *partial_bytes = partial;
   if (counter_bytes) *counter_bytes = counter;
@@ -211,21 +243,22 @@ int saber_iu8_attn(saber_iu8_ctx *ctx, const void *q, uint32_t q_row, const sabe
   if (!cu_q) max_q = 1;
   Plan p;
   const bool f8 = cache->kind == SABER_IU8_KV_E4M3;
-  if (int rc = attn_args(op, seqs, max_q, max_kv, heads, cache->kv_heads, D, f8, &p)) return rc;
-  if (!partial || !counter) p.splits = 1, p.chunk = WHOLE;  // in one piece
+  if (int rc = attn_plan(op, seqs, max_q, max_kv, heads, cache->kv_heads, D, f8, !partial || !counter, (uint64_t)cache->table_stride * cache->page_tokens, &p)) return rc;
   const char *kind = f8 ? "e4m3" : "bf16";
   saber_iu8_desc d;
-  const uint32_t grid[3] = {(uint32_t)(p.items * p.splits), 1, 1};
+  const uint32_t grid[3] = {(uint32_t)p.grid, 1, 1};
   const std::string name = p.few() ? fmt("attn_few_%s_d%u_r%u", kind, D, p.rows) : fmt("attn_many_%s_d%u", kind, D);
   if (int rc = saber_iu8_describe_raw(name.c_str(), "attn_paged", grid, 256, &d)) return rc;
   copy_name(d.op, sizeof d.op, op);
   set_i32(&d, "q_row", q_row), set_i32(&d, "tokens", tokens), set_i32(&d, "shape", heads | cache->kv_heads << 16);
   set_i32(&d, "page_shift", log2_of(cache->page_tokens)), set_i32(&d, "pages", cache->pages), set_i32(&d, "table_stride", cache->table_stride);
-  set_i32(&d, "chunk", p.chunk), set_i32(&d, "splits", p.splits), set_i32(&d, "qtiles", p.qtiles);
+  set_i32(&d, "qtiles", p.qtiles);
+  if (p.few()) set_i32(&d, "seqs", seqs), set_i32(&d, "unit_shift", p.unit_shift);
+  else set_i32(&d, "chunk", p.chunk), set_i32(&d, "splits", p.splits);
   set_f32(&d, "scale", scale);
   if (!f8) set_null(&d, "k_scale"), set_null(&d, "v_scale");
   if (!cu_q) set_null(&d, "cu_q");
-  if (p.splits == 1) set_null(&d, "partial"), set_null(&d, "counter");
+  if (!p.partial) set_null(&d, "partial"), set_null(&d, "counter");
   const saber_iu8_binding b[] = {{"q", (void *)q},
                                  {"kc", cache->k},
                                  {"vc", cache->v},

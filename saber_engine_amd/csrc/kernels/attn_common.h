@@ -24,7 +24,24 @@ struct AtCache {
   int kv_heads, page_shift, pages, table_stride;
 };
 
+// what a scheduling group counts
+constexpr int AT_MFMA = 0x8, AT_DS_READ = 0x100;
+
+// A lane's value beside the one of lane ^ 32 (or ^ 16): what both have, by one exchange between registers.
+template <int X, class F>
+static __device__ __forceinline__ float at_both(float v, F f) {
+  const unsigned u = __float_as_uint(v);
+  iu8_v2u r;
+  if constexpr (X == 32) r = __builtin_bit_cast(iu8_v2u, __builtin_amdgcn_permlane32_swap(u, u, false, false));
+  else r = __builtin_bit_cast(iu8_v2u, __builtin_amdgcn_permlane16_swap(u, u, false, false));
+  return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+static __device__ __forceinline__ float at_max2(float a, float b) { return fmaxf(a, b); }
+static __device__ __forceinline__ float at_sum2(float a, float b) { return a + b; }
+
 static __device__ __forceinline__ int at_uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+static __device__ __forceinline__ float at_uniform_f(float x) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(x))); }
 
 // Tokens of sequence s, bounded by what its row of the page table can hold.
 static __device__ __forceinline__ int at_len(const int *kv_len, int s, int table_stride, int page_shift) {
@@ -77,6 +94,13 @@ static __device__ __forceinline__ void at_four(const unsigned char *p, float (&v
   v[2] = __uint_as_float(x[1] << 16), v[3] = __uint_as_float(x[1] & 0xFFFF0000u);
 }
 
-// f32 partials of a split: 16 bytes a store / load that are coherent across the XCDs' L2s by themselves (iu8_common.h).
+// f32 partials of a split: 16 bytes a store / load that are coherent across the XCDs' L2s by themselves (iu8_common.h). The loads are
+// buffer loads, whose cache policy (both scope bits) the compiler lets one name at 16 bytes and still counts, so many can be in
+// flight; `offset` in bytes from the uniform address the resource was made of.
 static __device__ __forceinline__ void at_store_through(float *p, iu8_v4f v) { iu8_store_through((int *)p, __builtin_bit_cast(iu8_v4i, v)); }
-static __device__ __forceinline__ iu8_v4f at_load_through(const float *p) { return __builtin_bit_cast(iu8_v4f, iu8_load_through((const int *)p)); }
+static __device__ __forceinline__ __amdgpu_buffer_rsrc_t at_resource(const float *p) {
+  return __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, 0xFFFFFFFFu, 0x00020000);
+}
+static __device__ __forceinline__ iu8_v4f at_load_through(__amdgpu_buffer_rsrc_t r, unsigned offset) {
+  return __builtin_bit_cast(iu8_v4f, __builtin_amdgcn_raw_buffer_load_b128(r, offset, 0, 1 | 16));
+}

@@ -46,23 +46,23 @@ static __device__ __forceinline__ void attn_many_body(
 
   __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * TILE];  // K, V of stage 0; K, V of stage 1
   __shared__ float s_il[R];
+  __shared__ int s_limit[R];  // the last position that each row sees
   __shared__ long long s_dst[R];
   __shared__ int s_last;
 
   const int r = qt * R + wave * 32 + n, i = r / G;
   const bool real = wave * 32 + n < live;
-  const int limit = real ? len - nq + i : len - 1;
+  if (hf == 0) s_limit[wave * 32 + n] = real ? len - nq + i : len - 1;
   const float ks_ = F8 ? k_scale[h] : 1.f, vs = F8 ? v_scale[h] : 1.f, cs = scale * AT_LOG2E * ks_;
   const unsigned flip = cs < 0.f ? 0x80008000u : 0u;  // attn_few.h
-  const float c = fmaxf(fabsf(cs), 1e-37f);
+  const float c = at_uniform_f(fmaxf(fabsf(cs), 1e-37f));
   iu8_v4u qf[KS];
   {
     const unsigned short *src = q + (size_t)(t0 + (real ? i : 0)) * q_row + (size_t)(h * G + (real ? r - i * G : 0)) * D;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) qf[ks] = real ? *(const iu8_v4u *)(src + 16 * ks + 8 * hf) ^ flip : iu8_v4u{0, 0, 0, 0};
   }
-  const long long dst = ((long long)(t0 + i) * heads + h * G + (r - i * G)) * D;
-  if (hf == 0) s_dst[wave * 32 + n] = dst;
+  if (hf == 0) s_dst[wave * 32 + n] = ((long long)(t0 + i) * heads + h * G + (r - i * G)) * D;
   const int begin = split * chunk, end = kv_end - begin > chunk ? begin + chunk : kv_end;
 
   const int *row = table + (size_t)s * table_stride;
@@ -78,15 +78,23 @@ static __device__ __forceinline__ void attn_many_body(
   };
   auto swz = [](int t) { return D == 256 ? t & 7 : D == 128 ? t & 3 : t & 1; };
 
+  const unsigned v_off = lane * 16 / ROWB * ROWB + ((lane % (ROWB / 16)) ^ (4 * swz(lane * 16 / ROWB))) * 16;
   constexpr int RAW = F8 ? BK * D / 256 / 16 : 1;  // 16-byte pieces of K (and of V) a thread, e4m3
   iu8_v4u raw[RAW];
+  // (a thread's number, made anew: what hangs on it would otherwise be kept across the loop, in registers that it lacks)
+  auto thread = [&]() {
+    int t = tid;
+    asm volatile("" : "+v"(t));
+    return t;
+  };
   auto fetch = [&](int tile, const unsigned char *src) {  // e4m3: a tile of K or of V into registers
+    const int me = thread();
 #pragma unroll
     for (int x = 0; x < RAW; ++x) {
       // (a block is D pieces: a wave's 64 lie in one)
       bool hole;
       const size_t at = block_at(tile + 16 * at_uniform((x * 256 + wave * 64) / D), hole);
-      raw[x] = *(const iu8_v4u *)(src + at + (size_t)((x * 256 + tid) % D) * 16);
+      raw[x] = *(const iu8_v4u *)(src + at + (unsigned)((x * 256 + me) % D) * 16);
     }
   };
   auto issue = [&](int tile, int stage) {  // bf16: a tile of both straight into a stage
@@ -96,29 +104,31 @@ static __device__ __forceinline__ void attn_many_body(
       for (int x = 0; x < LOADS / 4; ++x) {
         const int ld = x * 4 + wave, blk = ld / BLK, part = ld % BLK;
         bool hole;
-        const size_t at = block_at(tile + 16 * blk, hole);
+        const size_t at = block_at(tile + 16 * blk, hole) + part * 1024;
         const unsigned lk = lds0 + stage * 2 * TILE + ld * 1024, lv = lk + TILE;
-        // V: lane's slot is row t, piece p; it holds piece p ^ 4 swz(t) of the row
-        const int t = part * (1024 / ROWB) + lane * 16 / ROWB, p = lane % (ROWB / 16);
-        const unsigned ok = part * 1024 + lane * 16, ov = t * ROWB + ((p ^ (4 * swz(t))) * 16);
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lk), "v"(ok), "s"(kc + at) : "memory", "m0");
+        // V: a lane's slot is row t, piece p; it holds piece p ^ 4 swz(t) of the row (of a whole kilobyte's rows, `part` shows in
+        // the piece at D = 256 alone)
+        const unsigned ov = D == 256 ? v_off ^ ((part & 3) * 128) : v_off;
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lk), "v"(lane * 16), "s"(kc + at) : "memory", "m0");
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lv), "v"(ov), "s"(vc + at) : "memory", "m0");
       }
     }
   };
   auto widen_k = [&](int stage) {
+    const int me = thread();
 #pragma unroll
     for (int x = 0; x < RAW; ++x) {
-      const int piece = x * 256 + tid, blk = piece / D, in = piece % D;
+      const int piece = x * 256 + me, blk = piece / D, in = piece % D;
       unsigned char *to = smem + stage * 2 * TILE + blk * 16 * ROWB + ((in / 16) * 32 + in % 16) * 16;
       *(iu8_v4u *)to = at_e4m3x8(raw[x][0], raw[x][1]);
       *(iu8_v4u *)(to + 256) = at_e4m3x8(raw[x][2], raw[x][3]);
     }
   };
   auto widen_v = [&](int stage) {
+    const int me = thread();
 #pragma unroll
     for (int x = 0; x < RAW; ++x) {
-      const int piece = x * 256 + tid, t = piece / (D / 16), p = piece % (D / 16) * 2;
+      const int piece = x * 256 + me, t = piece / (D / 16), p = piece % (D / 16) * 2;
       unsigned char *to = smem + (stage * 2 + 1) * TILE + t * ROWB + ((p ^ (4 * swz(t))) * 16);
       *(iu8_v4u *)to = at_e4m3x8(raw[x][0], raw[x][1]);
       *(iu8_v4u *)(to + 16) = at_e4m3x8(raw[x][2], raw[x][3]);
@@ -133,9 +143,12 @@ static __device__ __forceinline__ void attn_many_body(
 #pragma unroll
   for (int x = 0; x < MT; ++x) o[x] = at_v16f{};
   float m = -__builtin_inff(), l = 0.f;
-  const unsigned k_lane = (n >> 4) * 16 * ROWB + hf * 256 + (n & 15) * 16;
+  auto k_lane = [&]() {
+    const int ln = (F8 ? thread() : tid) & 63;
+    return (unsigned)(((ln >> 4) & 1) * 16 * ROWB + (ln >> 5) * 256 + (ln & 15) * 16);
+  };
   const int vrow = 4 * hf + ((lane & 15) >> 2);
-  const unsigned v_lane = vrow * ROWB + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
+  const unsigned v_lane = vrow * ROWB + swz(vrow) * 64 + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;  // ^ 64 mt: channel block mt
 
   if (begin < end) {
     if constexpr (F8) {
@@ -164,10 +177,9 @@ static __device__ __forceinline__ void attn_many_body(
       holes |= (hole ? 1u : 0u) << b;
     }
     const bool special = holes || tile + BK > min(end, free_end);
-    auto piece = [&](int t, int x) -> unsigned char * { return sv + t * ROWB + ((x ^ (4 * swz(t))) * 16); };
     int odd = 0;  // a value that is not finite among tokens that some rows see and others do not
     if (special) {
-      for (int x = tid; x < BK * (ROWB / 16); x += 256) {
+      for (int x = thread(); x < BK * (ROWB / 16); x += 256) {
         const int t = x / (ROWB / 16);
         iu8_v4u *at = (iu8_v4u *)(sv + x * 16);
         if (tile + t >= end || (holes >> (t >> 4) & 1)) {  // takes no part: a weight of zero would keep its NaNs
@@ -183,20 +195,37 @@ static __device__ __forceinline__ void attn_many_body(
     // scores. (The products are read in the block that makes them: behind a branch this compiler leaves too few wait states
     // between a matrix instruction and the first read of its result, seen as wrong scores.)
     float st[HB][16];
+    {
+      at_v16f sc[HB];
+      iu8_v4u kf[HB][KS];
+      const unsigned char *ka = sk + k_lane();
 #pragma unroll
-    for (int hb = 0; hb < HB; ++hb) {
-      at_v16f sc = at_v16f{};
+      for (int hb = 0; hb < HB; ++hb)
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        const iu8_v4u a = *(const iu8_v4u *)(sk + k_lane + hb * 32 * ROWB + ks * 512);
-        sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at_bf(a), at_bf(qf[ks]), sc, 0, 0, 0);
+        for (int ks = 0; ks < KS; ++ks) kf[hb][ks] = *(const iu8_v4u *)(ka + hb * 32 * ROWB + ks * 512);
+#pragma unroll
+      for (int hb = 0; hb < HB; ++hb) {
+        sc[hb] = at_v16f{};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) sc[hb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at_bf(kf[hb][ks]), at_bf(qf[ks]), sc[hb], 0, 0, 0);
       }
+      // the order of issue: reads ahead of the products by a few (attn_few.h)
+      constexpr int AHEAD = D == 256 ? (F8 ? 2 : 3) : 4;
+      __builtin_amdgcn_sched_group_barrier(AT_DS_READ, AHEAD, 0);
 #pragma unroll
-      for (int x = 0; x < 16; ++x) {
-        float y = sc[x];
-        asm volatile("" : "+v"(y));
-        st[hb][x] = y;
+      for (int x = 0; x < HB * KS - AHEAD; ++x) {
+        __builtin_amdgcn_sched_group_barrier(AT_MFMA, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(AT_DS_READ, 1, 0);
       }
+      __builtin_amdgcn_sched_group_barrier(AT_MFMA, AHEAD, 0);
+#pragma unroll
+      for (int hb = 0; hb < HB; ++hb)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+          float y = sc[hb][x];
+          asm volatile("" : "+v"(y));
+          st[hb][x] = y;
+        }
     }
     if constexpr (F8) {
       if (more) {
@@ -205,12 +234,15 @@ static __device__ __forceinline__ void attn_many_body(
       }
     }
     if (special) {
+      int ln = lane;
+      asm volatile("" : "+v"(ln));  // (what this rare block needs is made here and not kept across the loop)
+      const int last = min(s_limit[wave * 32 + (ln & 31)], end - 1) - tile - 4 * (ln >> 5);
 #pragma unroll
       for (int hb = 0; hb < HB; ++hb)
 #pragma unroll
         for (int x = 0; x < 16; ++x) {
-          const int t = 32 * hb + 8 * (x >> 2) + 4 * hf + (x & 3);
-          if (tile + t > limit || tile + t >= end || (holes >> (t >> 4) & 1)) st[hb][x] = -__builtin_inff();
+          const int t = 32 * hb + 8 * (x >> 2) + (x & 3);  // + 4 half
+          if (t > last || (holes >> (t >> 4) & 1)) st[hb][x] = -__builtin_inff();
         }
     }
     float top = st[0][0];
@@ -218,7 +250,7 @@ static __device__ __forceinline__ void attn_many_body(
     for (int hb = 0; hb < HB; ++hb)
 #pragma unroll
       for (int x = 0; x < 16; ++x) top = fmaxf(top, st[hb][x]);
-    top = fmaxf(top, __shfl_xor(top, 32));
+    top = at_both<32>(top, at_max2);
     // The maximum that the weights are taken against moves only when a score passes it by 2^8 or more (and at the first key): until
     // then weights of up to 256 are as exact, and the sums' rescale is saved.
     if (__any((top - m) * c > 8.f)) {
@@ -240,55 +272,71 @@ static __device__ __forceinline__ void attn_many_body(
         pf[hb][x / 2] = iu8_bf16_pack(st[hb][x], st[hb][x + 1]);
       }
     if (odd) {  // these tokens' values by lane arithmetic, for the rows that see them; the product then finds zeros
-      const int from = max(free_end - tile, 0), to = min(end - tile, BK);
+      int ln = lane;
+      asm volatile("" : "+v"(ln));
+      const int from = max(free_end - tile, 0), to = min(end - tile, BK), last = s_limit[wave * 32 + (ln & 31)] - tile;
 #pragma unroll
       for (int hb = 0; hb < HB; ++hb)
 #pragma unroll 1
         for (int t = max(from - 32 * hb, 0); t < min(to - 32 * hb, 32); ++t) {
-          float pj = st[hb][0];
+          unsigned w = pf[hb][0];
+          const int j = (t >> 3) * 4 + (t & 3), tt = t + 32 * hb;
 #pragma unroll
-          for (int x = 1; x < 16; ++x) pj = (t >> 3) * 4 + (t & 3) == x ? st[hb][x] : pj;
-          pj = __shfl(pj, n + 32 * ((t >> 2) & 1));
-          const int tt = t + 32 * hb;
-          if (tile + tt <= limit && !(holes >> (tt >> 4) & 1)) {
+          for (int x = 1; x < 8; ++x) w = j >> 1 == x ? pf[hb][x] : w;
+          const float pj = __shfl(__uint_as_float(j & 1 ? w & 0xFFFF0000u : w << 16), (ln & 31) + 32 * ((t >> 2) & 1));
+          if (tt <= last && !(holes >> (tt >> 4) & 1)) {
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
               for (int x = 0; x < 16; x += 4) {
                 float v[4];
-                at_four<false>(piece(tt, 4 * mt + x / 4) + 8 * hf, v);
+                at_four<false>(sv + tt * ROWB + ((4 * (mt ^ swz(tt)) + x / 4) * 16) + 8 * (ln >> 5), v);
 #pragma unroll
                 for (int r2 = 0; r2 < 4; ++r2) o[mt][x + r2] = fmaf(pj, v[r2], o[mt][x + r2]);
               }
           }
         }
       __syncthreads();
-      for (int x = tid; x < BK * (ROWB / 16); x += 256)
+      for (int x = thread(); x < BK * (ROWB / 16); x += 256)
         if (x / (ROWB / 16) >= from) *(iu8_v4u *)(sv + x * 16) = iu8_v4u{0, 0, 0, 0};
       __syncthreads();
     }
+    {
+      constexpr int NP = MT * HB * 2;  // products, two reads each
+      unsigned va = (unsigned)(size_t)(__attribute__((address_space(3))) unsigned char *)sv + v_lane;
+      asm volatile("" : "+v"(va));  // (the addresses are made from it here: kept across the loop they would be registers that it lacks)
+      iu8_v2u vf[NP][2];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      const unsigned char *pv = sv + v_lane + ((mt ^ swz(vrow)) * 64);
+      for (int x = 0; x < NP; ++x) {
+        const int mt = x / (2 * HB), t16 = x % (2 * HB);
+        auto *pv = (__attribute__((address_space(3))) unsigned char *)(size_t)(va ^ (mt * 64)) + 16 * t16 * ROWB;
+        vf[x][0] = __builtin_bit_cast(iu8_v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) at_v4s *)pv));
+        vf[x][1] = __builtin_bit_cast(iu8_v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) at_v4s *)(pv + 8 * ROWB)));
+      }
 #pragma unroll
-      for (int hb = 0; hb < HB; ++hb)
+      for (int x = 0; x < NP; ++x) {
+        const int mt = x / (2 * HB), t16 = x % (2 * HB);
+        const unsigned *w = &pf[t16 / 2][t16 % 2 * 4];
+        o[mt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at_bf(vf[x][0][0], vf[x][0][1], vf[x][1][0], vf[x][1][1]), at_bf(w[0], w[1], w[2], w[3]), o[mt], 0, 0, 0);
+      }
+      constexpr int AHEAD = D == 256 ? 2 : 3;
+      __builtin_amdgcn_sched_group_barrier(AT_DS_READ, 2 * AHEAD, 1);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const at_v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) at_v4s *)(pv + (32 * hb + 16 * t) * ROWB));
-          const at_v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) at_v4s *)(pv + (32 * hb + 16 * t + 8) * ROWB));
-          const iu8_v2u a0 = __builtin_bit_cast(iu8_v2u, lo), a1 = __builtin_bit_cast(iu8_v2u, hi);
-          o[mt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at_bf(a0[0], a0[1], a1[0], a1[1]), at_bf(pf[hb][4 * t], pf[hb][4 * t + 1], pf[hb][4 * t + 2], pf[hb][4 * t + 3]),
-                                                          o[mt], 0, 0, 0);
-        }
+      for (int x = 0; x < NP - AHEAD; ++x) {
+        __builtin_amdgcn_sched_group_barrier(AT_MFMA, 1, 1);
+        __builtin_amdgcn_sched_group_barrier(AT_DS_READ, 2, 1);
+      }
+      __builtin_amdgcn_sched_group_barrier(AT_MFMA, AHEAD, 1);
     }
     if constexpr (F8) {
       if (more) widen_v(stage ^ 1);
     }
     arrived();
   }
-  l += __shfl_xor(l, 32);
+  l = at_both<32>(l, at_sum2);
   if (ns == 1) {
     const float il = l == 0.f ? 0.f : vs / l;
+    const long long dst = s_dst[wave * 32 + n];
     if (real) {
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
@@ -299,16 +347,16 @@ static __device__ __forceinline__ void attn_many_body(
     }
     return;
   }
-  const size_t per = (size_t)R * (D + 4);
-  float *part = partial + (size_t)item * splits * per, *ml = part + (size_t)splits * R * D;
+  constexpr size_t SLOT = (size_t)R * (D + 4);
+  float *part = partial + (size_t)item * splits * SLOT, *mine = part + (size_t)split * SLOT;
   if (real) {
-    float *p = part + ((size_t)split * R + wave * 32 + n) * D;
+    float *p = mine + (wave * 32 + n) * D;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
       for (int x = 0; x < 16; x += 4)
         at_store_through(p + 32 * mt + 2 * x + 4 * hf, iu8_v4f{o[mt][x], o[mt][x + 1], o[mt][x + 2], o[mt][x + 3]});
-    if (hf == 0) at_store_through(ml + ((size_t)split * R + wave * 32 + n) * 4, iu8_v4f{m * c, l, 0.f, 0.f});
+    if (hf == 0) at_store_through(mine + R * D + (wave * 32 + n) * 4, iu8_v4f{m * c, l, 0.f, 0.f});
   }
   iu8_stores_done();
   __syncthreads();
@@ -319,5 +367,5 @@ static __device__ __forceinline__ void attn_many_body(
   }
   __syncthreads();
   if (!s_last) return;
-  at_join<D, R, 256, 2, 8>(part, ml, ns, live, vs, tid, out, s_dst, s_il, (float *)smem);
+  at_join<D, R, 256, 2, 8>(part, 0, SLOT, ns, live, vs, tid, out, s_dst, s_il, (float *)smem);
 }

@@ -24,10 +24,10 @@
       const unsigned short *__restrict__ q, const unsigned char *__restrict__ kc, const unsigned char *__restrict__ vc,           \
       const float *__restrict__ k_scale, const float *__restrict__ v_scale, const int *__restrict__ table,                        \
       const int *__restrict__ kv_len, const int *__restrict__ cu_q, unsigned short *__restrict__ out, float *__restrict__ partial, \
-      int *__restrict__ counter, int q_row, int tokens, int shape, int page_shift, int pages, int table_stride, int chunk,        \
-      int splits, int qtiles, float scale) {                                                                                      \
-    attn_few_body<D, F8, RT>(q, kc, vc, k_scale, v_scale, table, kv_len, cu_q, out, partial, counter, q_row, tokens, shape,       \
-                             page_shift, pages, table_stride, chunk, splits, scale);                                              \
+      int *__restrict__ counter, int q_row, int tokens, int seqs, int shape, int page_shift, int pages, int table_stride,         \
+      int unit_shift, int qtiles, float scale) {                                                                                  \
+    attn_few_body<D, F8, RT>(q, kc, vc, k_scale, v_scale, table, kv_len, cu_q, out, partial, counter, q_row, tokens, seqs, shape, \
+                             page_shift, pages, table_stride, unit_shift, qtiles, scale);                                             \
   }
 #define ATTN_MANY(name, D, F8)                                                                                                    \
   extern "C" __global__ __launch_bounds__(256, 2) void attn_many_##name##_d##D(                                                      \
