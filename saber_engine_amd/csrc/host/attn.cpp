@@ -2,6 +2,7 @@
 // launches. No counterpart among the reference's interfaces for this path.
 #include <algorithm>
 #include <cmath>
+#include <cstddef>
 
 #include "../../../include/saber_iu8.h"
 #include "rules.h"
@@ -17,11 +18,6 @@ constexpr int FEW_UNIT_SHIFT = 7, WHOLE_SHIFT = 31;  // log2 of the tokens a uni
 constexpr uint32_t MANY_PARTS = 32;  // parts of an item at most: their maxima and sums lie in one workgroup's LDS when they are joined
 constexpr uint32_t I32_MAX = 0x7FFFFFFFu;
 constexpr uint32_t WHOLE = 0x7FFFFF00u;  // a part that holds any sequence: the positions a table's row may reach
-
-void set_f32(saber_iu8_desc *d, const char *name, float v) {
-  for (uint32_t i = 0; i < d->n_args; ++i)
-    if (!strcmp(d->args[i].name, name)) d->args[i].kind = SABER_IU8_ARG_F32, d->args[i].fval = v;
-}
 
 int log2_of(uint32_t x) {
   int s = 0;
@@ -105,6 +101,50 @@ int attn_plan(const char *op, uint32_t seqs, uint32_t max_q, uint32_t max_kv, ui
   return 0;
 }
 
+// The kernels' arguments as abi.cpp declares them (natural alignment: the order says it all). An operator of a decode step is a few
+// microseconds on the card and called from a serving loop, so its image is laid out here: through a descriptor and its names the
+// call took 5.0 us on the host, 2.5 of them the runtime's.
+struct Cache {
+  const void *k, *v, *k_scale, *v_scale, *table, *kv_len;
+};
+struct AppendArgs {
+  const void *q, *k, *v, *q_out;
+  Cache cache;
+  const void *cu_q, *q_norm, *k_norm, *inv_freq;
+  int32_t q_row, q_head, kv_row, tokens, seqs, shape, form, pages, table_stride;
+  float eps;
+};
+struct AttnArgs {
+  const void *q;
+  Cache cache;
+  const void *cu_q, *out, *partial, *counter;
+  int32_t q_row;
+  union {
+    struct {
+      int32_t tokens, seqs, shape, page_shift, pages, table_stride, unit_shift, qtiles;
+      float scale;
+    } few;
+    struct {
+      int32_t tokens, shape, page_shift, pages, table_stride, chunk, splits, qtiles;
+      float scale;
+    } many;
+  };
+};
+static_assert(sizeof(AppendArgs) == 152 && offsetof(AppendArgs, eps) == 148 && sizeof(AttnArgs) == 128 && offsetof(AttnArgs, few.scale) == 124, "as abi.cpp packs them");
+
+Cache cache_of(const saber_iu8_kv_cache *c) {
+  const bool f8 = c->kind == SABER_IU8_KV_E4M3;
+  return Cache{c->k, c->v, f8 ? c->k_scale : nullptr, f8 ? c->v_scale : nullptr, c->page_table, c->kv_len};
+}
+
+// [e4m3][64, 128, 256]
+#define NAMES(stem, tail) \
+  { {stem "_bf16_d64" tail, stem "_bf16_d128" tail, stem "_bf16_d256" tail}, {stem "_e4m3_d64" tail, stem "_e4m3_d128" tail, stem "_e4m3_d256" tail} }
+constexpr const char *APPEND[2][3] = NAMES("kv_append", ""), *FEW16[2][3] = NAMES("attn_few", "_r16"), *FEW32[2][3] = NAMES("attn_few", "_r32"),
+                     *MANY[2][3] = NAMES("attn_many", "");
+#undef NAMES
+int dim_index(uint32_t dim) { return dim == 64 ? 0 : dim == 128 ? 1 : 2; }
+
 const saber_iu8_slot *slot(const saber_iu8_desc *d, const char *name) {
   for (uint32_t i = 0; i < d->n_args; ++i)
     if (!strcmp(d->args[i].name, name)) return &d->args[i];
@@ -166,8 +206,7 @@ uint64_t saber_iu8_kv_v_offset(uint32_t page, uint32_t kv_head, uint32_t token, 
 int saber_iu8_kv_append(saber_iu8_ctx *ctx, const void *q, const void *k, const void *v, void *q_out, const saber_iu8_kv_cache *cache,
                         const int32_t *cu_q, uint32_t tokens, uint32_t seqs, uint32_t heads, uint32_t q_row, uint32_t q_head, uint32_t kv_row,
                         const double *inv_freq, uint32_t rot_dim, int interleaved, const void *q_norm, const void *k_norm, float eps, void *stream) {
-  const char *op = "kv_append";
-  if (int rc = cache_check(op, cache, heads, seqs, tokens, cu_q)) return rc;
+  if (int rc = cache_check("kv_append", cache, heads, seqs, tokens, cu_q)) return rc;
   const uint32_t D = cache->head_dim;
   if (!q || !k || !v || !q_out) return fail(SABER_IU8_E_ARG, "kv_append: null rows");
   if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q_out | (uintptr_t)q_norm | (uintptr_t)k_norm) % 16)
@@ -183,36 +222,10 @@ int saber_iu8_kv_append(saber_iu8_ctx *ctx, const void *q, const void *k, const 
   const uint64_t all = (uint64_t)tokens * waves;
   if (all > I32_MAX) return fail(SABER_IU8_E_RULE, fmt("kv_append: %u rows of %u heads pass a launch's 32-bit sizes", tokens, heads));
   const bool f8 = cache->kind == SABER_IU8_KV_E4M3;
-  saber_iu8_desc d;
-  const uint32_t grid[3] = {(uint32_t)((all + 3) / 4), 1, 1};
-  if (int rc = saber_iu8_describe_raw(fmt("kv_append_%s_d%u", f8 ? "e4m3" : "bf16", D).c_str(), "attn_paged", grid, 256, &d)) return rc;
-  copy_name(d.op, sizeof d.op, op);
-  set_i32(&d, "q_row", q_row), set_i32(&d, "q_head", q_head), set_i32(&d, "kv_row", kv_row);
-  set_i32(&d, "tokens", tokens), set_i32(&d, "seqs", seqs);
-  set_i32(&d, "shape", heads | cache->kv_heads << 16);
-  set_i32(&d, "form", log2_of(cache->page_tokens) | (interleaved ? 0x100 : 0) | rot_dim << 16);
-  set_i32(&d, "pages", cache->pages), set_i32(&d, "table_stride", cache->table_stride);
-  set_f32(&d, "eps", eps);
-  if (!f8) set_null(&d, "k_scale"), set_null(&d, "v_scale");
-  if (!cu_q) set_null(&d, "cu_q");
-  if (!q_norm) set_null(&d, "q_norm");
-  if (!k_norm) set_null(&d, "k_norm");
-  if (!rot_dim) set_null(&d, "inv_freq");
-  const saber_iu8_binding b[] = {{"q", (void *)q},
-                                 {"k", (void *)k},
-                                 {"v", (void *)v},
-                                 {"q_out", q_out},
-                                 {"kc", cache->k},
-                                 {"vc", cache->v},
-                                 {"k_scale", (void *)cache->k_scale},
-                                 {"v_scale", (void *)cache->v_scale},
-                                 {"table", (void *)cache->page_table},
-                                 {"kv_len", (void *)cache->kv_len},
-                                 {"cu_q", (void *)cu_q},
-                                 {"q_norm", (void *)q_norm},
-                                 {"k_norm", (void *)k_norm},
-                                 {"inv_freq", (void *)inv_freq}};
-  return saber_iu8_launch(ctx, &d, b, 14, stream);
+  AppendArgs x{q, k, v, q_out, cache_of(cache), cu_q, q_norm, k_norm, rot_dim ? inv_freq : nullptr, (int32_t)q_row, (int32_t)q_head, (int32_t)kv_row,
+               (int32_t)tokens, (int32_t)seqs, (int32_t)(heads | cache->kv_heads << 16),
+               (int32_t)(log2_of(cache->page_tokens) | (interleaved ? 0x100 : 0) | rot_dim << 16), (int32_t)cache->pages, (int32_t)cache->table_stride, eps};
+  return launch_image(ctx, APPEND[f8][dim_index(D)], (uint32_t)((all + 3) / 4), 256, &x, sizeof x, stream);
 }
 
 int saber_iu8_attn_workspace(uint32_t seqs, uint32_t max_q, uint32_t max_kv, uint32_t heads, uint32_t kv_heads, uint32_t head_dim,
@@ -232,8 +245,7 @@ int saber_iu8_attn_workspace(uint32_t seqs, uint32_t max_q, uint32_t max_kv, uin
 
 int saber_iu8_attn(saber_iu8_ctx *ctx, const void *q, uint32_t q_row, const saber_iu8_kv_cache *cache, const int32_t *cu_q, void *out, uint32_t tokens,
                    uint32_t seqs, uint32_t max_q, uint32_t max_kv, uint32_t heads, float scale, void *partial, void *counter, void *stream) {
-  const char *op = "attn";
-  if (int rc = cache_check(op, cache, heads, seqs, tokens, cu_q)) return rc;
+  if (int rc = cache_check("attn", cache, heads, seqs, tokens, cu_q)) return rc;
   const uint32_t D = cache->head_dim;
   if (!q || !out) return fail(SABER_IU8_E_ARG, "attn: null rows");
   if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)partial) % 16 || (uintptr_t)counter % 4) return fail(SABER_IU8_E_ARG, "attn: rows and partials must lie on 16 bytes");
@@ -243,34 +255,16 @@ int saber_iu8_attn(saber_iu8_ctx *ctx, const void *q, uint32_t q_row, const sabe
   if (!cu_q) max_q = 1;
   Plan p;
   const bool f8 = cache->kind == SABER_IU8_KV_E4M3;
-  if (int rc = attn_plan(op, seqs, max_q, max_kv, heads, cache->kv_heads, D, f8, !partial || !counter, (uint64_t)cache->table_stride * cache->page_tokens, &p)) return rc;
-  const char *kind = f8 ? "e4m3" : "bf16";
-  saber_iu8_desc d;
-  const uint32_t grid[3] = {(uint32_t)p.grid, 1, 1};
-  const std::string name = p.few() ? fmt("attn_few_%s_d%u_r%u", kind, D, p.rows) : fmt("attn_many_%s_d%u", kind, D);
-  if (int rc = saber_iu8_describe_raw(name.c_str(), "attn_paged", grid, 256, &d)) return rc;
-  copy_name(d.op, sizeof d.op, op);
-  set_i32(&d, "q_row", q_row), set_i32(&d, "tokens", tokens), set_i32(&d, "shape", heads | cache->kv_heads << 16);
-  set_i32(&d, "page_shift", log2_of(cache->page_tokens)), set_i32(&d, "pages", cache->pages), set_i32(&d, "table_stride", cache->table_stride);
-  set_i32(&d, "qtiles", p.qtiles);
-  if (p.few()) set_i32(&d, "seqs", seqs), set_i32(&d, "unit_shift", p.unit_shift);
-  else set_i32(&d, "chunk", p.chunk), set_i32(&d, "splits", p.splits);
-  set_f32(&d, "scale", scale);
-  if (!f8) set_null(&d, "k_scale"), set_null(&d, "v_scale");
-  if (!cu_q) set_null(&d, "cu_q");
-  if (!p.partial) set_null(&d, "partial"), set_null(&d, "counter");
-  const saber_iu8_binding b[] = {{"q", (void *)q},
-                                 {"kc", cache->k},
-                                 {"vc", cache->v},
-                                 {"k_scale", (void *)cache->k_scale},
-                                 {"v_scale", (void *)cache->v_scale},
-                                 {"table", (void *)cache->page_table},
-                                 {"kv_len", (void *)cache->kv_len},
-                                 {"cu_q", (void *)cu_q},
-                                 {"out", out},
-                                 {"partial", partial},
-                                 {"counter", counter}};
-  return saber_iu8_launch(ctx, &d, b, 11, stream);
+  if (int rc = attn_plan("attn", seqs, max_q, max_kv, heads, cache->kv_heads, D, f8, !partial || !counter, (uint64_t)cache->table_stride * cache->page_tokens, &p)) return rc;
+  AttnArgs x{};
+  x.q = q, x.cache = cache_of(cache), x.cu_q = cu_q, x.out = out, x.q_row = (int32_t)q_row;
+  if (p.partial) x.partial = partial, x.counter = counter;
+  const int32_t shape = (int32_t)(heads | cache->kv_heads << 16), page_shift = log2_of(cache->page_tokens), pages = (int32_t)cache->pages,
+                stride = (int32_t)cache->table_stride;
+  if (p.few()) x.few = {(int32_t)tokens, (int32_t)seqs, shape, page_shift, pages, stride, p.unit_shift, (int32_t)p.qtiles, scale};
+  else x.many = {(int32_t)tokens, shape, page_shift, pages, stride, (int32_t)p.chunk, (int32_t)p.splits, (int32_t)p.qtiles, scale};
+  const auto &names = p.rows == 16 ? FEW16 : p.rows == FEW_ROWS ? FEW32 : MANY;
+  return launch_image(ctx, names[f8][dim_index(D)], (uint32_t)p.grid, 256, &x, sizeof x, stream);
 }
 
 }  // extern "C"

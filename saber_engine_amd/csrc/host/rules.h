@@ -124,6 +124,8 @@ std::string device_profile_toml();
 
 // The scalars of a descriptor of the paged cache's kernels (attn.cpp).
 int attn_guard(const saber_iu8_desc *d);
+// A launch of a kernarg image that its operator has laid out itself (runtime.cpp): saber_iu8_launch without the descriptor.
+int launch_image(saber_iu8_ctx *ctx, const char *kernel, uint32_t grid, uint32_t block, void *image, size_t bytes, void *stream);
 
 // Fills name/offset/size of every slot from the kernel's signature; kinds default to BUFFER.
 int fill_slots(const std::string &kernel, saber_iu8_desc *d);

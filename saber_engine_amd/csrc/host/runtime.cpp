@@ -487,6 +487,21 @@ int saber_iu8_launch(saber_iu8_ctx *ctx, const saber_iu8_desc *d, const saber_iu
   return 0;
 }
 
+}  // extern "C"
+int iu8::launch_image(saber_iu8_ctx *ctx, const char *kernel, uint32_t grid, uint32_t block, void *image, size_t bytes, void *stream) {
+  if (!ctx) return fail(SABER_IU8_E_ARG, "launch: null argument");
+  const auto it = ctx->fn.find(std::string_view(kernel));
+  if (it == ctx->fn.end()) return fail(SABER_IU8_E_NOTLOADED, std::string(kernel) + ": not in the loaded plugin set");
+  if (block != it->second.max_threads)
+    return fail(SABER_IU8_E_RULE, fmt("%s: a block of %u threads; the gfx950 kernel is written for %u", kernel, block, it->second.max_threads));
+  void *extra[] = {HIP_LAUNCH_PARAM_BUFFER_POINTER, image, HIP_LAUNCH_PARAM_BUFFER_SIZE, &bytes, HIP_LAUNCH_PARAM_END};
+  const hipError_t e = hipModuleLaunchKernel(it->second.fn, grid, 1, 1, block, 1, 1, 0, (hipStream_t)stream, nullptr, extra);
+  if (e != hipSuccess) return hip_fail(kernel, e);
+  ctx->counters.launches++;
+  return 0;
+}
+extern "C" {
+
 int saber_iu8_quant(saber_iu8_ctx *ctx, const void *x, void *q, float *scale, uint32_t m, uint32_t k, void *stream) {
   saber_iu8_desc d;
   if (int rc = resolve_quant(m, k, &d)) return rc;

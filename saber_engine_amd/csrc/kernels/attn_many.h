@@ -56,12 +56,6 @@ static __device__ __forceinline__ void attn_many_body(
   const float ks_ = F8 ? k_scale[h] : 1.f, vs = F8 ? v_scale[h] : 1.f, cs = scale * AT_LOG2E * ks_;
   const unsigned flip = cs < 0.f ? 0x80008000u : 0u;  // attn_few.h
   const float c = at_uniform_f(fmaxf(fabsf(cs), 1e-37f));
-  iu8_v4u qf[KS];
-  {
-    const unsigned short *src = q + (size_t)(t0 + (real ? i : 0)) * q_row + (size_t)(h * G + (real ? r - i * G : 0)) * D;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) qf[ks] = real ? *(const iu8_v4u *)(src + 16 * ks + 8 * hf) ^ flip : iu8_v4u{0, 0, 0, 0};
-  }
   if (hf == 0) s_dst[wave * 32 + n] = ((long long)(t0 + i) * heads + h * G + (r - i * G)) * D;
   const int begin = split * chunk, end = kv_end - begin > chunk ? begin + chunk : kv_end;
 
@@ -70,11 +64,30 @@ static __device__ __forceinline__ void attn_many_body(
   const int mask = (1 << page_shift) - 1;
   const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) unsigned char *)smem;
 
-  // where a block of 16 tokens lies (a block past the end or in a hole: page 0, masked later)
-  auto block_at = [&](int tok, bool &hole) -> size_t {
-    const int p = tok < end ? at_uniform(row[tok >> page_shift]) : -1;
-    hole = (unsigned)p >= (unsigned)pages;
-    return hole ? 0 : (((size_t)p * kv_heads + h) * head_elems + (size_t)(tok & mask) * D) * ES;
+  // where a tile's blocks of 16 tokens lie (a block past the end or in a hole: page 0, masked later); the pages are looked up a
+  // tile ahead
+  constexpr int NB = BK / 16;
+  size_t at[NB];
+  int page[NB];
+  auto look_up = [&](int tile) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b) page[b] = row[min((unsigned)(tile + 16 * b) >> page_shift, (unsigned)table_stride - 1u)];
+  };
+  auto locate = [&](int tile) {
+    unsigned holes = 0;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const bool hole = tile + 16 * b >= end || (unsigned)page[b] >= (unsigned)pages;
+      holes |= hole ? 1u << b : 0u;
+      at[b] = hole ? 0 : (((size_t)page[b] * kv_heads + h) * head_elems + (size_t)((tile + 16 * b) & mask) * D) * ES;
+    }
+    return holes;
+  };
+  auto block = [&](int first, int more) {  // (the wave's: `more` is uniform)
+    size_t x = at[first];
+#pragma unroll
+    for (int b = first + 1; b < NB; ++b) x = b == first + more ? at[b] : x;
+    return x;
   };
   auto swz = [](int t) { return D == 256 ? t & 7 : D == 128 ? t & 3 : t & 1; };
 
@@ -87,30 +100,25 @@ static __device__ __forceinline__ void attn_many_body(
     asm volatile("" : "+v"(t));
     return t;
   };
-  auto fetch = [&](int tile, const unsigned char *src) {  // e4m3: a tile of K or of V into registers
+  auto fetch = [&](const unsigned char *src) {  // e4m3: a tile of K or of V into registers
     const int me = thread();
 #pragma unroll
-    for (int x = 0; x < RAW; ++x) {
-      // (a block is D pieces: a wave's 64 lie in one)
-      bool hole;
-      const size_t at = block_at(tile + 16 * at_uniform((x * 256 + wave * 64) / D), hole);
-      raw[x] = *(const iu8_v4u *)(src + at + (unsigned)((x * 256 + me) % D) * 16);
-    }
+    for (int x = 0; x < RAW; ++x)  // (a block is D pieces: a wave's 64 lie in one)
+      raw[x] = *(const iu8_v4u *)(src + block(x * 256 / D, wave * 64 / D) + (unsigned)((x * 256 + me) % D) * 16);
   };
-  auto issue = [&](int tile, int stage) {  // bf16: a tile of both straight into a stage
+  auto issue = [&](int stage) {  // bf16: a tile of both straight into a stage
     if constexpr (!F8) {
       constexpr int BLK = 16 * ROWB / 1024, LOADS = BK / 16 * BLK;  // wave-loads of 1 KiB a block, a tile
 #pragma unroll
       for (int x = 0; x < LOADS / 4; ++x) {
-        const int ld = x * 4 + wave, blk = ld / BLK, part = ld % BLK;
-        bool hole;
-        const size_t at = block_at(tile + 16 * blk, hole) + part * 1024;
+        const int ld = x * 4 + wave, part = ld % BLK;
+        const size_t from = block(x * 4 / BLK, BLK < 4 ? wave / BLK : 0) + part * 1024;
         const unsigned lk = lds0 + stage * 2 * TILE + ld * 1024, lv = lk + TILE;
         // V: a lane's slot is row t, piece p; it holds piece p ^ 4 swz(t) of the row (of a whole kilobyte's rows, `part` shows in
         // the piece at D = 256 alone)
         const unsigned ov = D == 256 ? v_off ^ ((part & 3) * 128) : v_off;
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lk), "v"(lane * 16), "s"(kc + at) : "memory", "m0");
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lv), "v"(ov), "s"(vc + at) : "memory", "m0");
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lk), "v"(lane * 16), "s"(kc + from) : "memory", "m0");
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lv), "v"(ov), "s"(vc + from) : "memory", "m0");
       }
     }
   };
@@ -150,45 +158,59 @@ static __device__ __forceinline__ void attn_many_body(
   const int vrow = 4 * hf + ((lane & 15) >> 2);
   const unsigned v_lane = vrow * ROWB + swz(vrow) * 64 + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;  // ^ 64 mt: channel block mt
 
+  unsigned holes_next = 0;
   if (begin < end) {
+    look_up(begin);
+    holes_next = locate(begin);
     if constexpr (F8) {
-      fetch(begin, kc);
+      fetch(kc);
       widen_k(0);
-      fetch(begin, vc);
+      fetch(vc);
       widen_v(0);
     } else {
-      issue(begin, 0);
+      issue(0);
+    }
+    look_up(begin + BK);
+  }
+  // query fragments
+  iu8_v4u qf[KS];
+  {
+    const unsigned short *src = q + (size_t)(t0 + (real ? i : 0)) * q_row + (size_t)(h * G + (real ? r - i * G : 0)) * D + 8 * hf;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = *(const iu8_v4u *)(src + 16 * ks);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      qf[ks] = (qf[ks] ^ flip) & (real ? ~0u : 0u);
+      asm volatile("" : "+v"(qf[ks]));  // here, not in the loop, is what waits for them
     }
   }
   arrived();
   int stage = 0;
   for (int tile = begin; tile < end; tile += BK, stage ^= 1) {
     const bool more = tile + BK < end;
+    const unsigned holes = holes_next;
     if (more) {
-      if constexpr (F8) fetch(tile + BK, kc);
-      else issue(tile + BK, stage ^ 1);
+      holes_next = locate(tile + BK);
+      if constexpr (F8) fetch(kc);
+      else issue(stage ^ 1);
+      look_up(tile + 2 * BK);
     }
     unsigned char *sk = smem + stage * 2 * TILE, *sv = sk + TILE;
-    unsigned holes = 0;
-#pragma unroll
-    for (int b = 0; b < BK / 16; ++b) {
-      bool hole;
-      (void)block_at(tile + 16 * b, hole);
-      holes |= (hole ? 1u : 0u) << b;
-    }
     const bool special = holes || tile + BK > min(end, free_end);
     int odd = 0;  // a value that is not finite among tokens that some rows see and others do not
     if (special) {
-      for (int x = thread(); x < BK * (ROWB / 16); x += 256) {
-        const int t = x / (ROWB / 16);
-        iu8_v4u *at = (iu8_v4u *)(sv + x * 16);
-        if (tile + t >= end || (holes >> (t >> 4) & 1)) {  // takes no part: a weight of zero would keep its NaNs
-          *at = iu8_v4u{0, 0, 0, 0};
-        } else if (tile + t >= free_end) {
-          const iu8_v4u v = *at;
+      constexpr int PR = ROWB / 16;  // pieces a row
+      const int stop = min(end - tile, BK), me = thread();
+      // what takes no part (rows behind the end, a hole's block): a weight of zero would keep its NaNs
+      for (int x = stop * PR + me; x < BK * PR; x += 256) *(iu8_v4u *)(sv + x * 16) = iu8_v4u{0, 0, 0, 0};
+      if (holes)
+        for (int x = me; x < BK * PR; x += 256)
+          if (holes >> (x / (16 * PR)) & 1) *(iu8_v4u *)(sv + x * 16) = iu8_v4u{0, 0, 0, 0};
+      for (int x = max(free_end - tile, 0) * PR + me; x < stop * PR; x += 256) {
+        const iu8_v4u v = *(const iu8_v4u *)(sv + x * 16);
+        if (holes >> (x / (16 * PR)) & 1) continue;
 #pragma unroll
-          for (int w = 0; w < 4; ++w) odd |= at_nonfinite2(v[w]);
-        }
+        for (int w = 0; w < 4; ++w) odd |= at_nonfinite2(v[w]);
       }
       odd = __syncthreads_or(odd);
     }
@@ -230,7 +252,7 @@ static __device__ __forceinline__ void attn_many_body(
     if constexpr (F8) {
       if (more) {
         widen_k(stage ^ 1);
-        fetch(tile + BK, vc);
+        fetch(vc);
       }
     }
     if (special) {
