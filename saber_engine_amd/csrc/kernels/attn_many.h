@@ -67,8 +67,10 @@ static __device__ __forceinline__ void attn_many_body(
   // where a tile's blocks of 16 tokens lie (a block past the end or in a hole: page 0, masked later); the pages are looked up a
   // tile ahead
   constexpr int NB = BK / 16;
-  size_t at[NB];
-  int page[NB];
+  typedef size_t places __attribute__((ext_vector_type(NB)));  // (vectors: an array here ends up in memory)
+  typedef int page_numbers __attribute__((ext_vector_type(NB)));
+  places at{};
+  page_numbers page{};
   auto look_up = [&](int tile) {
 #pragma unroll
     for (int b = 0; b < NB; ++b) page[b] = row[min((unsigned)(tile + 16 * b) >> page_shift, (unsigned)table_stride - 1u)];
@@ -83,10 +85,10 @@ static __device__ __forceinline__ void attn_many_body(
     }
     return holes;
   };
-  auto block = [&](int first, int more) {  // (the wave's: `more` is uniform)
-    size_t x = at[first];
+  auto block = [](places of, int first, int more) {  // (the wave's: `more` is uniform)
+    size_t x = of[first];
 #pragma unroll
-    for (int b = first + 1; b < NB; ++b) x = b == first + more ? at[b] : x;
+    for (int b = first + 1; b < NB; ++b) x = b == first + more ? of[b] : x;
     return x;
   };
   auto swz = [](int t) { return D == 256 ? t & 7 : D == 128 ? t & 3 : t & 1; };
@@ -100,26 +102,36 @@ static __device__ __forceinline__ void attn_many_body(
     asm volatile("" : "+v"(t));
     return t;
   };
-  auto fetch = [&](const unsigned char *src) {  // e4m3: a tile of K or of V into registers
+  auto fetch = [&](const unsigned char *src, places of) {  // e4m3: a tile of K or of V into registers
     const int me = thread();
 #pragma unroll
     for (int x = 0; x < RAW; ++x)  // (a block is D pieces: a wave's 64 lie in one)
-      raw[x] = *(const iu8_v4u *)(src + block(x * 256 / D, wave * 64 / D) + (unsigned)((x * 256 + me) % D) * 16);
+      raw[x] = *(const iu8_v4u *)(src + block(of, x * 256 / D, wave * 64 / D) + (unsigned)((x * 256 + me) % D) * 16);
   };
-  auto issue = [&](int stage) {  // bf16: a tile of both straight into a stage
-    if constexpr (!F8) {
-      constexpr int BLK = 16 * ROWB / 1024, LOADS = BK / 16 * BLK;  // wave-loads of 1 KiB a block, a tile
+  constexpr int BLK = 16 * ROWB / 1024, LOADS = BK / 16 * BLK;  // wave-loads of 1 KiB a block, a tile
+  auto issue_k = [&](int stage, places of) {  // bf16: a tile straight into a stage
 #pragma unroll
-      for (int x = 0; x < LOADS / 4; ++x) {
-        const int ld = x * 4 + wave, part = ld % BLK;
-        const size_t from = block(x * 4 / BLK, BLK < 4 ? wave / BLK : 0) + part * 1024;
-        const unsigned lk = lds0 + stage * 2 * TILE + ld * 1024, lv = lk + TILE;
-        // V: a lane's slot is row t, piece p; it holds piece p ^ 4 swz(t) of the row (of a whole kilobyte's rows, `part` shows in
-        // the piece at D = 256 alone)
-        const unsigned ov = D == 256 ? v_off ^ ((part & 3) * 128) : v_off;
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lk), "v"(lane * 16), "s"(kc + from) : "memory", "m0");
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lv), "v"(ov), "s"(vc + from) : "memory", "m0");
-      }
+    for (int x = 0; x < LOADS / 4; ++x) {
+      const int ld = x * 4 + wave, part = ld % BLK;
+      const size_t from = block(of, x * 4 / BLK, BLK < 4 ? wave / BLK : 0) + part * 1024;
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                   :
+                   : "s"(lds0 + stage * 2 * TILE + ld * 1024), "v"(lane * 16), "s"(kc + from)
+                   : "memory", "m0");
+    }
+  };
+  auto issue_v = [&](int stage, places of) {
+#pragma unroll
+    for (int x = 0; x < LOADS / 4; ++x) {
+      const int ld = x * 4 + wave, part = ld % BLK;
+      const size_t from = block(of, x * 4 / BLK, BLK < 4 ? wave / BLK : 0) + part * 1024;
+      // a lane's slot is row t, piece p; it holds piece p ^ 4 swz(t) of the row (of a whole kilobyte's rows, `part` shows in
+      // the piece at D = 256 alone)
+      const unsigned ov = D == 256 ? v_off ^ ((part & 3) * 128) : v_off;
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                   :
+                   : "s"(lds0 + (stage * 2 + 1) * TILE + ld * 1024), "v"(ov), "s"(vc + from)
+                   : "memory", "m0");
     }
   };
   auto widen_k = [&](int stage) {
@@ -151,30 +163,171 @@ static __device__ __forceinline__ void attn_many_body(
 #pragma unroll
   for (int x = 0; x < MT; ++x) o[x] = at_v16f{};
   float m = -__builtin_inff(), l = 0.f;
-  auto k_lane = [&]() {
-    const int ln = (F8 ? thread() : tid) & 63;
-    return (unsigned)(((ln >> 4) & 1) * 16 * ROWB + (ln >> 5) * 256 + (ln & 15) * 16);
-  };
   const int vrow = 4 * hf + ((lane & 15) >> 2);
   const unsigned v_lane = vrow * ROWB + swz(vrow) * 64 + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;  // ^ 64 mt: channel block mt
-
-  unsigned holes_next = 0;
-  if (begin < end) {
-    look_up(begin);
-    holes_next = locate(begin);
-    if constexpr (F8) {
-      fetch(kc);
-      widen_k(0);
-      fetch(vc);
-      widen_v(0);
-    } else {
-      issue(0);
-    }
-    look_up(begin + BK);
-  }
-  // query fragments
   iu8_v4u qf[KS];
-  {
+
+  // ---- the steps of a tile
+  // V before its product: zeros in what takes no part (rows behind the end, a hole's block), whose NaNs a weight of zero would
+  // keep; whether a value that is not finite lies among tokens that some rows see and others do not
+  auto clean = [&](int tile, unsigned holes, unsigned char *sv) -> int {
+    constexpr int PR = ROWB / 16;  // pieces a row
+    const int stop = min(end - tile, BK), me = thread();
+    int odd = 0;
+    for (int x = stop * PR + me; x < BK * PR; x += 256) *(iu8_v4u *)(sv + x * 16) = iu8_v4u{0, 0, 0, 0};
+    if (holes)
+      for (int x = me; x < BK * PR; x += 256)
+        if (holes >> (x / (16 * PR)) & 1) *(iu8_v4u *)(sv + x * 16) = iu8_v4u{0, 0, 0, 0};
+    for (int x = max(free_end - tile, 0) * PR + me; x < stop * PR; x += 256) {
+      const iu8_v4u v = *(const iu8_v4u *)(sv + x * 16);
+      if (holes >> (x / (16 * PR)) & 1) continue;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) odd |= at_nonfinite2(v[w]);
+    }
+    return __syncthreads_or(odd);
+  };
+  // S^T = K Q^T of a stage's K into st; VALU: what lies in the same block and may be issued between the products
+  auto scores = [&](const unsigned char *sk, at_v16f (&sc)[HB]) {
+    const int ln = (F8 ? thread() : tid) & 63;
+    const unsigned char *ka = sk + ((ln >> 4) & 1) * 16 * ROWB + (ln >> 5) * 256 + (ln & 15) * 16;
+    iu8_v4u kf[HB][KS];
+#pragma unroll
+    for (int hb = 0; hb < HB; ++hb)
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) kf[hb][ks] = *(const iu8_v4u *)(ka + hb * 32 * ROWB + ks * 512);
+#pragma unroll
+    for (int hb = 0; hb < HB; ++hb) {
+      sc[hb] = at_v16f{};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) sc[hb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at_bf(kf[hb][ks]), at_bf(qf[ks]), sc[hb], 0, 0, 0);
+    }
+  };
+  // (The products are read in the block that makes them: behind a branch this compiler can leave too few wait states between a
+  // matrix instruction and the first read of its result, seen as wrong scores.)
+  auto settle = [&](const at_v16f (&sc)[HB], float (&st)[HB][16]) {
+#pragma unroll
+    for (int hb = 0; hb < HB; ++hb)
+#pragma unroll
+      for (int x = 0; x < 16; ++x) {
+        float y = sc[hb][x];
+        asm volatile("" : "+v"(y));
+        st[hb][x] = y;
+      }
+  };
+  // the order of issue: reads ahead of the products by a few (attn_few.h)
+  auto order_scores = [&]() {
+    constexpr int AHEAD = D == 256 ? (F8 ? 2 : 3) : 4;
+    __builtin_amdgcn_sched_group_barrier(AT_DS_READ, AHEAD, 0);
+#pragma unroll
+    for (int x = 0; x < HB * KS - AHEAD; ++x) {
+      __builtin_amdgcn_sched_group_barrier(AT_MFMA, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(AT_DS_READ, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(AT_MFMA, AHEAD, 0);
+  };
+  auto hide = [&](int tile, unsigned holes, float (&st)[HB][16]) {  // what a row does not see
+    int ln = lane;
+    asm volatile("" : "+v"(ln));  // (what this rare block needs is made here and not kept across the loop)
+    const int last = min(s_limit[wave * 32 + (ln & 31)], end - 1) - tile - 4 * (ln >> 5);
+#pragma unroll
+    for (int hb = 0; hb < HB; ++hb)
+#pragma unroll
+      for (int x = 0; x < 16; ++x) {
+        const int t = 32 * hb + 8 * (x >> 2) + (x & 3);  // + 4 half
+        if (t > last || (holes >> (t >> 4) & 1)) st[hb][x] = -__builtin_inff();
+      }
+  };
+  // The maximum that the weights are taken against moves only when a score passes it by 2^8 or more (and at the first key): until
+  // then weights of up to 256 are as exact, and the sums' rescale is saved. Returns it in units of log2.
+  auto maximum = [&](const float (&st)[HB][16]) -> float {
+    float top = st[0][0];
+#pragma unroll
+    for (int hb = 0; hb < HB; ++hb)
+#pragma unroll
+      for (int x = 0; x < 16; ++x) top = fmaxf(top, st[hb][x]);
+    top = at_both<32>(top, at_max2);
+    if (__any((top - m) * c > 8.f)) {
+      const float mn = fmaxf(m, top), f = __builtin_amdgcn_exp2f((m - (mn == -__builtin_inff() ? 0.f : mn)) * c);
+      l *= f;
+#pragma unroll
+      for (int x = 0; x < MT; ++x) o[x] *= f;
+      m = mn;
+    }
+    return m == -__builtin_inff() ? 0.f : m * c;
+  };
+  auto weights = [&](const float (&st)[HB][16], float mc, unsigned (&pf)[HB][8]) {
+#pragma unroll
+    for (int hb = 0; hb < HB; ++hb)
+#pragma unroll
+      for (int x = 0; x < 16; x += 2) {
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(st[hb][x], c, -mc)), p1 = __builtin_amdgcn_exp2f(fmaf(st[hb][x + 1], c, -mc));
+        l += p0 + p1;
+        pf[hb][x / 2] = iu8_bf16_pack(p0, p1);
+      }
+  };
+  // the tokens from free_end on by lane arithmetic, for the rows that see them; the product then finds zeros
+  auto by_lanes = [&](int tile, unsigned holes, unsigned char *sv, const unsigned (&pf)[HB][8]) {
+    int ln = lane;
+    asm volatile("" : "+v"(ln));
+    const int from = max(free_end - tile, 0), to = min(end - tile, BK), last = s_limit[wave * 32 + (ln & 31)] - tile;
+#pragma unroll
+    for (int hb = 0; hb < HB; ++hb)
+#pragma unroll 1
+      for (int t = max(from - 32 * hb, 0); t < min(to - 32 * hb, 32); ++t) {
+        unsigned w = pf[hb][0];
+        const int j = (t >> 3) * 4 + (t & 3), tt = t + 32 * hb;
+#pragma unroll
+        for (int x = 1; x < 8; ++x) {
+          unsigned p = pf[hb][x];
+          asm volatile("" : "+v"(p));  // (or the choice becomes an index, and the weights of every tile go to memory)
+          w = j >> 1 == x ? p : w;
+        }
+        const float pj = __shfl(__uint_as_float(j & 1 ? w & 0xFFFF0000u : w << 16), (ln & 31) + 32 * ((t >> 2) & 1));
+        if (tt <= last && !(holes >> (tt >> 4) & 1)) {
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int x = 0; x < 16; x += 4) {
+              float v[4];
+              at_four<false>(sv + tt * ROWB + ((4 * (mt ^ swz(tt)) + x / 4) * 16) + 8 * (ln >> 5), v);
+#pragma unroll
+              for (int r2 = 0; r2 < 4; ++r2) o[mt][x + r2] = fmaf(pj, v[r2], o[mt][x + r2]);
+            }
+        }
+      }
+    __syncthreads();
+    for (int x = thread(); x < BK * (ROWB / 16); x += 256)
+      if (x / (ROWB / 16) >= from) *(iu8_v4u *)(sv + x * 16) = iu8_v4u{0, 0, 0, 0};
+    __syncthreads();
+  };
+  auto product = [&](unsigned char *sv, const unsigned (&pf)[HB][8]) {  // O^T += V^T P^T
+    constexpr int NP = MT * HB * 2;                                      // two reads each
+    unsigned va = (unsigned)(size_t)(__attribute__((address_space(3))) unsigned char *)sv + v_lane;
+    asm volatile("" : "+v"(va));  // (the addresses are made from it here: kept across the loop they would be registers that it lacks)
+    iu8_v2u vf[NP][2];
+#pragma unroll
+    for (int x = 0; x < NP; ++x) {
+      const int mt = x / (2 * HB), t16 = x % (2 * HB);
+      auto *pv = (__attribute__((address_space(3))) unsigned char *)(size_t)(va ^ (mt * 64)) + 16 * t16 * ROWB;
+      vf[x][0] = __builtin_bit_cast(iu8_v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) at_v4s *)pv));
+      vf[x][1] = __builtin_bit_cast(iu8_v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) at_v4s *)(pv + 8 * ROWB)));
+    }
+#pragma unroll
+    for (int x = 0; x < NP; ++x) {
+      const int mt = x / (2 * HB), t16 = x % (2 * HB);
+      const unsigned *w = &pf[t16 / 2][t16 % 2 * 4];
+      o[mt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at_bf(vf[x][0][0], vf[x][0][1], vf[x][1][0], vf[x][1][1]), at_bf(w[0], w[1], w[2], w[3]), o[mt], 0, 0, 0);
+    }
+    constexpr int AHEAD = D == 256 ? 2 : 3;
+    __builtin_amdgcn_sched_group_barrier(AT_DS_READ, 2 * AHEAD, 1);
+#pragma unroll
+    for (int x = 0; x < NP - AHEAD; ++x) {
+      __builtin_amdgcn_sched_group_barrier(AT_MFMA, 1, 1);
+      __builtin_amdgcn_sched_group_barrier(AT_DS_READ, 2, 1);
+    }
+    __builtin_amdgcn_sched_group_barrier(AT_MFMA, AHEAD, 1);
+  };
+  auto queries = [&]() {
     const unsigned short *src = q + (size_t)(t0 + (real ? i : 0)) * q_row + (size_t)(h * G + (real ? r - i * G : 0)) * D + 8 * hf;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) qf[ks] = *(const iu8_v4u *)(src + 16 * ks);
@@ -183,177 +336,157 @@ static __device__ __forceinline__ void attn_many_body(
       qf[ks] = (qf[ks] ^ flip) & (real ? ~0u : 0u);
       asm volatile("" : "+v"(qf[ks]));  // here, not in the loop, is what waits for them
     }
-  }
-  arrived();
-  int stage = 0;
-  for (int tile = begin; tile < end; tile += BK, stage ^= 1) {
-    const bool more = tile + BK < end;
-    const unsigned holes = holes_next;
-    if (more) {
-      holes_next = locate(tile + BK);
-      if constexpr (F8) fetch(kc);
-      else issue(stage ^ 1);
-      look_up(tile + 2 * BK);
-    }
-    unsigned char *sk = smem + stage * 2 * TILE, *sv = sk + TILE;
-    const bool special = holes || tile + BK > min(end, free_end);
-    int odd = 0;  // a value that is not finite among tokens that some rows see and others do not
-    if (special) {
-      constexpr int PR = ROWB / 16;  // pieces a row
-      const int stop = min(end - tile, BK), me = thread();
-      // what takes no part (rows behind the end, a hole's block): a weight of zero would keep its NaNs
-      for (int x = stop * PR + me; x < BK * PR; x += 256) *(iu8_v4u *)(sv + x * 16) = iu8_v4u{0, 0, 0, 0};
-      if (holes)
-        for (int x = me; x < BK * PR; x += 256)
-          if (holes >> (x / (16 * PR)) & 1) *(iu8_v4u *)(sv + x * 16) = iu8_v4u{0, 0, 0, 0};
-      for (int x = max(free_end - tile, 0) * PR + me; x < stop * PR; x += 256) {
-        const iu8_v4u v = *(const iu8_v4u *)(sv + x * 16);
-        if (holes >> (x / (16 * PR)) & 1) continue;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) odd |= at_nonfinite2(v[w]);
+  };
+
+  if constexpr (D == 256) {
+    // a tile at a time; the next one's K and V are on the way
+    unsigned holes_next = 0;
+    if (begin < end) {
+      look_up(begin);
+      holes_next = locate(begin);
+      if constexpr (F8) {
+        fetch(kc, at);
+        widen_k(0);
+        fetch(vc, at);
+        widen_v(0);
+      } else {
+        issue_k(0, at);
+        issue_v(0, at);
       }
-      odd = __syncthreads_or(odd);
+      look_up(begin + BK);
     }
-    // scores. (The products are read in the block that makes them: behind a branch this compiler leaves too few wait states
-    // between a matrix instruction and the first read of its result, seen as wrong scores.)
-    float st[HB][16];
-    {
-      at_v16f sc[HB];
-      iu8_v4u kf[HB][KS];
-      const unsigned char *ka = sk + k_lane();
-#pragma unroll
-      for (int hb = 0; hb < HB; ++hb)
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) kf[hb][ks] = *(const iu8_v4u *)(ka + hb * 32 * ROWB + ks * 512);
-#pragma unroll
-      for (int hb = 0; hb < HB; ++hb) {
-        sc[hb] = at_v16f{};
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) sc[hb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at_bf(kf[hb][ks]), at_bf(qf[ks]), sc[hb], 0, 0, 0);
-      }
-      // the order of issue: reads ahead of the products by a few (attn_few.h)
-      constexpr int AHEAD = D == 256 ? (F8 ? 2 : 3) : 4;
-      __builtin_amdgcn_sched_group_barrier(AT_DS_READ, AHEAD, 0);
-#pragma unroll
-      for (int x = 0; x < HB * KS - AHEAD; ++x) {
-        __builtin_amdgcn_sched_group_barrier(AT_MFMA, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(AT_DS_READ, 1, 0);
-      }
-      __builtin_amdgcn_sched_group_barrier(AT_MFMA, AHEAD, 0);
-#pragma unroll
-      for (int hb = 0; hb < HB; ++hb)
-#pragma unroll
-        for (int x = 0; x < 16; ++x) {
-          float y = sc[hb][x];
-          asm volatile("" : "+v"(y));
-          st[hb][x] = y;
-        }
-    }
-    if constexpr (F8) {
-      if (more) {
-        widen_k(stage ^ 1);
-        fetch(vc);
-      }
-    }
-    if (special) {
-      int ln = lane;
-      asm volatile("" : "+v"(ln));  // (what this rare block needs is made here and not kept across the loop)
-      const int last = min(s_limit[wave * 32 + (ln & 31)], end - 1) - tile - 4 * (ln >> 5);
-#pragma unroll
-      for (int hb = 0; hb < HB; ++hb)
-#pragma unroll
-        for (int x = 0; x < 16; ++x) {
-          const int t = 32 * hb + 8 * (x >> 2) + (x & 3);  // + 4 half
-          if (t > last || (holes >> (t >> 4) & 1)) st[hb][x] = -__builtin_inff();
-        }
-    }
-    float top = st[0][0];
-#pragma unroll
-    for (int hb = 0; hb < HB; ++hb)
-#pragma unroll
-      for (int x = 0; x < 16; ++x) top = fmaxf(top, st[hb][x]);
-    top = at_both<32>(top, at_max2);
-    // The maximum that the weights are taken against moves only when a score passes it by 2^8 or more (and at the first key): until
-    // then weights of up to 256 are as exact, and the sums' rescale is saved.
-    if (__any((top - m) * c > 8.f)) {
-      const float mn = fmaxf(m, top), f = __builtin_amdgcn_exp2f((m - (mn == -__builtin_inff() ? 0.f : mn)) * c);
-      l *= f;
-#pragma unroll
-      for (int x = 0; x < MT; ++x) o[x] *= f;
-      m = mn;
-    }
-    const float mc = m == -__builtin_inff() ? 0.f : m * c;
-    unsigned pf[HB][8];
-#pragma unroll
-    for (int hb = 0; hb < HB; ++hb)
-#pragma unroll
-      for (int x = 0; x < 16; x += 2) {
-        st[hb][x] = __builtin_amdgcn_exp2f(fmaf(st[hb][x], c, -mc));
-        st[hb][x + 1] = __builtin_amdgcn_exp2f(fmaf(st[hb][x + 1], c, -mc));
-        l += st[hb][x] + st[hb][x + 1];
-        pf[hb][x / 2] = iu8_bf16_pack(st[hb][x], st[hb][x + 1]);
-      }
-    if (odd) {  // these tokens' values by lane arithmetic, for the rows that see them; the product then finds zeros
-      int ln = lane;
-      asm volatile("" : "+v"(ln));
-      const int from = max(free_end - tile, 0), to = min(end - tile, BK), last = s_limit[wave * 32 + (ln & 31)] - tile;
-#pragma unroll
-      for (int hb = 0; hb < HB; ++hb)
-#pragma unroll 1
-        for (int t = max(from - 32 * hb, 0); t < min(to - 32 * hb, 32); ++t) {
-          unsigned w = pf[hb][0];
-          const int j = (t >> 3) * 4 + (t & 3), tt = t + 32 * hb;
-#pragma unroll
-          for (int x = 1; x < 8; ++x) w = j >> 1 == x ? pf[hb][x] : w;
-          const float pj = __shfl(__uint_as_float(j & 1 ? w & 0xFFFF0000u : w << 16), (ln & 31) + 32 * ((t >> 2) & 1));
-          if (tt <= last && !(holes >> (tt >> 4) & 1)) {
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-              for (int x = 0; x < 16; x += 4) {
-                float v[4];
-                at_four<false>(sv + tt * ROWB + ((4 * (mt ^ swz(tt)) + x / 4) * 16) + 8 * (ln >> 5), v);
-#pragma unroll
-                for (int r2 = 0; r2 < 4; ++r2) o[mt][x + r2] = fmaf(pj, v[r2], o[mt][x + r2]);
-              }
-          }
-        }
-      __syncthreads();
-      for (int x = thread(); x < BK * (ROWB / 16); x += 256)
-        if (x / (ROWB / 16) >= from) *(iu8_v4u *)(sv + x * 16) = iu8_v4u{0, 0, 0, 0};
-      __syncthreads();
-    }
-    {
-      constexpr int NP = MT * HB * 2;  // products, two reads each
-      unsigned va = (unsigned)(size_t)(__attribute__((address_space(3))) unsigned char *)sv + v_lane;
-      asm volatile("" : "+v"(va));  // (the addresses are made from it here: kept across the loop they would be registers that it lacks)
-      iu8_v2u vf[NP][2];
-#pragma unroll
-      for (int x = 0; x < NP; ++x) {
-        const int mt = x / (2 * HB), t16 = x % (2 * HB);
-        auto *pv = (__attribute__((address_space(3))) unsigned char *)(size_t)(va ^ (mt * 64)) + 16 * t16 * ROWB;
-        vf[x][0] = __builtin_bit_cast(iu8_v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) at_v4s *)pv));
-        vf[x][1] = __builtin_bit_cast(iu8_v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) at_v4s *)(pv + 8 * ROWB)));
-      }
-#pragma unroll
-      for (int x = 0; x < NP; ++x) {
-        const int mt = x / (2 * HB), t16 = x % (2 * HB);
-        const unsigned *w = &pf[t16 / 2][t16 % 2 * 4];
-        o[mt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at_bf(vf[x][0][0], vf[x][0][1], vf[x][1][0], vf[x][1][1]), at_bf(w[0], w[1], w[2], w[3]), o[mt], 0, 0, 0);
-      }
-      constexpr int AHEAD = D == 256 ? 2 : 3;
-      __builtin_amdgcn_sched_group_barrier(AT_DS_READ, 2 * AHEAD, 1);
-#pragma unroll
-      for (int x = 0; x < NP - AHEAD; ++x) {
-        __builtin_amdgcn_sched_group_barrier(AT_MFMA, 1, 1);
-        __builtin_amdgcn_sched_group_barrier(AT_DS_READ, 2, 1);
-      }
-      __builtin_amdgcn_sched_group_barrier(AT_MFMA, AHEAD, 1);
-    }
-    if constexpr (F8) {
-      if (more) widen_v(stage ^ 1);
-    }
+    queries();
     arrived();
+    int stage = 0;
+    for (int tile = begin; tile < end; tile += BK, stage ^= 1) {
+      const bool more = tile + BK < end;
+      const unsigned holes = holes_next;
+      if (more) {
+        holes_next = locate(tile + BK);
+        if constexpr (F8) {
+          fetch(kc, at);
+        } else {
+          issue_k(stage ^ 1, at);
+          issue_v(stage ^ 1, at);
+        }
+        look_up(tile + 2 * BK);
+      }
+      unsigned char *sk = smem + stage * 2 * TILE, *sv = sk + TILE;
+      const bool special = holes || tile + BK > min(end, free_end);
+      int odd = 0;
+      if (special) odd = clean(tile, holes, sv);
+      float st[HB][16];
+      {
+        at_v16f sc[HB];
+        scores(sk, sc);
+        order_scores();
+        settle(sc, st);
+      }
+      if constexpr (F8) {
+        if (more) {
+          widen_k(stage ^ 1);
+          fetch(vc, at);
+        }
+      }
+      if (special) hide(tile, holes, st);
+      const float mc = maximum(st);
+      unsigned pf[HB][8];
+      weights(st, mc, pf);
+      if (odd) by_lanes(tile, holes, sv, pf);
+      product(sv, pf);
+      if constexpr (F8) {
+        if (more) widen_v(stage ^ 1);
+      }
+      arrived();
+    }
+  } else {
+    // A tile's scores are made while the weights of the one before it are, in one block: matrix instructions and the
+    // exponentials' lane arithmetic side by side. K is a tile ahead of V: while tile j is weighed, K of j + 1 and V of j are here, K of
+    // j + 2 and V of j + 1 on the way.
+    unsigned holes = 0, holes_1 = 0, holes_2 = 0;
+    float st[2][HB][16];
+    if (begin < end) {
+      look_up(begin);
+      holes = locate(begin);
+      look_up(begin + BK);
+      if constexpr (F8) {
+        fetch(kc, at);
+        widen_k(0);
+        fetch(vc, at);
+        widen_v(0);
+      } else {
+        issue_k(0, at);
+        issue_v(0, at);
+      }
+      holes_1 = locate(begin + BK);
+      look_up(begin + 2 * BK);
+      if constexpr (F8) {
+        fetch(kc, at);
+        widen_k(1);
+      } else {
+        issue_k(1, at);
+      }
+    }
+    queries();
+    arrived();
+    if (begin < end) {
+      at_v16f sc[HB];
+      scores(smem, sc);
+      order_scores();
+      settle(sc, st[0]);
+    }
+    __syncthreads();
+    auto step = [&](int tile, int stage, float (&now_st)[HB][16], float (&next_st)[HB][16]) {
+      unsigned char *sv = smem + (stage * 2 + 1) * TILE;
+      const places at_v = at;  // V's, of the tile before K's
+      holes_2 = locate(tile + 2 * BK);
+      look_up(tile + 3 * BK);
+      const bool more = tile + BK < end, more_2 = tile + 2 * BK < end;
+      if constexpr (F8) {
+        if (more_2) fetch(kc, at);
+      } else {
+        if (more_2) issue_k(stage, at);
+        if (more) issue_v(stage ^ 1, at_v);
+      }
+      const bool special = holes || tile + BK > min(end, free_end);
+      int odd = 0;
+      if (special) {
+        odd = clean(tile, holes, sv);
+        hide(tile, holes, now_st);
+      }
+      const float mc = maximum(now_st);
+      unsigned pf[HB][8];
+      {
+        // (behind the last tile the scores are of whatever the stage holds, and not looked at)
+        at_v16f sc[HB];
+        scores(smem + (stage ^ 1) * 2 * TILE, sc);
+        weights(now_st, mc, pf);
+        constexpr int AHEAD = 4, NM = HB * KS, PER = (HB * 16 * 7 / 2 + NM - 1) / NM;
+        __builtin_amdgcn_sched_group_barrier(AT_DS_READ, AHEAD, 0);
+#pragma unroll
+        for (int x = 0; x < NM; ++x) {
+          __builtin_amdgcn_sched_group_barrier(AT_MFMA, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(AT_VALU, PER, 0);
+          if (x + AHEAD < NM) __builtin_amdgcn_sched_group_barrier(AT_DS_READ, 1, 0);
+        }
+        settle(sc, next_st);
+      }
+      if constexpr (F8) {
+        if (more_2) widen_k(stage);
+        if (more) fetch(vc, at_v);
+      }
+      if (odd) by_lanes(tile, holes, sv, pf);
+      product(sv, pf);
+      if constexpr (F8) {
+        if (more) widen_v(stage ^ 1);
+      }
+      holes = holes_1, holes_1 = holes_2;
+      arrived();
+    };
+    for (int tile = begin; tile < end; tile += 2 * BK) {
+      step(tile, 0, st[0], st[1]);
+      if (tile + BK < end) step(tile + BK, 1, st[1], st[0]);
+    }
   }
   l = at_both<32>(l, at_sum2);
   if (ns == 1) {
