@@ -608,11 +608,13 @@ int saber_iu8_kv_append(saber_iu8_ctx *ctx, const void *q, const void *k, const 
  * q rows `q_row` elements apart, heads head_dim apart; out bf16 [tokens, heads, head_dim]. A row that sees no key gives zeros; rows behind
  * the last sequence are left as they were. max_q: the most new rows of a sequence (rows past it are not computed); max_kv: what
  * kv_len is expected to reach, for the split of the cache's length alone (a longer one is right, and slower).
- * Up to 32 rows a kv head (new rows x group) run on the few-row kernels, which stream the cache; more on the many-row kernels,
- * 128 a workgroup. Both share the cache's length among workgroups where the grid would leave the card idle, with
- * the workspaces of saber_iu8_attn_workspace: `partial` (scratch) and `counter` (zeroed once, left zero); either NULL: in one piece.
- * Calls that share them must not overlap in time. Scores and sums in f32, the softmax's weights rounded to bf16 for the
- * second product, the output rounded once; the same bytes on every run of one plan. Asynchronous. */
+ * Up to 32 rows a kv head (new rows x group), and somewhat more on a long cache, run on the few-row kernels, which stream the
+ * cache; the rest on the many-row kernels, 128 rows a workgroup. Both share the cache's length among workgroups where the grid would
+ * leave the card idle, with the workspaces of saber_iu8_attn_workspace: `partial` (scratch) and `counter` (zeroed once, left zero);
+ * either NULL: in one piece. Workspaces made for (seqs, max_q, max_kv) hold every call of the same heads with at most these,
+ * on a cache of either kind. Calls that share them must not overlap in time. Scores and sums in f32, the softmax's weights rounded to
+ * bf16 for the second product, the output rounded once; the same bytes on every run of one plan. Values that are not finite stay in
+ * the rows that see them. q may be anywhere but in `out`. Asynchronous. */
 int saber_iu8_attn_workspace(uint32_t seqs, uint32_t max_q, uint32_t max_kv, uint32_t heads, uint32_t kv_heads, uint32_t head_dim,
                              uint64_t *partial_bytes, uint64_t *counter_bytes);
 int saber_iu8_attn(saber_iu8_ctx *ctx, const void *q, uint32_t q_row, const saber_iu8_kv_cache *cache, const int32_t *cu_q, void *out, uint32_t tokens,

@@ -16,6 +16,8 @@ constexpr uint32_t FEW_ROWS = 32;    // rows a kv head and sequence up to which 
 constexpr uint32_t MANY_ROWS = 128;  // rows a workgroup of the many-row kernels
 constexpr int FEW_UNIT_SHIFT = 7, WHOLE_SHIFT = 31;  // log2 of the tokens a unit of the few-row kernels' deal (attn_few.h)
 constexpr uint32_t MANY_PARTS = 32;  // parts of an item at most: their maxima and sums lie in one workgroup's LDS when they are joined
+constexpr uint64_t FEW_UNITS_MIN = 8, FEW_UNITS_MAX = 5 * CU_COUNT;  // more than 32 rows on the few-row kernels: units a row tile from, units of all up to
+constexpr uint64_t MANY_TARGET = 2 * CU_COUNT, MANY_LEAST = 512;     // workgroups that the parts aim at, tokens a part from
 constexpr uint32_t I32_MAX = 0x7FFFFFFFu;
 constexpr uint32_t WHOLE = 0x7FFFFF00u;  // a part that holds any sequence: the positions a table's row may reach
 
@@ -67,7 +69,7 @@ Plan plan(uint32_t seqs, uint32_t max_q, uint32_t max_kv, uint32_t heads, uint32
   Plan p{};
   const uint64_t rows = (uint64_t)max_q * (heads / kv_heads), units = max_kv ? ((max_kv - 1) >> FEW_UNIT_SHIFT) + 1 : 1;
   const uint64_t all32 = (uint64_t)seqs * kv_heads * ((rows + FEW_ROWS - 1) / FEW_ROWS) * units;
-  p.rows = rows <= 16 ? 16 : rows <= FEW_ROWS || (!whole && units >= 8 && all32 <= 5 * CU_COUNT) ? FEW_ROWS : MANY_ROWS;
+  p.rows = rows <= 16 ? 16 : rows <= FEW_ROWS || (!whole && units >= FEW_UNITS_MIN && all32 <= FEW_UNITS_MAX) ? FEW_ROWS : MANY_ROWS;
   p.qtiles = (rows + p.rows - 1) / p.rows;
   p.items = (uint64_t)seqs * kv_heads * p.qtiles;
   p.splits = 1, p.chunk = WHOLE, p.unit_shift = WHOLE_SHIFT;
@@ -82,8 +84,7 @@ Plan plan(uint32_t seqs, uint32_t max_q, uint32_t max_kv, uint32_t heads, uint32
     if (split) p.partial = p.grid * 2 * p.rows * (dim + 4) * 4, p.counter = p.items * 4;
     return p;
   }
-  const uint64_t target = 2 * CU_COUNT, least = 512;
-  const uint64_t parts = std::min<uint64_t>({std::max<uint64_t>(1, target / p.items), MANY_PARTS, std::max<uint64_t>(1, (max_kv + least - 1) / least)});
+  const uint64_t parts = std::min<uint64_t>({std::max<uint64_t>(1, MANY_TARGET / p.items), MANY_PARTS, std::max<uint64_t>(1, (max_kv + MANY_LEAST - 1) / MANY_LEAST)});
   if (!whole && parts > 1) {
     p.chunk = (uint32_t)(((max_kv + parts - 1) / parts + 127) / 128 * 128);
     p.splits = (max_kv + p.chunk - 1) / p.chunk;
@@ -93,11 +94,28 @@ Plan plan(uint32_t seqs, uint32_t max_q, uint32_t max_kv, uint32_t heads, uint32
   return p;
 }
 
+// What the plan of any call of up to these sizes takes, caches of either kind: fewer sequences or shorter ones may be cut into more
+// parts, and a server allocates once. Few rows: two slots a workgroup, at most 512 of 16 rows or 256 of 32; many: a slot a
+// workgroup, at most 512.
+void workspace(uint64_t seqs, uint64_t max_q, uint64_t max_kv, uint64_t group, uint64_t kv_heads, uint64_t dim, uint64_t *partial, uint64_t *counter) {
+  const uint64_t rows = max_q * group, units = max_kv ? ((max_kv - 1) >> FEW_UNIT_SHIFT) + 1 : 1, row = (dim + 4) * 4;
+  auto want = [&](uint64_t items, uint64_t slots, uint64_t a_slot) { *partial = std::max(*partial, slots * a_slot * row), *counter = std::max(*counter, items * 4); };
+  if (units < 2) return;
+  if (group <= 16) want(seqs * kv_heads, std::min<uint64_t>(2 * CU_COUNT, seqs * kv_heads * units), 2 * 16);
+  if (rows > 16) {
+    const uint64_t items = std::max(seqs * kv_heads, std::min<uint64_t>(seqs * kv_heads * ((rows + FEW_ROWS - 1) / FEW_ROWS), FEW_UNITS_MAX / FEW_UNITS_MIN));
+    want(items, std::min<uint64_t>(CU_COUNT, items * units), 2 * FEW_ROWS);
+  }
+  const uint64_t items = seqs * kv_heads * ((rows + MANY_ROWS - 1) / MANY_ROWS), parts = std::min<uint64_t>(MANY_PARTS, (max_kv + MANY_LEAST - 1) / MANY_LEAST);
+  if (rows > FEW_ROWS && parts > 1) want(std::min(items, MANY_TARGET / 2), std::min(items * parts, MANY_TARGET), MANY_ROWS);
+}
+
 int attn_plan(const char *op, uint32_t seqs, uint32_t max_q, uint32_t max_kv, uint32_t heads, uint32_t kv_heads, uint32_t dim, bool f8, bool whole, uint64_t held, Plan *p) {
   if (!max_q || max_kv > I32_MAX) return fail(SABER_IU8_E_RULE, fmt("%s: at most %u new rows and %u keys a sequence: from 1 and below 2^31", op, max_q, max_kv));
-  *p = plan(seqs, max_q, max_kv, heads, kv_heads, dim, f8, whole, held);
-  if ((uint64_t)max_q * (heads / kv_heads) > I32_MAX || p->items > I32_MAX || p->grid > I32_MAX)
+  const uint64_t rows = (uint64_t)max_q * (heads / kv_heads);
+  if (rows > I32_MAX || (__int128)seqs * kv_heads * ((rows + MANY_ROWS - 1) / MANY_ROWS) > (int64_t)I32_MAX)
     return fail(SABER_IU8_E_RULE, fmt("%s: %u sequences of up to %u new rows and %u heads pass a launch's 32-bit sizes", op, seqs, max_q, heads));
+  *p = plan(seqs, max_q, max_kv, heads, kv_heads, dim, f8, whole, held);
   return 0;
 }
 
@@ -230,14 +248,12 @@ int saber_iu8_kv_append(saber_iu8_ctx *ctx, const void *q, const void *k, const 
 
 int saber_iu8_attn_workspace(uint32_t seqs, uint32_t max_q, uint32_t max_kv, uint32_t heads, uint32_t kv_heads, uint32_t head_dim,
                              uint64_t *partial_bytes, uint64_t *counter_bytes) {
-  if (!seqs || !heads || !kv_heads || heads % kv_heads || (head_dim != 64 && head_dim != 128 && head_dim != 256))
+  if (!seqs || !heads || !kv_heads || heads % kv_heads || heads > 0xFFFF || kv_heads > 0x7FFF || (head_dim != 64 && head_dim != 128 && head_dim != 256))
     return fail(SABER_IU8_E_RULE, fmt("attn_workspace: %u sequences of %u heads over %u kv heads of %u", seqs, heads, kv_heads, head_dim));
+  Plan p;
+  if (int rc = attn_plan("attn_workspace", seqs, max_q, max_kv, heads, kv_heads, head_dim, false, false, max_kv, &p)) return rc;
   uint64_t partial = 0, counter = 0;
-  for (bool f8 : {false, true}) {  // enough for a cache of either kind
-    Plan p;
-    if (int rc = attn_plan("attn_workspace", seqs, max_q, max_kv, heads, kv_heads, head_dim, f8, false, max_kv, &p)) return rc;
-    partial = std::max(partial, p.partial), counter = std::max(counter, p.counter);
-  }
+  workspace(seqs, max_q, max_kv, heads / kv_heads, kv_heads, head_dim, &partial, &counter);
   if (partial_bytes) *partial_bytes = partial;
   if (counter_bytes) *counter_bytes = counter;
   return 0;

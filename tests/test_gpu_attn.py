@@ -6,9 +6,11 @@ import numpy as np
 import pytest
 import torch
 
-from saber_engine_amd import iu8
+from oracle import ref
+from saber_engine_amd import iu8, synth
+from saber_engine_amd.attn import AttnLayerIU8, PagedKvCache
 from tests.attn_util import BF16, E4M3, Paged, Workspace, attention, check, f64, random_rows
-from tests.gpu_util import say
+from tests.gpu_util import dev_bf16_bits, dev_f32, dev_u8, host_u16, say
 
 pytestmark = pytest.mark.gpu
 
@@ -198,7 +200,7 @@ def attn_case(ctx, dim, heads, kvh, lens, news, page=64, e4m3=False, packed=True
     return c, q, out
 
 
-KINDS = [(64, 8, 8), (64, 14, 2), (128, 5, 1), (128, 16, 1), (256, 12, 2), (256, 4, 4)]
+KINDS = [(64, 8, 8), (64, 14, 2), (128, 5, 1), (128, 16, 1), (256, 10, 2), (256, 4, 4)]
 
 
 @pytest.mark.parametrize("e4m3", [False, True])
@@ -225,7 +227,7 @@ def test_attn_many_rows(ctx, dim, heads, kvh, e4m3):
 
 @pytest.mark.parametrize("split", [False, True])
 @pytest.mark.parametrize("dim,heads,kvh,lens,news", [
-    (128, 5, 1, [3001, 129, 5], [1, 1, 1]), (256, 6, 1, [4099], [5]), (64, 4, 1, [2600, 700], [40, 50]), (256, 12, 2, [1900], [90]), (128, 16, 2, [1500], [64])])
+    (128, 5, 1, [3001, 129, 5], [1, 1, 1]), (256, 6, 1, [4099], [5]), (64, 4, 1, [2600, 700], [40, 50]), (256, 10, 2, [1900], [90]), (128, 16, 2, [1500], [64])])
 def test_attn_split_over_the_cache(ctx, dim, heads, kvh, lens, news, split):
     say(f"attn, split {dim} {heads} {kvh} {lens} {news} {split}")
     assert iu8.attn_workspace(len(lens), max(news), max(lens), heads, kvh, dim)[0] > 0
@@ -290,3 +292,264 @@ def test_attn_values_that_are_not_finite_where_a_row_does_not_look(ctx, dim, hea
     want, tol = attention(f64(q[:last].float()).reshape(last, heads, dim), k, v, there, 1 / math.sqrt(dim))
     check(f64(out[:last].float()), want, tol, "rows before the NaN")
     assert torch.isnan(out[last]).all()
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("most_new", [1, 3])
+def test_attn_among_many_sequences(ctx, most_new, e4m3):
+    """More sequences than a wave has lanes, ragged, idle ones and empty ones among them: the deal of the units."""
+    say(f"attn, 150 sequences of up to {most_new} rows {e4m3}")
+    rng = np.random.default_rng(most_new)
+    lens = [int(x) for x in rng.integers(0, 500, 150)]
+    news = [int(x) for x in rng.integers(0, most_new + 1, 150)]
+    lens[7], news[7], lens[149], news[149], news[0] = 0, most_new, 3, 2, 0
+    attn_case(ctx, 64, 4, 2, lens, news, page=32, e4m3=e4m3, behind=1)
+
+
+@pytest.mark.parametrize("dim,heads,kvh,total,new", [(64, 4, 1, 40000, 1), (64, 20, 1, 30000, 1), (64, 8, 2, 20000, 40), (128, 2, 1, 16500, 1)])
+def test_attn_as_many_parts_as_a_join_holds(ctx, dim, heads, kvh, total, new):
+    say(f"attn, one long sequence {dim} {heads} {kvh} {total} {new}")
+    attn_case(ctx, dim, heads, kvh, [total], [new], page=256)
+
+
+@pytest.mark.parametrize("dim,heads,kvh,total,new", [(64, 5, 1, 1500, 9), (128, 4, 2, 2100, 33), (256, 6, 1, 1100, 15)])
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_attn_row_tiles_of_the_few_row_kernels(ctx, dim, heads, kvh, total, new, e4m3):
+    say(f"attn, {new} rows of group {heads // kvh} behind {total} keys {e4m3}")
+    attn_case(ctx, dim, heads, kvh, [total, 40, 1300], [new, new - 1, 1], e4m3=e4m3)
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_attn_lengths_around_a_tile(ctx, dim, e4m3):
+    """Prompts that end one before, at and behind a tile (32 and 64 tokens), a row tile (128 rows) and a page."""
+    say(f"attn, lengths around a tile {dim} {e4m3}")
+    lens = [31, 32, 33, 63, 64, 65, 127, 128, 129, 191, 193]
+    attn_case(ctx, dim, 2, 1, lens, lens, page=16, e4m3=e4m3)
+    attn_case(ctx, dim, 2, 1, [x + 100 for x in lens], lens, page=128, e4m3=e4m3)
+
+
+def test_attn_one_workspace_for_every_smaller_call(ctx):
+    """Workspaces of the largest call, smaller ones in them, with what lies behind them looked at."""
+    say("attn, shared workspaces")
+    heads, kvh, dim, seqs, most = 4, 2, 64, 6, 4000
+    pb, cb = iu8.attn_workspace(seqs, 70, most, heads, kvh, dim)
+    partial, counter = torch.full((pb // 4 + 64,), 3.0, device="cuda"), torch.zeros(cb // 4 + 64, dtype=torch.int32, device="cuda")
+    counter[cb // 4:] = 5
+    g = torch.Generator().manual_seed(8)
+    c = Paged(seqs, kvh, dim, 64, most, fill=0.0)
+    for s in range(seqs):
+        c.put(s, 0, random_rows(g, most, kvh, dim), random_rows(g, most, kvh, dim))
+    for n_seqs, new, total in ((6, 70, 4000), (1, 1, 4000), (6, 1, 4000), (2, 9, 3000), (1, 70, 4000), (3, 40, 700), (6, 5, 129), (1, 33, 2000)):
+        c.kv_len[:n_seqs] = total
+        tokens = n_seqs * new
+        q, out = random_rows(g, tokens, heads * dim), torch.zeros(tokens, heads, dim, dtype=torch.bfloat16, device="cuda")
+        ctx.attn(q.data_ptr(), heads * dim, c.desc(), ends([new] * n_seqs).data_ptr(), out.data_ptr(), tokens, n_seqs, new, total, heads, 0.125,
+                 partial.data_ptr(), counter.data_ptr())
+        torch.cuda.synchronize()
+        assert (partial[pb // 4:] == 3).all() and (counter[cb // 4:] == 5).all() and not counter[:cb // 4].any(), (n_seqs, new, total)
+        s = n_seqs - 1
+        k, v, there = c.rows(s, total)
+        want, tol = attention(f64(q[-new:].float()).reshape(new, heads, dim), k, v, there, 0.125)
+        check(f64(out[-new:].float()), want, tol, f"{n_seqs} sequences of {new} rows on {total}")
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_cache_past_four_gibibytes(ctx, new):
+    """A pool of pages whose byte offsets pass 32 bits: append into its far end, attention over it."""
+    say(f"cache of 5 GiB, {new} new rows")
+    heads, kvh, dim, page, total, pages = 4, 1, 256, 256, 900, 40000
+    g = torch.Generator().manual_seed(9)
+    c = Paged(1, kvh, dim, page, total, pages=pages, fill=0.0)
+    c.table[0] = torch.tensor([pages - 1, 3, 33000, pages - 2])
+    assert iu8.kv_bytes(pages, kvh, dim, page) > 1 << 32
+    c.put(0, 0, random_rows(g, total - new, kvh, dim), random_rows(g, total - new, kvh, dim))
+    c.kv_len[0] = total
+    row = heads * dim + 2 * dim
+    x, q = random_rows(g, new, row), torch.zeros(new, heads, dim, dtype=torch.bfloat16, device="cuda")
+    out, cu, p, ws = torch.zeros_like(q), ends([new]), x.data_ptr(), Workspace(1, new, total, heads, kvh, dim)
+    ctx.kv_append(p, p + 2 * heads * dim, p + 2 * (heads + 1) * dim, q.data_ptr(), c.desc(), cu.data_ptr(), new, 1, heads, row, dim, row)
+    ctx.attn(q.data_ptr(), heads * dim, c.desc(), cu.data_ptr(), out.data_ptr(), new, 1, new, total, heads, 1 / 16,
+             *ws.args())
+    torch.cuda.synchronize()
+    assert torch.equal(q.view(new, -1), x[:, :heads * dim])
+    k, v, there = c.rows(0, total)
+    src = f64(x.float())
+    assert np.array_equal(k[-new:, 0], src[:, heads * dim:-dim]) and np.array_equal(v[-new:, 0], src[:, -dim:])
+    want, tol = attention(f64(q.float()), k, v, there, 1 / 16)
+    check(f64(out.float()), want, tol, "rows on far pages")
+
+
+def test_append_in_place(ctx):
+    say("append: q_out is q")
+    heads, kvh, dim, n = 6, 2, 128, 9
+    freq = torch.tensor([1e4 ** (-i / 32) for i in range(32)], dtype=torch.float64).cuda()
+    got = []
+    for in_place in (False, True):
+        c = Paged(1, kvh, dim, 32, n, fill=0.0)
+        c.kv_len[0] = n
+        q, kv = random_rows(torch.Generator().manual_seed(5), n, heads * dim), random_rows(torch.Generator().manual_seed(6), n, 2 * kvh * dim)
+        to = q if in_place else torch.zeros_like(q)
+        ctx.kv_append(q.data_ptr(), kv.data_ptr(), kv.data_ptr() + 2 * kvh * dim, to.data_ptr(), c.desc(), ends([n]).data_ptr(), n, 1, heads, heads * dim, dim,
+                      2 * kvh * dim, freq.data_ptr(), 64)
+        torch.cuda.synchronize()
+        got.append((to, c.k, c.v))
+    assert all(torch.equal(a.view(torch.int16), b.view(torch.int16)) for a, b in zip(*got))
+
+
+# ------------------------------------------------------------------ the run of them
+
+def layer(ctx, cache, tokens, max_q, gated, heads, hidden, weights, freq, **more):
+    n = AttnLayerIU8(ctx, cache, tokens, heads, hidden, max_q=max_q, gated=gated, inv_freq=freq, **more)
+    n.set_weights(*weights)
+    return n
+
+
+def layer_weights(heads, kvh, dim, hidden, gated, seed):
+    n_core, n_qkv = heads * dim, heads * dim * (2 if gated else 1) + 2 * kvh * dim
+    a, b = synth.dense_case(1, n_qkv, hidden, seed=seed), synth.dense_case(1, hidden, n_core, seed=seed + 1)
+    rng = np.random.default_rng(seed + 2)
+    t = rng.choice([-1.0, 1.0], size=n_core).astype(np.float32)
+    norms = [torch.from_numpy(rng.standard_normal(dim).astype(np.float32) * 0.2).bfloat16().cuda() for _ in range(2)]
+    host = dict(qkv=a, o=b, t=t, norms=norms)
+    return host, (dev_u8(iu8.repack_w4(a["W"])), dev_f32(a["ws"]), dev_u8(iu8.repack_w4(b["W"])), dev_f32(b["ws"]), dev_f32(t) if gated else None, *norms)
+
+
+def check_layer(n, host, x, news, before, kv):
+    """Every step of a call from the one before it: the linears' bytes are the oracle's, what lies between them within the rounding."""
+    cache, T, D = n.cache, n.T, n.cache.head_dim
+    live = sum(news)
+    qkv = host_u16(n.qkv)
+    np.testing.assert_array_equal(qkv, ref.linear(x, host["qkv"]["W"], host["qkv"]["ws"], False, threads=8)["C"])
+    rows = f64(n.qkv.view(torch.bfloat16).float())
+    fr = f64(n.inv_freq)
+    q = f64(n.q.view(torch.bfloat16).float()).reshape(T, n.heads, D)
+    core = f64(n.core.view(torch.bfloat16).float()).reshape(T, n.heads, D)
+    t = 0
+    for s, new in enumerate(news):
+        total = before[s] + new
+        k, v, there = kv.rows(s, total)
+        if new:
+            pos = np.arange(before[s], total)
+            x0 = rows[t:t + new]
+            wq = normed(np.stack([x0[:, h * n.q_head:h * n.q_head + D] for h in range(n.heads)], 1), host["norms"][0], n.eps)
+            wk = normed(x0[:, n.heads * n.q_head:][:, :kv.h * D].reshape(new, kv.h, D), host["norms"][1], n.eps)
+            slack = lambda y: 1.5e-5 * (np.abs(y).max(-1, keepdims=True) + 1e-30)  # noqa: E731
+            for got, want in ((q[t:t + new], wq), (k[before[s]:], wk)):
+                turned = rotated(want, pos, fr, 2 * len(fr), n.interleaved)
+                check(got, turned, np.abs(turned) * BF16 * 1.01 + slack(want), f"sequence {s}")
+            assert np.array_equal(v[before[s]:], x0[:, n.heads * n.q_head + kv.h * D:].reshape(new, kv.h, D))
+            want, tol = attention(q[t:t + new], k, v, there, n.scale)
+            check(core[t:t + new], want, tol, f"attention of sequence {s}")
+        t += new
+    bits = host_u16(n.core).reshape(T, -1)[:live]
+    if n.gated:
+        codes, scales = ref.attn_gate_quant_had(bits, qkv[:live], host["t"], D)
+        S, _ = ref.gemm_fast(codes, host["o"]["W"], False, threads=8)
+        want = ref.epilogue(S, scales, host["o"]["ws"], False)
+    else:
+        want = ref.linear(bits, host["o"]["W"], host["o"]["ws"], False, threads=8)["C"]
+    np.testing.assert_array_equal(host_u16(n.out)[:live], want)
+
+
+class Rows:
+    """PagedKvCache's rows as attn_util's Paged gives them."""
+
+    def __init__(self, c):
+        self.h, d, page = c.kv_heads, c.head_dim, c.page_tokens
+        self.p = Paged.__new__(Paged)
+        self.p.h, self.p.dim, self.p.page, self.p.e4m3, self.p.e, self.p.pages, self.p.kind, self.p.table = self.h, d, page, False, 8, c.pages, torch.bfloat16, c.table
+        self.p.k = c.k.view(torch.bfloat16).view(c.pages, self.h, page // 16, d // 8, 16, 8)
+        self.p.v = c.v.view(torch.bfloat16).view(c.pages, self.h, page, d)
+
+    def rows(self, s, n):
+        return self.p.rows(s, n)
+
+
+@pytest.mark.parametrize("gated,heads,kvh,dim,hidden,interleaved", [(True, 4, 1, 256, 512, False), (False, 8, 2, 128, 256, True)])
+def test_layer_prompts_then_single_tokens(ctx, gated, heads, kvh, dim, hidden, interleaved):
+    """Packed prompts of ragged lengths, a chunk behind them, then decode steps captured once and replayed while the counts and the page
+    table change and eager work runs between; a prompt train of another graph beside it."""
+    say(f"attention layer, gated {gated}, {heads} heads of {dim}")
+    rng = np.random.default_rng(dim)
+    host, weights = layer_weights(heads, kvh, dim, hidden, gated, 40 + dim)
+    freq = torch.tensor([1e6 ** (-i / 32) for i in range(32)], dtype=torch.float64).cuda()
+    cache = PagedKvCache(3, kvh, dim, 600, page_tokens=32)
+    kv = Rows(cache)
+    lens = [0, 0, 0]
+
+    def prompt(news, T):
+        n = layer(ctx, cache, T, max(news), gated, heads, hidden, weights, freq, interleaved=interleaved)
+        x = synth.activations(rng, T, hidden)
+        n.cu_q.copy_(ends(news))
+        before = list(lens)
+        for s, new in enumerate(news):
+            lens[s] += new
+            cache.reserve(s, lens[s])
+        cache.kv_len.copy_(torch.tensor(lens))
+        n.forward(dev_bf16_bits(x))
+        torch.cuda.synchronize()
+        check_layer(n, host, x, news, before, kv)
+
+    prompt([70, 0, 200], 272)
+    prompt([30, 129, 5], 164)
+    n = layer(ctx, cache, 3, 1, gated, heads, hidden, weights, freq, interleaved=interleaved)
+    x_dev = torch.zeros((3, hidden), dtype=torch.int16, device="cuda")
+    stream, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g, stream=stream):
+        n.forward(x_dev, stream.cuda_stream)
+    for step in range(4):
+        if step == 2:                     # a sequence leaves, another takes its pages and its place
+            cache.release(0)
+            lens[0] = 0
+        before = list(lens)
+        for s in range(3):
+            lens[s] += 1
+            cache.reserve(s, lens[s])
+        cache.kv_len.copy_(torch.tensor(lens))
+        x = synth.activations(rng, 3, hidden)
+        x_dev.copy_(dev_bf16_bits(x))
+        n.core.fill_(0x7FC0)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            g.replay()
+        torch.cuda.synchronize()
+        check_layer(n, host, x, [1, 1, 1], before, kv)
+        assert n._attn_ws[1] is None or not n._attn_ws[1].any()
+
+
+def test_two_captured_trains_at_once(ctx):
+    """Two graphs, each with its own cache and workspaces, replayed on two streams at once: the bytes of each by itself."""
+    say("two captured attention layers at once")
+    heads, kvh, dim, hidden = 8, 2, 64, 256
+    host, weights = layer_weights(heads, kvh, dim, hidden, False, 90)
+    freq = torch.tensor([1e4 ** (-i / 16) for i in range(16)], dtype=torch.float64).cuda()
+    trains = []
+    for i in range(2):
+        cache = PagedKvCache(2, kvh, dim, 3000, page_tokens=64)
+        for s in range(2):
+            cache.reserve(s, 3000)
+        gen = torch.Generator().manual_seed(i)
+        for t in (cache.k, cache.v):
+            t.view(torch.bfloat16).copy_(torch.randn(t.numel() // 2, generator=gen))
+        cache.kv_len.copy_(torch.tensor([2900 + i, 1700]))
+        n = layer(ctx, cache, 2, 1, False, heads, hidden, weights, freq)
+        x = dev_bf16_bits(synth.activations(np.random.default_rng(i), 2, hidden))
+        n.forward(x)
+        torch.cuda.synchronize()
+        want, core = n.out.clone(), n.core.clone()
+        stream, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            n.forward(x, stream.cuda_stream)
+        trains.append((n, x, want, core, stream, g))
+    for rep in range(4):
+        for n, *_ in trains:
+            n.out.zero_(), n.core.zero_()
+        torch.cuda.synchronize()
+        for *_, stream, g in trains:
+            with torch.cuda.stream(stream):
+                g.replay()
+        torch.cuda.synchronize()
+        for n, _, want, core, *_ in trains:
+            assert torch.equal(n.out, want) and torch.equal(n.core, core) and want.any(), rep
