@@ -17,7 +17,7 @@ constexpr uint32_t MANY_ROWS = 128;  // rows a workgroup of the many-row kernels
 constexpr int FEW_UNIT_SHIFT = 7, WHOLE_SHIFT = 31;  // log2 of the tokens a unit of the few-row kernels' deal (attn_few.h)
 constexpr uint32_t MANY_PARTS = 32;  // parts of an item at most: their maxima and sums lie in one workgroup's LDS when they are joined
 constexpr uint64_t FEW_UNITS_MIN = 8, FEW_UNITS_MAX = 5 * CU_COUNT;  // more than 32 rows on the few-row kernels: units a row tile from, units of all up to
-constexpr uint64_t MANY_TARGET = 2 * CU_COUNT, MANY_LEAST = 512;     // workgroups that the parts aim at, tokens a part from
+constexpr uint64_t MANY_TARGET = 2 * CU_COUNT, MANY_LEAST = 320, MANY_LONG = 2048;  // workgroups that parts aim at, at most; tokens a part, from; long ones
 constexpr uint32_t I32_MAX = 0x7FFFFFFFu;
 constexpr uint32_t WHOLE = 0x7FFFFF00u;  // a part that holds any sequence: the positions a table's row may reach
 
@@ -57,19 +57,21 @@ struct Plan {
 };
 
 // Which kernels, and the grid. Few rows (attn_few.h) up to 32 a kv head and sequence; above, still where a long cache meets so
-// few rows that its tiles of 32 make at most five units a CU -- 40 new tokens of group 6 on 4,000 keys, head width 256, 30 us
-// against 51 of the many-row kernel; 100 on 8,000 (19 units a CU) 119 against 71; 40 of group 5 on 4,000, width 128 (7) 32.5 / 32.3.
-// Their grid: the workgroups that the card holds at once (by their LDS: two a CU, or one), which deal the units level; three
-// quarters of the CUs where each then has 16 units and more (131,072 keys, 4 kv heads of 256: 192 workgroups 93 us, 256 96; 64
-// sequences of up to 8,192, 8 heads of 128: 199 against 203 of 512).
-// Many rows: parts of at least 512 tokens where the row tiles alone are fewer than two workgroups a CU (512 rows of group 6
-// on 16,896 keys: one part 1,140 us, five 281).
+// few rows that its tiles of 32 make at most a unit a CU (60 new tokens of group 6 on 300 keys, head width 256: 19.7 us against 21.2 of
+// the many-row kernel; 60 on 600 24.6 / 31.7; 60 of group 5 on 300, width 128, 13.3 / 16.3 -- but not whole prompts of one or two units, half of
+// which is masked: 200 on 200, 20.9 / 17.9) or, on eight units and more, five a CU (200 of group 6 on 1,000 35 / 45; on 1,600, at eight
+// a CU, 56 / 44). Their grid: the workgroups that the card holds at once (by their LDS: two a CU, or one), which deal the units
+// level; three quarters of the CUs where each then has 16 units and more (131,072 keys, 4 kv heads of 256: 192 workgroups 92 us,
+// 256 96; 64 sequences of up to 8,192, 8 heads of 128: 199 against 203 of 512).
+// Many rows: parts where the row tiles alone are fewer than the CUs, one workgroup a CU (400 rows of group 6, 76 tiles, on 3,000 keys:
+// one part 112 us, three 62, four 68, six 69 to 85), two a CU where the parts are long (512 rows, 96 tiles, on 16,896: two parts
+// 395 us, five 248 to 271).
 // `whole`: no workspaces, every item in one piece; `held`: the tokens that a sequence's row of the page table can hold.
 Plan plan(uint32_t seqs, uint32_t max_q, uint32_t max_kv, uint32_t heads, uint32_t kv_heads, uint32_t dim, bool f8, bool whole, uint64_t held) {
   Plan p{};
   const uint64_t rows = (uint64_t)max_q * (heads / kv_heads), units = max_kv ? ((max_kv - 1) >> FEW_UNIT_SHIFT) + 1 : 1;
   const uint64_t all32 = (uint64_t)seqs * kv_heads * ((rows + FEW_ROWS - 1) / FEW_ROWS) * units;
-  p.rows = rows <= 16 ? 16 : rows <= FEW_ROWS || (!whole && units >= FEW_UNITS_MIN && all32 <= FEW_UNITS_MAX) ? FEW_ROWS : MANY_ROWS;
+  p.rows = rows <= 16 ? 16 : rows <= FEW_ROWS || (!whole && ((units >= FEW_UNITS_MIN && all32 <= FEW_UNITS_MAX) || (units >= 3 && all32 <= CU_COUNT))) ? FEW_ROWS : MANY_ROWS;
   p.qtiles = (rows + p.rows - 1) / p.rows;
   p.items = (uint64_t)seqs * kv_heads * p.qtiles;
   p.splits = 1, p.chunk = WHOLE, p.unit_shift = WHOLE_SHIFT;
@@ -84,7 +86,9 @@ Plan plan(uint32_t seqs, uint32_t max_q, uint32_t max_kv, uint32_t heads, uint32
     if (split) p.partial = p.grid * 2 * p.rows * (dim + 4) * 4, p.counter = p.items * 4;
     return p;
   }
-  const uint64_t parts = std::min<uint64_t>({std::max<uint64_t>(1, MANY_TARGET / p.items), MANY_PARTS, std::max<uint64_t>(1, (max_kv + MANY_LEAST - 1) / MANY_LEAST)});
+  uint64_t parts = std::max<uint64_t>(1, CU_COUNT / p.items);
+  if (max_kv > MANY_LONG * parts) parts = std::max<uint64_t>(1, MANY_TARGET / p.items);
+  parts = std::min<uint64_t>({parts, MANY_PARTS, std::max<uint64_t>(1, (max_kv + MANY_LEAST - 1) / MANY_LEAST)});
   if (!whole && parts > 1) {
     p.chunk = (uint32_t)(((max_kv + parts - 1) / parts + 127) / 128 * 128);
     p.splits = (max_kv + p.chunk - 1) / p.chunk;

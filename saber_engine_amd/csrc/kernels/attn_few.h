@@ -44,7 +44,7 @@ static __device__ __forceinline__ int at_chunk(int len, int chunk, int splits) {
 // row (one 16-byte store); rows r < live go out. The parts come from memory (other XCDs wrote them), so as many loads as registers allow are
 // in flight, U items x K parts a thread, the first of them beside the (m, l). `s_f`: ns * live floats of LDS; ns at most 128 (R = 128: 32).
 template <int D, int R, int T, int U, int K>
-static __device__ __forceinline__ void at_join(const float *__restrict__ part, size_t first, size_t step, int ns, int live, float vs, int tid,
+static __device__ __forceinline__ void at_join_of(const float *__restrict__ part, size_t first, size_t step, int ns, int live, float vs, int tid,
                                                unsigned short *__restrict__ out, const long long *s_dst, float *s_il, float *s_f) {
   constexpr int D4 = D / 4, NI = (R * D4 + T - 1) / T;
   const int all = live * D4;
@@ -120,6 +120,14 @@ static __device__ __forceinline__ void at_join(const float *__restrict__ part, s
   }
 }
 
+template <int D, int R, int T, int U, int K>
+static __device__ __forceinline__ void at_join(const float *__restrict__ part, size_t first, size_t step, int ns, int live, float vs, int tid,
+                                               unsigned short *__restrict__ out, const long long *s_dst, float *s_il, float *s_f) {
+  if (ns <= 2) at_join_of<D, R, T, U * K / 2, 2>(part, first, step, ns, live, vs, tid, out, s_dst, s_il, s_f);
+  else if (ns <= 4) at_join_of<D, R, T, U * K / 4, 4>(part, first, step, ns, live, vs, tid, out, s_dst, s_il, s_f);
+  else at_join_of<D, R, T, U, K>(part, first, step, ns, live, vs, tid, out, s_dst, s_il, s_f);
+}
+
 template <int D, bool F8>
 struct AtFew {
   static constexpr int ES = F8 ? 1 : 2, ROWB = D * ES, TILE = 32 * ROWB, NL = TILE / 1024;  // wave-loads of 1 KiB a tile
@@ -152,6 +160,13 @@ static __device__ __forceinline__ void attn_few_body(
   unsigned char *sk = smem + wave * REGION, *sv = sk + TILE;
   const size_t head_elems = (size_t)D << page_shift;
   const int mask = (1 << page_shift) - 1;
+
+  // (Where a workgroup's 32 rows leave few registers: a number made anew, with the addresses that follow from it, which kept across the tiles would be registers
+  // that the loop lacks)
+  auto anew = [](int x) {
+    if constexpr (RT == 2 || (F8 && D == 256)) asm volatile("" : "+v"(x));
+    return x;
+  };
 
   // ---- this workgroup's units
   struct Seq {
@@ -405,6 +420,7 @@ static __device__ __forceinline__ void attn_few_body(
       else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       if (special) {
         auto piece = [&](int t, int x) -> unsigned char * { return sv + t * ROWB + ((x ^ A::swz(t)) * 16); };
+        const int ln = anew(lane), lane = ln, n = ln & 15, g = ln >> 4;
         constexpr int PR = ROWB / 16;  // pieces a row
         const int stop = min(end - tile, 32);
         // what takes no part: rows behind the end, a hole's block
@@ -448,6 +464,7 @@ static __device__ __forceinline__ void attn_few_body(
       {
         constexpr int RD = F8 ? 1 : 2;  // reads a channel block
         iu8_v2u vf[DT][RD];
+        const int ln = anew(lane), n = ln & 15, g = ln >> 4;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
           if constexpr (F8) {
@@ -512,7 +529,8 @@ static __device__ __forceinline__ void attn_few_body(
     const unsigned start = at_unit - u0;  // the item's first unit
     const bool leads = at_unit == blockIdx.x * share;
     float *slot = partial + (size_t)(blockIdx.x * 2 + !leads) * SLOT;
-    for (int e = tid; e < live * (D / 4); e += 256) {
+    const int me = anew(tid);
+    for (int e = me; e < live * (D / 4); e += 256) {
       const int r = e / (D / 4), d = (e % (D / 4)) * 4;
       const float *x0 = (const float *)smem + r * (D + 4) + d;
       iu8_v4f x = *(const iu8_v4f *)x0;
@@ -538,7 +556,7 @@ static __device__ __forceinline__ void attn_few_body(
       }
       __syncthreads();
       if (s_last)
-        at_join<D, R, 256, 2, RT == 1 ? 16 : 8>(partial + (size_t)first * 2 * SLOT, start == first * share ? 0 : SLOT, 2 * SLOT, ns, live, vs, tid, out, s_dst, s_il,
+        at_join<D, R, 256, 2, RT == 1 ? 16 : 8>(partial + (size_t)first * 2 * SLOT, start == first * share ? 0 : SLOT, 2 * SLOT, ns, live, vs, me, out, s_dst, s_il,
                                   (float *)smem);
     }
     at_unit += u1 - u0;

@@ -489,29 +489,31 @@ static __device__ __forceinline__ void attn_many_body(
     }
   }
   l = at_both<32>(l, at_sum2);
+  const int end_n = thread() & 31, end_hf = (thread() & 63) >> 5;
+  const bool end_real = wave * 32 + end_n < live;
   if (ns == 1) {
     const float il = l == 0.f ? 0.f : vs / l;
-    const long long dst = s_dst[wave * 32 + n];
-    if (real) {
+    const long long dst = s_dst[wave * 32 + end_n];
+    if (end_real) {
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int x = 0; x < 16; x += 4)
-          *(iu8_v2u *)(out + dst + 32 * mt + 2 * x + 4 * hf) =
+          *(iu8_v2u *)(out + dst + 32 * mt + 2 * x + 4 * end_hf) =
               iu8_v2u{iu8_bf16_pack(o[mt][x] * il, o[mt][x + 1] * il), iu8_bf16_pack(o[mt][x + 2] * il, o[mt][x + 3] * il)};
     }
     return;
   }
   constexpr size_t SLOT = (size_t)R * (D + 4);
   float *part = partial + (size_t)item * splits * SLOT, *mine = part + (size_t)split * SLOT;
-  if (real) {
-    float *p = mine + (wave * 32 + n) * D;
+  if (end_real) {
+    float *p = mine + (wave * 32 + end_n) * D;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
       for (int x = 0; x < 16; x += 4)
-        at_store_through(p + 32 * mt + 2 * x + 4 * hf, iu8_v4f{o[mt][x], o[mt][x + 1], o[mt][x + 2], o[mt][x + 3]});
-    if (hf == 0) at_store_through(mine + R * D + (wave * 32 + n) * 4, iu8_v4f{m * c, l, 0.f, 0.f});
+        at_store_through(p + 32 * mt + 2 * x + 4 * end_hf, iu8_v4f{o[mt][x], o[mt][x + 1], o[mt][x + 2], o[mt][x + 3]});
+    if (end_hf == 0) at_store_through(mine + R * D + (wave * 32 + end_n) * 4, iu8_v4f{m * c, l, 0.f, 0.f});
   }
   iu8_stores_done();
   __syncthreads();
@@ -522,5 +524,5 @@ static __device__ __forceinline__ void attn_many_body(
   }
   __syncthreads();
   if (!s_last) return;
-  at_join<D, R, 256, 2, 8>(part, 0, SLOT, ns, live, vs, tid, out, s_dst, s_il, (float *)smem);
+  at_join<D, R, 256, 2, 8>(part, 0, SLOT, ns, live, vs, thread(), out, s_dst, s_il, (float *)smem);
 }

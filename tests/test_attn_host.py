@@ -228,8 +228,7 @@ def test_every_kernel_is_there_with_its_signature():
             for stem, tail in (("kv_append", ""), ("attn_few", "_r16"), ("attn_few", "_r32"), ("attn_many", ""))}
     assert set(re.findall(r'name = "((?:kv_append|attn)_\w+)"', text)) >= want
     scratch = {n: int(b) for n, b in re.findall(r'name = "(\w+)"(?:(?!\[\[kernel\]\]).)*?private_segment_fixed_size = (\d+)', text, flags=re.S) if int(b)}
-    # what lies in memory is touched in front of a tile loop and in the rare tiles' branch, not in the loop's common path
-    assert all(b <= 48 for b in scratch.values()) and set(scratch) <= {"attn_few_bf16_d256_r32", "attn_many_e4m3_d128", "attn_many_e4m3_d256"}, scratch
+    assert not scratch, scratch
     lds = [int(x) for x in re.findall(r"group_segment_fixed_size = (\d+)", text)]
     assert max(lds) <= 160 * 1024
 
