@@ -179,17 +179,17 @@ static __device__ __forceinline__ void attn_few_body(
     x.len = at_len(kv_len, i, table_stride, page_shift);
     return x;
   };
-  auto units_of = [&](const Seq &x) { return (unsigned)((max(x.len, 1) - 1) >> unit_shift) + 1; };
+  auto own_units = [&](const Seq &x) { return (unsigned)((max(x.len, 1) - 1) >> unit_shift) + 1; };
   auto tiles_of = [&](const Seq &x) { return x.nq > 0 ? (unsigned)min((x.nq * G - 1) / R + 1, qtiles) : 0u; };
   unsigned mine = 0, before = 0, total, longest = 0;  // (units: the launch law keeps their sum below 2^31)
   const int per_lane = (seqs - 1) / 64 + 1;
   if (seqs == 1) {
     const Seq x = sequence(0);
-    total = mine = units_of(x) * tiles_of(x) * kv_heads, longest = units_of(x);
+    total = mine = own_units(x) * tiles_of(x) * kv_heads, longest = own_units(x);
   } else {
     for (int i = lane * per_lane; i < min(lane * per_lane + per_lane, seqs); ++i) {
       const Seq x = sequence(i);
-      const unsigned u = units_of(x), t = tiles_of(x);
+      const unsigned u = own_units(x), t = tiles_of(x);
       mine += u * t * kv_heads, longest = max(longest, t ? u : 0u);
     }
     before = mine;
@@ -209,6 +209,34 @@ static __device__ __forceinline__ void attn_few_body(
   // A join costs a workgroup about what four units do: whole items where they are no more than that longer.
   const unsigned over = share % longest, lone = longest - over;
   if (over && lone <= 4) share += lone;
+  // Where the items' parts of `share` units fit the grid, each item begins with a workgroup of its own, as if its last part were
+  // whole: no workgroup then has the end of one item and the beginning of another. (9 x 5 new rows
+  // of group 6 on 4,000 keys 52.6 us -> 47.1; 100 on 1,000 35.0 -> 26.3; the look at the lengths costs 0.5 us.)
+  bool apart = share > 1 && (long long)seqs * kv_heads * qtiles <= grid;
+  if (apart) {
+    unsigned parts = 0, ahead, all;
+    if (seqs == 1) {
+      all = ahead = parts = ((longest - 1) / share + 1) * (total / longest);
+    } else {
+      for (int i = lane * per_lane; i < min(lane * per_lane + per_lane, seqs); ++i) {
+        const Seq x = sequence(i);
+        parts += ((own_units(x) - 1) / share + 1) * tiles_of(x) * kv_heads;
+      }
+      ahead = parts;
+#pragma unroll
+      for (int x = 1; x < 64; x *= 2) {
+        const unsigned y = __shfl_up(ahead, x);
+        ahead += lane >= x ? y : 0;
+      }
+      all = __builtin_amdgcn_readlane(ahead, 63);
+    }
+    apart = all <= grid;
+    if (apart) mine = parts * share, before = (ahead - parts) * share, total = all * share;
+  }
+  auto units_of = [&](const Seq &x) {
+    const unsigned u = own_units(x);
+    return apart ? ((u - 1) / share + 1) * share : u;
+  };
   if (blockIdx.x > (total - 1) / share) return;
   unsigned at_unit = blockIdx.x * share;
   const unsigned last_unit = min(at_unit + share, total);
