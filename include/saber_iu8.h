@@ -590,8 +590,8 @@ uint64_t saber_iu8_kv_v_offset(uint32_t page, uint32_t kv_head, uint32_t token, 
                                uint32_t page_tokens, uint32_t kind);
 
 /* The new tokens of `seqs` sequences into the cache. Rows cu_q[s] .. cu_q[s + 1] - 1 (device, [seqs + 1]) are sequence s's newest
- * tokens, at positions kv_len[s] - n .. kv_len[s] - 1; cu_q NULL: one row a sequence. Rows behind the last sequence (of `tokens`),
- * and rows whose position would be negative, are left as they were, in q_out as in the cache.
+ * tokens, at positions kv_len[s] - n .. kv_len[s] - 1; cu_q NULL: one row a sequence. Rows in front of the first sequence and behind the
+ * last (of `tokens`), and rows whose position would be negative, are left as they were, in q_out as in the cache.
  *   q [tokens] rows `q_row` elements apart, head h at h * q_head (q_head = 2 * head_dim reads a gated projection's [q | gate] heads
  *   in place); k, v rows `kv_row` apart, heads head_dim apart; q_out [tokens, heads, head_dim].
  *   q_norm, k_norm (bf16 [head_dim], may be NULL): x * 1/sqrt(mean(x^2) + eps) * (1 + w) over the head's channels.
@@ -605,8 +605,8 @@ int saber_iu8_kv_append(saber_iu8_ctx *ctx, const void *q, const void *k, const 
 
 /* The new rows' attention over the cache, causal: row i of sequence s's n new ones sees positions 0 .. kv_len[s] - n + i.
  *   out[t, h] = sum_j softmax_j(scale * q[t, h] . k_j) v_j, heads in groups of heads / kv_heads a kv head
- * q rows `q_row` elements apart, heads head_dim apart; out bf16 [tokens, heads, head_dim]. A row that sees no key gives zeros; rows behind
- * the last sequence are left as they were. max_q: the most new rows of a sequence (rows past it are not computed); max_kv: what
+ * q rows `q_row` elements apart, heads head_dim apart; out bf16 [tokens, heads, head_dim]. A row that sees no key gives zeros; rows in
+ * front of the first sequence and behind the last are left as they were. max_q: the most new rows of a sequence (rows past it are not computed); max_kv: what
  * kv_len is expected to reach, for the split of the cache's length alone (a longer one is right, and slower).
  * Up to 32 rows a kv head (new rows x group), and somewhat more on a long cache, run on the few-row kernels, which stream the
  * cache; the rest on the many-row kernels, 128 rows a workgroup. Both share the cache's length among workgroups where the grid would

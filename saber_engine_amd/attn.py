@@ -9,7 +9,7 @@ from . import iu8
 
 class PagedKvCache:
     """The pages of one layer's sequences. The host deals pages (reserve, release); the table and the counts lie on the device, where
-    the kernels read them, so that a captured step follows them."""
+    the kernels read them, so that a captured step follows them; reserve and release write there on torch's current stream."""
 
     def __init__(self, seqs, kv_heads, head_dim, max_kv, pages=None, page_tokens=64, kind=iu8.KV_BF16, k_scale=None, v_scale=None, device="cuda"):
         """max_kv: the most tokens a sequence may hold; pages: of all sequences together (None: enough for all at that length);
@@ -86,9 +86,12 @@ class AttnLayerIU8:
         self._w = (wqkv_frag, wsqkv, wo_frag, wso)
         self.had_t, self.q_norm, self.k_norm = had_t, q_norm, k_norm
 
-    def forward(self, x, stream=0):
+    def forward(self, x, stream=0, max_kv=None):
         """x bf16 bits [T, H] (int16 tensor), the newest tokens of the cache's sequences, whose kv_len already counts them and whose
-        pages are reserved; every launch on `stream`."""
+        pages are reserved; every launch on `stream`. max_kv: what kv_len reaches in this call, where the caller knows it (a
+        captured call: in any replay); the cache's length is shared among workgroups accordingly."""
+        if tuple(x.shape) != (self.T, self.H):
+            raise iu8.IU8Error(iu8.E_RULE, f"rows of shape {tuple(x.shape)}; the train is made for {(self.T, self.H)}")
         c, T, D, P = self.ctx, self.T, self.cache.head_dim, lambda t: t.data_ptr() if t is not None else None  # noqa: E731
         wqkv, wsqkv, wo, wso = self._w
         cache, qkv, cu = self.cache.desc, self.qkv.data_ptr(), P(self.cu_q)
@@ -98,8 +101,8 @@ class AttnLayerIU8:
         c.kv_append(qkv, k, k + 2 * self.cache.kv_heads * D, P(self.q), cache, cu, T, self.cache.seqs, self.heads, self.n_qkv, self.q_head,
                     self.n_qkv, P(self.inv_freq), 2 * len(self.inv_freq) if self.inv_freq is not None else 0, self.interleaved,
                     P(self.q_norm), P(self.k_norm), self.eps, stream)
-        c.attn(P(self.q), self.n_core, cache, cu, P(self.core), T, self.cache.seqs, self.max_q, self.cache.max_kv, self.heads, self.scale,
-               *map(P, self._attn_ws), stream)
+        c.attn(P(self.q), self.n_core, cache, cu, P(self.core), T, self.cache.seqs, self.max_q,
+               self.cache.max_kv if max_kv is None else min(max_kv, self.cache.max_kv), self.heads, self.scale,               *map(P, self._attn_ws), stream)
         if self.gated:
             c.attn_gate_quant_had(P(self.core), qkv, P(self.a2), P(self.s2), T, self.n_core, D, self.n_qkv, P(self.had_t), stream)
         else:

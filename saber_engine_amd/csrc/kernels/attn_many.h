@@ -3,8 +3,15 @@
 //
 // One workgroup: 128 rows of one kv head of one sequence, 32 a wave; row r is new token r / G, head r % G of the group, so every
 // head of the group shares the staged keys and a short prompt still fills its rows. K and V come tile by tile (BK tokens, two
-// LDS stages): bf16 straight from memory into LDS, e4m3 through registers, widened once for all four waves. Bound by the matrix
-// cores and the LDS that feeds them.
+// LDS stages): bf16 straight from memory into LDS, e4m3 through registers, widened once for all four waves. Two workgroups a compute
+// unit (256 registers a lane, 64 KiB of LDS), so that one's softmax runs under the other's products; up to 128 channels, where the
+// registers allow, also under its own (the scores of the next tile in the block of this one's weights: 8,192 tokens of 40 heads of
+// 128 channels 696 us -> 672).
+//
+// Bound by the matrix cores at the clock that they leave (60 % of their cycles busy at 8,192 tokens of 24 heads of 256: 719 to 745 us,
+// 1,107 to 1,147 TF/s, where the library's largest plain product reaches 1,348), and on short prompts by the chain of a workgroup's
+// beginning and end, about four tiles' time: five prompts of 883 to 2,100 tokens, 40 heads of 128, 185 to 192 us, 138 GF. LDS: 30 % of
+// the cycles, no conflicts (e4m3: 14 % of its accesses).
 //
 // Both products have the row as the MFMA's column (attn_few.h has why): S^T = K Q^T leaves lane (row, half) the tokens
 // 8 i + 4 half + r, which is the token order that P's operand of O^T = V^T P^T then has, and the LDS's transposing read gives V^T

@@ -218,6 +218,8 @@ def test_layer_refusals():
     layer = attn.AttnLayerIU8(None, c, 3, 4, 256)
     with pytest.raises(iu8.IU8Error, match="had_t"):
         layer.set_weights(None, None, None, None)
+    with pytest.raises(iu8.IU8Error, match="made for"):
+        layer.forward(torch.zeros((2, 256), dtype=torch.int16))
 
 
 # ------------------------------------------------------------------ the built kernels

@@ -380,6 +380,31 @@ def test_cache_past_four_gibibytes(ctx, new):
     check(f64(out.float()), want, tol, "rows on far pages")
 
 
+def test_rows_in_front_of_the_first_sequence(ctx):
+    """cu_q that does not begin at 0: the rows in front belong to nobody, in the cache as in the outputs."""
+    say("rows in front of the first sequence")
+    heads, kvh, dim, lens, news, front = 4, 2, 64, [30, 9], [4, 9], 3
+    c = Paged(2, kvh, dim, 16, 32, fill=0.0)
+    c.kv_len.copy_(torch.tensor(lens))
+    g = torch.Generator().manual_seed(3)
+    tokens, row = front + sum(news), (heads + 2 * kvh) * dim
+    x = random_rows(g, tokens, row)
+    q, out = (torch.full((tokens, heads, dim), 7.0, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    cu, p = ends(news) + front, x.data_ptr()
+    ctx.kv_append(p, p + 2 * heads * dim, p + 2 * (heads + kvh) * dim, q.data_ptr(), c.desc(), cu.data_ptr(), tokens, 2, heads, row, dim, row)
+    ctx.attn(q.data_ptr(), heads * dim, c.desc(), cu.data_ptr(), out.data_ptr(), tokens, 2, 9, 30, heads, 0.125)
+    torch.cuda.synchronize()
+    assert (q[:front] == 7).all() and (out[:front] == 7).all()
+    t = front
+    for s, n in enumerate(news):
+        k, v, there = c.rows(s, lens[s])
+        assert not k[:-n].any() and not v[:-n].any()
+        assert np.array_equal(k[-n:].reshape(n, -1), f64(x[t:t + n, heads * dim:(heads + kvh) * dim].float()))
+        want, tol = attention(f64(x[t:t + n, :heads * dim].float()).reshape(n, heads, dim), k, v, there, 0.125)
+        check(f64(out[t:t + n].float()), want, tol, f"sequence {s}")
+        t += n
+
+
 def test_append_in_place(ctx):
     say("append: q_out is q")
     heads, kvh, dim, n = 6, 2, 128, 9
@@ -487,7 +512,7 @@ def test_layer_prompts_then_single_tokens(ctx, gated, heads, kvh, dim, hidden, i
             lens[s] += new
             cache.reserve(s, lens[s])
         cache.kv_len.copy_(torch.tensor(lens))
-        n.forward(dev_bf16_bits(x))
+        n.forward(dev_bf16_bits(x), max_kv=max(lens))
         torch.cuda.synchronize()
         check_layer(n, host, x, news, before, kv)
 
