@@ -17,6 +17,7 @@ constexpr uint32_t MANY_ROWS = 128;  // rows a workgroup of the many-row kernels
 constexpr int FEW_UNIT_SHIFT = 7, WHOLE_SHIFT = 31;  // log2 of the tokens a unit of the few-row kernels' deal (attn_few.h)
 constexpr uint32_t MANY_PARTS = 32;  // parts of an item at most: their maxima and sums lie in one workgroup's LDS when they are joined
 constexpr uint64_t FEW_UNITS_MIN = 8, FEW_UNITS_MAX = 5 * CU_COUNT;  // more than 32 rows on the few-row kernels: units a row tile from, units of all up to
+constexpr uint64_t FEW_BRIEF = 1200;  // units of all below which a part's beginning and end weigh more than its bytes
 constexpr uint64_t MANY_TARGET = 2 * CU_COUNT, MANY_LEAST = 320, MANY_LONG = 2048;  // workgroups that parts aim at, at most; tokens a part, from; long ones
 constexpr uint32_t I32_MAX = 0x7FFFFFFFu;
 constexpr uint32_t WHOLE = 0x7FFFFF00u;  // a part that holds any sequence: the positions a table's row may reach
@@ -60,9 +61,10 @@ struct Plan {
 // few rows that its tiles of 32 make at most a unit a CU (60 new tokens of group 6 on 300 keys, head width 256: 19.7 us against 21.2 of
 // the many-row kernel; 60 on 600 24.6 / 31.7; 60 of group 5 on 300, width 128, 13.3 / 16.3 -- but not whole prompts of one or two units, half of
 // which is masked: 200 on 200, 20.9 / 17.9) or, on eight units and more, five a CU (200 of group 6 on 1,000 35 / 45; on 1,600, at eight
-// a CU, 56 / 44). Their grid: the workgroups that the card holds at once (by their LDS: two a CU, or one), which deal the units
-// level; three quarters of the CUs where each then has 16 units and more (131,072 keys, 4 kv heads of 256: 192 workgroups 92 us,
-// 256 96; 64 sequences of up to 8,192, 8 heads of 128: 199 against 203 of 512).
+// a CU, 56 / 44). Their grid, among which the units are dealt level: a workgroup a CU; two where both fit one's LDS and the items
+// suffice for nearly all of them to stay whole (256 sequences of 1,000 keys, 8 heads of 128 in e4m3: 256 workgroups 98 us, 512 86; 32 of 2,400 in
+// bf16, 256 items: 51 against 55); fewer where few items would be cut into many parts, whose join costs a round of loads for every
+// 16 (5,000 keys, 8 heads of 128: 128 workgroups 13.5 us, 256 15.7, 512 20.0; 4 heads of 256 on 131,072: 128 102, 192 92, 256 96).
 // Many rows: parts where the row tiles alone are fewer than the CUs, one workgroup a CU (400 rows of group 6, 76 tiles, on 3,000 keys:
 // one part 112 us, three 62, four 68, six 69 to 85), two a CU where the parts are long (512 rows, 96 tiles, on 16,896: two parts
 // 395 us, five 248 to 271).
@@ -76,7 +78,8 @@ Plan plan(uint32_t seqs, uint32_t max_q, uint32_t max_kv, uint32_t heads, uint32
   p.items = (uint64_t)seqs * kv_heads * p.qtiles;
   p.splits = 1, p.chunk = WHOLE, p.unit_shift = WHOLE_SHIFT;
   if (p.few()) {
-    const uint64_t slots = p.items * units >= 16 * CU_COUNT ? CU_COUNT * 3 / 4 : CU_COUNT * (p.rows == 16 && (f8 || dim < 256) ? 2 : 1);
+    const bool two = p.rows == 16 && (f8 || dim < 256) && p.items >= 2 * CU_COUNT, brief = p.items * units < FEW_BRIEF;
+    const uint64_t slots = two ? 2 * CU_COUNT : std::clamp<uint64_t>((brief ? 16 : 48) * p.items, brief ? CU_COUNT / 2 : CU_COUNT * 3 / 4, CU_COUNT);
     if (!whole && units > 1) {
       p.unit_shift = FEW_UNIT_SHIFT;
       while (p.unit_shift < WHOLE_SHIFT && p.items * ((held >> p.unit_shift) + 1) > I32_MAX) ++p.unit_shift;  // the kernel counts them in 32 bits
