@@ -18,7 +18,8 @@ constexpr int FEW_UNIT_SHIFT = 7, WHOLE_SHIFT = 31;  // log2 of the tokens a uni
 constexpr uint32_t MANY_PARTS = 32;  // parts of an item at most: their maxima and sums lie in one workgroup's LDS when they are joined
 constexpr uint64_t FEW_UNITS_MIN = 8, FEW_UNITS_MAX = 5 * CU_COUNT;  // more than 32 rows on the few-row kernels: units a row tile from, units of all up to
 constexpr uint64_t FEW_BRIEF = 1200;  // units of all below which a part's beginning and end weigh more than its bytes
-constexpr uint64_t MANY_TARGET = 2 * CU_COUNT, MANY_LEAST = 320, MANY_LONG = 2048;  // workgroups that parts aim at, at most; tokens a part, from; long ones
+constexpr uint64_t MANY_TARGET = 2 * CU_COUNT, MANY_LEAST = 320, MANY_LONG = 2048;  // workgroups that the card holds; tokens a part, from; long ones
+constexpr uint64_t MANY_UNEVEN = 448, MANY_LONGEST = 8192;  // row tiles that leave an eighth of the places empty, up to; keys that make that worth more parts
 constexpr uint32_t I32_MAX = 0x7FFFFFFFu;
 constexpr uint32_t WHOLE = 0x7FFFFF00u;  // a part that holds any sequence: the positions a table's row may reach
 
@@ -67,7 +68,8 @@ struct Plan {
 // 16 (5,000 keys, 8 heads of 128: 128 workgroups 13.5 us, 256 15.7, 512 20.0; 4 heads of 256 on 131,072: 128 102, 192 92, 256 96).
 // Many rows: parts where the row tiles alone are fewer than the CUs, one workgroup a CU (400 rows of group 6, 76 tiles, on 3,000 keys:
 // one part 112 us, three 62, four 68, six 69 to 85), two a CU where the parts are long (512 rows, 96 tiles, on 16,896: two parts
-// 395 us, five 248 to 271).
+// 395 us, five 248 to 271), three or two each where the row tiles are between one and two a CU and the keys many (1,200 rows of 32 heads on 8
+// of 64, 304 tiles, on 20,000: one part 424 us, three 290; 40 on 8 of 128, 376 tiles: 546 and, in two, 525).
 // `whole`: no workspaces, every item in one piece; `held`: the tokens that a sequence's row of the page table can hold.
 Plan plan(uint32_t seqs, uint32_t max_q, uint32_t max_kv, uint32_t heads, uint32_t kv_heads, uint32_t dim, bool f8, bool whole, uint64_t held) {
   Plan p{};
@@ -91,6 +93,7 @@ Plan plan(uint32_t seqs, uint32_t max_q, uint32_t max_kv, uint32_t heads, uint32
   }
   uint64_t parts = std::max<uint64_t>(1, CU_COUNT / p.items);
   if (max_kv > MANY_LONG * parts) parts = std::max<uint64_t>(1, MANY_TARGET / p.items);
+  if (p.items > CU_COUNT && p.items <= MANY_UNEVEN && max_kv >= MANY_LONGEST) parts = 2 * MANY_TARGET / p.items;
   parts = std::min<uint64_t>({parts, MANY_PARTS, std::max<uint64_t>(1, (max_kv + MANY_LEAST - 1) / MANY_LEAST)});
   if (!whole && parts > 1) {
     p.chunk = (uint32_t)(((max_kv + parts - 1) / parts + 127) / 128 * 128);
@@ -103,7 +106,7 @@ Plan plan(uint32_t seqs, uint32_t max_q, uint32_t max_kv, uint32_t heads, uint32
 
 // What the plan of any call of up to these sizes takes, caches of either kind: fewer sequences or shorter ones may be cut into more
 // parts, and a server allocates once. Few rows: two slots a workgroup, at most 512 of 16 rows or 256 of 32; many: a slot a
-// workgroup, at most 512.
+// workgroup, at most 512, on long caches 1,024.
 void workspace(uint64_t seqs, uint64_t max_q, uint64_t max_kv, uint64_t group, uint64_t kv_heads, uint64_t dim, uint64_t *partial, uint64_t *counter) {
   const uint64_t rows = max_q * group, units = max_kv ? ((max_kv - 1) >> FEW_UNIT_SHIFT) + 1 : 1, row = (dim + 4) * 4;
   auto want = [&](uint64_t items, uint64_t slots, uint64_t a_slot) { *partial = std::max(*partial, slots * a_slot * row), *counter = std::max(*counter, items * 4); };
@@ -114,7 +117,7 @@ void workspace(uint64_t seqs, uint64_t max_q, uint64_t max_kv, uint64_t group, u
     want(items, std::min<uint64_t>(CU_COUNT, items * units), 2 * FEW_ROWS);
   }
   const uint64_t items = seqs * kv_heads * ((rows + MANY_ROWS - 1) / MANY_ROWS), parts = std::min<uint64_t>(MANY_PARTS, (max_kv + MANY_LEAST - 1) / MANY_LEAST);
-  if (rows > FEW_ROWS && parts > 1) want(std::min(items, MANY_TARGET / 2), std::min(items * parts, MANY_TARGET), MANY_ROWS);
+  if (rows > FEW_ROWS && parts > 1) want(std::min(items, MANY_UNEVEN), std::min(items * parts, max_kv < MANY_LONGEST ? MANY_TARGET : 2 * MANY_TARGET), MANY_ROWS);
 }
 
 int attn_plan(const char *op, uint32_t seqs, uint32_t max_q, uint32_t max_kv, uint32_t heads, uint32_t kv_heads, uint32_t dim, bool f8, bool whole, uint64_t held, Plan *p) {
