@@ -569,7 +569,8 @@ int saber_iu8_silu_table(saber_iu8_ctx *ctx, void *out_u16, void *stream);
  * [16 tokens][E], V [pages][kv_heads][page_tokens][head_dim] (saber_iu8_kv_k_offset, _v_offset). head_dim 64, 128 or 256; page_tokens a
  * power of two from 16 to 256. An e4m3 cache holds value / scale, a scale a kv head, rounded to nearest even and saturated at 448;
  * the attention multiplies by it. Entry [s * table_stride + p] of the page table is the page that holds tokens p * page_tokens ... of
- * sequence s; an entry outside 0 .. pages - 1 is a hole: nothing is written there and its keys take no part. kv_len[s] counts
+ * sequence s; an entry outside 0 .. pages - 1 is a hole: nothing is written there and its keys take no part. Sequences
+ * may share pages that no call writes. kv_len[s] counts
  * the sequence's tokens, the call's new ones included (both operators of a step read the same number); counts above
  * table_stride * page_tokens are taken as that, below 0 as 0. The counts and the table are read on the device, so a captured launch
  * follows them. */

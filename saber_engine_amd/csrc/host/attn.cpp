@@ -16,7 +16,7 @@ constexpr uint32_t FEW_ROWS = 32;    // rows a kv head and sequence up to which 
 constexpr uint32_t MANY_ROWS = 128;  // rows a workgroup of the many-row kernels
 constexpr int FEW_UNIT_SHIFT = 7, WHOLE_SHIFT = 31;  // log2 of the tokens a unit of the few-row kernels' deal (attn_few.h)
 constexpr uint32_t MANY_PARTS = 32;  // parts of an item at most: their maxima and sums lie in one workgroup's LDS when they are joined
-constexpr uint64_t FEW_UNITS_MIN = 8, FEW_UNITS_MAX = 5 * CU_COUNT;  // more than 32 rows on the few-row kernels: units a row tile from, units of all up to
+constexpr uint64_t FEW_UNITS_MIN = 8, FEW_UNITS_MAX = 5 * CU_COUNT, FEW_UNITS_MAX_E4M3 = 16 * CU_COUNT;  // more than 32 rows on the few-row kernels: units a row tile from, units of all up to
 constexpr uint64_t FEW_BRIEF = 1200;  // units of all below which a part's beginning and end weigh more than its bytes
 constexpr uint64_t MANY_TARGET = 2 * CU_COUNT, MANY_LEAST = 320, MANY_LONG = 2048;  // workgroups that the card holds; tokens a part, from; long ones
 constexpr uint64_t MANY_UNEVEN = 448, MANY_LONGEST = 8192;  // row tiles that leave an eighth of the places empty, up to; keys that make that worth more parts
@@ -62,7 +62,8 @@ struct Plan {
 // few rows that its tiles of 32 make at most a unit a CU (60 new tokens of group 6 on 300 keys, head width 256: 19.7 us against 21.2 of
 // the many-row kernel; 60 on 600 24.6 / 31.7; 60 of group 5 on 300, width 128, 13.3 / 16.3 -- but not whole prompts of one or two units, half of
 // which is masked: 200 on 200, 20.9 / 17.9) or, on eight units and more, five a CU (200 of group 6 on 1,000 35 / 45; on 1,600, at eight
-// a CU, 56 / 44). Their grid, among which the units are dealt level: a workgroup a CU; two where both fit one's LDS and the items
+// a CU, 56 / 44), sixteen a CU in e4m3, which the many-row kernel widens through registers (60 of group 6 on 4,000: 39 / 61; 8 sequences
+// of 8 rows each 35 / 44; 32 of them, at 32 a CU, 94 / 93). Their grid, among which the units are dealt level: a workgroup a CU; two where both fit one's LDS and the items
 // suffice for nearly all of them to stay whole (256 sequences of 1,000 keys, 8 heads of 128 in e4m3: 256 workgroups 98 us, 512 86; 32 of 2,400 in
 // bf16, 256 items: 51 against 55); fewer where few items would be cut into many parts, whose join costs a round of loads for every
 // 16 (5,000 keys, 8 heads of 128: 128 workgroups 13.5 us, 256 15.7, 512 20.0; 4 heads of 256 on 131,072: 128 102, 192 92, 256 96).
@@ -75,7 +76,7 @@ Plan plan(uint32_t seqs, uint32_t max_q, uint32_t max_kv, uint32_t heads, uint32
   Plan p{};
   const uint64_t rows = (uint64_t)max_q * (heads / kv_heads), units = max_kv ? ((max_kv - 1) >> FEW_UNIT_SHIFT) + 1 : 1;
   const uint64_t all32 = (uint64_t)seqs * kv_heads * ((rows + FEW_ROWS - 1) / FEW_ROWS) * units;
-  p.rows = rows <= 16 ? 16 : rows <= FEW_ROWS || (!whole && ((units >= FEW_UNITS_MIN && all32 <= FEW_UNITS_MAX) || (units >= 3 && all32 <= CU_COUNT))) ? FEW_ROWS : MANY_ROWS;
+  p.rows = rows <= 16 ? 16 : rows <= FEW_ROWS || (!whole && ((units >= FEW_UNITS_MIN && all32 <= (f8 ? FEW_UNITS_MAX_E4M3 : FEW_UNITS_MAX)) || (units >= 3 && all32 <= CU_COUNT))) ? FEW_ROWS : MANY_ROWS;
   p.qtiles = (rows + p.rows - 1) / p.rows;
   p.items = (uint64_t)seqs * kv_heads * p.qtiles;
   p.splits = 1, p.chunk = WHOLE, p.unit_shift = WHOLE_SHIFT;
@@ -113,7 +114,7 @@ void workspace(uint64_t seqs, uint64_t max_q, uint64_t max_kv, uint64_t group, u
   if (units < 2) return;
   if (group <= 16) want(seqs * kv_heads, std::min<uint64_t>(2 * CU_COUNT, seqs * kv_heads * units), 2 * 16);
   if (rows > 16) {
-    const uint64_t items = std::max(seqs * kv_heads, std::min<uint64_t>(seqs * kv_heads * ((rows + FEW_ROWS - 1) / FEW_ROWS), FEW_UNITS_MAX / FEW_UNITS_MIN));
+    const uint64_t items = std::max(seqs * kv_heads, std::min<uint64_t>(seqs * kv_heads * ((rows + FEW_ROWS - 1) / FEW_ROWS), FEW_UNITS_MAX_E4M3 / FEW_UNITS_MIN));
     want(items, std::min<uint64_t>(CU_COUNT, items * units), 2 * FEW_ROWS);
   }
   const uint64_t items = seqs * kv_heads * ((rows + MANY_ROWS - 1) / MANY_ROWS), parts = std::min<uint64_t>(MANY_PARTS, (max_kv + MANY_LEAST - 1) / MANY_LEAST);

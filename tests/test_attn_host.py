@@ -118,7 +118,7 @@ def test_workspaces_hold_every_smaller_call():
         less = [rng.randint(1, x) for x in most]
         big, small = (iu8.attn_workspace(*s, kvh * group, kvh, dim) for s in (most, less))
         assert small[0] <= big[0] and small[1] <= big[1], (most, less, kvh, group, dim)
-        assert big[0] <= 1024 * 128 * (dim + 4) * 4 and big[1] <= 4 * max(most[0] * kvh, 448)
+        assert big[0] <= 1024 * 128 * (dim + 4) * 4 and big[1] <= 4 * max(most[0] * kvh, 512)
 
 
 class Other(iu8.KvCache):

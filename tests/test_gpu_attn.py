@@ -319,6 +319,24 @@ def test_attn_row_tiles_of_the_few_row_kernels(ctx, dim, heads, kvh, total, new,
     attn_case(ctx, dim, heads, kvh, [total, 40, 1300], [new, new - 1, 1], e4m3=e4m3)
 
 
+@pytest.mark.parametrize("dim,heads,kvh,lens,news", [
+    (64, 200, 1, [300, 41], [1, 2]), (64, 300, 300, [70, 1, 150], [1, 1, 1]), (64, 2, 2, [20 + i % 50 for i in range(300)], [20 + i % 17 for i in range(300)])])
+def test_attn_wide_groups_many_heads_many_prompts(ctx, dim, heads, kvh, lens, news):
+    say(f"attn, {heads} heads on {kvh}, {len(lens)} sequences")
+    attn_case(ctx, dim, heads, kvh, lens, news, page=16, e4m3=kvh == 300)
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("new", [1, 40])
+def test_attn_over_pages_that_sequences_share(ctx, new, e4m3):
+    """A prefix that lies in the same pages for every sequence, the rest in pages of its own."""
+    say(f"attn, a shared prefix, {new} new rows {e4m3}")
+    def share(c):
+        c.table[1, :3] = c.table[0, :3]
+        c.table[2, :2] = c.table[0, :2]
+    attn_case(ctx, 128, 4, 2, [150, 170, 100], [new] * 3, page=32, e4m3=e4m3, spoil=share)
+
+
 @pytest.mark.parametrize("e4m3", [False, True])
 @pytest.mark.parametrize("dim", [64, 128, 256])
 def test_attn_lengths_around_a_tile(ctx, dim, e4m3):
