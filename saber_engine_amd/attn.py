@@ -72,6 +72,8 @@ class AttnLayerIU8:
         self.cu_q = torch.zeros(cache.seqs + 1, dtype=torch.int32, device=device) if max_q > 1 else None
         self._ws = [self._workspace(iu8.gemm_workspace(iu8.W4, tokens, n, k)) for n, k in ((self.n_qkv, hidden), (hidden, self.n_core))]
         self._attn_ws = self._workspace(iu8.attn_workspace(cache.seqs, max_q, cache.max_kv, heads, kvh, D))
+        # few rows: quantisation and GEMM of a linear in one launch, where the launch law holds it
+        self.fused_qkv, self.fused_o = (iu8.fused_holds(tokens, k) for k in (hidden, self.n_core))
         self.had_t = self.q_norm = self.k_norm = None
 
     def _workspace(self, sizes):  # (scratch, counters: zeroed once, left zero by the kernels)
@@ -96,8 +98,11 @@ class AttnLayerIU8:
         wqkv, wsqkv, wo, wso = self._w
         cache, qkv, cu = self.cache.desc, self.qkv.data_ptr(), P(self.cu_q)
         k = qkv + 2 * self.heads * self.q_head
-        c.quant(x.data_ptr(), P(self.a1), P(self.s1), T, self.H, stream)
-        c.gemm(iu8.W4, P(self.a1), P(self.s1), P(wqkv), P(wsqkv), qkv, T, self.n_qkv, self.H, *map(P, self._ws[0]), stream)
+        if self.fused_qkv:
+            c.linear_fused(iu8.W4, x.data_ptr(), P(wqkv), P(wsqkv), qkv, T, self.n_qkv, self.H, stream=stream)
+        else:
+            c.quant(x.data_ptr(), P(self.a1), P(self.s1), T, self.H, stream)
+            c.gemm(iu8.W4, P(self.a1), P(self.s1), P(wqkv), P(wsqkv), qkv, T, self.n_qkv, self.H, *map(P, self._ws[0]), stream)
         c.kv_append(qkv, k, k + 2 * self.cache.kv_heads * D, P(self.q), cache, cu, T, self.cache.seqs, self.heads, self.n_qkv, self.q_head,
                     self.n_qkv, P(self.inv_freq), 2 * len(self.inv_freq) if self.inv_freq is not None else 0, self.interleaved,
                     P(self.q_norm), P(self.k_norm), self.eps, stream)
@@ -105,6 +110,9 @@ class AttnLayerIU8:
                self.cache.max_kv if max_kv is None else min(max_kv, self.cache.max_kv), self.heads, self.scale,               *map(P, self._attn_ws), stream)
         if self.gated:
             c.attn_gate_quant_had(P(self.core), qkv, P(self.a2), P(self.s2), T, self.n_core, D, self.n_qkv, P(self.had_t), stream)
+        elif self.fused_o:
+            c.linear_fused(iu8.W4, P(self.core), P(wo), P(wso), P(self.out), T, self.H, self.n_core, stream=stream)
+            return self.out
         else:
             c.quant(P(self.core), P(self.a2), P(self.s2), T, self.n_core, stream)
         c.gemm(iu8.W4, P(self.a2), P(self.s2), P(wo), P(wso), P(self.out), T, self.H, self.n_core, *map(P, self._ws[1]), stream)

@@ -16,11 +16,12 @@ constexpr uint32_t FEW_ROWS = 32;    // rows a kv head and sequence up to which 
 constexpr uint32_t MANY_ROWS = 128;  // rows a workgroup of the many-row kernels
 constexpr int FEW_UNIT_SHIFT = 7, WHOLE_SHIFT = 31;  // log2 of the tokens a unit of the few-row kernels' deal (attn_few.h)
 constexpr uint32_t MANY_PARTS = 32;  // parts of an item at most: their maxima and sums lie in one workgroup's LDS when they are joined
-constexpr uint64_t FEW_UNITS_MIN = 8, FEW_UNITS_MAX = 5 * CU_COUNT, FEW_UNITS_MAX_E4M3 = 16 * CU_COUNT;  // more than 32 rows on the few-row kernels: units a row tile from, units of all up to
+// more than 32 rows on the few-row kernels: units a row tile from, units of all up to
+constexpr uint64_t FEW_UNITS_MIN = 8, FEW_UNITS_MAX = 5 * CU_COUNT, FEW_UNITS_MAX_E4M3 = 16 * CU_COUNT;
 constexpr uint64_t FEW_BRIEF = 1200;  // units of all below which a part's beginning and end weigh more than its bytes
 constexpr uint64_t MANY_TARGET = 2 * CU_COUNT, MANY_LEAST = 320, MANY_LONG = 2048;  // workgroups that the card holds; tokens a part, from; long ones
 constexpr uint64_t MANY_UNEVEN = 448, MANY_LONGEST = 8192;  // row tiles that leave an eighth of the places empty, up to; keys that make that worth more parts
-constexpr uint32_t I32_MAX = 0x7FFFFFFFu;
+constexpr uint32_t I32_MAX = 0x7FFFFFFFu, GRID_MAX = 0xFFFFFFu;  // workgroups of 256 whose threads a launch counts in 32 bits
 constexpr uint32_t WHOLE = 0x7FFFFF00u;  // a part that holds any sequence: the positions a table's row may reach
 
 int log2_of(uint32_t x) {
@@ -76,7 +77,8 @@ Plan plan(uint32_t seqs, uint32_t max_q, uint32_t max_kv, uint32_t heads, uint32
   Plan p{};
   const uint64_t rows = (uint64_t)max_q * (heads / kv_heads), units = max_kv ? ((max_kv - 1) >> FEW_UNIT_SHIFT) + 1 : 1;
   const uint64_t all32 = (uint64_t)seqs * kv_heads * ((rows + FEW_ROWS - 1) / FEW_ROWS) * units;
-  p.rows = rows <= 16 ? 16 : rows <= FEW_ROWS || (!whole && ((units >= FEW_UNITS_MIN && all32 <= (f8 ? FEW_UNITS_MAX_E4M3 : FEW_UNITS_MAX)) || (units >= 3 && all32 <= CU_COUNT))) ? FEW_ROWS : MANY_ROWS;
+  const bool sparse = !whole && ((units >= FEW_UNITS_MIN && all32 <= (f8 ? FEW_UNITS_MAX_E4M3 : FEW_UNITS_MAX)) || (units >= 3 && all32 <= CU_COUNT));
+  p.rows = rows <= 16 ? 16 : rows <= FEW_ROWS || sparse ? FEW_ROWS : MANY_ROWS;
   p.qtiles = (rows + p.rows - 1) / p.rows;
   p.items = (uint64_t)seqs * kv_heads * p.qtiles;
   p.splits = 1, p.chunk = WHOLE, p.unit_shift = WHOLE_SHIFT;
@@ -127,6 +129,7 @@ int attn_plan(const char *op, uint32_t seqs, uint32_t max_q, uint32_t max_kv, ui
   if (rows > I32_MAX || (__int128)seqs * kv_heads * ((rows + MANY_ROWS - 1) / MANY_ROWS) > (int64_t)I32_MAX)
     return fail(SABER_IU8_E_RULE, fmt("%s: %u sequences of up to %u new rows and %u heads pass a launch's 32-bit sizes", op, seqs, max_q, heads));
   *p = plan(seqs, max_q, max_kv, heads, kv_heads, dim, f8, whole, held);
+  if (p->grid > GRID_MAX) return fail(SABER_IU8_E_RULE, fmt("%s: %u sequences of up to %u new rows and %u heads pass a launch's 32-bit sizes", op, seqs, max_q, heads));
   return 0;
 }
 
@@ -249,7 +252,7 @@ int saber_iu8_kv_append(saber_iu8_ctx *ctx, const void *q, const void *k, const 
   if ((q_norm || k_norm) && !(eps >= 0.f && std::isfinite(eps))) return fail(SABER_IU8_E_RULE, "kv_append: eps must be a number from 0");
   const uint32_t heads_a_wave = 64 / (D / 16), waves = (heads + 2 * cache->kv_heads + heads_a_wave - 1) / heads_a_wave;
   const uint64_t all = (uint64_t)tokens * waves;
-  if (all > I32_MAX) return fail(SABER_IU8_E_RULE, fmt("kv_append: %u rows of %u heads pass a launch's 32-bit sizes", tokens, heads));
+  if ((all + 3) / 4 > GRID_MAX) return fail(SABER_IU8_E_RULE, fmt("kv_append: %u rows of %u heads pass a launch's 32-bit sizes", tokens, heads));
   const bool f8 = cache->kind == SABER_IU8_KV_E4M3;
   AppendArgs x{q, k, v, q_out, cache_of(cache), cu_q, q_norm, k_norm, rot_dim ? inv_freq : nullptr, (int32_t)q_row, (int32_t)q_head, (int32_t)kv_row,
                (int32_t)tokens, (int32_t)seqs, (int32_t)(heads | cache->kv_heads << 16),

@@ -193,7 +193,7 @@ static __device__ __forceinline__ void attn_many_body(
     }
     return __syncthreads_or(odd);
   };
-  // S^T = K Q^T of a stage's K into st; VALU: what lies in the same block and may be issued between the products
+  // S^T = K Q^T of a stage's K
   auto scores = [&](const unsigned char *sk, at_v16f (&sc)[HB]) {
     const int ln = (F8 ? thread() : tid) & 63;
     const unsigned char *ka = sk + ((ln >> 4) & 1) * 16 * ROWB + (ln >> 5) * 256 + (ln & 15) * 16;

@@ -80,6 +80,7 @@ def test_caches_that_are_refused(ctx, bad, code, words):
     (dict(rot_dim=8), iu8.E_RULE, "rotated"), (dict(rot_dim=272), iu8.E_RULE, "rotated"), (dict(inv_freq=None), iu8.E_ARG, "inv_freq"),
     (dict(eps=-1.0), iu8.E_RULE, "eps"), (dict(eps=math.nan), iu8.E_RULE, "eps"), (dict(eps=math.inf), iu8.E_RULE, "eps"),
     (dict(heads=0), iu8.E_RULE, "whole groups"), (dict(heads=65536), iu8.E_RULE, "whole groups"), (dict(tokens=0x7FFFFFFF), iu8.E_RULE, "32-bit sizes"),
+    (dict(tokens=8388608), iu8.E_RULE, "32-bit sizes"), (dict(tokens=8388607), iu8.E_ARG, "null argument"),
     (dict(), iu8.E_ARG, "null argument"), (dict(rot_dim=0, inv_freq=None), iu8.E_ARG, "null argument"),
     (dict(q_norm=None, k_norm=None, eps=-1.0), iu8.E_ARG, "null argument"), (dict(cu_q=None, tokens=3), iu8.E_ARG, "null argument"),
     (dict(q_row=23 * 512 + 256), iu8.E_ARG, "null argument")])       # a last head without its gate behind it
@@ -92,7 +93,8 @@ def test_append_refusals(ctx, bad, code, words):
     (dict(partial=P + 4), iu8.E_ARG, "16 bytes"), (dict(counter=P + 2), iu8.E_ARG, "16 bytes"), (dict(q_row=24 * 256 - 8), iu8.E_RULE, "cover"),
     (dict(q_row=24 * 256 + 4), iu8.E_RULE, "cover"), (dict(scale=math.nan), iu8.E_RULE, "scale"), (dict(scale=math.inf), iu8.E_RULE, "scale"),
     (dict(max_q=0), iu8.E_RULE, "from 1"), (dict(max_kv=1 << 31), iu8.E_RULE, "below 2\\^31"), (dict(max_q=0xFFFFFFFF), iu8.E_RULE, "32-bit sizes"),
-    (dict(seqs=0x7FFFFFFE, max_q=1000), iu8.E_RULE, "32-bit sizes"), (dict(cu_q=None), iu8.E_RULE, "one row a sequence"),
+    (dict(seqs=0x7FFFFFFE, max_q=1000), iu8.E_RULE, "32-bit sizes"),
+    (dict(seqs=1 << 22, max_q=40, partial=None), iu8.E_RULE, "32-bit sizes"), (dict(seqs=(1 << 21) - 1, max_q=40), iu8.E_ARG, "null argument"), (dict(cu_q=None), iu8.E_RULE, "one row a sequence"),
     (dict(), iu8.E_ARG, "null argument"), (dict(partial=None, counter=None), iu8.E_ARG, "null argument"),
     (dict(cu_q=None, seqs=9, max_q=0), iu8.E_ARG, "null argument"), (dict(max_kv=0), iu8.E_ARG, "null argument")])
 def test_attn_refusals(ctx, bad, code, words):
