@@ -25,7 +25,7 @@ struct AtCache {
 };
 
 // what a scheduling group counts
-constexpr int AT_VALU = 0x2, AT_MFMA = 0x8, AT_DS_READ = 0x100;
+constexpr int AT_VALU = 0x2, AT_MFMA = 0x8, AT_DS_READ = 0x100, AT_TRANS = 0x400;
 
 // A lane's value beside the one of lane ^ 32 (or ^ 16): what both have, by one exchange between registers.
 template <int X, class F>
