@@ -10,7 +10,7 @@
 //
 // Bound by the matrix cores at the clock that they leave (60 % of their cycles busy at 8,192 tokens of 24 heads of 256: 719 to 745 us,
 // 1,107 to 1,147 TF/s, where the library's largest plain product reaches 1,348), and on short prompts by the chain of a workgroup's
-// beginning and end, about four tiles' time: five prompts of 883 to 2,100 tokens, 40 heads of 128, 185 to 192 us, 138 GF. LDS: 30 % of
+// beginning and end, about four tiles' time: five prompts of 883 to 2,100 tokens, 40 heads of 128, 180 to 189 us, 138 GF. LDS: 30 % of
 // the cycles, no conflicts (e4m3: 14 % of its accesses).
 //
 // Both products have the row as the MFMA's column (attn_few.h has why): S^T = K Q^T leaves lane (row, half) the tokens
