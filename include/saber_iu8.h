@@ -572,8 +572,9 @@ int saber_iu8_silu_table(saber_iu8_ctx *ctx, void *out_u16, void *stream);
  * sequence s; an entry outside 0 .. pages - 1 is a hole: nothing is written there and its keys take no part. Sequences
  * may share pages that no call writes. kv_len[s] counts
  * the sequence's tokens, the call's new ones included (both operators of a step read the same number); counts above
- * table_stride * page_tokens are taken as that, below 0 as 0. The counts and the table are read on the device, so a captured launch
- * follows them. */
+ * table_stride * page_tokens are taken as that, below 0 as 0. The counts, the table and cu_q are read on the device, so a captured
+ * launch follows them; they must stand still while a call runs, since a kernel reads them more than once: order whatever writes them with the
+ * calls' stream. (A count that changes under a call leaves that call's outputs, and its workspaces' counters, undefined: zero them again.) */
 #define SABER_IU8_KV_BF16 0
 #define SABER_IU8_KV_E4M3 1
 typedef struct {

@@ -9,7 +9,9 @@ from . import iu8
 
 class PagedKvCache:
     """The pages of one layer's sequences. The host deals pages (reserve, release); the table and the counts lie on the device, where
-    the kernels read them, so that a captured step follows them; reserve and release write there on torch's current stream."""
+    the kernels read them, so that a captured step follows them; reserve and release write there on torch's current stream. While a step
+    runs they must stand still: where steps take another stream than torch's current one, order the two (make it current around reserve, release
+    and writes of kv_len, or wait for the step)."""
 
     def __init__(self, seqs, kv_heads, head_dim, max_kv, pages=None, page_tokens=64, kind=iu8.KV_BF16, k_scale=None, v_scale=None, device="cuda"):
         """max_kv: the most tokens a sequence may hold; pages: of all sequences together (None: enough for all at that length);

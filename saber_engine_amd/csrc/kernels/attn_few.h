@@ -32,10 +32,9 @@
 // itself, the sum of weights taken of the unrounded ones), the output once to bf16.
 #pragma once
 #include "attn_common.h"
+#include "attn_deal.h"
 
 constexpr float AT_LOG2E = 1.44269504088896340736f;
-
-constexpr int AT_PARTS = 128;  // parts of an item at most
 
 // The tokens of a part of the many-row kernels: as the launch law cut them, or equal shares where the sequence is longer than the
 // law was told.
@@ -251,12 +250,8 @@ static __device__ __forceinline__ void attn_few_body(
     s = owner * per_lane, base = __builtin_amdgcn_readlane(before, owner);
   }
   Seq q_;
-  for (;; ++s) {
-    q_ = sequence(s);
-    const unsigned all = units_of(q_) * tiles_of(q_) * kv_heads;
-    if (base + all > at_unit) break;
-    base += all;
-  }
+  s = at_walk([&](int i) { return q_ = sequence(i), units_of(q_) * tiles_of(q_) * kv_heads; }, s, seqs, base, at_unit);
+  if (s >= seqs) return;
   unsigned u0, h, qt;
   {
     const unsigned u = units_of(q_), it = (at_unit - base) / u, tiles = tiles_of(q_);
@@ -578,7 +573,7 @@ static __device__ __forceinline__ void attn_few_body(
       if (tid < live) at_store_through(slot + R * D + tid * 4, iu8_v4f{s_m[tid], s_il[tid], 0.f, 0.f});
       iu8_stores_done();
       __syncthreads();
-      const int first = start / share, ns = (int)((start + units - 1) / share) - first + 1;  // the workgroups that have parts
+      const int first = start / share, ns = at_parts_of(start, units, share, first, grid);  // the workgroups that have parts
       if (tid == 0) {
         int *count = counter + ((size_t)s * kv_heads + h) * qtiles + qt;
         const int arrived = iu8_arrive(count);
@@ -598,8 +593,8 @@ static __device__ __forceinline__ void attn_few_body(
       qt = 0;
       if (++h == (unsigned)kv_heads) {
         h = 0;
-        do q_ = sequence(++s);
-        while (tiles_of(q_) == 0);
+        s = at_next([&](int i) { return q_ = sequence(i), tiles_of(q_); }, s, seqs);
+        if (s >= seqs) return;
       }
     }
   }
