@@ -621,6 +621,10 @@ int saber_iu8_attn_workspace(uint32_t seqs, uint32_t max_q, uint32_t max_kv, uin
                              uint64_t *partial_bytes, uint64_t *counter_bytes);
 int saber_iu8_attn(saber_iu8_ctx *ctx, const void *q, uint32_t q_row, const saber_iu8_kv_cache *cache, const int32_t *cu_q, void *out, uint32_t tokens,
                    uint32_t seqs, uint32_t max_q, uint32_t max_kv, uint32_t heads, float scale, void *partial, void *counter, void *stream);
+/* The launch that saber_iu8_attn makes of these sizes (kernel, grid, units or parts, this call's own share of the workspaces), for hosts that
+ * plan or record their launches; saber_iu8_launch runs it with the buffers bound by name. `packed`: with cu_q; `split`: with the workspaces. */
+int saber_iu8_resolve_attn(const saber_iu8_kv_cache *cache, uint32_t q_row, int packed, uint32_t tokens, uint32_t seqs, uint32_t max_q, uint32_t max_kv,
+                           uint32_t heads, float scale, int split, saber_iu8_desc *out);
 
 /* ---- tier packs ("SBRPACK1"): reading the iu8 records of a built pack ------------------------------
  * The byte layout of include/saber_abi.h:541-944 and the open-time rules of

@@ -3,6 +3,8 @@
 #include <algorithm>
 #include <cmath>
 #include <cstddef>
+#include <string_view>
+#include <utility>
 
 #include "../../../include/saber_iu8.h"
 #include "rules.h"
@@ -30,7 +32,7 @@ int log2_of(uint32_t x) {
   return s;
 }
 
-int cache_check(const char *op, const saber_iu8_kv_cache *c, uint32_t heads, uint32_t seqs, uint32_t tokens, const int32_t *cu_q) {
+int cache_check(const char *op, const saber_iu8_kv_cache *c, uint32_t heads, uint32_t seqs, uint32_t tokens, bool packed) {
   if (!c) return fail(SABER_IU8_E_ARG, fmt("%s: null cache", op));
   if (!c->k || !c->v || !c->page_table || !c->kv_len) return fail(SABER_IU8_E_ARG, fmt("%s: the cache's k, v, page_table and kv_len must be given", op));
   if (c->kind != SABER_IU8_KV_BF16 && c->kind != SABER_IU8_KV_E4M3) return fail(SABER_IU8_E_ARG, fmt("%s: unknown cache kind %u", op, c->kind));
@@ -46,7 +48,7 @@ int cache_check(const char *op, const saber_iu8_kv_cache *c, uint32_t heads, uin
   if (!c->pages || c->pages > I32_MAX || !c->table_stride || (uint64_t)c->table_stride * c->page_tokens > WHOLE)
     return fail(SABER_IU8_E_RULE, fmt("%s: %u pages, %u of %u tokens a sequence: at least one, positions below 2^31 - 256", op, c->pages, c->table_stride, c->page_tokens));
   if (!seqs || !tokens || seqs >= I32_MAX || tokens > I32_MAX) return fail(SABER_IU8_E_RULE, fmt("%s: %u rows of %u sequences has nothing to do", op, tokens, seqs));
-  if (!cu_q && tokens != seqs) return fail(SABER_IU8_E_RULE, fmt("%s: %u rows of %u sequences without cu_q (one row a sequence)", op, tokens, seqs));
+  if (!packed && tokens != seqs) return fail(SABER_IU8_E_RULE, fmt("%s: %u rows of %u sequences without cu_q (one row a sequence)", op, tokens, seqs));
   return 0;
 }
 
@@ -181,6 +183,21 @@ constexpr const char *APPEND[2][3] = NAMES("kv_append", ""), *FEW16[2][3] = NAME
 #undef NAMES
 int dim_index(uint32_t dim) { return dim == 64 ? 0 : dim == 128 ? 1 : 2; }
 
+const char *kernel_of(const Plan &p, const saber_iu8_kv_cache *c) {
+  const auto &names = p.rows == 16 ? FEW16 : p.rows == FEW_ROWS ? FEW32 : MANY;
+  return names[c->kind == SABER_IU8_KV_E4M3][dim_index(c->head_dim)];
+}
+
+// The scalars of a call on a cache that cache_check has passed, and its plan; `split`: the workspaces are there.
+int attn_law(const char *op, const saber_iu8_kv_cache *c, uint32_t q_row, bool packed, uint32_t seqs, uint32_t max_q, uint32_t max_kv, uint32_t heads, float scale,
+             bool split, Plan *p) {
+  if (q_row % 8 || q_row > I32_MAX || q_row < (uint64_t)heads * c->head_dim)
+    return fail(SABER_IU8_E_RULE, fmt("%s: rows of %u elements: whole 16-byte pieces that cover %u heads of %u", op, q_row, heads, c->head_dim));
+  if (!std::isfinite(scale)) return fail(SABER_IU8_E_RULE, fmt("%s: the scale must be a number", op));
+  return attn_plan(op, seqs, packed ? max_q : 1, max_kv, heads, c->kv_heads, c->head_dim, c->kind == SABER_IU8_KV_E4M3, !split,
+                   (uint64_t)c->table_stride * c->page_tokens, p);
+}
+
 const saber_iu8_slot *slot(const saber_iu8_desc *d, const char *name) {
   for (uint32_t i = 0; i < d->n_args; ++i)
     if (!strcmp(d->args[i].name, name)) return &d->args[i];
@@ -242,7 +259,7 @@ uint64_t saber_iu8_kv_v_offset(uint32_t page, uint32_t kv_head, uint32_t token, 
 int saber_iu8_kv_append(saber_iu8_ctx *ctx, const void *q, const void *k, const void *v, void *q_out, const saber_iu8_kv_cache *cache,
                         const int32_t *cu_q, uint32_t tokens, uint32_t seqs, uint32_t heads, uint32_t q_row, uint32_t q_head, uint32_t kv_row,
                         const double *inv_freq, uint32_t rot_dim, int interleaved, const void *q_norm, const void *k_norm, float eps, void *stream) {
-  if (int rc = cache_check("kv_append", cache, heads, seqs, tokens, cu_q)) return rc;
+  if (int rc = cache_check("kv_append", cache, heads, seqs, tokens, cu_q != nullptr)) return rc;
   const uint32_t D = cache->head_dim;
   if (!q || !k || !v || !q_out) return fail(SABER_IU8_E_ARG, "kv_append: null rows");
   if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q_out | (uintptr_t)q_norm | (uintptr_t)k_norm) % 16)
@@ -279,17 +296,11 @@ int saber_iu8_attn_workspace(uint32_t seqs, uint32_t max_q, uint32_t max_kv, uin
 
 int saber_iu8_attn(saber_iu8_ctx *ctx, const void *q, uint32_t q_row, const saber_iu8_kv_cache *cache, const int32_t *cu_q, void *out, uint32_t tokens,
                    uint32_t seqs, uint32_t max_q, uint32_t max_kv, uint32_t heads, float scale, void *partial, void *counter, void *stream) {
-  if (int rc = cache_check("attn", cache, heads, seqs, tokens, cu_q)) return rc;
-  const uint32_t D = cache->head_dim;
+  if (int rc = cache_check("attn", cache, heads, seqs, tokens, cu_q != nullptr)) return rc;
   if (!q || !out) return fail(SABER_IU8_E_ARG, "attn: null rows");
   if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)partial) % 16 || (uintptr_t)counter % 4) return fail(SABER_IU8_E_ARG, "attn: rows and partials must lie on 16 bytes");
-  if (q_row % 8 || q_row > I32_MAX || q_row < (uint64_t)heads * D)
-    return fail(SABER_IU8_E_RULE, fmt("attn: rows of %u elements: whole 16-byte pieces that cover %u heads of %u", q_row, heads, D));
-  if (!std::isfinite(scale)) return fail(SABER_IU8_E_RULE, "attn: the scale must be a number");
-  if (!cu_q) max_q = 1;
   Plan p;
-  const bool f8 = cache->kind == SABER_IU8_KV_E4M3;
-  if (int rc = attn_plan("attn", seqs, max_q, max_kv, heads, cache->kv_heads, D, f8, !partial || !counter, (uint64_t)cache->table_stride * cache->page_tokens, &p)) return rc;
+  if (int rc = attn_law("attn", cache, q_row, cu_q != nullptr, seqs, max_q, max_kv, heads, scale, partial && counter, &p)) return rc;
   AttnArgs x{};
   x.q = q, x.cache = cache_of(cache), x.cu_q = cu_q, x.out = out, x.q_row = (int32_t)q_row;
   if (p.partial) x.partial = partial, x.counter = counter;
@@ -297,8 +308,39 @@ int saber_iu8_attn(saber_iu8_ctx *ctx, const void *q, uint32_t q_row, const sabe
                 stride = (int32_t)cache->table_stride;
   if (p.few()) x.few = {(int32_t)tokens, (int32_t)seqs, shape, page_shift, pages, stride, p.unit_shift, (int32_t)p.qtiles, scale};
   else x.many = {(int32_t)tokens, shape, page_shift, pages, stride, (int32_t)p.chunk, (int32_t)p.splits, (int32_t)p.qtiles, scale};
-  const auto &names = p.rows == 16 ? FEW16 : p.rows == FEW_ROWS ? FEW32 : MANY;
-  return launch_image(ctx, names[f8][dim_index(D)], (uint32_t)p.grid, 256, &x, sizeof x, stream);
+  return launch_image(ctx, kernel_of(p, cache), (uint32_t)p.grid, 256, &x, sizeof x, stream);
+}
+
+int saber_iu8_resolve_attn(const saber_iu8_kv_cache *cache, uint32_t q_row, int packed, uint32_t tokens, uint32_t seqs, uint32_t max_q, uint32_t max_kv,
+                           uint32_t heads, float scale, int split, saber_iu8_desc *d) {
+  if (!d) return fail(SABER_IU8_E_ARG, "resolve_attn: null descriptor");
+  if (int rc = cache_check("resolve_attn", cache, heads, seqs, tokens, packed)) return rc;
+  Plan p;
+  if (int rc = attn_law("resolve_attn", cache, q_row, packed, seqs, max_q, max_kv, heads, scale, split, &p)) return rc;
+  const uint32_t grid[3] = {(uint32_t)p.grid, 1, 1};
+  if (int rc = saber_iu8_describe_raw(kernel_of(p, cache), "attn_paged", grid, 256, d)) return rc;
+  snprintf(d->op, sizeof d->op, "attn");
+  const std::pair<const char *, int64_t> scalars[] = {
+      {"q_row", q_row}, {"tokens", tokens}, {"seqs", seqs}, {"shape", heads | (int64_t)cache->kv_heads << 16}, {"page_shift", log2_of(cache->page_tokens)},
+      {"pages", cache->pages}, {"table_stride", cache->table_stride}, {"unit_shift", p.unit_shift}, {"chunk", p.chunk}, {"splits", p.splits}, {"qtiles", (int64_t)p.qtiles}};
+  for (const auto &[name, value] : scalars)
+    if (slot(d, name)) (void)saber_iu8_desc_set_i32(d, name, value);
+  for (uint32_t i = 0; i < d->n_args; ++i) {
+    saber_iu8_slot &s = d->args[i];
+    const std::string_view name = s.name;
+    if (name == "scale") s.fval = scale;
+    if ((!packed && name == "cu_q") || (cache->kind != SABER_IU8_KV_E4M3 && (name == "k_scale" || name == "v_scale")) ||
+        (!p.partial && (name == "partial" || name == "counter")))
+      s.kind = SABER_IU8_ARG_NULL_BUFFER;
+  }
+  if (p.partial) {
+    d->n_workspaces = 2;
+    snprintf(d->workspaces[0].name, sizeof d->workspaces[0].name, "partial");
+    d->workspaces[0].kind = SABER_IU8_WS_SCRATCH, d->workspaces[0].bytes = p.partial;
+    snprintf(d->workspaces[1].name, sizeof d->workspaces[1].name, "counter");
+    d->workspaces[1].kind = SABER_IU8_WS_PERSISTENT, d->workspaces[1].bytes = p.counter, d->workspaces[1].zero_once = 1;
+  }
+  return 0;
 }
 
 }  // extern "C"

@@ -185,6 +185,7 @@ def lib():
         L.saber_iu8_attn_workspace.argtypes = [C.c_uint32] * 6 + [C.POINTER(C.c_uint64)] * 2
         L.saber_iu8_attn.argtypes = ([C.c_void_p, C.c_void_p, C.c_uint32, C.POINTER(KvCache), C.c_void_p, C.c_void_p] + [C.c_uint32] * 5 +
                                      [C.c_float] + [C.c_void_p] * 3)
+        L.saber_iu8_resolve_attn.argtypes = ([C.POINTER(KvCache), C.c_uint32, C.c_int] + [C.c_uint32] * 5 + [C.c_float, C.c_int, C.POINTER(Desc)])
         L.saber_iu8_silu_table.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p]
         _lib = L
     return _lib
@@ -606,6 +607,13 @@ def attn_workspace(seqs, max_q, max_kv, heads, kv_heads, head_dim):
     p, c = C.c_uint64(), C.c_uint64()
     _check(lib().saber_iu8_attn_workspace(seqs, max_q, max_kv, heads, kv_heads, head_dim, C.byref(p), C.byref(c)))
     return p.value, c.value
+
+
+def resolve_attn(cache, q_row, tokens, seqs, max_q, max_kv, heads, scale, packed=True, split=True):
+    """The launch that attn() makes of these sizes (packed: with cu_q; split: with the workspaces)."""
+    d = Desc()
+    _check(lib().saber_iu8_resolve_attn(C.byref(cache), q_row, int(packed), tokens, seqs, max_q, max_kv, heads, scale, int(split), C.byref(d)))
+    return d
 
 
 def kv_bytes(pages, kv_heads, head_dim, page_tokens, kind=KV_BF16):

@@ -1,0 +1,67 @@
+"""CPU tests of the launch that `attn` makes (csrc/host/attn.cpp), as resolve_attn describes it."""
+import random
+
+import pytest
+
+from saber_engine_amd import iu8
+
+P = 1 << 40        # an address: nothing here is launched
+
+
+def cache(kvh, dim, e4m3=False, page=64, stride=4096):
+    return iu8.KvCache.of(P, P, P, P, kv_heads=kvh, head_dim=dim, page_tokens=page, pages=1000, table_stride=stride, kind=iu8.KV_E4M3 if e4m3 else iu8.KV_BF16,
+                          k_scale=P if e4m3 else None, v_scale=P if e4m3 else None)
+
+
+def plan(dim, kvh, group, e4m3, seqs, max_q, max_kv, tokens=None, packed=True, split=True, **more):
+    heads = kvh * group
+    tokens = (seqs * max_q if packed else seqs) if tokens is None else tokens
+    return iu8.resolve_attn(cache(kvh, dim, e4m3, **more), heads * dim, tokens, seqs, max_q, max_kv, heads, 0.125, packed, split)
+
+
+def scalar(d, name):
+    return next(s.ival for s in d.args[:d.n_args] if s.name == name.encode())
+
+
+def kinds(d):
+    return {s.name.decode(): s.kind for s in d.args[:d.n_args]}
+
+
+def test_the_descriptor_says_what_the_call_takes():
+    d = plan(256, 4, 6, False, 1, 1, 1800, packed=False)
+    assert (d.op, d.plugin, d.kernel, d.grid[0], d.block[0]) == (b"attn", b"attn_paged", b"attn_few_bf16_d256_r16", 60, 256)
+    k = kinds(d)
+    assert k["cu_q"] == k["k_scale"] == k["v_scale"] == iu8.ARG_NULL_BUFFER and k["partial"] == k["counter"] == k["q"] == iu8.ARG_BUFFER
+    assert [(w.name, w.bytes, w.zero_once) for w in d.workspaces[:d.n_workspaces]] == [(b"partial", 60 * 2 * 16 * 260 * 4, 0), (b"counter", 16, 1)]
+    assert scalar(d, "shape") == 24 | 4 << 16 and scalar(d, "unit_shift") == 7 and scalar(d, "page_shift") == 6 and scalar(d, "q_row") == 24 * 256
+    d = plan(128, 2, 6, True, 1, 300, 6000)
+    assert d.kernel == b"attn_many_e4m3_d128" and scalar(d, "splits") > 1 and d.grid[0] == 2 * 15 * scalar(d, "splits")
+    assert kinds(d)["k_scale"] == kinds(d)["cu_q"] == iu8.ARG_BUFFER
+    d = plan(128, 2, 6, True, 1, 300, 6000, split=False)
+    assert d.kernel == b"attn_many_e4m3_d128" and scalar(d, "splits") == 1 and d.n_workspaces == 0 and kinds(d)["partial"] == iu8.ARG_NULL_BUFFER
+
+
+def test_the_descriptor_is_refused_as_the_call_is():
+    for bad, words in ((dict(max_q=0, tokens=5), "from 1"), (dict(max_kv=1 << 31), "below 2"), (dict(tokens=0), "nothing to do"), (dict(tokens=2, packed=False), "one row a sequence"),
+                       (dict(stride=1 << 26), "positions below")):
+        a = dict(dim=64, kvh=2, group=2, e4m3=False, seqs=1, max_q=5, max_kv=100)
+        a.update(bad)
+        with pytest.raises(iu8.IU8Error, match=words) as e:
+            plan(**a)
+        assert e.value.code == iu8.E_RULE
+    with pytest.raises(iu8.IU8Error, match="cover"):
+        iu8.resolve_attn(cache(2, 64), 252, 1, 1, 1, 100, 4, 0.125)
+    with pytest.raises(iu8.IU8Error, match="number"):
+        iu8.resolve_attn(cache(2, 64), 256, 1, 1, 1, 100, 4, float("nan"))
+
+
+def test_a_call_takes_no_more_than_its_workspaces():
+    rng = random.Random(5)
+    for _ in range(4000):
+        kvh, group, dim, e4m3 = rng.choice([1, 2, 4, 8]), rng.choice([1, 3, 5, 6, 8, 16, 17, 40]), rng.choice([64, 128, 256]), rng.random() < 0.5
+        most = [rng.choice([1, 2, 9, 64, 300]), rng.choice([1, 2, 5, 40, 200, 1000, 9000]), rng.choice([1, 129, 600, 1500, 5000, 140000])]
+        less = [rng.randint(1, x) for x in most]
+        sizes = iu8.attn_workspace(*most, kvh * group, kvh, dim)
+        d = plan(dim, kvh, group, e4m3, *less)
+        took = [w.bytes for w in d.workspaces[:d.n_workspaces]] or [0, 0]
+        assert took[0] <= sizes[0] and took[1] <= sizes[1], (most, less, kvh, group, dim, e4m3)
