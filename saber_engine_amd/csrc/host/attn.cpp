@@ -18,8 +18,8 @@ constexpr uint32_t FEW_ROWS = 32;    // rows a kv head and sequence up to which 
 constexpr uint32_t MANY_ROWS = 128;  // rows a workgroup of the many-row kernels
 constexpr int FEW_UNIT_SHIFT = 7, WHOLE_SHIFT = 31;  // log2 of the tokens a unit of the few-row kernels' deal (attn_few.h)
 constexpr uint32_t MANY_PARTS = 32;  // parts of an item at most: their maxima and sums lie in one workgroup's LDS when they are joined
-// more than 32 rows on the few-row kernels: units a row tile from, units of all up to
-constexpr uint64_t FEW_UNITS_MIN = 8, FEW_UNITS_MAX = 5 * CU_COUNT, FEW_UNITS_MAX_E4M3 = 16 * CU_COUNT;
+// more than 32 rows on the few-row kernels: units a row tile from, units of all up to, and up to for whole prompts
+constexpr uint64_t FEW_UNITS_MIN = 8, FEW_UNITS_MAX = 5 * CU_COUNT, FEW_UNITS_MAX_E4M3 = 16 * CU_COUNT, FEW_UNITS_PROMPT = 3 * CU_COUNT, FEW_UNITS_PROMPT_E4M3 = 8 * CU_COUNT;
 constexpr uint64_t FEW_BRIEF = 1200, FEW_LONG = 48;  // units of all below which a part's beginning and end weigh more than its bytes; units of a long item
 constexpr uint64_t MANY_TARGET = 2 * CU_COUNT, MANY_LEAST = 320, MANY_LONG = 2048;  // workgroups that the card holds; tokens a part, from; long ones
 constexpr uint64_t MANY_UNEVEN = 448, MANY_LONGEST = 8192;  // row tiles that leave an eighth of the places empty, up to; keys that make that worth more parts
@@ -63,10 +63,14 @@ struct Plan {
 
 // Which kernels, and the grid. Few rows (attn_few.h) up to 32 a kv head and sequence; above, still where a long cache meets so
 // few rows that its tiles of 32 make at most a unit a CU (60 new tokens of group 6 on 300 keys, head width 256: 19.7 us against 21.2 of
-// the many-row kernel; 60 on 600 24.6 / 31.7; 60 of group 5 on 300, width 128, 13.3 / 16.3 -- but not whole prompts of one or two units, half of
-// which is masked: 200 on 200, 20.9 / 17.9) or, on eight units and more, five a CU (200 of group 6 on 1,000 35 / 45; on 1,600, at eight
+// the many-row kernel; 60 on 600 24.6 / 31.7; 60 of group 5 on 300, width 128, 13.3 / 16.3) or, on eight units and more, five a CU (200 of group 6 on 1,000 35 / 45; on 1,600, at eight
 // a CU, 56 / 44), sixteen a CU in e4m3, which the many-row kernel widens through registers (60 of group 6 on 4,000: 39 / 61; 8 sequences
-// of 8 rows each 35 / 44; 32 of them, at 32 a CU, 94 / 93). Their grid, among which the units are dealt level: a workgroup a CU; two where both fit one's LDS and the items
+// of 8 rows each 35 / 44; 32 of them, at 32 a CU, 94 / 93). Of a whole prompt causality hides half, which the few-row kernels walk all the same and
+// the many-row kernels do not, so where the new rows are most of the keys the bounds lie lower: three units a CU in bf16 (900 of group 3 on
+// themselves, 2.7 units a CU, width 64 / 128 / 256: 14 / 19 / 30 us against 17 / 24 / 39; of group 4, 3.5: 20 / 28 / 45 against 17 / 23 / 39; 900 on 1,200, 4.4: 17 / 24 / 38
+// against 18 / 25 / 42), eight in e4m3 (900 of 8 heads on 2, 7.1: 18 / 23 / 34 against 19 / 27 / 44; 1,150, 10: 29 / 40 / 60 against 19 / 27 / 42; 1,400 of 8 on 1, 15: 37 / 48 / 73
+// against 25 / 34 / 55), and four units, in e4m3 three, where all make at most one a CU (bf16, 300 of group 4: 11 / 15 / 24 against 11 / 14 / 20, 400: 13 / 17 / 27 against 13 /
+// 18 / 29; e4m3, 300: 10 / 13 / 18 against 13 / 17 / 22; of one or two units, 200 on 200, bf16: 21 / 18 at width 256). Their grid, among which the units are dealt level: a workgroup a CU; two where both fit one's LDS and the items
 // suffice for nearly all of them to stay whole (256 sequences of 1,000 keys, 8 heads of 128 in e4m3: 256 workgroups 98 us, 512 86; 32 of 2,400 in
 // bf16, 256 items: 51 against 55); fewer where few items would be cut into many parts, whose join costs a round of loads for every
 // 16 (5,000 keys, 8 heads of 128: 128 workgroups 13.5 us, 256 15.7, 512 20.0; 4 heads of 256 on 131,072: 128 102, 192 92, 256 96).
@@ -81,7 +85,9 @@ Plan plan(uint32_t seqs, uint32_t max_q, uint32_t max_kv, uint32_t heads, uint32
   Plan p{};
   const uint64_t rows = (uint64_t)max_q * (heads / kv_heads), units = max_kv ? ((max_kv - 1) >> FEW_UNIT_SHIFT) + 1 : 1;
   const uint64_t all32 = (uint64_t)seqs * kv_heads * ((rows + FEW_ROWS - 1) / FEW_ROWS) * units;
-  const bool sparse = !whole && ((units >= FEW_UNITS_MIN && all32 <= (f8 ? FEW_UNITS_MAX_E4M3 : FEW_UNITS_MAX)) || (units >= 3 && all32 <= CU_COUNT));
+  const bool prompt = (uint64_t)max_q * 8 > (uint64_t)max_kv * 7;  // new rows are most of the keys
+  const uint64_t most = prompt ? (f8 ? FEW_UNITS_PROMPT_E4M3 : FEW_UNITS_PROMPT) : f8 ? FEW_UNITS_MAX_E4M3 : FEW_UNITS_MAX;
+  const bool sparse = !whole && ((units >= FEW_UNITS_MIN && all32 <= most) || (units >= (prompt && !f8 ? 4 : 3) && all32 <= CU_COUNT));
   p.rows = rows <= 16 ? 16 : rows <= FEW_ROWS || sparse ? FEW_ROWS : MANY_ROWS;
   p.qtiles = (rows + p.rows - 1) / p.rows;
   p.items = (uint64_t)seqs * kv_heads * p.qtiles;

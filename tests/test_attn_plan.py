@@ -65,3 +65,17 @@ def test_a_call_takes_no_more_than_its_workspaces():
         d = plan(dim, kvh, group, e4m3, *less)
         took = [w.bytes for w in d.workspaces[:d.n_workspaces]] or [0, 0]
         assert took[0] <= sizes[0] and took[1] <= sizes[1], (most, less, kvh, group, dim, e4m3)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_whole_prompts_take_the_kernels_that_skip_what_causality_hides(dim):
+    """The few-row kernels walk a prompt's hidden half, the many-row kernels do not: from three (bf16) and eight (e4m3) units of 128 keys a CU on
+    a whole prompt is the many-row kernels'; the same rows behind a prefix, and prompts below, stay."""
+    def many(e4m3, kvh, group, new, kv, seqs=1):
+        return b"many" in plan(dim, kvh, group, e4m3, seqs, new, kv).kernel
+    for e4m3, kvh, group, new in ((True, 2, 8, 1024), (True, 1, 8, 1400), (True, 1, 5, 1700), (True, 2, 4, 1150), (True, 2, 8, 900), (False, 1, 4, 900), (False, 1, 4, 1000),
+                                  (False, 1, 2, 300), (False, 1, 8, 300), (False, 1, 6, 200), (True, 4, 6, 200)):
+        assert many(e4m3, kvh, group, new, new), (e4m3, kvh, group, new)
+    for e4m3, kvh, group, new, kv in ((True, 2, 4, 900, 900), (True, 1, 8, 300, 300), (True, 1, 5, 1000, 1000), (False, 1, 3, 900, 900), (False, 1, 1, 1400, 1400), (False, 1, 4, 400, 400),
+                                      (True, 2, 8, 500, 1000), (True, 1, 8, 1000, 1333), (False, 1, 4, 900, 1200), (False, 1, 8, 220, 293), (True, 1, 8, 300, 4800)):
+        assert not many(e4m3, kvh, group, new, kv), (e4m3, kvh, group, new, kv)
