@@ -20,7 +20,7 @@ constexpr int FEW_UNIT_SHIFT = 7, WHOLE_SHIFT = 31;  // log2 of the tokens a uni
 constexpr uint32_t MANY_PARTS = 32;  // parts of an item at most: their maxima and sums lie in one workgroup's LDS when they are joined
 // more than 32 rows on the few-row kernels: units a row tile from, units of all up to, and up to for whole prompts
 constexpr uint64_t FEW_UNITS_MIN = 8, FEW_UNITS_MAX = 5 * CU_COUNT, FEW_UNITS_MAX_E4M3 = 16 * CU_COUNT, FEW_UNITS_PROMPT = 3 * CU_COUNT, FEW_UNITS_PROMPT_E4M3 = 8 * CU_COUNT;
-constexpr uint64_t FEW_BRIEF = 1200, FEW_LONG = 48;  // units of all below which a part's beginning and end weigh more than its bytes; units of a long item
+constexpr uint64_t FEW_BRIEF = 1200;  // units of all below which a part's beginning and end weigh more than its bytes
 constexpr uint64_t MANY_TARGET = 2 * CU_COUNT, MANY_LEAST = 320, MANY_LONG = 2048;  // workgroups that the card holds; tokens a part, from; long ones
 constexpr uint64_t MANY_UNEVEN = 448, MANY_LONGEST = 8192;  // row tiles that leave an eighth of the places empty, up to; keys that make that worth more parts
 constexpr uint32_t I32_MAX = 0x7FFFFFFFu, GRID_MAX = 0xFFFFFFu;  // workgroups of 256 whose threads a launch counts in 32 bits
@@ -74,8 +74,9 @@ struct Plan {
 // suffice for nearly all of them to stay whole (256 sequences of 1,000 keys, 8 heads of 128 in e4m3: 256 workgroups 98 us, 512 86; 32 of 2,400 in
 // bf16, 256 items: 51 against 55); fewer where few items would be cut into many parts, whose join costs a round of loads for every
 // 16 (5,000 keys, 8 heads of 128: 128 workgroups 13.5 us, 256 15.7, 512 20.0; 4 heads of 256 on 131,072: 128 102, 192 92, 256 96).
-// Long bf16 streams on every CU take three quarters of them (64 sequences of up to 8,192, 8 heads of 128: 192 198, 256 203, 512 201; 32 of 20,000
-// 381 / 387 / 389; 32 of 10,000 level; e4m3 loses by it, 112 / 105).
+// Long streams as the others: fewer workgroups gain nothing where tiles are large (64 sequences of up to 8,192, 8 heads of 128, 192 / 256 / 512: 201 / 201 /
+// 200; 32 of 20,000 382 / 386 / 388; 128 of 8,192, 4 heads of 256, 192 / 256: 646 / 620) and lose bytes in flight where they are small (64 of up to 8,192, 8 heads of
+// 64: 120 / 112 / 105; 32 of 20,000, tiles of 32 rows, 192 / 256: 226 / 206).
 // Many rows: parts where the row tiles alone are fewer than the CUs, one workgroup a CU (400 rows of group 6, 76 tiles, on 3,000 keys:
 // one part 112 us, three 62, four 68, six 69 to 85), two a CU where the parts are long (512 rows, 96 tiles, on 16,896: two parts
 // 395 us, five 248 to 271), three or two each where the row tiles are between one and two a CU and the keys many (1,200 rows of 32 heads on 8
@@ -94,9 +95,8 @@ Plan plan(uint32_t seqs, uint32_t max_q, uint32_t max_kv, uint32_t heads, uint32
   p.splits = 1, p.chunk = WHOLE, p.unit_shift = WHOLE_SHIFT;
   if (p.few()) {
     const bool two = p.rows == 16 && (f8 || dim < 256) && p.items >= 2 * CU_COUNT, brief = p.items * units < FEW_BRIEF;
-    const bool stream = !f8 && units >= FEW_LONG && p.items * units >= 64 * CU_COUNT;
-    const uint64_t slots = stream ? CU_COUNT * 3 / 4 : two ? 2 * CU_COUNT
-                                  : std::clamp<uint64_t>((brief ? 16 : 48) * p.items, brief ? CU_COUNT / 2 : CU_COUNT * 3 / 4, CU_COUNT);
+    const uint64_t slots = two ? 2 * CU_COUNT
+                               : std::clamp<uint64_t>((brief ? 16 : 48) * p.items, brief ? CU_COUNT / 2 : CU_COUNT * 3 / 4, CU_COUNT);
     if (!whole && units > 1) {
       p.unit_shift = FEW_UNIT_SHIFT;
       while (p.unit_shift < WHOLE_SHIFT && p.items * ((held >> p.unit_shift) + 1) > I32_MAX) ++p.unit_shift;  // the kernel counts them in 32 bits

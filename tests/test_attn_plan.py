@@ -79,3 +79,12 @@ def test_whole_prompts_take_the_kernels_that_skip_what_causality_hides(dim):
     for e4m3, kvh, group, new, kv in ((True, 2, 4, 900, 900), (True, 1, 8, 300, 300), (True, 1, 5, 1000, 1000), (False, 1, 3, 900, 900), (False, 1, 1, 1400, 1400), (False, 1, 4, 400, 400),
                                       (True, 2, 8, 500, 1000), (True, 1, 8, 1000, 1333), (False, 1, 4, 900, 1200), (False, 1, 8, 220, 293), (True, 1, 8, 300, 4800)):
         assert not many(e4m3, kvh, group, new, kv), (e4m3, kvh, group, new, kv)
+
+
+@pytest.mark.parametrize("dim,kvh,group,max_q,seqs,kv,grid", [
+    (64, 8, 1, 1, 64, 8192, 512), (64, 8, 5, 1, 256, 8192, 512), (64, 8, 5, 1, 32, 20000, 256), (64, 8, 4, 8, 64, 8192, 256), (128, 8, 5, 1, 64, 8192, 512),
+    (128, 8, 4, 8, 32, 20000, 256), (256, 4, 6, 1, 128, 8192, 256), (256, 4, 6, 5, 128, 8192, 256)])
+def test_long_streams_take_every_compute_unit(dim, kvh, group, max_q, seqs, kv, grid):
+    """As many as fit: a workgroup's tiles are what is in flight, 32 KiB of them at width 64."""
+    d = plan(dim, kvh, group, False, seqs, max_q, kv)
+    assert b"few" in d.kernel and d.grid[0] == grid == plan(dim, kvh, group, False, seqs, max_q, 6000).grid[0]
