@@ -592,7 +592,8 @@ uint64_t saber_iu8_kv_v_offset(uint32_t page, uint32_t kv_head, uint32_t token, 
                                uint32_t page_tokens, uint32_t kind);
 
 /* The new tokens of `seqs` sequences into the cache. Rows cu_q[s] .. cu_q[s + 1] - 1 (device, [seqs + 1]) are sequence s's newest
- * tokens, at positions kv_len[s] - n .. kv_len[s] - 1; cu_q NULL: one row a sequence. Rows in front of the first sequence and behind the
+ * tokens, at positions kv_len[s] - n .. kv_len[s] - 1; cu_q NULL: one row a sequence. An end past `tokens` counts for the positions (of this call
+ * and of the attention's); only the rows of `tokens` are read and written. Rows in front of the first sequence and behind the
  * last (of `tokens`), and rows whose position would be negative, are left as they were, in q_out as in the cache.
  *   q [tokens] rows `q_row` elements apart, head h at h * q_head (q_head = 2 * head_dim reads a gated projection's [q | gate] heads
  *   in place); k, v rows `kv_row` apart, heads head_dim apart; q_out [tokens, heads, head_dim].

@@ -172,13 +172,15 @@ static __device__ __forceinline__ void attn_few_body(
 
   // ---- this workgroup's units
   struct Seq {
-    int t0, nq, len;
+    int t0, nq, pos, len;
   };
-  auto sequence = [&](int i) {  // its new rows and its length
+  auto sequence = [&](int i) {  // its new rows (those of `tokens`), the first one's position, its length
     Seq x;
     x.t0 = cu_q ? cu_q[i] : i;
-    x.nq = min((cu_q ? cu_q[i + 1] : i + 1), tokens) - x.t0;
+    const int to = cu_q ? cu_q[i + 1] : i + 1;
+    x.nq = min(to, tokens) - x.t0;
     x.len = at_len(kv_len, i, table_stride, page_shift);
+    x.pos = x.len - (to - x.t0);
     return x;
   };
   auto own_units = [&](const Seq &x) { return (unsigned)((max(x.len, 1) - 1) >> unit_shift) + 1; };
@@ -282,9 +284,9 @@ static __device__ __forceinline__ void attn_few_body(
   for (;;) {
     // ---- a segment: units u0 .. of one item
     const unsigned units = units_of(q_), u1 = min(units, u0 + (last_unit - at_unit));
-    const int nq = q_.nq, t0 = q_.t0, len = q_.len, begin = u0 << unit_shift, end = u1 == units ? len : (int)(u1 << unit_shift);
+    const int nq = q_.nq, t0 = q_.t0, pos = q_.pos, len = q_.len, begin = u0 << unit_shift, end = u1 == units ? len : (int)(u1 << unit_shift);
     const int live = (int)min((long long)nq * G - (long long)qt * R, (long long)R);
-    const int free_end = len - nq + (int)(qt * R) / G + 1;  // tokens below it are seen by every row
+    const int free_end = pos + (int)(qt * R) / G + 1;  // tokens below it are seen by every row
     const int *row = table + (size_t)s * table_stride;
     auto fetch = [&](int tile, int (&p)[2]) {
 #pragma unroll
@@ -322,7 +324,7 @@ static __device__ __forceinline__ void attn_few_body(
     for (int rt = 0; rt < RT; ++rt) {
       const int r = (int)qt * R + rt * 16 + n, i = r / G;
       const bool real = rt * 16 + n < live;
-      limit[rt] = real ? len - nq + i : len - 1;
+      limit[rt] = real ? pos + i : len - 1;
       const unsigned short *src = q + (size_t)(t0 + (real ? i : 0)) * q_row + (size_t)(h * G + (real ? r - i * G : 0)) * D;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {

@@ -40,13 +40,13 @@ static __device__ __forceinline__ void attn_many_body(
   const int tid = threadIdx.x, lane = tid & 63, wave = at_uniform(tid >> 6), n = lane & 31, hf = lane >> 5;
 
   const int t0 = cu_q ? cu_q[s] : s;
-  const int nq = min((cu_q ? cu_q[s + 1] : s + 1), tokens) - t0;
-  const int len = at_len(kv_len, s, table_stride, page_shift);
+  const int to = cu_q ? cu_q[s + 1] : s + 1, nq = min(to, tokens) - t0;
+  const int len = at_len(kv_len, s, table_stride, page_shift), pos = len - (to - t0);  // of the first new row
   const long long all = (long long)max(nq, 0) * G;
   if ((long long)qt * R >= all) return;
   const int live = (int)min((long long)R, all - (long long)qt * R);
   const int i_first = qt * R / G, i_last = (qt * R + live - 1) / G;
-  const int kv_end = max(min(len, len - nq + i_last + 1), 0), free_end = len - nq + i_first + 1;
+  const int kv_end = max(min(len, pos + i_last + 1), 0), free_end = pos + i_first + 1;
   chunk = at_chunk(kv_end, chunk, splits);
   const int ns = kv_end > chunk ? (kv_end + chunk - 1) / chunk : 1;
   if (split >= ns) return;
@@ -59,7 +59,7 @@ static __device__ __forceinline__ void attn_many_body(
 
   const int r = qt * R + wave * 32 + n, i = r / G;
   const bool real = wave * 32 + n < live;
-  if (hf == 0) s_limit[wave * 32 + n] = real ? len - nq + i : len - 1;
+  if (hf == 0) s_limit[wave * 32 + n] = real ? pos + i : len - 1;
   const float ks_ = F8 ? k_scale[h] : 1.f, vs = F8 ? v_scale[h] : 1.f, cs = scale * AT_LOG2E * ks_;
   const unsigned flip = cs < 0.f ? 0x80008000u : 0u;  // attn_few.h
   const float c = at_uniform_f(fmaxf(fabsf(cs), 1e-37f));

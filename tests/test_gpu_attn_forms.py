@@ -199,3 +199,32 @@ def test_few_rows_by_their_descriptor(ctx, e4m3):
         again = torch.zeros_like(c.out)
         c.launch(ctx, again)
         assert torch.equal(again.view(torch.int16), c.out.view(torch.int16)) and not c.ws.counter.any()
+
+
+# ------------------------------------------------------------------ rows and positions
+
+@pytest.mark.parametrize("dim,heads,kvh,lens,news,form", [
+    (64, 4, 2, [50, 300], [3, 6], "attn_few_r16"), (128, 8, 2, [50, 300], [3, 8], "attn_few_r32"), (256, 4, 2, [50, 200], [30, 130], "attn_many"),
+    (128, 4, 2, [50, 200], [30, 130], "attn_many")])
+def test_an_end_past_the_call_s_rows_counts_for_the_positions(ctx, dim, heads, kvh, lens, news, form):
+    """The last sequence's end lies behind `tokens`: both operators give the rows that are there what they are given in the whole call, and
+    touch no others."""
+    say(f"end past tokens {form} {dim}")
+    c = Call(dim, heads, kvh, lens, news, split=False).takes(form, False)
+    whole, less = c.run(ctx).clone(), c.tokens - 2
+    c.check([(1, news[1] - 3)])
+    c.out.fill_(7.0)
+    c.tokens = less
+    c.run(ctx)
+    assert torch.equal(c.out[:less].view(torch.int16), whole[:less].view(torch.int16)) and (c.out[less:] == 7).all()
+    rows = random_rows(torch.Generator().manual_seed(3), sum(news), (heads + 2 * kvh) * dim)
+    p, row, got = rows.data_ptr(), rows.shape[1], []
+    for tokens in (sum(news), less):
+        c.c.k.view(torch.uint8).zero_(), c.c.v.view(torch.uint8).zero_()
+        q_out = torch.full((sum(news), heads * dim), 7.0, dtype=torch.bfloat16, device="cuda")
+        ctx.kv_append(p, p + 2 * heads * dim, p + 2 * (heads + kvh) * dim, q_out.data_ptr(), c.c.desc(), c.cu.data_ptr(), tokens, 2, heads, row, dim, row)
+        torch.cuda.synchronize()
+        got.append((q_out, *c.c.rows(1, lens[1])[:2]))
+    (q0, k0, v0), (q1, k1, v1) = got
+    assert torch.equal(q0[:less], q1[:less]) and (q1[less:] == 7).all()
+    assert k0[-1].any() and np.array_equal(k0[:-2], k1[:-2]) and np.array_equal(v0[:-2], v1[:-2]) and not k1[-2:].any() and not v1[-2:].any()
