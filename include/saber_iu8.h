@@ -567,8 +567,8 @@ int saber_iu8_silu_table(saber_iu8_ctx *ctx, void *out_u16, void *stream);
  *
  * The cache in the gfx950 order, E = the elements of 16 bytes (8 bf16, 16 e4m3): K [pages][kv_heads][page_tokens / 16][head_dim / E]
  * [16 tokens][E], V [pages][kv_heads][page_tokens][head_dim] (saber_iu8_kv_k_offset, _v_offset). head_dim 64, 128 or 256; page_tokens a
- * power of two from 16 to 256. An e4m3 cache holds value / scale, a scale a kv head, rounded to nearest even and saturated at 448;
- * the attention multiplies by it. Entry [s * table_stride + p] of the page table is the page that holds tokens p * page_tokens ... of
+ * power of two from 16 to 256. An e4m3 cache holds value / scale (the f32 quotient), a scale a kv head, rounded to nearest even and saturated
+ * at 448; the attention multiplies by it. Scales are finite and not zero. Entry [s * table_stride + p] of the page table is the page that holds tokens p * page_tokens ... of
  * sequence s; an entry outside 0 .. pages - 1 is a hole: nothing is written there and its keys take no part. Sequences
  * may share pages that no call writes. kv_len[s] counts
  * the sequence's tokens, the call's new ones included (both operators of a step read the same number); counts above

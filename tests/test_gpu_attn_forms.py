@@ -201,6 +201,33 @@ def test_few_rows_by_their_descriptor(ctx, e4m3):
         assert torch.equal(again.view(torch.int16), c.out.view(torch.int16)) and not c.ws.counter.any()
 
 
+# ------------------------------------------------------------------ rounding
+
+@pytest.mark.parametrize("scale", [0.3, 0.7, 1.0, 0.0123, 3.1415927, 1 / 448])
+def test_e4m3_values_are_the_rounded_quotients(ctx, scale):
+    """Every bf16 value as k and as v: the byte of value / scale, an f32 quotient rounded to nearest even, saturated, a NaN kept."""
+    say(f"append e4m3, every bf16 value at a scale of {scale}")
+    n, dim = 256, 256
+    c = Paged(1, 1, dim, 64, n, True)
+    c.scales = [torch.full((1,), scale, device="cuda") for _ in range(2)]
+    c.kv_len[0] = n
+    values = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(torch.bfloat16).view(n, dim)
+    rows = torch.cat((torch.zeros(n, dim, dtype=torch.bfloat16), values, values.flip(0)), 1).cuda()
+    q_out, p = torch.zeros(n, dim, dtype=torch.bfloat16, device="cuda"), rows.data_ptr()
+    ctx.kv_append(p, p + 2 * dim, p + 4 * dim, q_out.data_ptr(), c.desc(), ends([n]).data_ptr(), n, 1, 1, 3 * dim, dim, 3 * dim)
+    torch.cuda.synchronize()
+    c.scales = [torch.ones(1, device="cuda")] * 2
+    k, v, _ = c.rows(0, n)
+    # (in the e4m3 grid: a step of 2^-9 below 2^-6, of 2^-3 of the binade above)
+    with np.errstate(invalid="ignore", over="ignore"):
+        x = f64(values.float()).astype(np.float32) / np.float32(scale)
+    x = np.clip(x.astype(np.float64), -448, 448)
+    with np.errstate(divide="ignore", invalid="ignore"):
+        step = 2.0 ** (np.maximum(np.floor(np.log2(np.abs(x))), -6) - 3)
+        want = np.where(x == 0, 0.0, np.rint(x / step) * step)
+    assert np.array_equal(k[:, 0], want, equal_nan=True) and np.array_equal(v[::-1, 0], want, equal_nan=True)
+
+
 # ------------------------------------------------------------------ rows and positions
 
 @pytest.mark.parametrize("dim,heads,kvh,lens,news,form", [
