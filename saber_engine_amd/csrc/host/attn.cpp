@@ -225,11 +225,18 @@ int iu8::attn_guard(const saber_iu8_desc *d) {
   const int64_t dim = w ? atoi(w + 2) : 0;
   bool ok = shape > 0 && kv_heads > 0 && heads > 0 && heads % kv_heads == 0 && form >= 0 && shift >= 4 && shift <= 8 && pages > 0 && stride > 0 &&
             (stride << shift) <= (int64_t)WHOLE && num("tokens") > 0 && d->grid[1] == 1 && d->grid[2] == 1;
+  auto given = [&](const char *name) {
+    const saber_iu8_slot *s = slot(d, name);
+    return s && s->kind == SABER_IU8_ARG_BUFFER;
+  };
+  for (const char *name : {"q", "kc", "vc", "table", "kv_len", append ? "q_out" : "out"}) ok = ok && given(name);
+  if (strstr(d->kernel, "_e4m3_")) ok = ok && given("k_scale") && given("v_scale");
   if (append) {
-    ok = ok && rot % 16 == 0 && rot <= dim && num("seqs") > 0;
+    ok = ok && rot % 16 == 0 && rot <= dim && num("seqs") > 0 && given("k") && given("v") && (!rot || given("inv_freq")) &&
+         (given("cu_q") || num("tokens") <= num("seqs"));  // without cu_q row t is sequence t's
   } else {
-    const saber_iu8_slot *part = slot(d, "partial"), *count = slot(d, "counter");
-    const bool bound = part && count && part->kind == SABER_IU8_ARG_BUFFER && count->kind == SABER_IU8_ARG_BUFFER;
+    const bool bound = given("partial") && given("counter");
+    ok = ok && form == shift;
     const int64_t qtiles = num("qtiles");
     if (few) {
       const int64_t unit = num("unit_shift"), seqs = num("seqs");

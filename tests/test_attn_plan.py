@@ -1,4 +1,5 @@
 """CPU tests of the launch that `attn` makes (csrc/host/attn.cpp), as resolve_attn describes it."""
+import ctypes
 import random
 
 import pytest
@@ -88,3 +89,29 @@ def test_long_streams_take_every_compute_unit(dim, kvh, group, max_q, seqs, kv, 
     """As many as fit: a workgroup's tiles are what is in flight, 32 KiB of them at width 64."""
     d = plan(dim, kvh, group, False, seqs, max_q, kv)
     assert b"few" in d.kernel and d.grid[0] == grid == plan(dim, kvh, group, False, seqs, max_q, 6000).grid[0]
+
+
+def test_descriptors_without_what_the_kernel_reads_are_refused():
+    """A buffer that a kernel reads, set to none by hand; rows of sequences that are not there; page sizes with more bits than a page has."""
+    guard = ctypes.CDLL(iu8.LIB_PATH)["_ZN3iu810attn_guardEPK14saber_iu8_desc"]
+    append = dict(shape=8 | 2 << 16, form=6 | 64 << 16, pages=10, table_stride=4, tokens=3, seqs=3)
+    few = dict(shape=8 | 2 << 16, page_shift=6, pages=10, table_stride=4, tokens=3, seqs=3, unit_shift=7, qtiles=1)
+    many = dict(shape=8 | 2 << 16, page_shift=6, pages=10, table_stride=4, tokens=300, chunk=128, splits=2, qtiles=3)
+
+    def check(kernel, scalars, none=(), **more):
+        d = iu8.describe_raw(kernel, (12, 1, 1), 256, "attn_paged", **dict(scalars, **more))
+        for s in d.args[:d.n_args]:
+            if s.name.decode() in none:
+                s.kind = iu8.ARG_NULL_BUFFER
+        return guard(ctypes.byref(d))
+
+    for kernel, scalars, needs in (("kv_append_bf16_d128", append, "q k v q_out kc vc table kv_len inv_freq"), ("kv_append_e4m3_d64", append, "q k_scale v_scale inv_freq"),
+                                   ("attn_few_bf16_d64_r16", few, "q kc vc table kv_len out partial counter"), ("attn_few_e4m3_d256_r32", few, "k_scale v_scale"),
+                                   ("attn_many_bf16_d256", many, "q kc vc table kv_len out partial counter"), ("attn_many_e4m3_d128", many, "k_scale v_scale")):
+        assert check(kernel, scalars) == 0
+        for name in needs.split():
+            assert check(kernel, scalars, (name,)) == iu8.E_RULE, (kernel, name)
+    assert check("kv_append_bf16_d64", append, ("k_scale", "v_scale", "cu_q", "q_norm", "k_norm")) == 0
+    assert check("kv_append_bf16_d64", append, ("inv_freq",), form=6) == 0
+    assert check("kv_append_bf16_d64", append, ("cu_q",), tokens=4) == iu8.E_RULE and check("kv_append_bf16_d64", append, (), tokens=4) == 0
+    assert check("attn_few_bf16_d64_r16", few, page_shift=6 | 1 << 8) == iu8.E_RULE and check("attn_many_bf16_d64", many, page_shift=5 | 1 << 16) == iu8.E_RULE
