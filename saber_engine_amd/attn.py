@@ -7,6 +7,12 @@ import torch
 from . import iu8
 
 
+def _is(t, dtype, n, device):
+    """n values of the type (int16: of its width) or more, in one piece on the device: what a kernel may read from the tensor's address."""
+    return (t is not None and (t.dtype == dtype or dtype is torch.int16 and t.dtype.itemsize == 2) and t.numel() >= n and t.is_contiguous() and
+            t.device.type == device.type and device.index in (None, t.device.index))
+
+
 class PagedKvCache:
     """The pages of one layer's sequences. The host deals pages (reserve, release); the table and the counts lie on the device, where
     the kernels read them, so that a captured step follows them; reserve and release write there on torch's current stream. While a step
@@ -19,6 +25,9 @@ class PagedKvCache:
         self.seqs, self.kv_heads, self.head_dim, self.page_tokens, self.kind = seqs, kv_heads, head_dim, page_tokens, kind
         self.max_kv, self.table_stride = max_kv, -(-max_kv // page_tokens)
         self.pages = pages or seqs * self.table_stride
+        for s in (k_scale, v_scale):
+            if kind == iu8.KV_E4M3 and not _is(s, torch.float32, kv_heads, torch.device(device)):
+                raise iu8.IU8Error(iu8.E_ARG, f"an e4m3 cache has a k_scale and a v_scale, f32 [{kv_heads}] on {device}")
         size = iu8.kv_bytes(self.pages, kv_heads, head_dim, page_tokens, kind)
         self.k, self.v = (torch.zeros(size, dtype=torch.uint8, device=device) for _ in range(2))
         self.k_scale, self.v_scale = k_scale, v_scale
@@ -60,6 +69,8 @@ class AttnLayerIU8:
         D, kvh, device = cache.head_dim, cache.kv_heads, cache.k.device
         if max_q == 1 and tokens != cache.seqs:
             raise iu8.IU8Error(iu8.E_RULE, f"{tokens} rows of {cache.seqs} sequences, one a sequence")
+        if inv_freq is not None and not (2 * len(inv_freq) <= D and _is(inv_freq, torch.float64, len(inv_freq), device)):
+            raise iu8.IU8Error(iu8.E_ARG, f"inv_freq: f64, at most {D // 2} of them, on {device}")
         self.gated, self.inv_freq, self.interleaved, self.eps = bool(gated), inv_freq, interleaved, eps
         self.scale = D ** -0.5 if scale is None else scale
         self.n_core, self.q_head = heads * D, 2 * D if gated else D
@@ -87,6 +98,12 @@ class AttnLayerIU8:
         bits [head_dim] or None."""
         if self.gated and had_t is None:
             raise iu8.IU8Error(iu8.E_ARG, "a gated layer's o linear lies in the Hadamard basis: had_t must be given")
+        device = self.cache.k.device
+        if self.gated and not _is(had_t, torch.float32, self.n_core, device):
+            raise iu8.IU8Error(iu8.E_ARG, f"had_t: f32 [{self.n_core}] on {device}")
+        for w in (q_norm, k_norm):
+            if w is not None and not _is(w, torch.int16, self.cache.head_dim, device):
+                raise iu8.IU8Error(iu8.E_ARG, f"head norms: bf16 bits [{self.cache.head_dim}] on {device}")
         self._w = (wqkv_frag, wsqkv, wo_frag, wso)
         self.had_t, self.q_norm, self.k_norm = had_t, q_norm, k_norm
 
@@ -96,6 +113,8 @@ class AttnLayerIU8:
         captured call: in any replay); the cache's length is shared among workgroups accordingly."""
         if tuple(x.shape) != (self.T, self.H):
             raise iu8.IU8Error(iu8.E_RULE, f"rows of shape {tuple(x.shape)}; the train is made for {(self.T, self.H)}")
+        if not _is(x, torch.int16, self.T * self.H, self.cache.k.device):
+            raise iu8.IU8Error(iu8.E_ARG, f"rows: bf16 bits in one piece on {self.cache.k.device}")
         c, T, D, P = self.ctx, self.T, self.cache.head_dim, lambda t: t.data_ptr() if t is not None else None  # noqa: E731
         wqkv, wsqkv, wo, wso = self._w
         cache, qkv, cu = self.cache.desc, self.qkv.data_ptr(), P(self.cu_q)
@@ -109,7 +128,7 @@ class AttnLayerIU8:
                     self.n_qkv, P(self.inv_freq), 2 * len(self.inv_freq) if self.inv_freq is not None else 0, self.interleaved,
                     P(self.q_norm), P(self.k_norm), self.eps, stream)
         c.attn(P(self.q), self.n_core, cache, cu, P(self.core), T, self.cache.seqs, self.max_q,
-               self.cache.max_kv if max_kv is None else min(max_kv, self.cache.max_kv), self.heads, self.scale,               *map(P, self._attn_ws), stream)
+               self.cache.max_kv if max_kv is None else min(max_kv, self.cache.max_kv), self.heads, self.scale, *map(P, self._attn_ws), stream)
         if self.gated:
             c.attn_gate_quant_had(P(self.core), qkv, P(self.a2), P(self.s2), T, self.n_core, D, self.n_qkv, P(self.had_t), stream)
         elif self.fused_o:
