@@ -68,6 +68,15 @@ def random_rows(g, *shape, e4m3=False):
     return (x * 60).clamp(-448, 448).to(torch.float8_e4m3fn).cuda() if e4m3 else x.to(torch.bfloat16).cuda()
 
 
+def e4m3_of(x, scale):
+    """What an e4m3 cache stores of x (f64, of bf16 or f32 values): the f32 quotient in the e4m3 grid (a step of 2^-9 below 2^-6, of 2^-3 of the
+    binade above), to nearest even, saturated."""
+    with np.errstate(invalid="ignore", over="ignore", divide="ignore"):
+        y = np.clip((x.astype(np.float32) / np.float32(scale)).astype(np.float64), -448, 448)
+        step = 2.0 ** (np.maximum(np.floor(np.log2(np.abs(y))), -6) - 3)
+        return np.where(y == 0, 0.0, np.rint(y / step) * step)
+
+
 def attention(q, k, v, there, scale):
     """q f64 [n, heads, dim], k, v f64 [len, kv_heads, dim]: the n rows are the last positions. Returns the output and how far a
     kernel may be off in each element: the weights rounded to bf16 (half a step of each), the output rounded once, the scores off by

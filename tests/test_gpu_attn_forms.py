@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from saber_engine_amd import iu8
-from tests.attn_util import Paged, Workspace, attention, check, f64, random_rows
+from tests.attn_util import Paged, Workspace, attention, check, e4m3_of, f64, random_rows
 from tests.gpu_util import say
 from tests.test_gpu_attn import ends
 
@@ -218,13 +218,7 @@ def test_e4m3_values_are_the_rounded_quotients(ctx, scale):
     torch.cuda.synchronize()
     c.scales = [torch.ones(1, device="cuda")] * 2
     k, v, _ = c.rows(0, n)
-    # (in the e4m3 grid: a step of 2^-9 below 2^-6, of 2^-3 of the binade above)
-    with np.errstate(invalid="ignore", over="ignore"):
-        x = f64(values.float()).astype(np.float32) / np.float32(scale)
-    x = np.clip(x.astype(np.float64), -448, 448)
-    with np.errstate(divide="ignore", invalid="ignore"):
-        step = 2.0 ** (np.maximum(np.floor(np.log2(np.abs(x))), -6) - 3)
-        want = np.where(x == 0, 0.0, np.rint(x / step) * step)
+    want = e4m3_of(f64(values.float()), scale)
     assert np.array_equal(k[:, 0], want, equal_nan=True) and np.array_equal(v[::-1, 0], want, equal_nan=True)
 
 
