@@ -609,7 +609,7 @@ int saber_iu8_kv_append(saber_iu8_ctx *ctx, const void *q, const void *k, const 
 /* The new rows' attention over the cache, causal: row i of sequence s's n new ones sees positions 0 .. kv_len[s] - n + i.
  *   out[t, h] = sum_j softmax_j(scale * q[t, h] . k_j) v_j, heads in groups of heads / kv_heads a kv head
  * q rows `q_row` elements apart, heads head_dim apart; out bf16 [tokens, heads, head_dim]. A row that sees no key gives zeros; rows in
- * front of the first sequence and behind the last are left as they were. max_q: the most new rows of a sequence (rows past it are not computed); max_kv: what
+ * front of the first sequence and behind the last are left as they were. max_q: the most new rows of a sequence (rows past it may be left as they were); max_kv: what
  * kv_len is expected to reach, for the split of the cache's length alone (a longer one is right, and slower).
  * Up to 32 rows a kv head (new rows x group), and somewhat more on a long cache, run on the few-row kernels, which stream the
  * cache; the rest on the many-row kernels, 128 rows a workgroup. Both share the cache's length among workgroups where the grid would

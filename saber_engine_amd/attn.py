@@ -1,6 +1,7 @@
 """The attention block of a decoder layer as a launch train over the C ABI: per-token quant -> q, k, v linear -> new tokens into the
 paged cache (head norms and rotation on the way) -> causal attention over it -> output gate and requant in the Hadamard basis (or the
-plain requant) -> o linear.  Every GEMM keeps the iu8 contract.  torch is used for device memory only.
+plain requant) -> o linear.  Every GEMM keeps the iu8 contract; the train's two linears are W4, as the served layers' are (with W8 ones
+the same operators are called one by one).  torch is used for device memory only.
 """
 import torch
 

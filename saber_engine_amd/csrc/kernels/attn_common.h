@@ -14,15 +14,8 @@
 #include "iu8_common.h"
 
 typedef __bf16 at_v8bf __attribute__((ext_vector_type(8)));
-typedef __bf16 at_v2bf __attribute__((ext_vector_type(2)));
 typedef float at_v16f __attribute__((ext_vector_type(16)));
 typedef short at_v4s __attribute__((ext_vector_type(4)));
-
-struct AtCache {
-  const unsigned char *k, *v;
-  const int *table, *kv_len;
-  int kv_heads, page_shift, pages, table_stride;
-};
 
 // what a scheduling group counts
 constexpr int AT_VALU = 0x2, AT_MFMA = 0x8, AT_DS_READ = 0x100, AT_TRANS = 0x400;
