@@ -15,7 +15,7 @@
 // straight from memory, and asks for the next K as soon as its scores are made, for the next V as soon as its product is: up to
 // 128 KiB a compute unit on the way, with no register held for it and no barrier between the waves. Measured: one row on 131,072 keys, 4
 // kv heads of 256, 537 MB of cache, 91 us (5.9 TB/s; a plain read reaches 6.0 to 6.4); 64 rows on up to 8,192, 8 heads of 128,
-// 1.27 GB, 200 us (6.3); 33 on up to 16,001 in e4m3, 586 MB, 102 us (5.7); 9 x 5 new rows of group 6 on up to 6,007, 154 MB, 46 us
+// 1.27 GB, 202 us (6.3); 33 on up to 16,001 in e4m3, 586 MB, 102 us (5.7); 9 x 5 new rows of group 6 on up to 6,007, 154 MB, 46 us
 // (3.4). One row on 1,800 keys 13 us: the chain of lengths, pages, keys, parts and join, behind 3 of the launch.
 //
 // Both products have the row as the MFMA's column (S^T = K Q^T, O^T = V^T P^T), so a lane keeps one row: its maximum, sum and
