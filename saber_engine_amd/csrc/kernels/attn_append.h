@@ -18,14 +18,15 @@
 
 // The quotient from the reciprocal, one of a head, and the remainder's correction (Markstein's: q + (x - q scale) / scale, each an fma), two operations
 // more than the product with the reciprocal, which is rounded twice on the way to the quotient and moved 26 of a million stored values of
-// bf16 rows at a scale of 0.3 to a neighbour. The first guess is bounded, so that an infinite x leaves no NaN in the remainder.
-static __device__ __forceinline__ unsigned at_e4m3x4(const float *x, float scale, float inv) {
+// bf16 rows at a scale of 0.3 to a neighbour. The remainder is taken the other way round and subtracted, which leaves a zero its sign. `most` is 448 scales,
+// within a rounding: x is bounded first, by operations that keep a NaN, so that an infinity leaves none in the remainder.
+static __device__ __forceinline__ unsigned at_e4m3x4(const float *x, float scale, float inv, float most) {
 #pragma clang fp contract(off)
   float y[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float q = __builtin_amdgcn_fmed3f(x[i] * inv, -1024.f, 1024.f), t = fmaf(fmaf(-q, scale, x[i]), inv, q);
-    y[i] = t != t ? t : __builtin_amdgcn_fmed3f(t, -448.f, 448.f);
+    const float b = __builtin_elementwise_minimum(__builtin_elementwise_maximum(x[i], -most), most), q = b * inv;
+    y[i] = fmaf(-fmaf(q, scale, -b), inv, q);
   }
   int r = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
   return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], r, true);
@@ -138,9 +139,9 @@ static __device__ __forceinline__ void kv_append_body(
   };
   unsigned char *dst = is_v ? vc : kc;
   if constexpr (F8) {
-    const float by = (is_v ? v_scale : k_scale)[h], inv = 1.f / by;
-    *(iu8_v2u *)(dst + at(c0)) = iu8_v2u{at_e4m3x4(a, by, inv), at_e4m3x4(a + 4, by, inv)};
-    *(iu8_v2u *)(dst + at(c1)) = iu8_v2u{at_e4m3x4(b, by, inv), at_e4m3x4(b + 4, by, inv)};
+    const float by = (is_v ? v_scale : k_scale)[h], inv = 1.f / by, most = 448.f * fabsf(by);
+    *(iu8_v2u *)(dst + at(c0)) = iu8_v2u{at_e4m3x4(a, by, inv, most), at_e4m3x4(a + 4, by, inv, most)};
+    *(iu8_v2u *)(dst + at(c1)) = iu8_v2u{at_e4m3x4(b, by, inv, most), at_e4m3x4(b + 4, by, inv, most)};
   } else {
     *(iu8_v4u *)(dst + 2 * at(c0)) = pack(a);
     *(iu8_v4u *)(dst + 2 * at(c1)) = pack(b);

@@ -220,6 +220,9 @@ def test_e4m3_values_are_the_rounded_quotients(ctx, scale):
     k, v, _ = c.rows(0, n)
     want = e4m3_of(f64(values.float()), scale)
     assert np.array_equal(k[:, 0], want, equal_nan=True) and np.array_equal(v[::-1, 0], want, equal_nan=True)
+    number = ~np.isnan(want)       # a zero keeps its value's sign
+    negative = np.signbit(f64(values.float()))[number]
+    assert np.array_equal(np.signbit(k[:, 0])[number], negative) and np.array_equal(np.signbit(v[::-1, 0])[number], negative)
 
 
 # ------------------------------------------------------------------ rows and positions
