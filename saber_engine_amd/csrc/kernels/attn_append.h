@@ -11,8 +11,8 @@
 //
 // Bound by the bytes (rows in, rows and pages out), and with few tokens by the launch. A lane owns 16 channels of one head: two
 // pieces of 8 that the rotation pairs, so a pair never crosses lanes. Measured: 6,772 tokens of 40 + 2 x 8 heads of 128 channels, 205 MB
-// of rows, 44 us (4.65 TB/s; a device copy reaches 4.9), up to 1,500 of 7 prompts into e4m3 38.5 (4.7); 64 tokens of 24 + 2 x 4 heads of 256 into e4m3
-// 4.3 us, one token 3.1.
+// of rows, 44 us (4.65 TB/s; a device copy reaches 4.9), up to 1,500 of 7 prompts into e4m3 39.8 (4.5); 64 tokens of 24 + 2 x 4 heads of 256 into e4m3
+// 4.1 us, one token 3.1.
 #pragma once
 #include "attn_common.h"
 
