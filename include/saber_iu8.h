@@ -627,6 +627,48 @@ int saber_iu8_attn(saber_iu8_ctx *ctx, const void *q, uint32_t q_row, const sabe
 int saber_iu8_resolve_attn(const saber_iu8_kv_cache *cache, uint32_t q_row, int packed, uint32_t tokens, uint32_t seqs, uint32_t max_q, uint32_t max_kv,
                            uint32_t heads, float scale, int split, saber_iu8_desc *out);
 
+/* Pages src[i] -> pages dst[i] of the cache's k and v, i < n (device arrays): a sequence forked, a pool compacted. A pair with a number outside 0 .. pages - 1 is passed
+ * over. No page may be written twice in a call, nor be both read and written. Of the cache's tables nothing is read. Asynchronous. */
+int saber_iu8_kv_copy(saber_iu8_ctx *ctx, const saber_iu8_kv_cache *cache, const int32_t *src, const int32_t *dst, uint32_t n, void *stream);
+
+/* ------------------------------------------------------------------ a delta-net layer's core */
+
+/* What stands between a delta-net layer's projections and its norm and output gate (saber_iu8_gdn_norm_quant_had). Rows are bf16; no counterpart
+ * among the reference's interfaces for this path.
+ *
+ * A sequence's memory lies in a slot of two pools: its tail, bf16 [slots][width - 1][channels], the convolution's last inputs, the oldest first;
+ * its state, f32 [slots][heads][128 of the key][128 of the value]. slot (device, [seqs]) names each sequence's (NULL: sequence s's is s); a
+ * sequence whose slot is outside 0 .. slots - 1 is passed over, its rows left as they were. No two sequences of a call may have the same slot. A sequence begins on zeros.
+ * Rows cu_q[s] .. cu_q[s + 1] - 1 (device, [seqs + 1], ascending) are sequence s's new ones, none: nothing happens to it; cu_q NULL: one row a
+ * sequence. Rows past `tokens` are not there; rows in front of the first sequence and behind the last are neither read nor written. kept (device, [seqs], may be
+ * NULL: all): the memory is moved on by the first kept[s] rows alone (bounded by 0 and the sequence's rows), while all rows are answered: drafted rows, of which a
+ * later call with the same rows makes the accepted ones count. Tables and kept must stand still while a call runs. Calls on the same slots must
+ * not overlap in time. All asynchronous; nothing is allocated.
+ *
+ * gdn_conv: out[t, c] = y sigmoid(y), y = bias[c] + sum_w weight[c, w] x[t - width + 1 + w, c], in f32, rounded once; what lies in front of a
+ * sequence's rows comes from its tail. weight bf16 [channels][width], bias bf16 [channels] or NULL; width 2 to 4, channels a multiple of 8. x rows
+ * `x_row`, out rows `out_row` elements apart; they must not overlap. Pointers on 16 bytes, strides multiples of 8. */
+int saber_iu8_gdn_conv(saber_iu8_ctx *ctx, const void *x, uint32_t x_row, const void *weight, const void *bias, void *tail, uint32_t slots, const int32_t *slot,
+                       const int32_t *cu_q, const int32_t *kept, void *out, uint32_t out_row, uint32_t tokens, uint32_t seqs, uint32_t channels, uint32_t width,
+                       void *stream);
+/* gdn, a row after the other, value head h with key head h / (heads / key_heads), all heads of 128:
+ *   k^ = k / sqrt(|k|^2 + eps), q^ = q / sqrt(|q|^2 + eps), decay = exp(-exp(a_log[h]) softplus(a + dt_bias[h])), beta = sigmoid(b)
+ *   S <- decay S + k^ (beta (v - (decay S)^T k^))^T,   out[t, h] = scale S^T q^
+ * q, k, v rows `row` elements apart, heads 128 apart; a, b rows `ab_row` apart, a value a head; a_log, dt_bias f32 [heads]; out bf16 [tokens, heads, 128], which
+ * must not overlap the rows, or NULL: the states alone (q may then be NULL). A decay below exp(-120) is zero. Values, states and gates are numbers: one that is not
+ * spoils its head's rows from its chunk of 64 on, and the state.
+ * max_q: the most new rows of a sequence, for the choice of the kernel alone. Long rows are taken in chunks of 64, with the workspace of saber_iu8_gdn_workspace (made
+ * for (tokens, seqs, max_q), it holds every call of the same heads with at most these; calls that share it must not overlap in time), the rest, and whatever has no
+ * workspace, kept, or no out, a row at a time: the same rule, other roundings. States, norms and sums in f32 (the chunks' matrix products hold 24 bits of
+ * what enters the state, 16 of what goes into the rows' answers alone), out rounded once; the same bytes on every run. */
+int saber_iu8_gdn_workspace(uint32_t tokens, uint32_t seqs, uint32_t max_q, uint32_t key_heads, uint32_t heads, uint64_t *bytes);
+int saber_iu8_gdn(saber_iu8_ctx *ctx, const void *q, const void *k, const void *v, uint32_t row, const void *a, const void *b, uint32_t ab_row, const float *a_log,
+                  const float *dt_bias, float *state, uint32_t slots, const int32_t *slot, const int32_t *cu_q, const int32_t *kept, void *out, uint32_t tokens,
+                  uint32_t seqs, uint32_t max_q, uint32_t key_heads, uint32_t heads, float eps, float scale, void *workspace, void *stream);
+/* States and tails of slots src[i] -> slots dst[i], i < n (device arrays), as saber_iu8_kv_copy does with pages. */
+int saber_iu8_gdn_copy(saber_iu8_ctx *ctx, float *state, void *tail, uint32_t slots, uint32_t heads, uint32_t channels, uint32_t width, const int32_t *src,
+                       const int32_t *dst, uint32_t n, void *stream);
+
 /* ---- tier packs ("SBRPACK1"): reading the iu8 records of a built pack ------------------------------
  * The byte layout of include/saber_abi.h:541-944 and the open-time rules of
  * crates/saber-mem/src/pack/{format,reader}.rs (PackReader::open_with / open_expecting): magic,

@@ -98,6 +98,24 @@ static const Signature SIG_ATTN_MANY = {
     {"tokens", K::I32},    {"shape", K::I32},    {"page_shift", K::I32}, {"pages", K::I32},  {"table_stride", K::I32}, {"chunk", K::I32},
     {"splits", K::I32},    {"qtiles", K::I32},   {"scale", K::F32}};
 
+// a delta-net layer's core, and the copies of a sequence (no counterpart lists in the reference)
+static const Signature SIG_DELTA_CONV = {
+    {"x", K::Buffer},    {"weight", K::Buffer}, {"bias", K::Buffer}, {"tail", K::Buffer}, {"slot", K::Buffer},  {"cu_q", K::Buffer}, {"kept", K::Buffer}, {"out", K::Buffer},
+    {"x_row", K::I32},   {"out_row", K::I32},   {"tokens", K::I32},  {"seqs", K::I32},    {"channels", K::I32}, {"slots", K::I32},   {"run", K::I32}};
+static const Signature SIG_DELTA_STEP = {
+    {"q", K::Buffer},    {"k", K::Buffer},    {"v", K::Buffer},    {"a", K::Buffer},   {"b", K::Buffer},  {"a_log", K::Buffer}, {"dt_bias", K::Buffer},
+    {"state", K::Buffer}, {"slot", K::Buffer}, {"cu_q", K::Buffer}, {"kept", K::Buffer}, {"out", K::Buffer}, {"row", K::I32},    {"ab_row", K::I32},
+    {"tokens", K::I32},  {"seqs", K::I32},    {"shape", K::I32},   {"slots", K::I32},  {"eps", K::F32},   {"scale", K::F32}};
+static const Signature SIG_DELTA_PREP = {
+    {"q", K::Buffer},    {"k", K::Buffer},    {"a", K::Buffer},    {"b", K::Buffer},   {"a_log", K::Buffer}, {"dt_bias", K::Buffer}, {"slot", K::Buffer},
+    {"cu_q", K::Buffer}, {"work", K::Buffer}, {"row", K::I32},     {"ab_row", K::I32}, {"tokens", K::I32},   {"seqs", K::I32},       {"shape", K::I32},
+    {"slots", K::I32},   {"eps", K::F32},     {"scale", K::F32}};
+static const Signature SIG_DELTA_SCAN = {
+    {"q", K::Buffer},    {"k", K::Buffer},   {"v", K::Buffer}, {"work", K::Buffer}, {"state", K::Buffer}, {"slot", K::Buffer}, {"cu_q", K::Buffer},
+    {"out", K::Buffer},  {"row", K::I32},    {"tokens", K::I32}, {"seqs", K::I32},  {"shape", K::I32},    {"slots", K::I32}};
+static const Signature SIG_BLOCK_COPY = {{"a", K::Buffer},   {"b", K::Buffer},   {"src", K::Buffer}, {"dst", K::Buffer},
+                                         {"a_bytes", K::I64}, {"b_bytes", K::I64}, {"blocks", K::I32}};
+
 static const Signature SIG_PROBE_READ = {{"src", K::Buffer}, {"out", K::Buffer}, {"n", K::I32}};
 static const Signature SIG_PROBE_COPY = {{"src", K::Buffer}, {"dst", K::Buffer}, {"n", K::I32}};
 
@@ -135,6 +153,11 @@ const Signature *signature_for(const std::string &k) {
   if (starts(k, "kv_append_")) return &SIG_KV_APPEND;
   if (starts(k, "attn_few_")) return &SIG_ATTN_FEW;
   if (starts(k, "attn_many_")) return &SIG_ATTN_MANY;
+  if (starts(k, "delta_conv_")) return &SIG_DELTA_CONV;
+  if (k == "delta_step") return &SIG_DELTA_STEP;
+  if (k == "delta_prep") return &SIG_DELTA_PREP;
+  if (starts(k, "delta_scan_")) return &SIG_DELTA_SCAN;
+  if (k == "block_copy") return &SIG_BLOCK_COPY;
   return nullptr;
 }
 

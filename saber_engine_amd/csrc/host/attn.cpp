@@ -32,26 +32,6 @@ int log2_of(uint32_t x) {
   return s;
 }
 
-int cache_check(const char *op, const saber_iu8_kv_cache *c, uint32_t heads, uint32_t seqs, uint32_t tokens, bool packed) {
-  if (!c) return fail(SABER_IU8_E_ARG, fmt("%s: null cache", op));
-  if (!c->k || !c->v || !c->page_table || !c->kv_len) return fail(SABER_IU8_E_ARG, fmt("%s: the cache's k, v, page_table and kv_len must be given", op));
-  if (c->kind != SABER_IU8_KV_BF16 && c->kind != SABER_IU8_KV_E4M3) return fail(SABER_IU8_E_ARG, fmt("%s: unknown cache kind %u", op, c->kind));
-  if (c->kind == SABER_IU8_KV_E4M3 && (!c->k_scale || !c->v_scale))
-    return fail(SABER_IU8_E_ARG, fmt("%s: an e4m3 cache has a k_scale and a v_scale a kv head", op));
-  if (((uintptr_t)c->k | (uintptr_t)c->v) % 16) return fail(SABER_IU8_E_ARG, fmt("%s: the cache's k and v must lie on 16 bytes", op));
-  if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256)
-    return fail(SABER_IU8_E_RULE, fmt("%s: head width %u; the kernels hold 64, 128 and 256", op, c->head_dim));
-  if (c->page_tokens < 16 || c->page_tokens > 256 || (c->page_tokens & (c->page_tokens - 1)))
-    return fail(SABER_IU8_E_RULE, fmt("%s: pages of %u tokens; a power of two from 16 to 256", op, c->page_tokens));
-  if (!heads || !c->kv_heads || heads % c->kv_heads || heads > 0xFFFF || c->kv_heads > 0x7FFF)
-    return fail(SABER_IU8_E_RULE, fmt("%s: %u heads over %u kv heads: whole groups, at most 65535 and 32767", op, heads, c->kv_heads));
-  if (!c->pages || c->pages > I32_MAX || !c->table_stride || (uint64_t)c->table_stride * c->page_tokens > WHOLE)
-    return fail(SABER_IU8_E_RULE, fmt("%s: %u pages, %u of %u tokens a sequence: at least one, positions below 2^31 - 256", op, c->pages, c->table_stride, c->page_tokens));
-  if (!seqs || !tokens || seqs >= I32_MAX || tokens > I32_MAX) return fail(SABER_IU8_E_RULE, fmt("%s: %u rows of %u sequences has nothing to do", op, tokens, seqs));
-  if (!packed && tokens != seqs) return fail(SABER_IU8_E_RULE, fmt("%s: %u rows of %u sequences without cu_q (one row a sequence)", op, tokens, seqs));
-  return 0;
-}
-
 struct Plan {
   uint32_t rows;        // a workgroup's: 16 or 32 (few), 128 (many)
   uint64_t qtiles, items, grid;
@@ -211,6 +191,26 @@ const saber_iu8_slot *slot(const saber_iu8_desc *d, const char *name) {
 }
 
 }  // namespace
+
+int iu8::cache_check(const char *op, const saber_iu8_kv_cache *c, uint32_t heads, uint32_t seqs, uint32_t tokens, bool packed) {
+  if (!c) return fail(SABER_IU8_E_ARG, fmt("%s: null cache", op));
+  if (!c->k || !c->v || !c->page_table || !c->kv_len) return fail(SABER_IU8_E_ARG, fmt("%s: the cache's k, v, page_table and kv_len must be given", op));
+  if (c->kind != SABER_IU8_KV_BF16 && c->kind != SABER_IU8_KV_E4M3) return fail(SABER_IU8_E_ARG, fmt("%s: unknown cache kind %u", op, c->kind));
+  if (c->kind == SABER_IU8_KV_E4M3 && (!c->k_scale || !c->v_scale))
+    return fail(SABER_IU8_E_ARG, fmt("%s: an e4m3 cache has a k_scale and a v_scale a kv head", op));
+  if (((uintptr_t)c->k | (uintptr_t)c->v) % 16) return fail(SABER_IU8_E_ARG, fmt("%s: the cache's k and v must lie on 16 bytes", op));
+  if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256)
+    return fail(SABER_IU8_E_RULE, fmt("%s: head width %u; the kernels hold 64, 128 and 256", op, c->head_dim));
+  if (c->page_tokens < 16 || c->page_tokens > 256 || (c->page_tokens & (c->page_tokens - 1)))
+    return fail(SABER_IU8_E_RULE, fmt("%s: pages of %u tokens; a power of two from 16 to 256", op, c->page_tokens));
+  if (!heads || !c->kv_heads || heads % c->kv_heads || heads > 0xFFFF || c->kv_heads > 0x7FFF)
+    return fail(SABER_IU8_E_RULE, fmt("%s: %u heads over %u kv heads: whole groups, at most 65535 and 32767", op, heads, c->kv_heads));
+  if (!c->pages || c->pages > I32_MAX || !c->table_stride || (uint64_t)c->table_stride * c->page_tokens > WHOLE)
+    return fail(SABER_IU8_E_RULE, fmt("%s: %u pages, %u of %u tokens a sequence: at least one, positions below 2^31 - 256", op, c->pages, c->table_stride, c->page_tokens));
+  if (!seqs || !tokens || seqs >= I32_MAX || tokens > I32_MAX) return fail(SABER_IU8_E_RULE, fmt("%s: %u rows of %u sequences has nothing to do", op, tokens, seqs));
+  if (!packed && tokens != seqs) return fail(SABER_IU8_E_RULE, fmt("%s: %u rows of %u sequences without cu_q (one row a sequence)", op, tokens, seqs));
+  return 0;
+}
 
 // What a hand-edited descriptor could get wrong for these kernels, whose walk over the cache follows their scalars.
 int iu8::attn_guard(const saber_iu8_desc *d) {

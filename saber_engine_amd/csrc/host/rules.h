@@ -124,6 +124,8 @@ std::string device_profile_toml();
 
 // The scalars of a descriptor of the paged cache's kernels (attn.cpp).
 int attn_guard(const saber_iu8_desc *d);
+// A cache, and the sizes of a call on it, as every operator of the cache takes them (attn.cpp); `packed`: with cu_q.
+int cache_check(const char *op, const saber_iu8_kv_cache *c, uint32_t heads, uint32_t seqs, uint32_t tokens, bool packed);
 // A launch of a kernarg image that its operator has laid out itself (runtime.cpp): saber_iu8_launch without the descriptor.
 int launch_image(saber_iu8_ctx *ctx, const char *kernel, uint32_t grid, uint32_t block, void *image, size_t bytes, void *stream);
 

@@ -397,6 +397,8 @@ static int launch_guard(const LoadedKernel &lk, const saber_iu8_desc *d) {
   if (int rc = counters_guard(d)) return rc;
   if (strncmp(d->kernel, "macaq_iu8f_mlp_", 15) == 0) return chain_guard(lk, d);
   if (!strncmp(d->kernel, "kv_append_", 10) || !strncmp(d->kernel, "attn_few_", 9) || !strncmp(d->kernel, "attn_many_", 10)) return attn_guard(d);
+  if (!strncmp(d->kernel, "delta_", 6) || !strcmp(d->kernel, "block_copy"))  // (their walks follow sizes that the operators check)
+    return fail(SABER_IU8_E_RULE, fmt("%s: launched by its operator alone", d->kernel));
   if (strncmp(d->kernel, "macaq_iu8f_gateup_act_", 22) == 0) {
     const int64_t m = i32_arg(d, "m"), n = i32_arg(d, "n"), k = i32_arg(d, "k");
     if (m <= 0 || n <= 0 || k <= 0 || !gate_up_act_holds((uint32_t)m, (uint32_t)k, (uint32_t)n))

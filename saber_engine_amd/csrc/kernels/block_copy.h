@@ -1,0 +1,30 @@
+// Blocks of two arrays to other blocks of them: block src[i] to block dst[i]. Pages of a key/value cache, states and tails of a delta-net layer.
+// A pair with a number outside the pool is passed over. Bound by the bytes; a workgroup takes 16 KiB of one block.
+#pragma once
+#include "iu8_common.h"
+
+constexpr int BLOCK_PIECE = 16384;
+
+static __device__ __forceinline__ void block_copy_body(unsigned char *__restrict__ a, unsigned char *__restrict__ b, const int *__restrict__ src,
+                                                       const int *__restrict__ dst, long long a_bytes, long long b_bytes, int blocks) {
+  const int a_pieces = (int)((a_bytes + BLOCK_PIECE - 1) / BLOCK_PIECE), b_pieces = (int)((b_bytes + BLOCK_PIECE - 1) / BLOCK_PIECE);
+  const int i = blockIdx.x / (unsigned)(a_pieces + b_pieces), piece = blockIdx.x - i * (a_pieces + b_pieces);
+  const int from = src[i], to = dst[i];
+  if ((unsigned)from >= (unsigned)blocks || (unsigned)to >= (unsigned)blocks || from == to) return;
+  unsigned char *base = piece < a_pieces ? a : b;
+  const long long bytes = piece < a_pieces ? a_bytes : b_bytes, at = (long long)(piece < a_pieces ? piece : piece - a_pieces) * BLOCK_PIECE;
+  const int left = (int)(bytes - at < BLOCK_PIECE ? bytes - at : BLOCK_PIECE);
+  const unsigned char *in = base + (size_t)from * bytes + at;
+  unsigned char *out = base + (size_t)to * bytes + at;
+  iu8_v4u v[4];
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    const int o = (x * 256 + (int)threadIdx.x) * 16;
+    if (o < left) v[x] = *(const iu8_v4u *)(in + o);
+  }
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    const int o = (x * 256 + (int)threadIdx.x) * 16;
+    if (o < left) *(iu8_v4u *)(out + o) = v[x];
+  }
+}

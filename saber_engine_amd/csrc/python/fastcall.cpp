@@ -81,7 +81,8 @@ struct Entry<F> {
   X(quant) X(quant_rowmajor) X(gemm) X(rowscale) X(linear_prefill_fused) X(gemm_static) X(gemm_pair) X(linear_fused) X(mlp_chain)  \
   X(gate_up_act) X(quant_had) X(silu_mul_quant_had) X(silu_mul_quant_had_lut) X(add_rms_quant_had) X(gdn_norm_quant_had)          \
   X(attn_gate_quant_had) X(attn_gate_quant_had_lut) X(moe_route) X(moe_route_quant) X(moe_grouped) X(moe_quant_rows)              \
-  X(moe_silu_mul_quant) X(moe_gate_up_act) X(moe_down_rows) X(moe_combine) X(kv_append) X(attn)
+  X(moe_silu_mul_quant) X(moe_gate_up_act) X(moe_down_rows) X(moe_combine) X(kv_append) X(attn)                     \
+  X(gdn_conv) X(gdn) X(kv_copy) X(gdn_copy)
 
 // bind(functions, tables, cache): {name: ctypes function}, the ctypes structures of the routed operators' tables and of the
 // key/value cache

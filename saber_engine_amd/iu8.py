@@ -186,6 +186,13 @@ def lib():
         L.saber_iu8_attn.argtypes = ([C.c_void_p, C.c_void_p, C.c_uint32, C.POINTER(KvCache), C.c_void_p, C.c_void_p] + [C.c_uint32] * 5 +
                                      [C.c_float] + [C.c_void_p] * 3)
         L.saber_iu8_resolve_attn.argtypes = ([C.POINTER(KvCache), C.c_uint32, C.c_int] + [C.c_uint32] * 5 + [C.c_float, C.c_int, C.POINTER(Desc)])
+        L.saber_iu8_gdn_conv.argtypes = ([C.c_void_p, C.c_void_p, C.c_uint32] + [C.c_void_p] * 3 + [C.c_uint32] + [C.c_void_p] * 4 + [C.c_uint32] * 5 +
+                                         [C.c_void_p])
+        L.saber_iu8_gdn_workspace.argtypes = [C.c_uint32] * 5 + [C.POINTER(C.c_uint64)]
+        L.saber_iu8_gdn.argtypes = ([C.c_void_p] * 4 + [C.c_uint32] + [C.c_void_p] * 2 + [C.c_uint32] + [C.c_void_p] * 3 + [C.c_uint32] + [C.c_void_p] * 4 +
+                                    [C.c_uint32] * 5 + [C.c_float] * 2 + [C.c_void_p] * 2)
+        L.saber_iu8_kv_copy.argtypes = [C.c_void_p, C.POINTER(KvCache), C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p]
+        L.saber_iu8_gdn_copy.argtypes = [C.c_void_p] * 3 + [C.c_uint32] * 4 + [C.c_void_p] * 2 + [C.c_uint32, C.c_void_p]
         L.saber_iu8_silu_table.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p]
         _lib = L
     return _lib
@@ -573,6 +580,27 @@ class Context:
         neither: in one piece."""
         _check(self._op.attn(self._addr, q, q_row, _tables(cache), cu_q, out, tokens, seqs, max_q, max_kv, heads, scale, partial, counter, stream))
 
+    def kv_copy(self, cache, src, dst, n, stream=0):
+        """Pages src[i] to pages dst[i] of k and v (int32 [n] on the device)."""
+        _check(self._op.kv_copy(self._addr, _tables(cache), src, dst, n, stream))
+
+    # ---- a delta-net layer's core
+    def gdn_conv(self, x, x_row, weight, tail, slots, out, out_row, tokens, seqs, channels, width, bias=None, slot=None, cu_q=None, kept=None, stream=0):
+        """The new rows' short causal convolution and SiLU, behind the inputs in the sequences' tails, which it moves on. cu_q None: one row a
+        sequence; slot None: sequence s's tail is s; kept: the rows that the tails move on by (None: all)."""
+        _check(self._op.gdn_conv(self._addr, x, x_row, weight, bias, tail, slots, slot, cu_q, kept, out, out_row, tokens, seqs, channels, width, stream))
+
+    def gdn(self, q, k, v, row, a, b, ab_row, a_log, dt_bias, state, slots, out, tokens, seqs, max_q, key_heads, heads, scale, eps=1e-6, slot=None, cu_q=None,
+            kept=None, workspace=None, stream=0):
+        """The gated delta rule over the new rows: out bf16 [tokens, heads, 128], the sequences' states moved on (by the first kept[s] rows, where
+        kept is given; out None: the states alone). The workspace of gdn_workspace, or none: a row at a time."""
+        _check(self._op.gdn(self._addr, q, k, v, row, a, b, ab_row, a_log, dt_bias, state, slots, slot, cu_q, kept, out, tokens, seqs, max_q, key_heads, heads,
+                            eps, scale, workspace, stream))
+
+    def gdn_copy(self, state, tail, slots, heads, channels, width, src, dst, n, stream=0):
+        """States and tails of slots src[i] to slots dst[i] (int32 [n] on the device)."""
+        _check(self._op.gdn_copy(self._addr, state, tail, slots, heads, channels, width, src, dst, n, stream))
+
 
 def moe_rows_cap(tokens, topk, experts, shared=False):
     return (lib().saber_iu8_moe_rows_cap_shared if shared else lib().saber_iu8_moe_rows_cap)(tokens, topk, experts)
@@ -607,6 +635,13 @@ def attn_workspace(seqs, max_q, max_kv, heads, kv_heads, head_dim):
     p, c = C.c_uint64(), C.c_uint64()
     _check(lib().saber_iu8_attn_workspace(seqs, max_q, max_kv, heads, kv_heads, head_dim, C.byref(p), C.byref(c)))
     return p.value, c.value
+
+
+def gdn_workspace(tokens, seqs, max_q, key_heads, heads):
+    """Bytes of gdn()'s workspace; 0 where it runs a row at a time."""
+    n = C.c_uint64()
+    _check(lib().saber_iu8_gdn_workspace(tokens, seqs, max_q, key_heads, heads, C.byref(n)))
+    return n.value
 
 
 def resolve_attn(cache, q_row, tokens, seqs, max_q, max_kv, heads, scale, packed=True, split=True):

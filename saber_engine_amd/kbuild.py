@@ -33,7 +33,7 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # -ffp-contract=off: every product and sum rounds where the source says (the epilogue contract);
 # the packed-fp32 feature is switched off for every device compile of this tree.
 FLAGS = f"--genco --offload-arch={ARCH} -O3 -ffp-contract=off -Xclang -target-feature -Xclang -packed-fp32-ops"
-PLUGINS = ("macaq_iu8", "macaq_iu8f", "macaq_i8q", "mxfp4_hadi8", "attn_glue_hadi8", "moe_iu8", "attn_paged", "iu8_probe")
+PLUGINS = ("macaq_iu8", "macaq_iu8f", "macaq_i8q", "mxfp4_hadi8", "attn_glue_hadi8", "moe_iu8", "attn_paged", "delta_net", "iu8_probe")
 # test infrastructure (accumulator and table taps of the parity suite): built beside the plugin
 # directory, where opening the plugin set does not see it
 TAPS = ("iu8_taps",)
