@@ -108,11 +108,11 @@ static const Signature SIG_DELTA_STEP = {
     {"tokens", K::I32},  {"seqs", K::I32},    {"shape", K::I32},   {"slots", K::I32},  {"eps", K::F32},   {"scale", K::F32}};
 static const Signature SIG_DELTA_PREP = {
     {"q", K::Buffer},    {"k", K::Buffer},    {"a", K::Buffer},    {"b", K::Buffer},   {"a_log", K::Buffer}, {"dt_bias", K::Buffer}, {"slot", K::Buffer},
-    {"cu_q", K::Buffer}, {"work", K::Buffer}, {"row", K::I32},     {"ab_row", K::I32}, {"tokens", K::I32},   {"seqs", K::I32},       {"shape", K::I32},
-    {"slots", K::I32},   {"eps", K::F32},     {"scale", K::F32}};
+    {"cu_q", K::Buffer}, {"keys", K::Buffer}, {"work", K::Buffer}, {"row", K::I32},    {"ab_row", K::I32},   {"tokens", K::I32},     {"seqs", K::I32},
+    {"shape", K::I32},   {"slots", K::I32},   {"places", K::I32},  {"eps", K::F32}};
 static const Signature SIG_DELTA_SCAN = {
-    {"q", K::Buffer},    {"k", K::Buffer},   {"v", K::Buffer}, {"work", K::Buffer}, {"state", K::Buffer}, {"slot", K::Buffer}, {"cu_q", K::Buffer},
-    {"out", K::Buffer},  {"row", K::I32},    {"tokens", K::I32}, {"seqs", K::I32},  {"shape", K::I32},    {"slots", K::I32}};
+    {"v", K::Buffer},   {"keys", K::Buffer}, {"work", K::Buffer}, {"state", K::Buffer}, {"slot", K::Buffer},  {"cu_q", K::Buffer}, {"out", K::Buffer},
+    {"row", K::I32},    {"tokens", K::I32},  {"seqs", K::I32},    {"shape", K::I32},    {"slots", K::I32},    {"scale", K::F32}};
 static const Signature SIG_BLOCK_COPY = {{"a", K::Buffer},   {"b", K::Buffer},   {"src", K::Buffer}, {"dst", K::Buffer},
                                          {"a_bytes", K::I64}, {"b_bytes", K::I64}, {"blocks", K::I32}};
 

@@ -13,8 +13,9 @@ using namespace iu8;
 namespace {
 
 constexpr uint32_t DIM = 128, CHUNK = 64, I32_MAX = 0x7FFFFFFFu, GRID_MAX = 0xFFFFFFu;  // workgroups of 256 whose threads a launch counts in 32 bits
-constexpr uint64_t PART = 31744;       // a chunk and value head's bytes of the workspace (delta_chunk.h)
+constexpr uint64_t KEYS = 32768, PART = 19456;  // a chunk and key head's, a chunk and value head's bytes of the workspace (delta_chunk.h)
 constexpr uint64_t PIECE = 16384;      // a workgroup's bytes of block_copy
+constexpr uint32_t ROW_MAX = 1u << 24;  // elements of a row: a chunk's bytes are counted in 32 bits
 constexpr uint32_t STEP_ROWS = 32;     // rows up to which the recurrent kernel runs
 
 // The kernels' arguments as abi.cpp declares them (natural alignment: the order says it all).
@@ -28,20 +29,21 @@ struct StepArgs {
   float eps, scale;
 };
 struct PrepArgs {
-  const void *q, *k, *a, *b, *a_log, *dt_bias, *slot, *cu_q, *work;
-  int32_t row, ab_row, tokens, seqs, shape, slots;
-  float eps, scale;
+  const void *q, *k, *a, *b, *a_log, *dt_bias, *slot, *cu_q, *keys, *work;
+  int32_t row, ab_row, tokens, seqs, shape, slots, places;
+  float eps;
 };
 struct ScanArgs {
-  const void *q, *k, *v, *work, *state, *slot, *cu_q, *out;
+  const void *v, *keys, *work, *state, *slot, *cu_q, *out;
   int32_t row, tokens, seqs, shape, slots;
+  float scale;
 };
 struct CopyArgs {
   const void *a, *b, *src, *dst;
   int64_t a_bytes, b_bytes;
   int32_t blocks;
 };
-static_assert(offsetof(ConvArgs, run) == 88 && offsetof(StepArgs, scale) == 124 && offsetof(PrepArgs, scale) == 100 && offsetof(ScanArgs, slots) == 80 &&
+static_assert(offsetof(ConvArgs, run) == 88 && offsetof(StepArgs, scale) == 124 && offsetof(PrepArgs, eps) == 108 && offsetof(ScanArgs, scale) == 76 &&
                   offsetof(CopyArgs, blocks) == 48,
               "as abi.cpp packs them");
 
@@ -104,7 +106,7 @@ int saber_iu8_gdn_workspace(uint32_t tokens, uint32_t seqs, uint32_t max_q, uint
   if (int rc = rows_check("gdn_workspace", tokens, seqs, seqs, true, true)) return rc;
   if (int rc = heads_check("gdn_workspace", key_heads, heads)) return rc;
   if (!bytes) return fail(SABER_IU8_E_ARG, "gdn_workspace: null argument");
-  *bytes = max_q <= STEP_ROWS ? 0 : ((uint64_t)tokens / CHUNK + seqs) * heads * PART;
+  *bytes = max_q <= STEP_ROWS ? 0 : ((uint64_t)tokens / CHUNK + seqs) * (key_heads * KEYS + heads * PART);
   return 0;
 }
 
@@ -118,7 +120,7 @@ int saber_iu8_gdn(saber_iu8_ctx *ctx, const void *q, const void *k, const void *
   if (int rc = rows_check("gdn", tokens, seqs, slots, cu_q, slot)) return rc;
   if (int rc = heads_check("gdn", key_heads, heads)) return rc;
   if (!max_q) return fail(SABER_IU8_E_RULE, "gdn: at most 0 new rows a sequence");
-  if (row % 8 || row > I32_MAX || row < (uint64_t)heads * DIM || ab_row > I32_MAX || ab_row < heads)
+  if (row % 8 || row > ROW_MAX || row < (uint64_t)heads * DIM || ab_row > I32_MAX || ab_row < heads)
     return fail(SABER_IU8_E_RULE, fmt("gdn: rows of %u elements (gates %u): whole 16-byte pieces that cover %u heads of 128", row, ab_row, heads));
   if (!(eps >= 0.f && std::isfinite(eps)) || !std::isfinite(scale)) return fail(SABER_IU8_E_RULE, "gdn: eps must be a number from 0, the scale a number");
   const int32_t shape = (int32_t)(heads | key_heads << 16);
@@ -128,15 +130,16 @@ int saber_iu8_gdn(saber_iu8_ctx *ctx, const void *q, const void *k, const void *
     StepArgs x{q, k, v, a, b, a_log, dt_bias, state, slot, cu_q, kept, out, (int32_t)row, (int32_t)ab_row, (int32_t)tokens, (int32_t)seqs, shape, (int32_t)slots, eps, scale};
     return launch_image(ctx, "delta_step", (uint32_t)items, 256, &x, sizeof x, stream);
   }
-  const uint64_t chunks = ((uint64_t)tokens / CHUNK + seqs) * heads;
-  // Waves a workgroup of the walk
-  const uint32_t waves = items >= 2 * CU_COUNT / 3 ? 8 : items * 2 > CU_COUNT ? 4 : 2;
-  const uint64_t walks = (items * (8 / waves) + 7) / 8 * 8;
+  const uint64_t places = (uint64_t)tokens / CHUNK + seqs, chunks = places * heads;
+  // Pairs of waves a workgroup of the walk
+  const uint32_t pairs = items * 4 <= CU_COUNT ? 2 : 4;
+  const uint64_t walks = (items * (8 / pairs) + 7) / 8 * 8;
   if (chunks > GRID_MAX || walks > GRID_MAX) return fail(SABER_IU8_E_RULE, fmt("gdn: %u rows of %u sequences and %u heads pass a launch's 32-bit sizes", tokens, seqs, heads));
-  PrepArgs p{q, k, a, b, a_log, dt_bias, slot, cu_q, workspace, (int32_t)row, (int32_t)ab_row, (int32_t)tokens, (int32_t)seqs, shape, (int32_t)slots, eps, scale};
-  if (int rc = launch_image(ctx, "delta_prep", (uint32_t)chunks, 256, &p, sizeof p, stream)) return rc;
-  ScanArgs x{q, k, v, workspace, state, slot, cu_q, out, (int32_t)row, (int32_t)tokens, (int32_t)seqs, shape, (int32_t)slots};
-  return launch_image(ctx, waves == 8 ? "delta_scan_w8" : waves == 4 ? "delta_scan_w4" : "delta_scan_w2", (uint32_t)walks, 64 * waves, &x, sizeof x, stream);
+  unsigned char *const keys = (unsigned char *)workspace, *const parts = keys + places * key_heads * KEYS;
+  PrepArgs p{q, k, a, b, a_log, dt_bias, slot, cu_q, keys, parts, (int32_t)row, (int32_t)ab_row, (int32_t)tokens, (int32_t)seqs, shape, (int32_t)slots, (int32_t)places, eps};
+  if (int rc = launch_image(ctx, "delta_prep", (uint32_t)((chunks + 7) / 8 * 8), 256, &p, sizeof p, stream)) return rc;
+  ScanArgs x{v, keys, parts, state, slot, cu_q, out, (int32_t)row, (int32_t)tokens, (int32_t)seqs, shape, (int32_t)slots, scale};
+  return launch_image(ctx, pairs == 2 ? "delta_scan_w2" : "delta_scan_w4", (uint32_t)walks, 128 * pairs, &x, sizeof x, stream);
 }
 
 int saber_iu8_kv_copy(saber_iu8_ctx *ctx, const saber_iu8_kv_cache *c, const int32_t *src, const int32_t *dst, uint32_t n, void *stream) {

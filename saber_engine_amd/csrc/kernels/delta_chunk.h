@@ -6,35 +6,43 @@
 //   U  = T diag(beta) (V - diag(exp G) K^ S0)
 //   O  = scale (diag(exp G) Q^ S0 + [exp(G_i - G_j) q^_i . k^_j, j <= i] U)
 //   S1 = exp(G_63) S0 + K^^T diag(exp(G_63 - G_j)) U
-// Two kernels. delta_prep makes, for all chunks at once, T diag(beta) and the inner matrix of O, each already as the other's operand, and the rows'
-// factors; delta_scan walks a sequence's chunks in order.
+// Two kernels. delta_prep makes, for all chunks at once, T diag(beta) and the inner matrix of O, each already as the other's operand, the rows'
+// factors, and K and Q as the walk reads them; delta_scan walks a sequence's chunks in order.
 //
-// Precision: the state and all that enters it is f32, on the bf16 matrix cores: a row of K or Q is bf16 as it comes (its norm's and decay's
-// factors are moved to the other side of the product), the other side is split into three bf16 terms, 24 bits (dn_split). What goes only
-// into the rows' bf16 answers takes two terms, 16 bits. G is summed, and its differences taken, in f64: after a strong decay the later rows'
-// differences would be left with the sum's digits.
+// Precision: the state and all that enters it is f32, on the f16 matrix cores. A row of K or Q, bf16 as it comes, is an f16 row times a power
+// of two (its largest value brought to 1 .. 2); its norm's and decay's factors are moved to the other side of the product; the other side is split
+// into two f16 terms, 22 bits (dn_split), in a column's own unit, a power of two that follows the column's largest value. What goes only into the rows' bf16 answers takes
+// one term, 11 bits. (Three bf16 terms, which need no units, are half as many products again and twice the lane arithmetic: the walk of 8,192 rows of 48
+// heads 304 us, with f16 235.) G is summed, and its differences taken, in f64: after a strong decay the later rows' differences would be left with the sum's digits.
 #pragma once
 #include "delta_step.h"
 
-// A chunk and value head's part of the workspace. Operands are kept as fragments, 64 lanes x 16 bytes: lane (l % 16, g = l / 16) has row l % 16 of 16 and
-// the columns 4 g .. 4 g + 3 of the first and of the second 16 of 32, which is how a product's result lies (dn_operand).
-// Fragment f of a lower triangle: row block 0, 1 of the first 32 columns; row blocks 2, 3 of the first and of the last.
-constexpr int DN_FRAGS = 6, DN_FRAG = 1024;
+// The workspace: of a chunk and key head K and Q, f16, 16 KiB each, row t's 16-byte pieces exchanged (piece ^ dn_swap(t)) as the walk keeps them in LDS; of a chunk and
+// value head T diag(beta) in two terms, the inner matrix in one, the factors. Operands are kept as fragments, 64 lanes x 16 bytes: lane (l % 16, g = l / 16) has row l % 16 of 16
+// and the columns 4 g .. 4 g + 3 of the first and of the second 16 of 32, which is how a product's result lies (dn_operand).
+// Fragment f of a lower triangle: row blocks 0, 1 of the first 32 columns; row blocks 2, 3 of the first and of the last.
+constexpr int DN_KEYS = 32768, DN_FRAGS = 6, DN_FRAG = 1024;
 static __host__ __device__ constexpr int dn_frag_block(int f) { return f < 2 ? f : 2 + (f - 2) / 2; }
 static __host__ __device__ constexpr int dn_frag_half(int f) { return f < 2 ? 0 : (f - 2) & 1; }
-constexpr int DN_T = 0, DN_INNER = 3 * DN_FRAGS * DN_FRAG, DN_FACTORS = DN_INNER + 2 * DN_FRAGS * DN_FRAG, DN_PART = DN_FACTORS + 1024;
-// the factors, f32: [64] exp(G_i) / |k_i|, [64] scale exp(G_i) / |q_i|, [64] exp(G_63 - G_i) / |k_i|, exp(G_63)
+constexpr int DN_T = 0, DN_INNER = 2 * DN_FRAGS * DN_FRAG, DN_FACTORS = DN_INNER + DN_FRAGS * DN_FRAG, DN_PART = DN_FACTORS + 1024;
+// the factors, f32: [64] exp(G_i) / |k_i|, [64] exp(G_i) / |q_i|, [64] exp(G_63 - G_i) / |k_i| (of the f16 rows), exp(G_63)
 
 static __device__ __forceinline__ int dn_chunk_id(const dn_rows &x) { return (x.t0 >> 6) + x.s; }  // of its first chunk: no two sequences' meet
+// Such that neither four neighbouring pieces of four neighbouring rows nor one piece of 16 rows share a bank.
+static __host__ __device__ constexpr int dn_swap(int t) { return (t & 3) << 2 | (t >> 2 & 3); }
 
 static __device__ __forceinline__ void delta_prep_body(const unsigned short *__restrict__ q, const unsigned short *__restrict__ k,
                                                        const unsigned short *__restrict__ a, const unsigned short *__restrict__ b,
                                                        const float *__restrict__ a_log, const float *__restrict__ dt_bias,
-                                                       const int *__restrict__ slot, const int *__restrict__ cu, unsigned char *__restrict__ work, int row,
-                                                       int ab_row, int tokens, int seqs, int shape, int slots, float eps, float scale) {
+                                                       const int *__restrict__ slot, const int *__restrict__ cu, unsigned char *__restrict__ keys,
+                                                       unsigned char *__restrict__ work, int row, int ab_row, int tokens, int seqs, int shape, int slots,
+                                                       int places, float eps) {
   constexpr int P = 68;  // floats of a row in LDS
-  const int heads = shape & 0xFFFF, group = heads / (shape >> 16);
-  const int id = blockIdx.x / heads, h = blockIdx.x - id * heads, hk = h / group;
+  const int heads = shape & 0xFFFF, key_heads = shape >> 16, group = heads / key_heads;
+  // (to one XCD the heads that read the same rows)
+  const int share = (int)(gridDim.x + 7) >> 3, item = (int)(blockIdx.x & 7) * share + (int)(blockIdx.x >> 3);
+  if (item >= places * heads) return;
+  const int id = item / heads, h = item - id * heads, hk = h / group;
   const int lane = threadIdx.x & 63, wave = at_uniform(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
   int s = -1;
   if (!cu) {
@@ -51,18 +59,22 @@ static __device__ __forceinline__ void delta_prep_body(const unsigned short *__r
   const int c0 = (id - dn_chunk_id(x)) * DN_CHUNK, m = min(x.n - c0, DN_CHUNK);  // the chunk's first row, its rows
   if (c0 < 0 || m <= 0) return;
 
-  __shared__ __attribute__((aligned(16))) float s_a[DN_CHUNK][P], s_i[DN_CHUNK][P], s_t[DN_CHUNK][P];
-  __shared__ double s_sum[DN_CHUNK];
+  // K and Q, 16 KiB each, then A (in the end T) and the inner matrix in their place
+  __shared__ __attribute__((aligned(16))) float s_m[2][DN_CHUNK][P];
+  __shared__ double s_sum[DN_CHUNK];  // in units of log 2
   __shared__ float s_beta[DN_CHUNK], s_rk[DN_CHUNK], s_rq[DN_CHUNK];
+  auto &s_a = s_m[0];
+  auto &s_i = s_m[1];
+  unsigned char *s_k = (unsigned char *)s_m, *s_q = s_k + DN_KEYS / 2;
 
-  // the products of the rows, row block `wave` with those up to it; a row past the end is the last one again, and takes no part
+  // a row past the end is the last one again, and takes no part
   const size_t t0 = x.t0 + c0;
-  auto fragment = [&](const unsigned short *from, int rb, int ks) {
-    return *(const iu8_v4u *)(from + (t0 + min(16 * rb + n, m - 1)) * row + hk * DN + 32 * ks + 8 * g);
-  };
-  iu8_v4u kf[4], qf[4];
+  iu8_v4u kr[4], qr[4];  // rows 16 wave + 4 i + lane / 16, piece lane % 16
 #pragma unroll
-  for (int ks = 0; ks < 4; ++ks) kf[ks] = fragment(k, wave, ks), qf[ks] = fragment(q, wave, ks);
+  for (int i = 0; i < 4; ++i) {
+    const size_t at = (t0 + min(16 * wave + 4 * i + g, m - 1)) * row + hk * DN + 8 * n;
+    kr[i] = *(const iu8_v4u *)(k + at), qr[i] = *(const iu8_v4u *)(q + at);
+  }
   if (wave == 0) {
     const int i = lane;
     float lg = 0.f, be = 0.f;
@@ -70,7 +82,7 @@ static __device__ __forceinline__ void delta_prep_body(const unsigned short *__r
       lg = dn_log_decay(iu8_bf16_f32(a[(t0 + i) * ab_row + h]), a_log[h], dt_bias[h]);
       be = dn_beta(iu8_bf16_f32(b[(t0 + i) * ab_row + h]));
     }
-    double sum = lg;
+    double sum = lg * 1.4426950408889634074;
 #pragma unroll
     for (int y = 1; y < 64; y *= 2) {
       const double z = __shfl_up(sum, y);
@@ -78,53 +90,63 @@ static __device__ __forceinline__ void delta_prep_body(const unsigned short *__r
     }
     s_sum[i] = sum, s_beta[i] = be;
   }
-  {
-    auto norm = [&](const iu8_v4u (&f)[4]) {
-      float ss = 0.f;
+  const int turned = (n ^ (g << 2)) << 4;  // piece n of row 16 wave + 4 i + g, ^ 16 i
 #pragma unroll
-      for (int ks = 0; ks < 4; ++ks)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float y = __uint_as_float(f[ks][e] << 16), z = __uint_as_float(f[ks][e] & 0xFFFF0000u);
-          ss = fmaf(y, y, fmaf(z, z, ss));
-        }
-      ss = at_both<32>(at_both<16>(ss, at_sum2), at_sum2);
-      return 1.f / sqrtf(ss + eps);
-    };
-    const float rk = norm(kf), rq = norm(qf);
-    const bool live = 16 * wave + n < m;
-    if (g == 0) s_rk[16 * wave + n] = live ? rk : 0.f, s_rq[16 * wave + n] = live ? rq * scale : 0.f;
-  }
-  iu8_v4f kk[4], qk[4];
-#pragma unroll
-  for (int jb = 0; jb < 4; ++jb) {
-    kk[jb] = qk[jb] = iu8_v4f{0.f, 0.f, 0.f, 0.f};
-    if (jb <= wave) {
-      iu8_v4u f[4];
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) f[ks] = fragment(k, jb, ks);
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) kk[jb] = dn_mfma(kf[ks], f[ks], kk[jb]), qk[jb] = dn_mfma(qf[ks], f[ks], qk[jb]);
-      dn_settle(kk[jb]), dn_settle(qk[jb]);
-    }
+  for (int i = 0; i < 4; ++i) {
+    const int at = (16 * wave + 4 * i + g) * 256 + (turned ^ (i << 4));
+    *(iu8_v4u *)(s_k + at) = kr[i], *(iu8_v4u *)(s_q + at) = qr[i];
   }
   __syncthreads();
+  // the products of the rows, row block `wave` with those up to it, and Q's with themselves
+  const int row_piece = n * 256 + ((g ^ (n >> 2)) << 4);
+  auto fragment = [&](const unsigned char *from, int rb, int ks) { return *(const iu8_v4u *)(from + rb * 4096 + row_piece + ((ks ^ (n & 3)) << 6)); };
+  iu8_v4f kk[4], qk[4], own = {0.f, 0.f, 0.f, 0.f}, qq = {0.f, 0.f, 0.f, 0.f};
+  {
+    iu8_v4u kf[4], qf[4];
 #pragma unroll
-  for (int jb = 0; jb < 4; ++jb) {
-    const int j = 16 * jb + n;
-    if (jb <= wave) {
-      const double sj = s_sum[j];
-      const float rj = s_rk[j];
+    for (int ks = 0; ks < 4; ++ks) kf[ks] = fragment(s_k, wave, ks), qf[ks] = fragment(s_q, wave, ks);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int i = 16 * wave + 4 * g + r;
-        const float w = i >= j ? expf((float)(s_sum[i] - sj)) * rj : 0.f;
-        s_a[i][j] = i > j ? s_beta[i] * s_rk[i] * w * kk[jb][r] : 0.f;
-        s_i[i][j] = s_rq[i] * w * qk[jb][r];
+    for (int ks = 0; ks < 4; ++ks) own = dn_mfma_bf(kf[ks], kf[ks], own), qq = dn_mfma_bf(qf[ks], qf[ks], qq);
+    dn_settle(own), dn_settle(qq);
+#pragma unroll
+    for (int jb = 0; jb < 4; ++jb) {
+      kk[jb] = qk[jb] = iu8_v4f{0.f, 0.f, 0.f, 0.f};
+      if (jb <= wave) {
+        iu8_v4u f[4];
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) f[ks] = fragment(s_k, jb, ks);
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) kk[jb] = dn_mfma_bf(kf[ks], f[ks], kk[jb]), qk[jb] = dn_mfma_bf(qf[ks], f[ks], qk[jb]);
+        dn_settle(kk[jb]), dn_settle(qk[jb]);
       }
-    } else {
+    }
+  }
+  // |k|^2 and |q|^2 stand on the diagonals; a row's unit is the power of two at or below its length (so that no value passes 2; lengths whose squares
+  // are no f32 count as 2^-63, below anything beside eps)
+  if (g == n >> 2) {
+    const float ks = (n & 2) ? ((n & 1) ? own[3] : own[2]) : ((n & 1) ? own[1] : own[0]), qs = (n & 2) ? ((n & 1) ? qq[3] : qq[2]) : ((n & 1) ? qq[1] : qq[0]);
+    const bool live = 16 * wave + n < m;
+    s_rk[16 * wave + n] = live ? ks : 0.f, s_rq[16 * wave + n] = live ? qs : 0.f;
+  }
+  __syncthreads();
+  auto unit_of = [](float ss) { return max(dn_exponent(sqrtf(ss)), 64); };
+  auto length_of = [&](float ss) { return 1.f / sqrtf(ss + eps); };
+  if (h - hk * group == 0) {
+    unsigned char *to = keys + ((size_t)id * key_heads + hk) * DN_KEYS;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) s_i[16 * wave + 4 * g + r][j] = 0.f, s_t[16 * wave + 4 * g + r][j] = 0.f;
+    for (int i = 0; i < 4; ++i) {
+      const int t = 16 * wave + 4 * i + g, at = t * 256 + (turned ^ (i << 4));
+      const float bk = dn_below(unit_of(s_rk[t])), bq = dn_below(unit_of(s_rq[t]));
+      auto as_f16 = [&](iu8_v4u f, float by) {
+        iu8_v4u y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const dn_v2h z = __builtin_convertvector(iu8_v2f{__uint_as_float(f[e] << 16) * by, __uint_as_float(f[e] & 0xFFFF0000u) * by}, dn_v2h);
+          y[e] = t < m ? __builtin_bit_cast(unsigned, z) : 0u;
+        }
+        return y;
+      };
+      *(iu8_v4u *)(to + at) = as_f16(kr[i], bk), *(iu8_v4u *)(to + DN_KEYS / 2 + at) = as_f16(qr[i], bq);
     }
   }
   unsigned char *mine = work + ((size_t)id * heads + h) * DN_PART;
@@ -132,239 +154,361 @@ static __device__ __forceinline__ void delta_prep_body(const unsigned short *__r
     const int i = lane;
     const double end = s_sum[DN_CHUNK - 1];
     float *f = (float *)(mine + DN_FACTORS);
-    const float eg = expf((float)s_sum[i]);
-    f[i] = eg * s_rk[i], f[64 + i] = eg * s_rq[i], f[128 + i] = expf((float)(end - s_sum[i])) * s_rk[i];
-    if (i == 0) f[192] = expf((float)end);
+    const float eg = __builtin_amdgcn_exp2f((float)s_sum[i]);
+    const float rk = i < m ? length_of(s_rk[i]) * dn_power(unit_of(s_rk[i])) : 0.f, rq = i < m ? length_of(s_rq[i]) * dn_power(unit_of(s_rq[i])) : 0.f;
+    f[i] = eg * rk, f[64 + i] = eg * rq, f[128 + i] = __builtin_amdgcn_exp2f((float)(end - s_sum[i])) * rk;
+    if (i == 0) f[192] = __builtin_amdgcn_exp2f((float)end);
   }
-  __syncthreads();
-  // T's blocks on the diagonal by substitution, a column a lane
-  if (g == 0) {
-    float y[16];
-    const float(*at)[P] = (const float(*)[P])(&s_a[16 * wave][16 * wave]);
+  {
+    float of_row[4], of_query[4];
+    double si[4];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float z = i == n ? 1.f : 0.f;
-#pragma unroll
-      for (int j = 0; j < i; ++j) z = fmaf(-at[i][j], y[j], z);
-      y[i] = z;
+    for (int r = 0; r < 4; ++r) {
+      const int i = 16 * wave + 4 * g + r;
+      of_row[r] = s_beta[i] * length_of(s_rk[i]), of_query[r] = length_of(s_rq[i]), si[r] = s_sum[i];
     }
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s_t[16 * wave + i][16 * wave + n] = y[i];
+    for (int jb = 0; jb < 4; ++jb) {
+      const int j = 16 * jb + n;
+      if (jb <= wave) {
+        const double sj = s_sum[j];
+        const float rj = j < m ? length_of(s_rk[j]) : 0.f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int i = 16 * wave + 4 * g + r;
+          const float w = i >= j ? __builtin_amdgcn_exp2f((float)(si[r] - sj)) * rj : 0.f;
+          s_a[i][j] = i > j ? of_row[r] * w * kk[jb][r] : 0.f;
+          s_i[i][j] = of_query[r] * w * qk[jb][r];
+        }
+      } else if (jb == wave + 1 && !(wave & 1)) {  // (the fragments' other block)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s_a[16 * wave + 4 * g + r][j] = 0.f, s_i[16 * wave + 4 * g + r][j] = 0.f;
+      }
+    }
+  }
+  __syncthreads();
+  auto give = [&](const float (*from)[P], int f, unsigned char *to, bool scaled, bool both) {
+    const int i = 16 * dn_frag_block(f) + n, j = 32 * dn_frag_half(f) + 4 * g;
+    iu8_v4f y = *(const iu8_v4f *)(from[i] + j), z = *(const iu8_v4f *)(from[i] + j + 16);
+    if (scaled) y = y * *(const iu8_v4f *)(s_beta + j), z = z * *(const iu8_v4f *)(s_beta + j + 16);
+    iu8_v4u w[2];
+    dn_operand<2>(y, z, w);
+    *(iu8_v4u *)(to + f * DN_FRAG + lane * 16) = w[0];
+    if (both) *(iu8_v4u *)(to + (DN_FRAGS + f) * DN_FRAG + lane * 16) = w[1];
+  };
+  for (int f = wave; f < DN_FRAGS; f += 4) give(s_i, f, mine + DN_INNER, false, false);
+  // T's blocks on the diagonal by substitution, a column a lane; in A's place
+  if (g == 0) {
+    float y[16];
+    float(*at)[P] = (float(*)[P])(&s_a[16 * wave][16 * wave]);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float z = i == n ? 1.f : 0.f, z1 = 0.f;
+#pragma unroll
+      for (int j = 0; j < i; ++j) {
+        if (j & 1) z1 = fmaf(-at[i][j], y[j], z1);
+        else z = fmaf(-at[i][j], y[j], z);
+      }
+      y[i] = z + z1;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) at[i][n] = y[i];
   }
   __syncthreads();
   // those under it, wave j the column of blocks j: T_ij = -T_ii sum_k A_ik T_kj, on the f32 matrix instruction; a result's rows 4 g + r are the next
   // product's places r of lane group g
-  {
-    iu8_v4f t[4];
+  iu8_v4f t[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) t[0][r] = s_t[16 * wave + 4 * g + r][16 * wave + n];
+  for (int r = 0; r < 4; ++r) t[0][r] = s_a[16 * wave + 4 * g + r][16 * wave + n];
 #pragma unroll
-    for (int d = 1; d < 4; ++d) {
-      const int i = wave + d;
-      if (i < 4) {
-        iu8_v4f y = {0.f, 0.f, 0.f, 0.f}, z = {0.f, 0.f, 0.f, 0.f};
+  for (int d = 1; d < 4; ++d) {
+    const int i = wave + d;
+    if (i < 4) {
+      iu8_v4f y = {0.f, 0.f, 0.f, 0.f}, z = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int e = 0; e < d; ++e) {
-          const iu8_v4f f = *(const iu8_v4f *)&s_a[16 * i + n][16 * (wave + e) + 4 * g];
+      for (int e = 0; e < d; ++e) {
+        const iu8_v4f f = *(const iu8_v4f *)&s_a[16 * i + n][16 * (wave + e) + 4 * g];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) y = __builtin_amdgcn_mfma_f32_16x16x4f32(f[r], t[e][r], y, 0, 0, 0);
-        }
-        dn_settle(y);
-        const iu8_v4f f = *(const iu8_v4f *)&s_t[16 * i + n][16 * i + 4 * g];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) z = __builtin_amdgcn_mfma_f32_16x16x4f32(f[r], y[r], z, 0, 0, 0);
-        dn_settle(z);
-        t[d] = -z;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) s_t[16 * i + 4 * g + r][16 * wave + n] = -z[r];
+        for (int r = 0; r < 4; ++r) y = __builtin_amdgcn_mfma_f32_16x16x4f32(f[r], t[e][r], y, 0, 0, 0);
       }
+      dn_settle(y);
+      const iu8_v4f f = *(const iu8_v4f *)&s_a[16 * i + n][16 * i + 4 * g];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) z = __builtin_amdgcn_mfma_f32_16x16x4f32(f[r], y[r], z, 0, 0, 0);
+      dn_settle(z);
+      t[d] = -z;
     }
   }
   __syncthreads();
-  // both as fragments
-  for (int f = wave; f < 2 * DN_FRAGS; f += 4) {
-    const bool inner = f >= DN_FRAGS;
-    const int ff = inner ? f - DN_FRAGS : f, i = 16 * dn_frag_block(ff) + n, j = 32 * dn_frag_half(ff) + 4 * g;
-    const float *from = inner ? s_i[i] : s_t[i];
-    iu8_v4f y = *(const iu8_v4f *)(from + j), z = *(const iu8_v4f *)(from + j + 16);
-    if (!inner) y = y * *(const iu8_v4f *)(s_beta + j), z = z * *(const iu8_v4f *)(s_beta + j + 16);
-    iu8_v4u w[3];
-    dn_operand<3>(y, z, w);
-    unsigned char *to = mine + (inner ? DN_INNER : DN_T) + ff * DN_FRAG + lane * 16;
 #pragma unroll
-    for (int e = 0; e < 3; ++e)
-      if (!inner || e < 2) *(iu8_v4u *)(to + e * DN_FRAGS * DN_FRAG) = w[e];
-  }
+  for (int d = 1; d < 4; ++d)
+    if (wave + d < 4) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s_a[16 * (wave + d) + 4 * g + r][16 * wave + n] = t[d][r];
+    }
+  __syncthreads();
+  for (int f = wave; f < DN_FRAGS; f += 4) give(s_a, f, mine + DN_T, true, true);
 }
 
-// The walk over a sequence's chunks. A wave has 16 columns of a head's state, 32 registers a lane, for the whole walk, and nothing passes between
+// The order of issue of what stands since the last such call: `AHEAD` reads, then M products, each with up to V lane operations and R reads (`READS` of
+// them in all) behind it. What is left follows.
+template <int M, int V, int R, int AHEAD, int READS>
+static __device__ __forceinline__ void dn_step() {
+  if constexpr (AHEAD > 0) __builtin_amdgcn_sched_group_barrier(AT_DS_READ, AHEAD, 0);
+#pragma unroll
+  for (int i = 0; i < M; ++i) {
+    __builtin_amdgcn_sched_group_barrier(AT_MFMA, 1, 0);
+    if (R > 0 && i * R < READS) __builtin_amdgcn_sched_group_barrier(AT_DS_READ, R, 0);
+    if constexpr (V > 0) __builtin_amdgcn_sched_group_barrier(AT_VALU, V, 0);
+  }
+  __builtin_amdgcn_sched_barrier(0);
+}
+static __device__ __forceinline__ iu8_v2u dn_transposed(const unsigned char *from) {
+  return __builtin_bit_cast(iu8_v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) at_v4s *)from));
+}
+
+// The walk over a sequence's chunks. A wave has 16 columns of a head's state, 32 registers a lane, for the whole walk, and no sum passes between
 // waves: with the state's columns as the MFMA's columns every product's result is the next one's operand where it lies (rows 4 g + r of two
 // blocks of 16 are the eight places of the next, dn_operand). So K's channels are taken 32 ks + 8 g + e by lane group g, as 16 bytes of a row hold
-// them, and row 4 p + r of block 2 ks + hb of K^T S's new state is channel 32 ks + 8 p + 4 hb + r, which the LDS's transposing reads give. Only O is taken
-// the other way round (the same registers, the operands exchanged), so that a lane has four neighbouring values of one row to store.
+// them, and row 4 p + r of block 2 ks + hb of K^T S's new state is channel 32 ks + 8 p + 4 hb + r, which the LDS's transposing reads give.
 //
-// The waves of a workgroup are W neighbouring column blocks of one head and share what they multiply by: a chunk's K, Q, T, inner matrix and factors and
-// each wave's own columns of V come straight from memory into one of two LDS stages, the next chunk's under this one's products; one barrier a
-// chunk.
+// The chunks' chain of products bounds a walk (a wave's lane arithmetic does not run under its own matrix instructions here), so its waves come in pairs: one walks
+// the chain (K S, V - .., U, the next S), the other does what hangs from it, the rows' answers, with the operands that the first leaves in LDS, and asks for K, Q,
+// T, the inner matrix, the factors and V two chunks ahead, which come straight from memory into one of two LDS stages as soon as it has been read. O is
+// taken the other way round (the operands exchanged), so that a lane has four neighbouring values of one row to store. Two meetings a chunk: behind U, where the
+// stage is free, and behind the next S. W pairs a workgroup share a stage.
 template <int W>
-static __device__ __forceinline__ void delta_scan_body(const unsigned short *__restrict__ q, const unsigned short *__restrict__ k,
-                                                       const unsigned short *__restrict__ v, const unsigned char *__restrict__ work,
-                                                       float *__restrict__ state, const int *__restrict__ slot, const int *__restrict__ cu,
-                                                       unsigned short *__restrict__ out, int row, int tokens, int seqs, int shape, int slots) {
-  constexpr int PARTS = 8 / W, K_AT = 0, Q_AT = 16384, W_AT = 32768, V_AT = W_AT + DN_PART, STAGE = V_AT + W * 2048;
-  constexpr int LOADS = 32 + DN_PART / 1024;  // wave-loads of 1 KiB of what is shared
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * STAGE];
-  const int heads = shape & 0xFFFF, group = heads / (shape >> 16);
+static __device__ __forceinline__ void delta_scan_body(const unsigned short *__restrict__ v, const unsigned char *__restrict__ keys,
+                                                       const unsigned char *__restrict__ work, float *__restrict__ state, const int *__restrict__ slot,
+                                                       const int *__restrict__ cu, unsigned short *__restrict__ out, int row, int tokens, int seqs, int shape,
+                                                       int slots, float scale) {
+  constexpr int PARTS = 8 / W, K_AT = 0, Q_AT = DN_KEYS / 2, W_AT = DN_KEYS, V_AT = W_AT + DN_PART, STAGE = V_AT + W * 2048, GIVEN = 8192 + 128;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * STAGE + W * GIVEN];  // stages; of each pair S in one term, U, the columns' units
+  const int heads = shape & 0xFFFF, key_heads = shape >> 16, group = heads / key_heads;
   // workgroups are dealt to the XCDs in turn: those of neighbouring heads, which read the same keys, to one
   const int all = seqs * heads * PARTS, share = (all + 7) / 8, item = (blockIdx.x & 7) * share + (blockIdx.x >> 3);
   if ((int)(blockIdx.x >> 3) >= share || item >= all) return;
   const int s = item / (heads * PARTS), h = item / PARTS - s * heads, hk = h / group, part = item % PARTS;
-  const int lane = threadIdx.x & 63, wave = at_uniform(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = at_uniform(threadIdx.x >> 6), pair = wave % W, n = lane & 15, g = lane >> 4;
   const dn_rows x = dn_sequence(cu, slot, s, tokens, slots);
   if (x.n <= 0) return;
-  const int chunks = (x.n + DN_CHUNK - 1) / DN_CHUNK, column = 16 * (W * part + wave);
+  const int chunks = (x.n + DN_CHUNK - 1) / DN_CHUNK, column = 16 * (W * part + pair);
   const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) unsigned char *)smem;
-  const unsigned char *parts = work + ((size_t)dn_chunk_id(x) * heads + h) * DN_PART;
+  unsigned char *given = smem + 2 * STAGE + pair * GIVEN;  // 1 KiB each: S's four steps, U's row blocks; the state's unit over U's, U's
+  float *units = (float *)(given + 8192);
+  const int row_piece = n * 256 + ((g ^ (n >> 2)) << 4);  // of K's and Q's row n; ^ 4 (ks ^ n % 4) pieces
+  auto meet = []() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
 
-  auto dma = [&](const unsigned char *from, unsigned to) {  // (a lane's own address; 64 x 16 bytes in a row in LDS)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(at_uniform((int)to)), "v"(from) : "memory", "m0");
-  };
-  auto issue = [&](int c, int stage) {
-    const int t0 = x.t0 + c * DN_CHUNK, last = x.t0 + x.n - 1;
-    const unsigned to = lds0 + stage * STAGE;
-    const unsigned char *p = parts + (size_t)c * heads * DN_PART;
+  if (wave < W) {  // ---- the chain
+    float *mine = state + ((size_t)x.slot * heads + h) * (DN * DN) + column + n;
+    auto channel = [&](int b, int r) { return 32 * (b >> 1) + 8 * g + 4 * (b & 1) + r; };
+    iu8_v4f st[8];  // in units of `unit`
+    float unit, per_unit, most = 0.f;  // most: the column's largest value, in units
+    iu8_v4u sw[4][2];
+    auto largest = [](float m, iu8_v4f y) { return fmaxf(fmaxf(fmaxf(fmaxf(m, fabsf(y[0])), fabsf(y[1])), fabsf(y[2])), fabsf(y[3])); };
+    auto give_state = [&](int ks) {
+      dn_operand<2>(st[2 * ks], st[2 * ks + 1], sw[ks]);
+      *(iu8_v4u *)(given + ks * 1024 + lane * 16) = sw[ks][0];
+    };
 #pragma unroll
-    for (int i = 0; i < (LOADS + W - 1) / W; ++i) {
-      const int l = i * W + wave;  // (uniform)
-      if (l < 32) {
-        const unsigned short *base = l < 16 ? k : q;
-        const int rb = (l & 15) >> 2, ks = l & 3;
-        dma((const unsigned char *)(base + (size_t)min(t0 + 16 * rb + n, last) * row + hk * DN + 32 * ks + 8 * g), to + l * 1024);
-      } else if (l < LOADS) {
-        dma(p + (l - 32) * 1024 + lane * 16, to + l * 1024);
-      }
+    for (int b = 0; b < 8; ++b) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) st[b][r] = mine[channel(b, r) * DN];
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      dma((const unsigned char *)(v + (size_t)min(t0 + 32 * i + (lane >> 1), last) * row + h * DN + column + 8 * (lane & 1)), to + V_AT + wave * 2048 + i * 1024);
-  };
-  auto transposed = [](const unsigned char *from) {
-    return __builtin_bit_cast(iu8_v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) at_v4s *)from));
-  };
-
-  issue(0, 0);
-  float *mine = state + ((size_t)x.slot * heads + h) * (DN * DN) + column + n;
-  auto channel = [&](int b, int r) { return 32 * (b >> 1) + 8 * g + 4 * (b & 1) + r; };
-  iu8_v4f st[8];
+    for (int b = 0; b < 8; ++b) most = largest(most, st[b]);
+    most = at_both<32>(at_both<16>(most, at_max2), at_max2);
+    {
+      const int e = most > 0.f ? dn_exponent(most) : 127;
+      unit = dn_power(e), per_unit = dn_below(e), most *= per_unit;
+    }
 #pragma unroll
-  for (int b = 0; b < 8; ++b)
+    for (int b = 0; b < 8; ++b) st[b] *= per_unit;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) st[b][r] = mine[channel(b, r) * DN];
-
-  for (int c = 0; c < chunks; ++c) {
-    unsigned char *at = smem + (c & 1) * STAGE;
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (c + 1 < chunks) issue(c + 1, (c + 1) & 1);
-    const unsigned char *wk = at + W_AT;
-    const float *factor = (const float *)(wk + DN_FACTORS);
-    auto frag = [&](int from, int f) { return *(const iu8_v4u *)(at + from + f * 1024 + lane * 16); };
-
-    // K S and (Q S)^T
-    iu8_v4f p[4], o[4];
+    for (int ks = 0; ks < 4; ++ks) give_state(ks);
+    meet();
+    for (int c = 0; c < chunks; ++c) {
+      const unsigned char *at = smem + (c & 1) * STAGE, *wk = at + W_AT;
+      const float *factor = (const float *)(wk + DN_FACTORS);
+      iu8_v4u kf[4][4], tf[DN_FRAGS][2], kt[8][2], rt[2][2], ru[2][2];
+      iu8_v4f p[4], u[4], er[4], ew[4];
+      iu8_v2u vv[4];
+      // K S; what the next steps need from LDS is asked for ahead of them
 #pragma unroll
-    for (int rb = 0; rb < 4; ++rb) p[rb] = o[rb] = iu8_v4f{0.f, 0.f, 0.f, 0.f};
+      for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      iu8_v4u w[3];
-      dn_operand<3>(st[2 * ks], st[2 * ks + 1], w);
+        for (int rb = 0; rb < 4; ++rb) kf[ks][rb] = *(const iu8_v4u *)(at + K_AT + rb * 4096 + row_piece + ((ks ^ (n & 3)) << 6));
 #pragma unroll
       for (int rb = 0; rb < 4; ++rb) {
-        const iu8_v4u kf = frag(K_AT, rb * 4 + ks), qf = frag(Q_AT, rb * 4 + ks);
-#pragma unroll
-        for (int e = 2; e >= 0; --e) p[rb] = dn_mfma(kf, w[e], p[rb]);
-        o[rb] = dn_mfma(w[1], qf, o[rb]);
-        o[rb] = dn_mfma(w[0], qf, o[rb]);
+        p[rb] = u[rb] = iu8_v4f{0.f, 0.f, 0.f, 0.f};
+        vv[rb] = dn_transposed(at + V_AT + (16 * rb + 4 * g + (n >> 2)) * (32 * W) + pair * 32 + (n & 3) * 8);
+        er[rb] = *(const iu8_v4f *)(factor + 16 * rb + 4 * g);
       }
-    }
 #pragma unroll
-    for (int rb = 0; rb < 4; ++rb) dn_settle(p[rb]), dn_settle(o[rb]);
-    // V - exp(G) / |k| K S
-    iu8_v4u rt[2][3];
+      for (int f = 0; f < DN_FRAGS; ++f)
 #pragma unroll
-    for (int rb = 0; rb < 4; ++rb) {
-      const iu8_v2u vv = transposed(at + V_AT + wave * 2048 + (16 * rb + 4 * g + (n >> 2)) * 32 + (n & 3) * 8);
-      const iu8_v4f er = *(const iu8_v4f *)(factor + 16 * rb + 4 * g);
-      const float vf[4] = {__uint_as_float(vv[0] << 16), __uint_as_float(vv[0] & 0xFFFF0000u), __uint_as_float(vv[1] << 16), __uint_as_float(vv[1] & 0xFFFF0000u)};
+        for (int e = 0; e < 2; ++e) tf[f][e] = *(const iu8_v4u *)(wk + DN_T + (e * DN_FRAGS + f) * DN_FRAG + lane * 16);
+      const float whole = factor[192];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) p[rb][r] = fmaf(-er[r], p[rb][r], vf[r]);
-      o[rb] *= factor[64 + 16 * rb + n];
-    }
+      for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
-    for (int i = 0; i < 2; ++i) dn_operand<3>(p[2 * i], p[2 * i + 1], rt[i]);
-    // U
-    iu8_v4f u[4];
+        for (int e = 1; e >= 0; --e)
 #pragma unroll
-    for (int rb = 0; rb < 4; ++rb) u[rb] = iu8_v4f{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int f = 0; f < DN_FRAGS; ++f) {
-      const int rb = dn_frag_block(f), i = dn_frag_half(f);
-      iu8_v4u w[3];
-#pragma unroll
-      for (int e = 0; e < 3; ++e) w[e] = frag(W_AT + DN_T, e * DN_FRAGS + f);
-#pragma unroll
-      for (int d = 2; d >= 0; --d)  // the smallest products first
-#pragma unroll
-        for (int e = 0; e <= d; ++e) u[rb] = dn_mfma(w[e], rt[i][d - e], u[rb]);
-    }
-#pragma unroll
-    for (int rb = 0; rb < 4; ++rb) dn_settle(u[rb]);
-    // the rows' answers
-    iu8_v4u ut[2][2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) dn_operand<2>(u[2 * i], u[2 * i + 1], ut[i]);
-#pragma unroll
-    for (int f = 0; f < DN_FRAGS; ++f) {
-      const int rb = dn_frag_block(f), i = dn_frag_half(f);
-      const iu8_v4u w0 = frag(W_AT + DN_INNER, f), w1 = frag(W_AT + DN_INNER, DN_FRAGS + f);
-      o[rb] = dn_mfma(ut[i][1], w0, o[rb]);
-      o[rb] = dn_mfma(ut[i][0], w1, o[rb]);
-      o[rb] = dn_mfma(ut[i][0], w0, o[rb]);
-    }
-#pragma unroll
-    for (int rb = 0; rb < 4; ++rb) dn_settle(o[rb]);
-    if (out) {
+          for (int rb = 0; rb < 4; ++rb) p[rb] = dn_mfma(kf[ks][rb], sw[ks][e], p[rb]);
+      dn_step<32, 0, 1, 8, 29>();
+      // V - exp(G) / |k| K S
+      float top = most;
 #pragma unroll
       for (int rb = 0; rb < 4; ++rb) {
-        const int t = c * DN_CHUNK + 16 * rb + n;
-        if (t < x.n)
-          *(iu8_v2u *)(out + ((size_t)(x.t0 + t) * heads + h) * DN + column + 4 * g) =
-              iu8_v2u{iu8_bf16_pack(o[rb][0], o[rb][1]), iu8_bf16_pack(o[rb][2], o[rb][3])};
+        const float vf[4] = {__uint_as_float(vv[rb][0] << 16), __uint_as_float(vv[rb][0] & 0xFFFF0000u), __uint_as_float(vv[rb][1] << 16),
+                             __uint_as_float(vv[rb][1] & 0xFFFF0000u)};
+#pragma unroll
+        for (int r = 0; r < 4; ++r) p[rb][r] = fmaf(vf[r], per_unit, -er[rb][r] * p[rb][r]);
+        top = largest(top, p[rb]);
       }
+      top = at_both<32>(at_both<16>(top, at_max2), at_max2);
+      // The unit moves only when the column's largest value has left 1/8 .. 32 of it: below, terms of f16 would lack bits, and above, 64 rows
+      // could bring the state past f16's range.
+      float was = unit;
+      if (__any(top > 32.f || (top < 0.125f && top > 0.f))) {
+        const int to = min(max(dn_exponent(unit) + (top > 0.f ? dn_exponent(top) - 127 : 0), 7), 247);
+        const float by = unit * dn_below(to);
+        unit = dn_power(to), per_unit = dn_below(to);
+#pragma unroll
+        for (int b = 0; b < 8; ++b) st[b] *= by;
+#pragma unroll
+        for (int rb = 0; rb < 4; ++rb) p[rb] *= by;
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) dn_operand<2>(p[2 * i], p[2 * i + 1], rt[i]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int b = 0; b < 8; ++b) {
+          const unsigned char *from = at + K_AT + (4 * g + (n >> 2)) * 256 + (((n & 3) ^ g) << 4) + (((b >> 1) ^ (n >> 2)) << 6) + (b & 1) * 8;
+          const iu8_v2u lo = dn_transposed(from + 2 * i * 4096), hi = dn_transposed(from + (2 * i + 1) * 4096);
+          kt[b][i] = iu8_v4u{lo[0], lo[1], hi[0], hi[1]};
+        }
+#pragma unroll
+      for (int rb = 0; rb < 4; ++rb) ew[rb] = *(const iu8_v4f *)(factor + 128 + 16 * rb + 4 * g);
+      // U, the smallest products first
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int y = 0; y < 3; ++y)
+#pragma unroll
+          for (int rb = 2 * i; rb < 4; ++rb) u[rb] = dn_mfma(tf[rb < 2 ? rb : 2 * rb - 2 + i][y == 1], rt[i][y == 0], u[rb]);
+#pragma unroll
+      for (int b = 0; b < 8; ++b) st[b] *= whole;
+#pragma unroll
+      for (int rb = 0; rb < 4; ++rb) *(iu8_v4f *)(given + (4 + rb) * 1024 + lane * 16) = u[rb];
+      if (g == 0) units[n] = was * per_unit, units[16 + n] = unit;
+      meet();
+      // the next state
+#pragma unroll
+      for (int rb = 0; rb < 4; ++rb) u[rb] *= ew[rb];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) dn_operand<2>(u[2 * i], u[2 * i + 1], ru[i]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 1; e >= 0; --e)
+#pragma unroll
+          for (int b = 0; b < 8; ++b) st[b] = dn_mfma(kt[b][i], ru[i][e], st[b]);
+      most = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        give_state(ks);
+        most = largest(largest(most, st[2 * ks]), st[2 * ks + 1]);
+      }
+      meet();
     }
-    // the next state
-#pragma unroll
-    for (int rb = 0; rb < 4; ++rb) u[rb] *= *(const iu8_v4f *)(factor + 128 + 16 * rb + 4 * g);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) dn_operand<3>(u[2 * i], u[2 * i + 1], rt[i]);
-    const float whole = factor[192];
-#pragma unroll
-    for (int b = 0; b < 8; ++b) st[b] *= whole;
 #pragma unroll
     for (int b = 0; b < 8; ++b)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const unsigned char *kt = at + K_AT + (b >> 1) * 1024 + ((n & 3) * 16 + 4 * g + (n >> 2)) * 16 + (b & 1) * 8;
-        const iu8_v2u lo = transposed(kt + 2 * i * 4096), hi = transposed(kt + (2 * i + 1) * 4096);
-        const iu8_v4u kf = {lo[0], lo[1], hi[0], hi[1]};
-#pragma unroll
-        for (int e = 2; e >= 0; --e) st[b] = dn_mfma(kf, rt[i][e], st[b]);
-      }
-#pragma unroll
-    for (int b = 0; b < 8; ++b) dn_settle(st[b]);
+      for (int r = 0; r < 4; ++r) mine[channel(b, r) * DN] = st[b][r] * unit;
+    return;
   }
+
+  // ---- the answers, and what comes from memory
+  const size_t id = dn_chunk_id(x);
+  const unsigned row_bytes = row * 2;
+  auto dma = [&](const unsigned char *from, unsigned off, unsigned to) {  // 64 lanes x 16 bytes, in a row in LDS
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(at_uniform((int)to)), "v"(off), "s"(from) : "memory", "m0");
+  };
+  constexpr int KEY_LOADS = DN_KEYS / 1024 / W, PART_LOADS = (DN_PART / 1024 + W - 1) / W, LOADS = KEY_LOADS + PART_LOADS + 2;  // a wave's
+  auto issue = [&](int c) {
+    const int last = x.n - c * DN_CHUNK - 1;  // (a row of V past the end is the last one again, and takes no part)
+    const unsigned to = lds0 + (c & 1) * STAGE;
+    const unsigned char *kp = keys + ((id + c) * key_heads + hk) * DN_KEYS, *p = work + ((id + c) * heads + h) * DN_PART;
+    const unsigned char *vp = (const unsigned char *)v + (size_t)(x.t0 + c * DN_CHUNK) * row_bytes + (h * DN + 16 * W * part) * 2;
 #pragma unroll
-  for (int b = 0; b < 8; ++b)
+    for (int i = 0; i < KEY_LOADS; ++i) dma(kp + (W * i + pair) * 1024, lane * 16, to + K_AT + (W * i + pair) * 1024);
+    // (as many a wave: the last one again where there are too few)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) mine[channel(b, r) * DN] = st[b][r];
+    for (int i = 0; i < PART_LOADS; ++i) {
+      const int l = min(W * i + pair, DN_PART / 1024 - 1);
+      dma(p + l * 1024, lane * 16, to + W_AT + l * 1024);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int l = W * i + pair;  // 32 / W rows of 32 W bytes
+      dma(vp, (unsigned)min(32 / W * l + lane / (2 * W), last) * row_bytes + lane % (2 * W) * 16, to + V_AT + l * 1024);
+    }
+  };
+  auto arrived = [&](bool more) {  // (loads are counted in order: all but the youngest chunk's)
+    if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  };
+  iu8_v2u y[4];
+  auto store = [&](int c) {
+#pragma unroll
+    for (int rb = 0; rb < 4; ++rb) {
+      const int t = c * DN_CHUNK + 16 * rb + n;
+      if (t < x.n) *(iu8_v2u *)(out + ((size_t)(x.t0 + t) * heads + h) * DN + column + 4 * g) = y[rb];
+    }
+  };
+  issue(0);
+  if (chunks > 1) issue(1);
+  arrived(chunks > 1);
+  meet();
+  for (int c = 0; c < chunks; ++c) {
+    const unsigned char *at = smem + (c & 1) * STAGE, *wk = at + W_AT;
+    const float *factor = (const float *)(wk + DN_FACTORS);
+    if (c) {
+      store(c - 1);
+      if (c + 1 < chunks) issue(c + 1);  // (its stage was read in the chunk before)
+    }
+    iu8_v4f o[4];
+    float eq[4];
+#pragma unroll
+    for (int rb = 0; rb < 4; ++rb) o[rb] = iu8_v4f{0.f, 0.f, 0.f, 0.f}, eq[rb] = factor[64 + 16 * rb + n];
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      const iu8_v4u w = *(const iu8_v4u *)(given + ks * 1024 + lane * 16);
+#pragma unroll
+      for (int rb = 0; rb < 4; ++rb) o[rb] = dn_mfma(w, *(const iu8_v4u *)(at + Q_AT + rb * 4096 + row_piece + ((ks ^ (n & 3)) << 6)), o[rb]);
+    }
+    iu8_v4u inner[DN_FRAGS];
+#pragma unroll
+    for (int f = 0; f < DN_FRAGS; ++f) inner[f] = *(const iu8_v4u *)(wk + DN_INNER + f * DN_FRAG + lane * 16);
+    meet();  // (the stage has been read)
+    const iu8_v4f ratio = *(const iu8_v4f *)(units + 4 * g), un = *(const iu8_v4f *)(units + 16 + 4 * g) * scale;
+    iu8_v4u ut[2][1];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      dn_operand<1>(*(const iu8_v4f *)(given + (4 + 2 * i) * 1024 + lane * 16), *(const iu8_v4f *)(given + (5 + 2 * i) * 1024 + lane * 16), ut[i]);
+#pragma unroll
+    for (int rb = 0; rb < 4; ++rb) o[rb] *= ratio * eq[rb];
+#pragma unroll
+    for (int f = 0; f < DN_FRAGS; ++f) o[dn_frag_block(f)] = dn_mfma(ut[dn_frag_half(f)][0], inner[f], o[dn_frag_block(f)]);
+#pragma unroll
+    for (int rb = 0; rb < 4; ++rb) {
+      o[rb] *= un;
+      y[rb] = iu8_v2u{iu8_bf16_pack(o[rb][0], o[rb][1]), iu8_bf16_pack(o[rb][2], o[rb][3])};
+    }
+    arrived(false);
+    meet();
+  }
+  store(chunks - 1);
 }

@@ -34,13 +34,20 @@ static __device__ __forceinline__ float dn_log_decay(float a, float a_log, float
 }
 static __device__ __forceinline__ float dn_beta(float b) { return 1.f / (1.f + expf(-b)); }
 
-// f32 as a sum of bf16: the first N terms, 8 bits of the mantissa each (three are all 24), of a pair of values at a time.
+typedef _Float16 dn_v8h __attribute__((ext_vector_type(8)));
+typedef _Float16 dn_v2h __attribute__((ext_vector_type(2)));
+
+// f32 as a sum of f16: the first N terms, 11 bits each, of a pair of values (of up to about 1: what two terms leave is 2^-25 at most, the f16's last
+// step below 2^-14, which the matrix instructions keep). What a term leaves is exact; v_fma_mix takes the f16 as it is, where conversion and
+// subtraction are two. (It is asm because the compiler makes those two of it. The conversion to f16 has read x and y in front of it, so a matrix result is there.)
 template <int N>
 static __device__ __forceinline__ void dn_split(float x, float y, unsigned (&t)[N]) {
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    t[i] = iu8_bf16_pack(x, y);
-    x -= __uint_as_float(t[i] << 16), y -= __uint_as_float(t[i] & 0xFFFF0000u);
+    const dn_v2h h = __builtin_convertvector(iu8_v2f{x, y}, dn_v2h);
+    t[i] = __builtin_bit_cast(unsigned, h);
+    if (i + 1 < N)
+      asm("v_fma_mix_f32 %0, %2, -1.0, %0 op_sel_hi:[1,0,0]\n\tv_fma_mix_f32 %1, %2, -1.0, %1 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "+v"(x), "+v"(y) : "v"(t[i]));
   }
 }
 // Two result blocks of a 16 x 16 product, rows 4 g + r of each, as the N terms of the next product's operand: its eight places
@@ -52,8 +59,15 @@ static __device__ __forceinline__ void dn_operand(iu8_v4f a, iu8_v4f b, iu8_v4u 
 #pragma unroll
   for (int i = 0; i < N; ++i) t[i] = iu8_v4u{x[0][i], x[1][i], x[2][i], x[3][i]};
 }
-static __device__ __forceinline__ iu8_v4f dn_mfma(iu8_v4u a, iu8_v4u b, iu8_v4f c) {
+static __device__ __forceinline__ iu8_v4f dn_mfma_bf(iu8_v4u a, iu8_v4u b, iu8_v4f c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(at_bf(a), at_bf(b), c, 0, 0, 0);
 }
+static __device__ __forceinline__ iu8_v4f dn_mfma(iu8_v4u a, iu8_v4u b, iu8_v4f c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(dn_v8h, a), __builtin_bit_cast(dn_v8h, b), c, 0, 0, 0);
+}
+// The power of two at or below |x| (x a number), and its reciprocal; both ordinary numbers.
+static __device__ __forceinline__ int dn_exponent(float x) { return min(max((int)(__float_as_uint(x) >> 23 & 255u), 7), 247); }
+static __device__ __forceinline__ float dn_power(int e) { return __uint_as_float((unsigned)e << 23); }
+static __device__ __forceinline__ float dn_below(int e) { return __uint_as_float((unsigned)(254 - e) << 23); }
 // A matrix instruction's result, read in the block that makes it (attn_few.h has why).
 static __device__ __forceinline__ void dn_settle(iu8_v4f &x) { asm volatile("" : "+v"(x)); }

@@ -3,7 +3,7 @@
 //
 //   delta_conv_w{2,3,4}     short causal convolution and SiLU of new rows (delta_conv.h)
 //   delta_step              the gated delta rule a row at a time (delta_step.h)
-//   delta_prep, delta_scan_w{2,4,8}  ... in chunks of 64 rows (delta_chunk.h)
+//   delta_prep, delta_scan_w{2,4}  ... in chunks of 64 rows (delta_chunk.h)
 //   block_copy              blocks of two arrays to other blocks (block_copy.h)
 #include "block_copy.h"
 #include "delta_chunk.h"
@@ -32,20 +32,19 @@ extern "C" __global__ __launch_bounds__(256) void delta_step(
 extern "C" __global__ __launch_bounds__(256) void delta_prep(
     const unsigned short *__restrict__ q, const unsigned short *__restrict__ k, const unsigned short *__restrict__ a, const unsigned short *__restrict__ b,
     const float *__restrict__ a_log, const float *__restrict__ dt_bias, const int *__restrict__ slot, const int *__restrict__ cu_q,
-    unsigned char *__restrict__ work, int row, int ab_row, int tokens, int seqs, int shape, int slots, float eps, float scale) {
-  delta_prep_body(q, k, a, b, a_log, dt_bias, slot, cu_q, work, row, ab_row, tokens, seqs, shape, slots, eps, scale);
+    unsigned char *__restrict__ keys, unsigned char *__restrict__ work, int row, int ab_row, int tokens, int seqs, int shape, int slots, int places, float eps) {
+  delta_prep_body(q, k, a, b, a_log, dt_bias, slot, cu_q, keys, work, row, ab_row, tokens, seqs, shape, slots, places, eps);
 }
 
-#define DELTA_SCAN(W)                                                                                                                  \
-  extern "C" __global__ __launch_bounds__(64 * W) void delta_scan_w##W(                                                                \
-      const unsigned short *__restrict__ q, const unsigned short *__restrict__ k, const unsigned short *__restrict__ v,                \
-      const unsigned char *__restrict__ work, float *__restrict__ state, const int *__restrict__ slot, const int *__restrict__ cu_q,   \
-      unsigned short *__restrict__ out, int row, int tokens, int seqs, int shape, int slots) {                                         \
-    delta_scan_body<W>(q, k, v, work, state, slot, cu_q, out, row, tokens, seqs, shape, slots);                                        \
+#define DELTA_SCAN(W)                                                                                                                         \
+  extern "C" __global__ __launch_bounds__(128 * W) void delta_scan_w##W(                                                                      \
+      const unsigned short *__restrict__ v, const unsigned char *__restrict__ keys, const unsigned char *__restrict__ work,                   \
+      float *__restrict__ state, const int *__restrict__ slot, const int *__restrict__ cu_q, unsigned short *__restrict__ out, int row,        \
+      int tokens, int seqs, int shape, int slots, float scale) {                                                                              \
+    delta_scan_body<W>(v, keys, work, state, slot, cu_q, out, row, tokens, seqs, shape, slots, scale);                                        \
   }
 DELTA_SCAN(2)
 DELTA_SCAN(4)
-DELTA_SCAN(8)
 
 extern "C" __global__ __launch_bounds__(256) void block_copy(unsigned char *__restrict__ a, unsigned char *__restrict__ b, const int *__restrict__ src,
                                                              const int *__restrict__ dst, long long a_bytes, long long b_bytes, int blocks) {

@@ -33,6 +33,9 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # -ffp-contract=off: every product and sum rounds where the source says (the epilogue contract);
 # the packed-fp32 feature is switched off for every device compile of this tree.
 FLAGS = f"--genco --offload-arch={ARCH} -O3 -ffp-contract=off -Xclang -target-feature -Xclang -packed-fp32-ops"
+# delta_net: matrix results in ordinary registers also where one wave a SIMD leaves it 512 of them (lane arithmetic reads most of them, each
+# through a copy otherwise)
+OWN_FLAGS = {"delta_net": "-mllvm -amdgpu-mfma-vgpr-form=1"}
 PLUGINS = ("macaq_iu8", "macaq_iu8f", "macaq_i8q", "mxfp4_hadi8", "attn_glue_hadi8", "moe_iu8", "attn_paged", "delta_net", "iu8_probe")
 # test infrastructure (accumulator and table taps of the parity suite): built beside the plugin
 # directory, where opening the plugin set does not see it
@@ -112,9 +115,10 @@ def build_plugin(stem, out_dir=PREBUILT):
     if src is None:
         raise FileNotFoundError(f"no source for `{stem}` under {KERNELS}")
     os.makedirs(out_dir, exist_ok=True)
-    flags = FLAGS.split()
+    all_flags = " ".join(filter(None, (FLAGS, OWN_FLAGS.get(stem))))
+    flags = all_flags.split()
     pp = _run([HIPCC] + flags + ["-E", "-P", src, "-o", "-"]).stdout.encode()
-    build_hash = hashlib.sha256(pp + FLAGS.encode()).hexdigest()
+    build_hash = hashlib.sha256(pp + all_flags.encode()).hexdigest()
     hsaco = os.path.join(out_dir, f"{stem}.hsaco")
     _run([HIPCC] + flags + [src, "-o", hsaco])
     with open(src, "rb") as f:
@@ -122,7 +126,7 @@ def build_plugin(stem, out_dir=PREBUILT):
     manifest = os.path.join(out_dir, f"{stem}.manifest.toml")
     L = _lib()
     rc = L.saber_iu8_manifest_write(hsaco.encode(), stem.encode(), ARCH.encode(), os.path.relpath(src, ROOT).encode(),
-                                    src_sha.encode(), FLAGS.encode(), build_hash.encode(), manifest.encode())
+                                    src_sha.encode(), all_flags.encode(), build_hash.encode(), manifest.encode())
     if rc != 0:
         raise RuntimeError(f"manifest for {stem}: {L.saber_iu8_last_error().decode()}")
     refusal = ctypes.c_int(0)

@@ -9,7 +9,8 @@ D = 128
 # chain of 16 and a tree of 3, or a matrix product's 12 steps of 32), the norm of k (sum, root, quotient, product: 12, twice), the gates
 # (exponentials and logarithms of 2 units each, 8), the update itself (3).
 ROW = 96
-TWO_TERMS = 2.0 ** -16       # of a product whose f32 factor is taken as two bf16 terms
+# What enters an answer alone is rounded to f16 in the chunked form (half a step of 2^-11 relative): the state of Q S, both factors of the inner matrix times U
+F16 = 2.0 ** -11
 
 
 def gates(a, b, a_log, dt_bias):
@@ -25,28 +26,29 @@ def rule(q, k, v, a, b, a_log, dt_bias, state, eps, scale, chunked=False):
 
     The tolerances: a column's error goes through each row's update as the column does, by decay (1 - beta k^ k^T), which lengthens nothing, and each row
     adds ROW roundings of the column's length and its value. An answer has the column's error (|q^| = 1), the same roundings of its own sum,
-    in the chunked form two-term products of the chunk's updates and of the state in front of it, and is rounded once. (In chunks: a row's update is
-    a sum of at most 64 inputs with weights of at most 1, so the same roundings as many times, which is what the rows' own add up to.)"""
+    in the chunked form f16 factors beside the state in front of the chunk and its updates, and is rounded once. (In chunks: a row's update is
+    a sum of at most 64 inputs with weights of at most 1, each factor of a product that is f32 taken to 2^-22, four roundings of f32, or to 2^-25 of the column's
+    unit, at most eight times its largest value: 64 roundings of the column's length once over the keys. Their 64-fold is less than what the chunk's rows add up to.)"""
     n, heads = v.shape[:2]
     of = np.arange(heads) // (heads // k.shape[1])
     decay, beta = gates(a, b, a_log, dt_bias)
     s, e = state.copy(), np.zeros((heads, D))
     out, tol, states, tols = np.zeros(v.shape), np.zeros(v.shape), [s.copy()], [e.copy()]
-    mass = np.zeros((heads, D))
+    mass = held = np.zeros((heads, D))
     for i in range(n):
         kh = k[i, of] / np.sqrt((k[i, of] ** 2).sum(-1, keepdims=True) + eps)
         qh = q[i, of] / np.sqrt((q[i, of] ** 2).sum(-1, keepdims=True) + eps)
         length = np.sqrt((s ** 2).sum(1))
         if i % 64 == 0:
-            mass = length.copy()
+            held, mass = length.copy(), np.zeros((heads, D))
         s = s * decay[i][:, None, None]
         u = beta[i][:, None] * (v[i] - np.einsum("hkv,hk->hv", s, kh))
         s = s + kh[:, :, None] * u[:, None, :]
         new = np.sqrt((s ** 2).sum(1))
         e = e * decay[i][:, None] + ROW * F32 * (length + new + np.abs(v[i]))
-        mass = mass * decay[i][:, None] + np.abs(u)
+        held, mass = held * decay[i][:, None], mass * decay[i][:, None] + np.abs(u)
         out[i] = scale * np.einsum("hkv,hk->hv", s, qh)
-        slack = e + ROW * F32 * (length + new + np.abs(v[i])) + (TWO_TERMS * mass if chunked else 0.0)
+        slack = e + ROW * F32 * (length + new + np.abs(v[i])) + (F16 * (held + 2.01 * mass) if chunked else 0.0)
         tol[i] = BF16 * np.abs(out[i]) * 1.01 + abs(scale) * slack + 1e-30
         states.append(s), tols.append(e.copy())
     return out, tol, states, [t[:, None, :] + 1e-30 for t in tols]
