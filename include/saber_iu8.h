@@ -660,7 +660,8 @@ int saber_iu8_gdn_conv(saber_iu8_ctx *ctx, const void *x, uint32_t x_row, const 
  * max_q: the most new rows of a sequence, for the choice of the kernel alone. Long rows are taken in chunks of 64, with the workspace of saber_iu8_gdn_workspace (made
  * for (tokens, seqs, max_q), it holds every call of the same heads with at most these; calls that share it must not overlap in time), the rest, and whatever has no
  * workspace, kept, or no out, a row at a time: the same rule, other roundings. States, norms and sums in f32 (the chunks' matrix products hold 22 bits of
- * what enters the state, 11 of what goes into the rows' answers alone), out rounded once; the same bytes on every run. */
+ * what enters the state, 11 of what goes into the rows' answers alone, and of both
+ * nothing below 2^-26 of the largest value that its column has in the 64 rows), out rounded once; the same bytes on every run. */
 int saber_iu8_gdn_workspace(uint32_t tokens, uint32_t seqs, uint32_t max_q, uint32_t key_heads, uint32_t heads, uint64_t *bytes);
 int saber_iu8_gdn(saber_iu8_ctx *ctx, const void *q, const void *k, const void *v, uint32_t row, const void *a, const void *b, uint32_t ab_row, const float *a_log,
                   const float *dt_bias, float *state, uint32_t slots, const int32_t *slot, const int32_t *cu_q, const int32_t *kept, void *out, uint32_t tokens,

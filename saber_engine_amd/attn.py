@@ -14,11 +14,19 @@ def _is(t, dtype, n, device):
             t.device.type == device.type and device.index in (None, t.device.index))
 
 
+def device_numbers(numbers, device):
+    return torch.tensor(numbers, dtype=torch.int32, device=device)
+
+
+def current_stream(device):
+    return torch.cuda.current_stream(device).cuda_stream if device.type == "cuda" else 0
+
+
 class PagedKvCache:
     """The pages of one layer's sequences. The host deals pages (reserve, release); the table and the counts lie on the device, where
-    the kernels read them, so that a captured step follows them; reserve and release write there on torch's current stream. While a step
+    the kernels read them, so that a captured step follows them; reserve, release, fork, trim and compact write there on torch's current stream. While a step
     runs they must stand still: where steps take another stream than torch's current one, order the two (make it current around reserve, release
-    and writes of kv_len, or wait for the step)."""
+    and writes of kv_len, or wait for the step). A page that several sequences share (fork) is whole, and written by none of them."""
 
     def __init__(self, seqs, kv_heads, head_dim, max_kv, pages=None, page_tokens=64, kind=iu8.KV_BF16, k_scale=None, v_scale=None, device="cuda"):
         """max_kv: the most tokens a sequence may hold; pages: of all sequences together (None: enough for all at that length);
@@ -35,6 +43,7 @@ class PagedKvCache:
         self.table = torch.full((seqs, self.table_stride), -1, dtype=torch.int32, device=device)
         self.kv_len = torch.zeros(seqs, dtype=torch.int32, device=device)
         self._free, self._held = list(range(self.pages - 1, -1, -1)), [[] for _ in range(seqs)]
+        self._holders = [0] * self.pages        # sequences that a page belongs to
         scale = [s.data_ptr() if s is not None else None for s in (k_scale, v_scale)]
         self.desc = iu8.KvCache.of(self.k.data_ptr(), self.v.data_ptr(), self.table.data_ptr(), self.kv_len.data_ptr(), kv_heads=kv_heads,
                                    head_dim=head_dim, page_tokens=page_tokens, pages=self.pages, table_stride=self.table_stride, kind=kind,
@@ -48,16 +57,89 @@ class PagedKvCache:
         if want - len(held) > len(self._free):
             raise iu8.IU8Error(iu8.E_RULE, f"{want - len(held)} more pages wanted, {len(self._free)} free")
         if want > len(held):
-            new = [self._free.pop() for _ in range(want - len(held))]
+            new = self._deal(want - len(held))
             self.table[seq, len(held):want] = torch.tensor(new, dtype=torch.int32, device=self.table.device)
             held += new
 
     def release(self, seq):
-        """The sequence's pages back, its count to zero."""
-        self._free += reversed(self._held[seq])
+        """The sequence's pages back (those that another sequence shares stay its), its count to zero."""
+        self._back(self._held[seq])
         self._held[seq] = []
         self.table[seq] = -1
         self.kv_len[seq] = 0
+
+    def _deal(self, n):
+        new = [self._free.pop() for _ in range(n)]
+        for p in new:
+            self._holders[p] = 1
+        return new
+
+    def _back(self, pages):
+        for p in reversed(pages):
+            self._holders[p] -= 1
+            if not self._holders[p]:
+                self._free.append(p)
+
+    def _copy(self, ctx, pairs):  # [(page, the page it is copied to)]
+        if pairs:
+            src, dst = (device_numbers([p[i] for p in pairs], self.table.device) for i in range(2))
+            ctx.kv_copy(self.desc, src.data_ptr(), dst.data_ptr(), len(pairs), current_stream(self.table.device))
+
+    def fork(self, ctx, src, dst, tokens):
+        """Sequence dst, which has none, gets sequence src's first `tokens` positions: the pages that they fill are shared, the last one, where
+        they end inside it, is copied. dst's count becomes `tokens`."""
+        held, whole, more = self._held[src], tokens // self.page_tokens, tokens % self.page_tokens > 0
+        if self._held[dst] or src == dst or tokens < 0 or whole + more > len(held):
+            raise iu8.IU8Error(iu8.E_RULE, f"{tokens} tokens of sequence {src}'s {len(held)} pages to sequence {dst}, which has {len(self._held[dst])}")
+        if more and not self._free:
+            raise iu8.IU8Error(iu8.E_RULE, "a page more wanted, none free")
+        new = held[:whole]
+        for p in new:
+            self._holders[p] += 1
+        if more:
+            new = new + self._deal(1)
+            self._copy(ctx, [(held[whole], new[whole])])
+        if new:
+            self.table[dst, :len(new)] = device_numbers(new, self.table.device)
+        self._held[dst] = new
+        self.kv_len[dst] = tokens
+
+    def trim(self, ctx, seq, tokens):
+        """The sequence's positions from `tokens` on back, as for drafted tokens that were not taken: pages behind them free, its count at most
+        `tokens`. A shared page that the sequence would write in next becomes a copy of its own."""
+        held, whole, more = self._held[seq], max(tokens, 0) // self.page_tokens, max(tokens, 0) % self.page_tokens > 0
+        if whole + more > len(held):
+            return
+        own = more and self._holders[held[whole]] > 1
+        if own and not self._free and all(self._holders[p] > 1 for p in held[whole + 1:]):
+            raise iu8.IU8Error(iu8.E_RULE, "a page more wanted, none free")
+        self._back(held[whole + more:])
+        last = held[whole:whole + more]
+        if own:
+            page = self._deal(1)
+            self._copy(ctx, [(last[0], page[0])])
+            self._back(last)
+            self.table[seq, whole] = page[0]
+            last = page
+        self.table[seq, whole + more:] = -1
+        self._held[seq] = held[:whole] + last
+        self.kv_len[seq].clamp_(max=max(tokens, 0))
+
+    def compact(self, ctx):
+        """The pages in use to the front of the pool; returns how many they are. Those behind them can then be given up, or another pool's."""
+        used = [p for p in range(self.pages) if self._holders[p]]
+        n = len(used)
+        to = dict(zip([p for p in used if p >= n], [p for p in range(n) if not self._holders[p]]))
+        self._copy(ctx, list(to.items()))
+        if to:
+            for old, new in to.items():
+                self._holders[new], self._holders[old] = self._holders[old], 0
+            for seq, held in enumerate(self._held):
+                if any(p in to for p in held):
+                    self._held[seq] = held = [to.get(p, p) for p in held]
+                    self.table[seq, :len(held)] = device_numbers(held, self.table.device)
+            self._free = list(range(self.pages - 1, n - 1, -1))
+        return n
 
 
 class AttnLayerIU8:

@@ -319,7 +319,7 @@ static __device__ __forceinline__ void delta_scan_body(const unsigned short *__r
     for (int b = 0; b < 8; ++b) most = largest(most, st[b]);
     most = at_both<32>(at_both<16>(most, at_max2), at_max2);
     {
-      const int e = most > 0.f ? dn_exponent(most) : 127;
+      const int e = most > 0.f ? max(dn_exponent(most) - 4, 7) : 127;
       unit = dn_power(e), per_unit = dn_below(e), most *= per_unit;
     }
 #pragma unroll
@@ -367,11 +367,11 @@ static __device__ __forceinline__ void delta_scan_body(const unsigned short *__r
         top = largest(top, p[rb]);
       }
       top = at_both<32>(at_both<16>(top, at_max2), at_max2);
-      // The unit moves only when the column's largest value has left 1/8 .. 32 of it: below, terms of f16 would lack bits, and above, 64 rows
-      // could bring the state past f16's range.
+      // The unit, in the beginning a 16th of the column's largest value, moves only when that has left 2 .. 256 of it: below, terms of f16 would lack bits; above,
+      // they could pass its range (inputs are at most 256 (1 + sqrt(128)), and 64 of them lengthen a column by no more than 8 of them).
       float was = unit;
-      if (__any(top > 32.f || (top < 0.125f && top > 0.f))) {
-        const int to = min(max(dn_exponent(unit) + (top > 0.f ? dn_exponent(top) - 127 : 0), 7), 247);
+      if (__any(top > 256.f || (top < 2.f && top > 0.f))) {
+        const int to = min(max(dn_exponent(unit) + (top > 0.f ? dn_exponent(top) - 131 : 0), 7), 247);
         const float by = unit * dn_below(to);
         unit = dn_power(to), per_unit = dn_below(to);
 #pragma unroll

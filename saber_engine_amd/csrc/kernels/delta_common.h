@@ -37,8 +37,8 @@ static __device__ __forceinline__ float dn_beta(float b) { return 1.f / (1.f + e
 typedef _Float16 dn_v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 dn_v2h __attribute__((ext_vector_type(2)));
 
-// f32 as a sum of f16: the first N terms, 11 bits each, of a pair of values (of up to about 1: what two terms leave is 2^-25 at most, the f16's last
-// step below 2^-14, which the matrix instructions keep). What a term leaves is exact; v_fma_mix takes the f16 as it is, where conversion and
+// f32 as a sum of f16: the first N terms, 11 bits each, of a pair of values (what two terms leave is 2^-22 of a value, and no less than half of f16's last
+// step, 2^-25; the matrix instructions keep values below 2^-14). What a term leaves is exact; v_fma_mix takes the f16 as it is, where conversion and
 // subtraction are two. (It is asm because the compiler makes those two of it. The conversion to f16 has read x and y in front of it, so a matrix result is there.)
 template <int N>
 static __device__ __forceinline__ void dn_split(float x, float y, unsigned (&t)[N]) {

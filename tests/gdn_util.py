@@ -11,6 +11,11 @@ D = 128
 ROW = 96
 # What enters an answer alone is rounded to f16 in the chunked form (half a step of 2^-11 relative): the state of Q S, both factors of the inner matrix times U
 F16 = 2.0 ** -11
+# ... and no finer than f16's last step, 2^-24, of the column's unit, which is at most half of the largest value that the column has in the chunk (its
+# inputs and the state in front of it): half a step of that, of the 128 values of S under |q^| = 1 (their sum at most sqrt(128)) and of the 64 of U; in the
+# state, of those of S under |k^| = 1, and of the 64 rests V - .. and the 64 updates that each chunk splits.
+STEP = 2.0 ** -26
+FLOOR, STATE_FLOOR = (128 ** 0.5 + 64) * STEP, (128 ** 0.5 + 128) * STEP
 
 
 def gates(a, b, a_log, dt_bias):
@@ -34,13 +39,15 @@ def rule(q, k, v, a, b, a_log, dt_bias, state, eps, scale, chunked=False):
     decay, beta = gates(a, b, a_log, dt_bias)
     s, e = state.copy(), np.zeros((heads, D))
     out, tol, states, tols = np.zeros(v.shape), np.zeros(v.shape), [s.copy()], [e.copy()]
-    mass = held = np.zeros((heads, D))
+    mass = held = floor = np.zeros((heads, D))
     for i in range(n):
         kh = k[i, of] / np.sqrt((k[i, of] ** 2).sum(-1, keepdims=True) + eps)
         qh = q[i, of] / np.sqrt((q[i, of] ** 2).sum(-1, keepdims=True) + eps)
         length = np.sqrt((s ** 2).sum(1))
         if i % 64 == 0:
-            held, mass = length.copy(), np.zeros((heads, D))
+            e = e + floor
+            floor = STATE_FLOOR * (length + np.abs(v[i:i + 64]).max(0)) * chunked
+            start, held, mass = length, length.copy(), np.zeros((heads, D))
         s = s * decay[i][:, None, None]
         u = beta[i][:, None] * (v[i] - np.einsum("hkv,hk->hv", s, kh))
         s = s + kh[:, :, None] * u[:, None, :]
@@ -48,9 +55,11 @@ def rule(q, k, v, a, b, a_log, dt_bias, state, eps, scale, chunked=False):
         e = e * decay[i][:, None] + ROW * F32 * (length + new + np.abs(v[i]))
         held, mass = held * decay[i][:, None], mass * decay[i][:, None] + np.abs(u)
         out[i] = scale * np.einsum("hkv,hk->hv", s, qh)
-        slack = e + ROW * F32 * (length + new + np.abs(v[i])) + (F16 * (held + 2.01 * mass) if chunked else 0.0)
+        slack = e + floor + ROW * F32 * (length + new + np.abs(v[i]))
+        if chunked:
+            slack += F16 * (held + 2.01 * mass) + FLOOR * (start + np.abs(v[i - i % 64:i - i % 64 + 64]).max(0))
         tol[i] = BF16 * np.abs(out[i]) * 1.01 + abs(scale) * slack + 1e-30
-        states.append(s), tols.append(e.copy())
+        states.append(s), tols.append(e + floor)
     return out, tol, states, [t[:, None, :] + 1e-30 for t in tols]
 
 
