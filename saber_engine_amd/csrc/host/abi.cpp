@@ -154,7 +154,7 @@ const Signature *signature_for(const std::string &k) {
   if (starts(k, "attn_few_")) return &SIG_ATTN_FEW;
   if (starts(k, "attn_many_")) return &SIG_ATTN_MANY;
   if (starts(k, "delta_conv_")) return &SIG_DELTA_CONV;
-  if (k == "delta_step") return &SIG_DELTA_STEP;
+  if (starts(k, "delta_step_")) return &SIG_DELTA_STEP;
   if (k == "delta_prep") return &SIG_DELTA_PREP;
   if (starts(k, "delta_scan_")) return &SIG_DELTA_SCAN;
   if (k == "block_copy") return &SIG_BLOCK_COPY;

@@ -15,6 +15,7 @@ namespace {
 constexpr uint32_t DIM = 128, CHUNK = 64, I32_MAX = 0x7FFFFFFFu, GRID_MAX = 0xFFFFFFu;  // workgroups of 256 whose threads a launch counts in 32 bits
 constexpr uint64_t KEYS = 32768, PART = 19456;  // a chunk and key head's, a chunk and value head's bytes of the workspace (delta_chunk.h)
 constexpr uint64_t PIECE = 16384;      // a workgroup's bytes of block_copy
+constexpr uint64_t STEP_NARROW = 256;  // heads and sequences up to which its waves take 16 columns each, not 32
 constexpr uint32_t ROW_MAX = 1u << 24;  // elements of a row: a chunk's bytes are counted in 32 bits
 constexpr uint32_t STEP_ROWS = 32;     // rows up to which the recurrent kernel runs
 
@@ -128,7 +129,8 @@ int saber_iu8_gdn(saber_iu8_ctx *ctx, const void *q, const void *k, const void *
   if (!workspace || kept || !out || !cu_q || max_q <= STEP_ROWS) {
     if (items > GRID_MAX) return fail(SABER_IU8_E_RULE, fmt("gdn: %u sequences of %u heads pass a launch's 32-bit sizes", seqs, heads));
     StepArgs x{q, k, v, a, b, a_log, dt_bias, state, slot, cu_q, kept, out, (int32_t)row, (int32_t)ab_row, (int32_t)tokens, (int32_t)seqs, shape, (int32_t)slots, eps, scale};
-    return launch_image(ctx, "delta_step", (uint32_t)items, 256, &x, sizeof x, stream);
+    const bool narrow = items <= STEP_NARROW;
+    return launch_image(ctx, narrow ? "delta_step_c16" : "delta_step_c32", (uint32_t)items, narrow ? 512 : 256, &x, sizeof x, stream);
   }
   const uint64_t places = (uint64_t)tokens / CHUNK + seqs, chunks = places * heads;
   // Pairs of waves a workgroup of the walk

@@ -20,11 +20,11 @@ static __device__ __forceinline__ void block_copy_body(unsigned char *__restrict
 #pragma unroll
   for (int x = 0; x < 4; ++x) {
     const int o = (x * 256 + (int)threadIdx.x) * 16;
-    if (o < left) v[x] = *(const iu8_v4u *)(in + o);
+    if (o < left) v[x] = __builtin_nontemporal_load((const iu8_v4u *)(in + o));
   }
 #pragma unroll
   for (int x = 0; x < 4; ++x) {
     const int o = (x * 256 + (int)threadIdx.x) * 16;
-    if (o < left) *(iu8_v4u *)(out + o) = v[x];
+    if (o < left) __builtin_nontemporal_store(v[x], (iu8_v4u *)(out + o));
   }
 }

@@ -2,7 +2,7 @@
 // sequence. No counterpart among the objects this library stands in for (the reference's delta-net kernels are outside the linear's path).
 //
 //   delta_conv_w{2,3,4}     short causal convolution and SiLU of new rows (delta_conv.h)
-//   delta_step              the gated delta rule a row at a time (delta_step.h)
+//   delta_step_c{16,32}     the gated delta rule a row at a time (delta_step.h)
 //   delta_prep, delta_scan_w{2,4}  ... in chunks of 64 rows (delta_chunk.h)
 //   block_copy              blocks of two arrays to other blocks (block_copy.h)
 #include "block_copy.h"
@@ -21,13 +21,17 @@ DELTA_CONV(2)
 DELTA_CONV(3)
 DELTA_CONV(4)
 
-extern "C" __global__ __launch_bounds__(256) void delta_step(
-    const unsigned short *__restrict__ q, const unsigned short *__restrict__ k, const unsigned short *__restrict__ v, const unsigned short *__restrict__ a,
-    const unsigned short *__restrict__ b, const float *__restrict__ a_log, const float *__restrict__ dt_bias, float *__restrict__ state,
-    const int *__restrict__ slot, const int *__restrict__ cu_q, const int *__restrict__ kept, unsigned short *__restrict__ out, int row, int ab_row,
-    int tokens, int seqs, int shape, int slots, float eps, float scale) {
-  delta_step_body(q, k, v, a, b, a_log, dt_bias, state, slot, cu_q, kept, out, row, ab_row, tokens, seqs, shape, slots, eps, scale);
-}
+#define DELTA_STEP(C)                                                                                                                            \
+  extern "C" __global__ __launch_bounds__(64 * 128 / C) void delta_step_c##C(                                                                    \
+      const unsigned short *__restrict__ q, const unsigned short *__restrict__ k, const unsigned short *__restrict__ v,                          \
+      const unsigned short *__restrict__ a, const unsigned short *__restrict__ b, const float *__restrict__ a_log,                               \
+      const float *__restrict__ dt_bias, float *__restrict__ state, const int *__restrict__ slot, const int *__restrict__ cu_q,                  \
+      const int *__restrict__ kept, unsigned short *__restrict__ out, int row, int ab_row, int tokens, int seqs, int shape, int slots, float eps, \
+      float scale) {                                                                                                                             \
+    delta_step_body<C>(q, k, v, a, b, a_log, dt_bias, state, slot, cu_q, kept, out, row, ab_row, tokens, seqs, shape, slots, eps, scale);        \
+  }
+DELTA_STEP(16)
+DELTA_STEP(32)
 
 extern "C" __global__ __launch_bounds__(256) void delta_prep(
     const unsigned short *__restrict__ q, const unsigned short *__restrict__ k, const unsigned short *__restrict__ a, const unsigned short *__restrict__ b,

@@ -169,13 +169,13 @@ def test_workspaces_hold_every_smaller_call():
 
 def test_every_kernel_is_there_without_scratch():
     text = open(os.path.join(iu8.PREBUILT, "delta_net.manifest.toml")).read()
-    want = {"block_copy", "delta_step", "delta_prep"} | {f"delta_conv_w{w}" for w in (2, 3, 4)} | {f"delta_scan_w{w}" for w in (2, 4)}
+    want = {"block_copy", "delta_step_c16", "delta_step_c32", "delta_prep"} | {f"delta_conv_w{w}" for w in (2, 3, 4)} | {f"delta_scan_w{w}" for w in (2, 4)}
     assert set(re.findall(r'name = "((?:delta_|block_)\w+)"', text)) >= want
     assert set(re.findall(r"private_segment_fixed_size = (\d+)", text)) == {"0"}
     assert max(int(x) for x in re.findall(r"group_segment_fixed_size = (\d+)", text)) <= 160 * 1024
 
 
-@pytest.mark.parametrize("kernel", ["delta_step", "delta_prep", "delta_scan_w4", "delta_conv_w3", "block_copy"])
+@pytest.mark.parametrize("kernel", ["delta_step_c16", "delta_prep", "delta_scan_w4", "delta_conv_w3", "block_copy"])
 def test_descriptors_of_the_kernels_are_refused(kernel):
     """Their walks follow sizes that the operators check: no launch by a descriptor that a caller has set up."""
     d = iu8.describe_raw(kernel, (1, 1, 1), 256, "delta_net")
