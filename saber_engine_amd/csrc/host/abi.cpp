@@ -109,7 +109,7 @@ static const Signature SIG_DELTA_STEP = {
 static const Signature SIG_DELTA_PREP = {
     {"q", K::Buffer},    {"k", K::Buffer},    {"a", K::Buffer},    {"b", K::Buffer},   {"a_log", K::Buffer}, {"dt_bias", K::Buffer}, {"slot", K::Buffer},
     {"cu_q", K::Buffer}, {"keys", K::Buffer}, {"work", K::Buffer}, {"row", K::I32},    {"ab_row", K::I32},   {"tokens", K::I32},     {"seqs", K::I32},
-    {"shape", K::I32},   {"slots", K::I32},   {"places", K::I32},  {"eps", K::F32}};
+    {"shape", K::I32},   {"slots", K::I32},   {"places", K::I32},  {"many", K::I32},    {"eps", K::F32}};
 static const Signature SIG_DELTA_SCAN = {
     {"v", K::Buffer},   {"keys", K::Buffer}, {"work", K::Buffer}, {"state", K::Buffer}, {"slot", K::Buffer},  {"cu_q", K::Buffer}, {"out", K::Buffer},
     {"row", K::I32},    {"tokens", K::I32},  {"seqs", K::I32},    {"shape", K::I32},    {"slots", K::I32},    {"scale", K::F32}};

@@ -15,6 +15,7 @@ namespace {
 constexpr uint32_t DIM = 128, CHUNK = 64, I32_MAX = 0x7FFFFFFFu, GRID_MAX = 0xFFFFFFu;  // workgroups of 256 whose threads a launch counts in 32 bits
 constexpr uint64_t KEYS = 32768, PART = 19456;  // a chunk and key head's, a chunk and value head's bytes of the workspace (delta_chunk.h)
 constexpr uint64_t PIECE = 16384;      // a workgroup's bytes of block_copy
+constexpr uint64_t PREP_FULL = 512;  // chunks and key heads from which a workgroup of the preparation takes several value heads
 constexpr uint64_t STEP_NARROW = 256;  // heads and sequences up to which its waves take 16 columns each, not 32
 constexpr uint32_t ROW_MAX = 1u << 24;  // elements of a row: a chunk's bytes are counted in 32 bits
 constexpr uint32_t STEP_ROWS = 32;     // rows up to which the recurrent kernel runs
@@ -31,7 +32,7 @@ struct StepArgs {
 };
 struct PrepArgs {
   const void *q, *k, *a, *b, *a_log, *dt_bias, *slot, *cu_q, *keys, *work;
-  int32_t row, ab_row, tokens, seqs, shape, slots, places;
+  int32_t row, ab_row, tokens, seqs, shape, slots, places, many;
   float eps;
 };
 struct ScanArgs {
@@ -44,7 +45,7 @@ struct CopyArgs {
   int64_t a_bytes, b_bytes;
   int32_t blocks;
 };
-static_assert(offsetof(ConvArgs, run) == 88 && offsetof(StepArgs, scale) == 124 && offsetof(PrepArgs, eps) == 108 && offsetof(ScanArgs, scale) == 76 &&
+static_assert(offsetof(ConvArgs, run) == 88 && offsetof(StepArgs, scale) == 124 && offsetof(PrepArgs, eps) == 112 && offsetof(ScanArgs, scale) == 76 &&
                   offsetof(CopyArgs, blocks) == 48,
               "as abi.cpp packs them");
 
@@ -132,13 +133,15 @@ int saber_iu8_gdn(saber_iu8_ctx *ctx, const void *q, const void *k, const void *
     const bool narrow = items <= STEP_NARROW;
     return launch_image(ctx, narrow ? "delta_step_c16" : "delta_step_c32", (uint32_t)items, narrow ? 512 : 256, &x, sizeof x, stream);
   }
-  const uint64_t places = (uint64_t)tokens / CHUNK + seqs, chunks = places * heads;
+  const uint64_t places = (uint64_t)tokens / CHUNK + seqs, group = heads / key_heads;
+  // Value heads a workgroup of the preparation: those of a key head share its rows' products, where the card is full without.
+  const uint64_t many = places * key_heads >= PREP_FULL ? std::min<uint64_t>(group, 4) : 1, chunks = places * key_heads * ((group + many - 1) / many);
   // Pairs of waves a workgroup of the walk
   const uint32_t pairs = items * 4 <= CU_COUNT ? 2 : 4;
   const uint64_t walks = (items * (8 / pairs) + 7) / 8 * 8;
   if (chunks > GRID_MAX || walks > GRID_MAX) return fail(SABER_IU8_E_RULE, fmt("gdn: %u rows of %u sequences and %u heads pass a launch's 32-bit sizes", tokens, seqs, heads));
   unsigned char *const keys = (unsigned char *)workspace, *const parts = keys + places * key_heads * KEYS;
-  PrepArgs p{q, k, a, b, a_log, dt_bias, slot, cu_q, keys, parts, (int32_t)row, (int32_t)ab_row, (int32_t)tokens, (int32_t)seqs, shape, (int32_t)slots, (int32_t)places, eps};
+  PrepArgs p{q, k, a, b, a_log, dt_bias, slot, cu_q, keys, parts, (int32_t)row, (int32_t)ab_row, (int32_t)tokens, (int32_t)seqs, shape, (int32_t)slots, (int32_t)places, (int32_t)many, eps};
   if (int rc = launch_image(ctx, "delta_prep", (uint32_t)((chunks + 7) / 8 * 8), 256, &p, sizeof p, stream)) return rc;
   ScanArgs x{v, keys, parts, state, slot, cu_q, out, (int32_t)row, (int32_t)tokens, (int32_t)seqs, shape, (int32_t)slots, scale};
   return launch_image(ctx, pairs == 2 ? "delta_scan_w2" : "delta_scan_w4", (uint32_t)walks, 128 * pairs, &x, sizeof x, stream);

@@ -36,23 +36,19 @@ static __device__ __forceinline__ void delta_prep_body(const unsigned short *__r
                                                        const float *__restrict__ a_log, const float *__restrict__ dt_bias,
                                                        const int *__restrict__ slot, const int *__restrict__ cu, unsigned char *__restrict__ keys,
                                                        unsigned char *__restrict__ work, int row, int ab_row, int tokens, int seqs, int shape, int slots,
-                                                       int places, float eps) {
+                                                       int places, int many, float eps) {
   constexpr int P = 68;  // floats of a row in LDS
   const int heads = shape & 0xFFFF, key_heads = shape >> 16, group = heads / key_heads;
-  // (to one XCD the heads that read the same rows)
-  const int share = (int)(gridDim.x + 7) >> 3, item = (int)(blockIdx.x & 7) * share + (int)(blockIdx.x >> 3);
-  if (item >= places * heads) return;
-  const int id = item / heads, h = item - id * heads, hk = h / group;
+  // a workgroup: `many` value heads (1 to 4) of a key head; to one XCD those that read the same rows
+  const int parts = (group + many - 1) / many, share = (int)(gridDim.x + 7) >> 3, item = (int)(blockIdx.x & 7) * share + (int)(blockIdx.x >> 3);
+  if (item >= places * key_heads * parts) return;
+  const int id = item / (key_heads * parts), hk = item / parts - id * key_heads, part = item % parts, h0 = hk * group + part * many;
+  const int count = min(many, group - part * many);
   const int lane = threadIdx.x & 63, wave = at_uniform(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
   int s = -1;
-  if (!cu) {
-    s = id - id / 65;  // (a sequence a row: (s >> 6) + s)
-    while ((s >> 6) + s > id) --s;
-  } else {
-    for (int base = 0; base < seqs; base += 64) {
-      const int i = base + lane;
-      s += __popcll(__ballot(i < seqs && (cu[i] >> 6) + i <= id));
-    }
+  for (int base = 0; base < seqs; base += 64) {
+    const int i = base + lane;
+    s += __popcll(__ballot(i < seqs && (cu[i] >> 6) + i <= id));
   }
   if (s < 0 || s >= seqs) return;
   const dn_rows x = dn_sequence(cu, slot, s, tokens, slots);
@@ -61,8 +57,9 @@ static __device__ __forceinline__ void delta_prep_body(const unsigned short *__r
 
   // K and Q, 16 KiB each, then A (in the end T) and the inner matrix in their place
   __shared__ __attribute__((aligned(16))) float s_m[2][DN_CHUNK][P];
-  __shared__ double s_sum[DN_CHUNK];  // in units of log 2
-  __shared__ float s_beta[DN_CHUNK], s_rk[DN_CHUNK], s_rq[DN_CHUNK];
+  __shared__ double s_sums[4][DN_CHUNK];  // in units of log 2
+  __shared__ __attribute__((aligned(16))) float s_betas[4][DN_CHUNK], s_rk[DN_CHUNK], s_rq[DN_CHUNK];
+  __shared__ int s_unit[DN_CHUNK];  // K's and Q's rows' units, as exponents
   auto &s_a = s_m[0];
   auto &s_i = s_m[1];
   unsigned char *s_k = (unsigned char *)s_m, *s_q = s_k + DN_KEYS / 2;
@@ -75,8 +72,8 @@ static __device__ __forceinline__ void delta_prep_body(const unsigned short *__r
     const size_t at = (t0 + min(16 * wave + 4 * i + g, m - 1)) * row + hk * DN + 8 * n;
     kr[i] = *(const iu8_v4u *)(k + at), qr[i] = *(const iu8_v4u *)(q + at);
   }
-  if (wave == 0) {
-    const int i = lane;
+  if (wave < count) {  // a head's gates a wave
+    const int i = lane, h = h0 + wave;
     float lg = 0.f, be = 0.f;
     if (i < m) {
       lg = dn_log_decay(iu8_bf16_f32(a[(t0 + i) * ab_row + h]), a_log[h], dt_bias[h]);
@@ -88,7 +85,7 @@ static __device__ __forceinline__ void delta_prep_body(const unsigned short *__r
       const double z = __shfl_up(sum, y);
       sum += i >= y ? z : 0.0;
     }
-    s_sum[i] = sum, s_beta[i] = be;
+    s_sums[wave][i] = sum, s_betas[wave][i] = be;
   }
   const int turned = (n ^ (g << 2)) << 4;  // piece n of row 16 wave + 4 i + g, ^ 16 i
 #pragma unroll
@@ -126,17 +123,17 @@ static __device__ __forceinline__ void delta_prep_body(const unsigned short *__r
   if (g == n >> 2) {
     const float ks = (n & 2) ? ((n & 1) ? own[3] : own[2]) : ((n & 1) ? own[1] : own[0]), qs = (n & 2) ? ((n & 1) ? qq[3] : qq[2]) : ((n & 1) ? qq[1] : qq[0]);
     const bool live = 16 * wave + n < m;
-    s_rk[16 * wave + n] = live ? ks : 0.f, s_rq[16 * wave + n] = live ? qs : 0.f;
+    auto unit_of = [](float ss) { return max(dn_exponent(sqrtf(ss)), 64); };
+    s_rk[16 * wave + n] = live ? 1.f / sqrtf(ks + eps) : 0.f, s_rq[16 * wave + n] = live ? 1.f / sqrtf(qs + eps) : 0.f;
+    s_unit[16 * wave + n] = unit_of(ks) | unit_of(qs) << 16;
   }
   __syncthreads();
-  auto unit_of = [](float ss) { return max(dn_exponent(sqrtf(ss)), 64); };
-  auto length_of = [&](float ss) { return 1.f / sqrtf(ss + eps); };
-  if (h - hk * group == 0) {
+  if (part == 0) {
     unsigned char *to = keys + ((size_t)id * key_heads + hk) * DN_KEYS;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int t = 16 * wave + 4 * i + g, at = t * 256 + (turned ^ (i << 4));
-      const float bk = dn_below(unit_of(s_rk[t])), bq = dn_below(unit_of(s_rq[t]));
+      const float bk = dn_below(s_unit[t] & 0xFFFF), bq = dn_below(s_unit[t] >> 16);
       auto as_f16 = [&](iu8_v4u f, float by) {
         iu8_v4u y;
 #pragma unroll
@@ -149,45 +146,13 @@ static __device__ __forceinline__ void delta_prep_body(const unsigned short *__r
       *(iu8_v4u *)(to + at) = as_f16(kr[i], bk), *(iu8_v4u *)(to + DN_KEYS / 2 + at) = as_f16(qr[i], bq);
     }
   }
-  unsigned char *mine = work + ((size_t)id * heads + h) * DN_PART;
-  if (wave == 3) {
-    const int i = lane;
-    const double end = s_sum[DN_CHUNK - 1];
-    float *f = (float *)(mine + DN_FACTORS);
-    const float eg = __builtin_amdgcn_exp2f((float)s_sum[i]);
-    const float rk = i < m ? length_of(s_rk[i]) * dn_power(unit_of(s_rk[i])) : 0.f, rq = i < m ? length_of(s_rq[i]) * dn_power(unit_of(s_rq[i])) : 0.f;
-    f[i] = eg * rk, f[64 + i] = eg * rq, f[128 + i] = __builtin_amdgcn_exp2f((float)(end - s_sum[i])) * rk;
-    if (i == 0) f[192] = __builtin_amdgcn_exp2f((float)end);
+  float of_row[4], of_query[4], of_key[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int i = 16 * wave + 4 * g + r, j = 16 * r + n;
+    of_row[r] = s_rk[i], of_query[r] = s_rq[i], of_key[r] = s_rk[j];
   }
-  {
-    float of_row[4], of_query[4];
-    double si[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int i = 16 * wave + 4 * g + r;
-      of_row[r] = s_beta[i] * length_of(s_rk[i]), of_query[r] = length_of(s_rq[i]), si[r] = s_sum[i];
-    }
-#pragma unroll
-    for (int jb = 0; jb < 4; ++jb) {
-      const int j = 16 * jb + n;
-      if (jb <= wave) {
-        const double sj = s_sum[j];
-        const float rj = j < m ? length_of(s_rk[j]) : 0.f;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int i = 16 * wave + 4 * g + r;
-          const float w = i >= j ? __builtin_amdgcn_exp2f((float)(si[r] - sj)) * rj : 0.f;
-          s_a[i][j] = i > j ? of_row[r] * w * kk[jb][r] : 0.f;
-          s_i[i][j] = of_query[r] * w * qk[jb][r];
-        }
-      } else if (jb == wave + 1 && !(wave & 1)) {  // (the fragments' other block)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) s_a[16 * wave + 4 * g + r][j] = 0.f, s_i[16 * wave + 4 * g + r][j] = 0.f;
-      }
-    }
-  }
-  __syncthreads();
-  auto give = [&](const float (*from)[P], int f, unsigned char *to, bool scaled, bool both) {
+  auto give = [&](const float (*from)[P], int f, unsigned char *to, const float *s_beta, bool scaled, bool both) {
     const int i = 16 * dn_frag_block(f) + n, j = 32 * dn_frag_half(f) + 4 * g;
     iu8_v4f y = *(const iu8_v4f *)(from[i] + j), z = *(const iu8_v4f *)(from[i] + j + 16);
     if (scaled) y = y * *(const iu8_v4f *)(s_beta + j), z = z * *(const iu8_v4f *)(s_beta + j + 16);
@@ -196,58 +161,98 @@ static __device__ __forceinline__ void delta_prep_body(const unsigned short *__r
     *(iu8_v4u *)(to + f * DN_FRAG + lane * 16) = w[0];
     if (both) *(iu8_v4u *)(to + (DN_FRAGS + f) * DN_FRAG + lane * 16) = w[1];
   };
-  for (int f = wave; f < DN_FRAGS; f += 4) give(s_i, f, mine + DN_INNER, false, false);
-  // T's blocks on the diagonal by substitution, a column a lane; in A's place
-  if (g == 0) {
-    float y[16];
-    float(*at)[P] = (float(*)[P])(&s_a[16 * wave][16 * wave]);
+  for (int hh = 0; hh < count; ++hh) {
+    if (hh) __syncthreads();
+    unsigned char *mine = work + ((size_t)id * heads + h0 + hh) * DN_PART;
+    const double *s_sum = s_sums[hh];
+    const float *s_beta = s_betas[hh];
+    if (wave == 3) {
+      const int i = lane;
+      const double end = s_sum[DN_CHUNK - 1];
+      float *f = (float *)(mine + DN_FACTORS);
+      const float eg = __builtin_amdgcn_exp2f((float)s_sum[i]);
+      const float rk = s_rk[i] * dn_power(s_unit[i] & 0xFFFF), rq = s_rq[i] * dn_power(s_unit[i] >> 16);
+      f[i] = eg * rk, f[64 + i] = eg * rq, f[128 + i] = __builtin_amdgcn_exp2f((float)(end - s_sum[i])) * rk;
+      if (i == 0) f[192] = __builtin_amdgcn_exp2f((float)end);
+    }
+    {
+      float be[4];
+      double si[4];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float z = i == n ? 1.f : 0.f, z1 = 0.f;
+      for (int r = 0; r < 4; ++r) be[r] = s_beta[16 * wave + 4 * g + r], si[r] = s_sum[16 * wave + 4 * g + r];
 #pragma unroll
-      for (int j = 0; j < i; ++j) {
-        if (j & 1) z1 = fmaf(-at[i][j], y[j], z1);
-        else z = fmaf(-at[i][j], y[j], z);
+      for (int jb = 0; jb < 4; ++jb) {
+        const int j = 16 * jb + n;
+        if (jb <= wave) {
+          const double sj = s_sum[j];
+          const float rj = of_key[jb];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int i = 16 * wave + 4 * g + r;
+            const float w = i >= j ? __builtin_amdgcn_exp2f((float)(si[r] - sj)) * rj : 0.f;
+            s_a[i][j] = i > j ? be[r] * of_row[r] * w * kk[jb][r] : 0.f;
+            s_i[i][j] = of_query[r] * w * qk[jb][r];
+          }
+        } else if (jb == wave + 1 && !(wave & 1)) {  // (the fragments' other block)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s_a[16 * wave + 4 * g + r][j] = 0.f, s_i[16 * wave + 4 * g + r][j] = 0.f;
+        }
       }
-      y[i] = z + z1;
     }
+    __syncthreads();
+    for (int f = wave; f < DN_FRAGS; f += 4) give(s_i, f, mine + DN_INNER, s_beta, false, false);
+    // T's blocks on the diagonal by substitution, a column a lane; in A's place
+    if (g == 0) {
+      float y[16];
+      float(*at)[P] = (float(*)[P])(&s_a[16 * wave][16 * wave]);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) at[i][n] = y[i];
-  }
-  __syncthreads();
-  // those under it, wave j the column of blocks j: T_ij = -T_ii sum_k A_ik T_kj, on the f32 matrix instruction; a result's rows 4 g + r are the next
-  // product's places r of lane group g
-  iu8_v4f t[4];
+      for (int i = 0; i < 16; ++i) {
+        float z = i == n ? 1.f : 0.f, z1 = 0.f;
 #pragma unroll
-  for (int r = 0; r < 4; ++r) t[0][r] = s_a[16 * wave + 4 * g + r][16 * wave + n];
-#pragma unroll
-  for (int d = 1; d < 4; ++d) {
-    const int i = wave + d;
-    if (i < 4) {
-      iu8_v4f y = {0.f, 0.f, 0.f, 0.f}, z = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int e = 0; e < d; ++e) {
-        const iu8_v4f f = *(const iu8_v4f *)&s_a[16 * i + n][16 * (wave + e) + 4 * g];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) y = __builtin_amdgcn_mfma_f32_16x16x4f32(f[r], t[e][r], y, 0, 0, 0);
+        for (int j = 0; j < i; ++j) {
+          if (j & 1) z1 = fmaf(-at[i][j], y[j], z1);
+          else z = fmaf(-at[i][j], y[j], z);
+        }
+        y[i] = z + z1;
       }
-      dn_settle(y);
-      const iu8_v4f f = *(const iu8_v4f *)&s_a[16 * i + n][16 * i + 4 * g];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) z = __builtin_amdgcn_mfma_f32_16x16x4f32(f[r], y[r], z, 0, 0, 0);
-      dn_settle(z);
-      t[d] = -z;
+      for (int i = 0; i < 16; ++i) at[i][n] = y[i];
     }
+    __syncthreads();
+    // those under it, wave j the column of blocks j: T_ij = -T_ii sum_k A_ik T_kj, on the f32 matrix instruction; a result's rows 4 g + r are the next
+    // product's places r of lane group g
+    iu8_v4f t[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) t[0][r] = s_a[16 * wave + 4 * g + r][16 * wave + n];
+#pragma unroll
+    for (int d = 1; d < 4; ++d) {
+      const int i = wave + d;
+      if (i < 4) {
+        iu8_v4f y = {0.f, 0.f, 0.f, 0.f}, z = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < d; ++e) {
+          const iu8_v4f f = *(const iu8_v4f *)&s_a[16 * i + n][16 * (wave + e) + 4 * g];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) y = __builtin_amdgcn_mfma_f32_16x16x4f32(f[r], t[e][r], y, 0, 0, 0);
+        }
+        dn_settle(y);
+        const iu8_v4f f = *(const iu8_v4f *)&s_a[16 * i + n][16 * i + 4 * g];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) z = __builtin_amdgcn_mfma_f32_16x16x4f32(f[r], y[r], z, 0, 0, 0);
+        dn_settle(z);
+        t[d] = -z;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int d = 1; d < 4; ++d)
+      if (wave + d < 4) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s_a[16 * (wave + d) + 4 * g + r][16 * wave + n] = t[d][r];
+      }
+    __syncthreads();
+    for (int f = wave; f < DN_FRAGS; f += 4) give(s_a, f, mine + DN_T, s_beta, true, true);
   }
-  __syncthreads();
-#pragma unroll
-  for (int d = 1; d < 4; ++d)
-    if (wave + d < 4) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r) s_a[16 * (wave + d) + 4 * g + r][16 * wave + n] = t[d][r];
-    }
-  __syncthreads();
-  for (int f = wave; f < DN_FRAGS; f += 4) give(s_a, f, mine + DN_T, true, true);
 }
 
 // The order of issue of what stands since the last such call: `AHEAD` reads, then M products, each with up to V lane operations and R reads (`READS` of

@@ -33,11 +33,12 @@ DELTA_CONV(4)
 DELTA_STEP(16)
 DELTA_STEP(32)
 
-extern "C" __global__ __launch_bounds__(256) void delta_prep(
+extern "C" __global__ __launch_bounds__(256, 4) void delta_prep(
     const unsigned short *__restrict__ q, const unsigned short *__restrict__ k, const unsigned short *__restrict__ a, const unsigned short *__restrict__ b,
     const float *__restrict__ a_log, const float *__restrict__ dt_bias, const int *__restrict__ slot, const int *__restrict__ cu_q,
-    unsigned char *__restrict__ keys, unsigned char *__restrict__ work, int row, int ab_row, int tokens, int seqs, int shape, int slots, int places, float eps) {
-  delta_prep_body(q, k, a, b, a_log, dt_bias, slot, cu_q, keys, work, row, ab_row, tokens, seqs, shape, slots, places, eps);
+    unsigned char *__restrict__ keys, unsigned char *__restrict__ work, int row, int ab_row, int tokens, int seqs, int shape, int slots, int places, int many,
+    float eps) {
+  delta_prep_body(q, k, a, b, a_log, dt_bias, slot, cu_q, keys, work, row, ab_row, tokens, seqs, shape, slots, places, many, eps);
 }
 
 #define DELTA_SCAN(W)                                                                                                                         \
