@@ -15,10 +15,20 @@ namespace {
 constexpr uint32_t DIM = 128, CHUNK = 64, I32_MAX = 0x7FFFFFFFu, GRID_MAX = 0xFFFFFFu;  // workgroups of 256 whose threads a launch counts in 32 bits
 constexpr uint64_t KEYS = 32768, PART = 19456;  // a chunk and key head's, a chunk and value head's bytes of the workspace (delta_chunk.h)
 constexpr uint64_t PIECE = 16384;      // a workgroup's bytes of block_copy
-constexpr uint64_t PREP_FULL = 512;  // chunks and key heads from which a workgroup of the preparation takes several value heads
-constexpr uint64_t STEP_NARROW = 256;  // heads and sequences up to which its waves take 16 columns each, not 32
+// Chunks and key heads from which a workgroup of the preparation takes the value heads of a key head, up to four, whose rows' products they share:
+// without, the card is not full. Three heads against one a workgroup, microseconds: 272 chunks and key heads 22.8 against 16.9, 528 23.7
+// against 24.4, 2064 67.6 against 79.
+constexpr uint64_t PREP_FULL = 512;
+// Sequences and heads up to which the recurrent kernel's waves take 16 columns each (512 threads a workgroup), not 32 (256). 1 / 5 / 8 rows,
+// microseconds: 48 items 6.7 / 9.8 / 12.0 on 16 columns, 8.3 / 10.6 / 12.9 on 32; 432 items 15.2 / 16.9 / 21.0 and 10.5 / 15.2 / 17.9.
+constexpr uint64_t STEP_NARROW = 256;
 constexpr uint32_t ROW_MAX = 1u << 24;  // elements of a row: a chunk's bytes are counted in 32 bits
-constexpr uint32_t STEP_ROWS = 32;     // rows up to which the recurrent kernel runs
+// Rows of a sequence up to which the recurrent kernel runs though a workspace is given: STEP_FEW where its workgroups (sequences and heads) are
+// few, STEP_MANY from STEP_ITEMS of them. Measured, microseconds of a call, recurrent against chunks: 1 sequence of 48 heads, 8 / 12 / 16 rows
+// 12.2 / 17.6 / 21.1 against 14.8 / 14.5 / 14.6; 16 of 8 heads 12.9 / 17.2 / 20.5 against 17.3 / 17.0 / 17.0; 4 of 48 heads, 12 / 16 / 24 rows
+// 17.9 / 21.0 / 28.7 against 20.7 / 23.0 / 21.8; 64 of 48 heads, 16 / 24 / 32 rows 131 / 179 / 230 against 174 / 174 / 179.
+constexpr uint32_t STEP_FEW = 10, STEP_MANY = 20;
+constexpr uint64_t STEP_ITEMS = 192;
 
 // The kernels' arguments as abi.cpp declares them (natural alignment: the order says it all).
 struct ConvArgs {
@@ -95,9 +105,11 @@ int saber_iu8_gdn_conv(saber_iu8_ctx *ctx, const void *x, uint32_t x_row, const 
   if (x_row % 8 || out_row % 8 || x_row < channels || out_row < channels || x_row > I32_MAX || out_row > I32_MAX)
     return fail(SABER_IU8_E_RULE, fmt("gdn_conv: rows of %u and %u elements: whole 16-byte pieces that cover %u channels", x_row, out_row, channels));
   const uint64_t per = (channels / 8 + 255) / 256;
-  // Rows a thread: as many as keep two workgroups a CU and more.
+  // Rows a thread: as many as leave a workgroup a CU. Measured at 10240 channels, microseconds with runs of 1 / 2 / 4 / 8 / 16 rows: 64 sequences
+  // of a row 4.4 / 4.8 / 6.5 / 9.6 / 15.9, 200 rows 5.3 / 4.8 / 4.6 / 5.4 / 7.2, 1000 rows 19.6 / 14.4 / 11.1 / 11.3 / 12.2, 6812 rows
+  // 111 / 77 / 57 / 53 / 54.
   uint32_t run = 1;
-  while (run < 16 && (uint64_t)tokens / (2 * run) * per >= 2 * CU_COUNT) run *= 2;
+  while (run < 8 && (uint64_t)tokens / (2 * run) * per >= CU_COUNT) run *= 2;
   const uint64_t grid = (tokens + run - 1) / run * per;
   if (grid > GRID_MAX) return fail(SABER_IU8_E_RULE, fmt("gdn_conv: %u rows of %u channels pass a launch's 32-bit sizes", tokens, channels));
   ConvArgs a{x, weight, bias, tail, slot, cu_q, kept, out, (int32_t)x_row, (int32_t)out_row, (int32_t)tokens, (int32_t)seqs, (int32_t)channels, (int32_t)slots, (int32_t)run};
@@ -108,7 +120,7 @@ int saber_iu8_gdn_workspace(uint32_t tokens, uint32_t seqs, uint32_t max_q, uint
   if (int rc = rows_check("gdn_workspace", tokens, seqs, seqs, true, true)) return rc;
   if (int rc = heads_check("gdn_workspace", key_heads, heads)) return rc;
   if (!bytes) return fail(SABER_IU8_E_ARG, "gdn_workspace: null argument");
-  *bytes = max_q <= STEP_ROWS ? 0 : ((uint64_t)tokens / CHUNK + seqs) * (key_heads * KEYS + heads * PART);
+  *bytes = max_q <= STEP_FEW ? 0 : ((uint64_t)tokens / CHUNK + seqs) * (key_heads * KEYS + heads * PART);
   return 0;
 }
 
@@ -127,24 +139,25 @@ int saber_iu8_gdn(saber_iu8_ctx *ctx, const void *q, const void *k, const void *
   if (!(eps >= 0.f && std::isfinite(eps)) || !std::isfinite(scale)) return fail(SABER_IU8_E_RULE, "gdn: eps must be a number from 0, the scale a number");
   const int32_t shape = (int32_t)(heads | key_heads << 16);
   const uint64_t items = (uint64_t)seqs * heads;
-  if (!workspace || kept || !out || !cu_q || max_q <= STEP_ROWS) {
+  if (!workspace || kept || !out || !cu_q || max_q <= (items < STEP_ITEMS ? STEP_FEW : STEP_MANY)) {
     if (items > GRID_MAX) return fail(SABER_IU8_E_RULE, fmt("gdn: %u sequences of %u heads pass a launch's 32-bit sizes", seqs, heads));
     StepArgs x{q, k, v, a, b, a_log, dt_bias, state, slot, cu_q, kept, out, (int32_t)row, (int32_t)ab_row, (int32_t)tokens, (int32_t)seqs, shape, (int32_t)slots, eps, scale};
     const bool narrow = items <= STEP_NARROW;
     return launch_image(ctx, narrow ? "delta_step_c16" : "delta_step_c32", (uint32_t)items, narrow ? 512 : 256, &x, sizeof x, stream);
   }
   const uint64_t places = (uint64_t)tokens / CHUNK + seqs, group = heads / key_heads;
-  // Value heads a workgroup of the preparation: those of a key head share its rows' products, where the card is full without.
-  const uint64_t many = places * key_heads >= PREP_FULL ? std::min<uint64_t>(group, 4) : 1, chunks = places * key_heads * ((group + many - 1) / many);
-  // Pairs of waves a workgroup of the walk
-  const uint32_t pairs = items * 4 <= CU_COUNT ? 2 : 4;
-  const uint64_t walks = (items * (8 / pairs) + 7) / 8 * 8;
-  if (chunks > GRID_MAX || walks > GRID_MAX) return fail(SABER_IU8_E_RULE, fmt("gdn: %u rows of %u sequences and %u heads pass a launch's 32-bit sizes", tokens, seqs, heads));
+  const uint64_t many = places * key_heads >= PREP_FULL ? std::min<uint64_t>(group, 4) : 1;
+  const uint64_t preps = (places * key_heads + 7) / 8 * 8 * ((group + many - 1) / many);
+  // Pairs of waves a workgroup of the walk: two, in twice the workgroups, while each has a CU of its own, else four. Microseconds of 4096 rows,
+  // two / four: 48 heads 111 / 128, 64 heads 116 / 129, 80 heads 209 / 133, 2 x 48 heads 219 / 149.
+  const uint64_t pairs = items * 4 <= CU_COUNT ? 2 : 4, walks = (items + 7) / 8 * 8 * (8 / pairs);
+  if (preps > GRID_MAX || walks > GRID_MAX * 2 / pairs)
+    return fail(SABER_IU8_E_RULE, fmt("gdn: %u rows of %u sequences and %u heads pass a launch's 32-bit sizes", tokens, seqs, heads));
   unsigned char *const keys = (unsigned char *)workspace, *const parts = keys + places * key_heads * KEYS;
   PrepArgs p{q, k, a, b, a_log, dt_bias, slot, cu_q, keys, parts, (int32_t)row, (int32_t)ab_row, (int32_t)tokens, (int32_t)seqs, shape, (int32_t)slots, (int32_t)places, (int32_t)many, eps};
-  if (int rc = launch_image(ctx, "delta_prep", (uint32_t)((chunks + 7) / 8 * 8), 256, &p, sizeof p, stream)) return rc;
+  if (int rc = launch_image(ctx, "delta_prep", (uint32_t)preps, 256, &p, sizeof p, stream)) return rc;
   ScanArgs x{v, keys, parts, state, slot, cu_q, out, (int32_t)row, (int32_t)tokens, (int32_t)seqs, shape, (int32_t)slots, scale};
-  return launch_image(ctx, pairs == 2 ? "delta_scan_w2" : "delta_scan_w4", (uint32_t)walks, 128 * pairs, &x, sizeof x, stream);
+  return launch_image(ctx, pairs == 2 ? "delta_scan_w2" : "delta_scan_w4", (uint32_t)walks, 128 * (uint32_t)pairs, &x, sizeof x, stream);
 }
 
 int saber_iu8_kv_copy(saber_iu8_ctx *ctx, const saber_iu8_kv_cache *c, const int32_t *src, const int32_t *dst, uint32_t n, void *stream) {

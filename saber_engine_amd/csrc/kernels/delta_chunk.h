@@ -13,13 +13,14 @@
 // of two (its largest value brought to 1 .. 2); its norm's and decay's factors are moved to the other side of the product; the other side is split
 // into two f16 terms, 22 bits (dn_split), in a column's own unit, a power of two that follows the column's largest value. What goes only into the rows' bf16 answers takes
 // one term, 11 bits. (Three bf16 terms, which need no units, are half as many products again and twice the lane arithmetic: the walk of 8,192 rows of 48
-// heads 304 us, with f16 235.) G is summed, and its differences taken, in f64: after a strong decay the later rows' differences would be left with the sum's digits.
+// heads 304 us, with f16 225.) G is summed, and its differences taken, in f64: after a strong decay the later rows' differences would be left with the sum's digits.
 #pragma once
 #include "delta_step.h"
 
-// The workspace: of a chunk and key head K and Q, f16, 16 KiB each, row t's 16-byte pieces exchanged (piece ^ dn_swap(t)) as the walk keeps them in LDS; of a chunk and
-// value head T diag(beta) in two terms, the inner matrix in one, the factors. Operands are kept as fragments, 64 lanes x 16 bytes: lane (l % 16, g = l / 16) has row l % 16 of 16
-// and the columns 4 g .. 4 g + 3 of the first and of the second 16 of 32, which is how a product's result lies (dn_operand).
+// The workspace: of a chunk and key head K and Q, f16, 16 KiB each, row t's 16-byte pieces exchanged (piece ^ (t % 4 * 4 + t / 4 % 4)) as the walk keeps them in
+// LDS, where neither four neighbouring pieces of four neighbouring rows nor one piece of 16 rows share a bank; of a chunk and value head T diag(beta) in two
+// terms, the inner matrix in one, the factors. Operands are kept as fragments, 64 lanes x 16 bytes: lane (l % 16, g = l / 16) has row l % 16 of 16 and the
+// columns 4 g .. 4 g + 3 of the first and of the second 16 of 32, which is how a product's result lies (dn_operand).
 // Fragment f of a lower triangle: row blocks 0, 1 of the first 32 columns; row blocks 2, 3 of the first and of the last.
 constexpr int DN_KEYS = 32768, DN_FRAGS = 6, DN_FRAG = 1024;
 static __host__ __device__ constexpr int dn_frag_block(int f) { return f < 2 ? f : 2 + (f - 2) / 2; }
@@ -28,8 +29,6 @@ constexpr int DN_T = 0, DN_INNER = 2 * DN_FRAGS * DN_FRAG, DN_FACTORS = DN_INNER
 // the factors, f32: [64] exp(G_i) / |k_i|, [64] exp(G_i) / |q_i|, [64] exp(G_63 - G_i) / |k_i| (of the f16 rows), exp(G_63)
 
 static __device__ __forceinline__ int dn_chunk_id(const dn_rows &x) { return (x.t0 >> 6) + x.s; }  // of its first chunk: no two sequences' meet
-// Such that neither four neighbouring pieces of four neighbouring rows nor one piece of 16 rows share a bank.
-static __host__ __device__ constexpr int dn_swap(int t) { return (t & 3) << 2 | (t >> 2 & 3); }
 
 static __device__ __forceinline__ void delta_prep_body(const unsigned short *__restrict__ q, const unsigned short *__restrict__ k,
                                                        const unsigned short *__restrict__ a, const unsigned short *__restrict__ b,
@@ -40,9 +39,9 @@ static __device__ __forceinline__ void delta_prep_body(const unsigned short *__r
   constexpr int P = 68;  // floats of a row in LDS
   const int heads = shape & 0xFFFF, key_heads = shape >> 16, group = heads / key_heads;
   // a workgroup: `many` value heads (1 to 4) of a key head; to one XCD those that read the same rows
-  const int parts = (group + many - 1) / many, share = (int)(gridDim.x + 7) >> 3, item = (int)(blockIdx.x & 7) * share + (int)(blockIdx.x >> 3);
-  if (item >= places * key_heads * parts) return;
-  const int id = item / (key_heads * parts), hk = item / parts - id * key_heads, part = item % parts, h0 = hk * group + part * many;
+  const int parts = (group + many - 1) / many, turn = (int)(blockIdx.x >> 3) / parts, item = turn * 8 + (int)(blockIdx.x & 7);
+  if (item >= places * key_heads) return;
+  const int id = item / key_heads, hk = item - id * key_heads, part = (int)(blockIdx.x >> 3) - turn * parts, h0 = hk * group + part * many;
   const int count = min(many, group - part * many);
   const int lane = threadIdx.x & 63, wave = at_uniform(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
   int s = -1;
@@ -281,7 +280,8 @@ static __device__ __forceinline__ iu8_v2u dn_transposed(const unsigned char *fro
 // the chain (K S, V - .., U, the next S), the other does what hangs from it, the rows' answers, with the operands that the first leaves in LDS, and asks for K, Q,
 // T, the inner matrix, the factors and V two chunks ahead, which come straight from memory into one of two LDS stages as soon as it has been read. O is
 // taken the other way round (the operands exchanged), so that a lane has four neighbouring values of one row to store. Two meetings a chunk: behind U, where the
-// stage is free, and behind the next S. W pairs a workgroup share a stage.
+// stage is free, and behind the next S. W pairs a workgroup share a stage. A chunk takes 1.8 us (8,192 rows of 48 heads 225 us; the chain with the
+// stages' loads alone 204).
 template <int W>
 static __device__ __forceinline__ void delta_scan_body(const unsigned short *__restrict__ v, const unsigned char *__restrict__ keys,
                                                        const unsigned char *__restrict__ work, float *__restrict__ state, const int *__restrict__ slot,
@@ -290,11 +290,23 @@ static __device__ __forceinline__ void delta_scan_body(const unsigned short *__r
   constexpr int PARTS = 8 / W, K_AT = 0, Q_AT = DN_KEYS / 2, W_AT = DN_KEYS, V_AT = W_AT + DN_PART, STAGE = V_AT + W * 2048, GIVEN = 8192 + 128;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * STAGE + W * GIVEN];  // stages; of each pair S in one term, U, the columns' units
   const int heads = shape & 0xFFFF, key_heads = shape >> 16, group = heads / key_heads;
-  // workgroups are dealt to the XCDs in turn: those of neighbouring heads, which read the same keys, to one
-  const int all = seqs * heads * PARTS, share = (all + 7) / 8, item = (blockIdx.x & 7) * share + (blockIdx.x >> 3);
-  if ((int)(blockIdx.x >> 3) >= share || item >= all) return;
-  const int s = item / (heads * PARTS), h = item / PARTS - s * heads, hk = h / group, part = item % PARTS;
+  // heads are dealt to the XCDs in turn, a head's workgroups, which read the same bytes, to one
+  const int turn = (int)(blockIdx.x >> 3), item = turn / PARTS * 8 + (int)(blockIdx.x & 7), part = turn % PARTS;
+  if (item >= seqs * heads) return;
   const int lane = threadIdx.x & 63, wave = at_uniform(threadIdx.x >> 6), pair = wave % W, n = lane & 15, g = lane >> 4;
+  int s = item / heads;
+  const int h = item - s * heads, hk = h / group;
+  // The longest walks first, where a lane a sequence can tell (prompts of 2100, 777, 1859, 903 and 1173 rows, 48 heads: 115 us; in the sequences'
+  // order, an eighth of the whole to each XCD, 158).
+  if (seqs <= 64) {
+    const int length = lane < seqs ? cu[lane + 1] - cu[lane] : 0;
+    int place = 0;
+    for (int i = 0; i < seqs; ++i) {
+      const int other = __builtin_amdgcn_readlane(length, i);
+      place += other > length || (other == length && i < lane);
+    }
+    s = __builtin_ctzll(__ballot(lane < seqs && place == s));
+  }
   const dn_rows x = dn_sequence(cu, slot, s, tokens, slots);
   if (x.n <= 0) return;
   const int chunks = (x.n + DN_CHUNK - 1) / DN_CHUNK, column = 16 * (W * part + pair);
@@ -466,12 +478,18 @@ static __device__ __forceinline__ void delta_scan_body(const unsigned short *__r
     else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   };
   iu8_v2u y[4];
-  auto store = [&](int c) {
+  unsigned short *to = out + ((size_t)(x.t0 + n) * heads + h) * DN + column + 4 * g;  // of the chunk's row n
+  const size_t block = (size_t)16 * heads * DN;
+  auto store = [&](int left) {  // (rows from the chunk's first on)
+    if (left >= DN_CHUNK) {
 #pragma unroll
-    for (int rb = 0; rb < 4; ++rb) {
-      const int t = c * DN_CHUNK + 16 * rb + n;
-      if (t < x.n) *(iu8_v2u *)(out + ((size_t)(x.t0 + t) * heads + h) * DN + column + 4 * g) = y[rb];
+      for (int rb = 0; rb < 4; ++rb) *(iu8_v2u *)(to + rb * block) = y[rb];
+    } else {
+#pragma unroll
+      for (int rb = 0; rb < 4; ++rb)
+        if (16 * rb + n < left) *(iu8_v2u *)(to + rb * block) = y[rb];
     }
+    to += 4 * block;
   };
   issue(0);
   if (chunks > 1) issue(1);
@@ -481,8 +499,8 @@ static __device__ __forceinline__ void delta_scan_body(const unsigned short *__r
     const unsigned char *at = smem + (c & 1) * STAGE, *wk = at + W_AT;
     const float *factor = (const float *)(wk + DN_FACTORS);
     if (c) {
-      store(c - 1);
       if (c + 1 < chunks) issue(c + 1);  // (its stage was read in the chunk before)
+      store(DN_CHUNK);
     }
     iu8_v4f o[4];
     float eq[4];
@@ -515,5 +533,5 @@ static __device__ __forceinline__ void delta_scan_body(const unsigned short *__r
     arrived(false);
     meet();
   }
-  store(chunks - 1);
+  store(x.n - (chunks - 1) * DN_CHUNK);
 }

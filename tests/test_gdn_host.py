@@ -72,7 +72,8 @@ def test_convolutions_that_are_refused(ctx, bad, code, words):
     (dict(heads=1 << 16, row=1 << 24, ab_row=1 << 16), iu8.E_RULE, "whole groups"), (dict(max_q=0), iu8.E_RULE, "at most 0"), (dict(row=48 * 128 - 8), iu8.E_RULE, "cover"),
     (dict(row=10244), iu8.E_RULE, "cover"), (dict(ab_row=40), iu8.E_RULE, "cover"), (dict(eps=-1.0), iu8.E_RULE, "eps"), (dict(eps=math.nan), iu8.E_RULE, "eps"),
     (dict(scale=math.inf), iu8.E_RULE, "scale"), (dict(seqs=1 << 20, tokens=1 << 20, slots=1 << 20, max_q=1), iu8.E_RULE, "32-bit sizes"),
-    (dict(seqs=1 << 20, tokens=1 << 22, slots=1 << 20), iu8.E_RULE, "32-bit sizes")])
+    (dict(seqs=1 << 20, tokens=1 << 22, slots=1 << 20), iu8.E_RULE, "32-bit sizes"), (dict(seqs=1 << 17, tokens=1 << 22, slots=1 << 17), iu8.E_RULE, "32-bit sizes"),
+    (dict(row=(1 << 24) + 8), iu8.E_RULE, "16777224 elements")])
 def test_rules_that_are_refused(ctx, bad, code, words):
     refused(lambda: rule(ctx, **bad), code, words)
 

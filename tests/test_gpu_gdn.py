@@ -154,6 +154,29 @@ def test_rule_in_chunks_by_the_waves_of_a_workgroup(ctx, kh, heads, seqs):
     rule_case(ctx, Rows(kh, heads, [70 + 13 * i % 60 for i in range(seqs)], seed=seqs), chunked=True)
 
 
+@pytest.mark.parametrize("seqs", [64, 65, 90])
+def test_rule_in_chunks_of_many_sequences(ctx, seqs):
+    """The longest are taken first where they are few; places of a batch that are idle, states that are nobody's."""
+    say(f"delta rule in chunks, {seqs} sequences")
+    r = Rows(1, 3, [(37 * i) % 71 for i in range(seqs)], front=2, behind=3, seed=seqs)
+    r.slot[5], r.slot[7] = -1, r.slots
+    rule_case(ctx, r, chunked=True)
+
+
+@pytest.mark.parametrize("lens,heads", [([10], 4), ([11, 3], 4), ([20, 9], 96), ([21, 2], 96)])
+def test_rule_by_its_longest_rows(ctx, lens, heads):
+    """The recurrent kernel up to a length, the chunks past it, whatever a workspace was made for."""
+    say(f"delta rule of {lens} rows, {heads} heads")
+    r = Rows(1, heads, lens, seed=heads)
+    ws = workspace(r, 64)
+    was = f64(r.state)
+    r.call(ctx, workspace=ws)
+    torch.cuda.synchronize()
+    for s, t, p, (want, tol, states, tols) in r.want(was, True):
+        check(f64(r.out[t:t + r.lens[s]].float()), want, tol, f"rows of sequence {s}")
+        check(f64(r.state[p]), states[-1], np.broadcast_to(tols[-1], states[-1].shape), f"state of sequence {s}")
+
+
 @pytest.mark.parametrize("chunked", [False, True])
 @pytest.mark.parametrize("like,a_at", [(0.0, 0.0), (1.0, -30.0), (0.9, -8.0), (0.0, 30.0), (0.5, 3000.0), (0.0, -3000.0)])
 def test_rule_of_like_keys_and_any_decay(ctx, like, a_at, chunked):
