@@ -16,9 +16,9 @@ constexpr uint32_t DIM = 128, CHUNK = 64, I32_MAX = 0x7FFFFFFFu, GRID_MAX = 0xFF
 constexpr uint64_t KEYS = 32768, PART = 19456;  // a chunk and key head's, a chunk and value head's bytes of the workspace (delta_chunk.h)
 constexpr uint64_t PIECE = 16384;      // a workgroup's bytes of block_copy
 // Chunks and key heads from which a workgroup of the preparation takes the value heads of a key head, up to four, whose rows' products they share:
-// without, the card is not full. Three heads against one a workgroup, microseconds: 272 chunks and key heads 22.8 against 16.9, 528 23.7
-// against 24.4, 2064 67.6 against 79.
-constexpr uint64_t PREP_FULL = 512;
+// without, the card is not full. Three heads against one a workgroup, microseconds: 272 chunks and key heads 17.0 against 15.5, 400 19.6
+// against 21.6, 528 20.5 against 26.0, 2064 59 against 76.
+constexpr uint64_t PREP_FULL = 384;
 // Sequences and heads up to which the recurrent kernel's waves take 16 columns each (512 threads a workgroup), not 32 (256). 1 / 5 / 8 rows,
 // microseconds: 48 items 6.7 / 9.8 / 12.0 on 16 columns, 8.3 / 10.6 / 12.9 on 32; 432 items 15.2 / 16.9 / 21.0 and 10.5 / 15.2 / 17.9.
 constexpr uint64_t STEP_NARROW = 256;

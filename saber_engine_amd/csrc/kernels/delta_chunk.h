@@ -30,6 +30,36 @@ constexpr int DN_T = 0, DN_INNER = 2 * DN_FRAGS * DN_FRAG, DN_FACTORS = DN_INNER
 
 static __device__ __forceinline__ int dn_chunk_id(const dn_rows &x) { return (x.t0 >> 6) + x.s; }  // of its first chunk: no two sequences' meet
 
+// A step of a running sum over the lanes.
+template <int X, int ROWS>
+static __device__ __forceinline__ void dn_scan_step(double &v) {
+  const iu8_v2u w = __builtin_bit_cast(iu8_v2u, v);
+  v += __builtin_bit_cast(double, iu8_v2u{(unsigned)__builtin_amdgcn_update_dpp(0, (int)w[0], X, ROWS, 0xF, false), (unsigned)__builtin_amdgcn_update_dpp(0, (int)w[1], X, ROWS, 0xF, false)});
+}
+// What lane I of each 16 holds.
+template <int I>
+static __device__ __forceinline__ float dn_shared(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x150 + I, 0xF, 0xF, false));
+}
+template <int I>
+static __device__ __forceinline__ double dn_shared(double v) {
+  const iu8_v2f w = __builtin_bit_cast(iu8_v2f, v);
+  return __builtin_bit_cast(double, iu8_v2f{dn_shared<I>(w[0]), dn_shared<I>(w[1])});
+}
+// Column n of the inverse of 1 + F, F strictly below the diagonal, in y, which begins as the identity's: from y_J on, y_i -= F_iJ y_J. (asm: the compiler makes
+// three instructions and a wait of it. f comes from LDS, so no lane operation has just written it.)
+template <int J, int I = J + 1>
+static __device__ __forceinline__ void dn_below_row(const float (&f)[16], float (&y)[16]) {
+  if constexpr (I < 16) {
+    asm("v_fmac_f32_dpp %0, -%1, %2 row_newbcast:%3 row_mask:0xf bank_mask:0xf" : "+v"(y[I]) : "v"(f[I]), "v"(y[J]), "n"(J));
+    dn_below_row<J, I + 1>(f, y);
+  } else if constexpr (J < 14) {
+    dn_below_row<J + 1>(f, y);
+  }
+}
+
+// Bound by what it moves and, a workgroup at a time, by the chain behind its loads: 8,192 rows of 16 and 48 heads, 67 MB in and 187 out, 59 us, a round
+// of workgroups some 15.
 static __device__ __forceinline__ void delta_prep_body(const unsigned short *__restrict__ q, const unsigned short *__restrict__ k,
                                                        const unsigned short *__restrict__ a, const unsigned short *__restrict__ b,
                                                        const float *__restrict__ a_log, const float *__restrict__ dt_bias,
@@ -44,23 +74,25 @@ static __device__ __forceinline__ void delta_prep_body(const unsigned short *__r
   const int id = item / key_heads, hk = item - id * key_heads, part = (int)(blockIdx.x >> 3) - turn * parts, h0 = hk * group + part * many;
   const int count = min(many, group - part * many);
   const int lane = threadIdx.x & 63, wave = at_uniform(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
-  int s = -1;
+  // the sequence of place `id`: the last whose first place is not behind it
+  dn_rows x;
+  x.n = 0;
   for (int base = 0; base < seqs; base += 64) {
-    const int i = base + lane;
-    s += __popcll(__ballot(i < seqs && (cu[i] >> 6) + i <= id));
+    const int i = min(base + lane, seqs - 1), from = cu[i], end = cu[i + 1], to = slot ? slot[i] : i;
+    const int below = __popcll(__ballot(base + lane < seqs && (from >> 6) + i <= id));
+    if (!below) break;
+    x = dn_rows_of(base + below - 1, __builtin_amdgcn_readlane(from, below - 1), __builtin_amdgcn_readlane(end, below - 1), __builtin_amdgcn_readlane(to, below - 1),
+                   tokens, slots);
   }
-  if (s < 0 || s >= seqs) return;
-  const dn_rows x = dn_sequence(cu, slot, s, tokens, slots);
+  if (x.n <= 0) return;
   const int c0 = (id - dn_chunk_id(x)) * DN_CHUNK, m = min(x.n - c0, DN_CHUNK);  // the chunk's first row, its rows
   if (c0 < 0 || m <= 0) return;
 
-  // K and Q, 16 KiB each, then A (in the end T) and the inner matrix in their place
+  // K and Q, 16 KiB each, then in their place of one head and the next A: blocks on the diagonal become T's, T's others stand in the block across it
   __shared__ __attribute__((aligned(16))) float s_m[2][DN_CHUNK][P];
-  __shared__ double s_sums[4][DN_CHUNK];  // in units of log 2
-  __shared__ __attribute__((aligned(16))) float s_betas[4][DN_CHUNK], s_rk[DN_CHUNK], s_rq[DN_CHUNK];
+  __shared__ __attribute__((aligned(16))) double s_sums[4][DN_CHUNK];  // in units of log 2
+  __shared__ __attribute__((aligned(16))) float s_betas[4][DN_CHUNK], s_in[4][DN_CHUNK], s_past[4][DN_CHUNK], s_rk[DN_CHUNK], s_rq[DN_CHUNK];
   __shared__ int s_unit[DN_CHUNK];  // K's and Q's rows' units, as exponents
-  auto &s_a = s_m[0];
-  auto &s_i = s_m[1];
   unsigned char *s_k = (unsigned char *)s_m, *s_q = s_k + DN_KEYS / 2;
 
   // a row past the end is the last one again, and takes no part
@@ -69,7 +101,7 @@ static __device__ __forceinline__ void delta_prep_body(const unsigned short *__r
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const size_t at = (t0 + min(16 * wave + 4 * i + g, m - 1)) * row + hk * DN + 8 * n;
-    kr[i] = *(const iu8_v4u *)(k + at), qr[i] = *(const iu8_v4u *)(q + at);
+    kr[i] = __builtin_nontemporal_load((const iu8_v4u *)(k + at)), qr[i] = __builtin_nontemporal_load((const iu8_v4u *)(q + at));
   }
   if (wave < count) {  // a head's gates a wave
     const int i = lane, h = h0 + wave;
@@ -79,12 +111,11 @@ static __device__ __forceinline__ void delta_prep_body(const unsigned short *__r
       be = dn_beta(iu8_bf16_f32(b[(t0 + i) * ab_row + h]));
     }
     double sum = lg * 1.4426950408889634074;
-#pragma unroll
-    for (int y = 1; y < 64; y *= 2) {
-      const double z = __shfl_up(sum, y);
-      sum += i >= y ? z : 0.0;
-    }
+    dn_scan_step<0x111, 0xF>(sum), dn_scan_step<0x112, 0xF>(sum), dn_scan_step<0x114, 0xF>(sum), dn_scan_step<0x118, 0xF>(sum);  // row_shr
+    dn_scan_step<0x142, 0xA>(sum), dn_scan_step<0x143, 0xC>(sum);                                                            // row_bcast
     s_sums[wave][i] = sum, s_betas[wave][i] = be;
+    // decays from the first of its 16 rows to it, from it to the last
+    s_in[wave][i] = __builtin_amdgcn_exp2f((float)(sum - dn_shared<0>(sum))), s_past[wave][i] = __builtin_amdgcn_exp2f((float)(dn_shared<15>(sum) - sum));
   }
   const int turned = (n ^ (g << 2)) << 4;  // piece n of row 16 wave + 4 i + g, ^ 16 i
 #pragma unroll
@@ -93,26 +124,26 @@ static __device__ __forceinline__ void delta_prep_body(const unsigned short *__r
     *(iu8_v4u *)(s_k + at) = kr[i], *(iu8_v4u *)(s_q + at) = qr[i];
   }
   __syncthreads();
-  // the products of the rows, row block `wave` with those up to it, and Q's with themselves
+  // the products of the rows, row block `wave` with those up to it, and Q's with themselves; row i = 16 wave + n, rows j = 16 jb + 4 g + r in place r
   const int row_piece = n * 256 + ((g ^ (n >> 2)) << 4);
   auto fragment = [&](const unsigned char *from, int rb, int ks) { return *(const iu8_v4u *)(from + rb * 4096 + row_piece + ((ks ^ (n & 3)) << 6)); };
-  iu8_v4f kk[4], qk[4], own = {0.f, 0.f, 0.f, 0.f}, qq = {0.f, 0.f, 0.f, 0.f};
+  iu8_v4f kk[3], qk[3], own = {0.f, 0.f, 0.f, 0.f}, qq = own, across = own;  // own, across: block `wave` itself
   {
     iu8_v4u kf[4], qf[4];
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) kf[ks] = fragment(s_k, wave, ks), qf[ks] = fragment(s_q, wave, ks);
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) own = dn_mfma_bf(kf[ks], kf[ks], own), qq = dn_mfma_bf(qf[ks], qf[ks], qq);
-    dn_settle(own), dn_settle(qq);
+    for (int ks = 0; ks < 4; ++ks) own = dn_mfma_bf(kf[ks], kf[ks], own), qq = dn_mfma_bf(qf[ks], qf[ks], qq), across = dn_mfma_bf(kf[ks], qf[ks], across);
+    dn_settle(own), dn_settle(qq), dn_settle(across);
 #pragma unroll
-    for (int jb = 0; jb < 4; ++jb) {
+    for (int jb = 0; jb < 3; ++jb) {
       kk[jb] = qk[jb] = iu8_v4f{0.f, 0.f, 0.f, 0.f};
-      if (jb <= wave) {
+      if (jb < wave) {
         iu8_v4u f[4];
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) f[ks] = fragment(s_k, jb, ks);
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) kk[jb] = dn_mfma_bf(kf[ks], f[ks], kk[jb]), qk[jb] = dn_mfma_bf(qf[ks], f[ks], qk[jb]);
+        for (int ks = 0; ks < 4; ++ks) kk[jb] = dn_mfma_bf(f[ks], kf[ks], kk[jb]), qk[jb] = dn_mfma_bf(f[ks], qf[ks], qk[jb]);
         dn_settle(kk[jb]), dn_settle(qk[jb]);
       }
     }
@@ -122,8 +153,10 @@ static __device__ __forceinline__ void delta_prep_body(const unsigned short *__r
   if (g == n >> 2) {
     const float ks = (n & 2) ? ((n & 1) ? own[3] : own[2]) : ((n & 1) ? own[1] : own[0]), qs = (n & 2) ? ((n & 1) ? qq[3] : qq[2]) : ((n & 1) ? qq[1] : qq[0]);
     const bool live = 16 * wave + n < m;
-    auto unit_of = [](float ss) { return max(dn_exponent(sqrtf(ss)), 64); };
-    s_rk[16 * wave + n] = live ? 1.f / sqrtf(ks + eps) : 0.f, s_rq[16 * wave + n] = live ? 1.f / sqrtf(qs + eps) : 0.f;
+    // half the exponent; v_rsq_f32 takes no subnormal
+    auto unit_of = [](float ss) { return max((dn_exponent(ss) + 127) >> 1, 64); };
+    auto inverse = [](float ss) { return ss < 0x1p-96f ? __builtin_amdgcn_rsqf(ss * 0x1p64f) * 0x1p32f : __builtin_amdgcn_rsqf(ss); };
+    s_rk[16 * wave + n] = live ? inverse(ks + eps) : 0.f, s_rq[16 * wave + n] = live ? inverse(qs + eps) : 0.f;
     s_unit[16 * wave + n] = unit_of(ks) | unit_of(qs) << 16;
   }
   __syncthreads();
@@ -145,112 +178,112 @@ static __device__ __forceinline__ void delta_prep_body(const unsigned short *__r
       *(iu8_v4u *)(to + at) = as_f16(kr[i], bk), *(iu8_v4u *)(to + DN_KEYS / 2 + at) = as_f16(qr[i], bq);
     }
   }
-  float of_row[4], of_query[4], of_key[4];
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int i = 16 * wave + 4 * g + r, j = 16 * r + n;
-    of_row[r] = s_rk[i], of_query[r] = s_rq[i], of_key[r] = s_rk[j];
-  }
-  auto give = [&](const float (*from)[P], int f, unsigned char *to, const float *s_beta, bool scaled, bool both) {
-    const int i = 16 * dn_frag_block(f) + n, j = 32 * dn_frag_half(f) + 4 * g;
-    iu8_v4f y = *(const iu8_v4f *)(from[i] + j), z = *(const iu8_v4f *)(from[i] + j + 16);
-    if (scaled) y = y * *(const iu8_v4f *)(s_beta + j), z = z * *(const iu8_v4f *)(s_beta + j + 16);
+  auto give = [&](iu8_v4f y, iu8_v4f z, int f, unsigned char *to, bool both) {
     iu8_v4u w[2];
     dn_operand<2>(y, z, w);
     *(iu8_v4u *)(to + f * DN_FRAG + lane * 16) = w[0];
     if (both) *(iu8_v4u *)(to + (DN_FRAGS + f) * DN_FRAG + lane * 16) = w[1];
   };
+  const iu8_v4f none = {0.f, 0.f, 0.f, 0.f};
+  const float rk = s_rk[16 * wave + n], rq = s_rq[16 * wave + n];
   for (int hh = 0; hh < count; ++hh) {
-    if (hh) __syncthreads();
     unsigned char *mine = work + ((size_t)id * heads + h0 + hh) * DN_PART;
     const double *s_sum = s_sums[hh];
     const float *s_beta = s_betas[hh];
-    if (wave == 3) {
-      const int i = lane;
-      const double end = s_sum[DN_CHUNK - 1];
-      float *f = (float *)(mine + DN_FACTORS);
-      const float eg = __builtin_amdgcn_exp2f((float)s_sum[i]);
-      const float rk = s_rk[i] * dn_power(s_unit[i] & 0xFFFF), rq = s_rq[i] * dn_power(s_unit[i] >> 16);
-      f[i] = eg * rk, f[64 + i] = eg * rq, f[128 + i] = __builtin_amdgcn_exp2f((float)(end - s_sum[i])) * rk;
-      if (i == 0) f[192] = __builtin_amdgcn_exp2f((float)end);
+    float(*s_a)[P] = s_m[hh & 1];
+    // exp(G_i - G_j) / |k_j|: on the diagonal by their difference; under it by three factors of at most 1, so that what is lost of one was lost of all
+    iu8_v4f w[3], wd;
+    const float *past = s_past[hh];
+    const float in = s_in[hh][16 * wave + n], by = s_beta[16 * wave + n] * rk;
+    const double si = s_sum[16 * wave + n], top = s_sum[16 * wave];
+    const iu8_v4f rd = *(const iu8_v4f *)(s_rk + 16 * wave + 4 * g);
+    double sd[4], ends[3];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) sd[r] = s_sum[16 * wave + 4 * g + r];
+#pragma unroll
+    for (int jb = 0; jb < 3; ++jb) {
+      w[jb] = *(const iu8_v4f *)(past + 16 * jb + 4 * g) * *(const iu8_v4f *)(s_rk + 16 * jb + 4 * g);
+      ends[jb] = s_sum[16 * jb + 15];
     }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) wd[r] = 4 * g + r <= n ? __builtin_amdgcn_exp2f((float)(si - sd[r])) * rd[r] : 0.f;
     {
-      float be[4];
-      double si[4];
+      iu8_v4f y = own * by * wd;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) be[r] = s_beta[16 * wave + 4 * g + r], si[r] = s_sum[16 * wave + 4 * g + r];
-#pragma unroll
-      for (int jb = 0; jb < 4; ++jb) {
-        const int j = 16 * jb + n;
-        if (jb <= wave) {
-          const double sj = s_sum[j];
-          const float rj = of_key[jb];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int i = 16 * wave + 4 * g + r;
-            const float w = i >= j ? __builtin_amdgcn_exp2f((float)(si[r] - sj)) * rj : 0.f;
-            s_a[i][j] = i > j ? be[r] * of_row[r] * w * kk[jb][r] : 0.f;
-            s_i[i][j] = of_query[r] * w * qk[jb][r];
-          }
-        } else if (jb == wave + 1 && !(wave & 1)) {  // (the fragments' other block)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) s_a[16 * wave + 4 * g + r][j] = 0.f, s_i[16 * wave + 4 * g + r][j] = 0.f;
-        }
-      }
+      for (int r = 0; r < 4; ++r) y[r] = 4 * g + r < n ? y[r] : 0.f;
+      *(iu8_v4f *)&s_a[16 * wave + n][16 * wave + 4 * g] = y;
     }
-    __syncthreads();
-    for (int f = wave; f < DN_FRAGS; f += 4) give(s_i, f, mine + DN_INNER, s_beta, false, false);
-    // T's blocks on the diagonal by substitution, a column a lane; in A's place
-    if (g == 0) {
-      float y[16];
+#pragma unroll
+    for (int jb = 0; jb < 3; ++jb) w[jb] *= in * __builtin_amdgcn_exp2f((float)(top - ends[jb]));
+#pragma unroll
+    for (int jb = 0; jb < 3; ++jb)
+      if (jb < wave) *(iu8_v4f *)&s_a[16 * wave + n][16 * jb + 4 * g] = kk[jb] * by * w[jb];
+    // T's blocks on the diagonal by substitution, a column a lane: of row i of F, whose 16 places 16 lanes hold, a place times what stands in y
+    {
       float(*at)[P] = (float(*)[P])(&s_a[16 * wave][16 * wave]);
+      __builtin_amdgcn_wave_barrier();
+      int column = n;  // (not known before this head: the 16 values would be kept)
+      asm volatile("" : "+v"(column));
+      float f[16], y[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float z = i == n ? 1.f : 0.f, z1 = 0.f;
-#pragma unroll
-        for (int j = 0; j < i; ++j) {
-          if (j & 1) z1 = fmaf(-at[i][j], y[j], z1);
-          else z = fmaf(-at[i][j], y[j], z);
-        }
-        y[i] = z + z1;
-      }
+      for (int i = 0; i < 16; ++i) f[i] = at[i][n], y[i] = i == column ? 1.f : 0.f;
+      dn_below_row<0>(f, y);
 #pragma unroll
       for (int i = 0; i < 16; ++i) at[i][n] = y[i];
     }
     __syncthreads();
     // those under it, wave j the column of blocks j: T_ij = -T_ii sum_k A_ik T_kj, on the f32 matrix instruction; a result's rows 4 g + r are the next
     // product's places r of lane group g
-    iu8_v4f t[4];
+    iu8_v4f t[3], f[6], of[3];
 #pragma unroll
     for (int r = 0; r < 4; ++r) t[0][r] = s_a[16 * wave + 4 * g + r][16 * wave + n];
 #pragma unroll
     for (int d = 1; d < 4; ++d) {
+      const int i = min(wave + d, 3);
+      of[d - 1] = *(const iu8_v4f *)&s_a[16 * i + n][16 * i + 4 * g];
+#pragma unroll
+      for (int e = 0; e < d; ++e) f[d * (d - 1) / 2 + e] = *(const iu8_v4f *)&s_a[16 * i + n][16 * min(wave + e, 3) + 4 * g];
+    }
+#pragma unroll
+    for (int d = 1; d < 4; ++d) {
       const int i = wave + d;
       if (i < 4) {
-        iu8_v4f y = {0.f, 0.f, 0.f, 0.f}, z = {0.f, 0.f, 0.f, 0.f};
+        iu8_v4f y = none, z = none;
 #pragma unroll
-        for (int e = 0; e < d; ++e) {
-          const iu8_v4f f = *(const iu8_v4f *)&s_a[16 * i + n][16 * (wave + e) + 4 * g];
+        for (int e = 0; e < d; ++e)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) y = __builtin_amdgcn_mfma_f32_16x16x4f32(f[r], t[e][r], y, 0, 0, 0);
-        }
+          for (int r = 0; r < 4; ++r) y = __builtin_amdgcn_mfma_f32_16x16x4f32(f[d * (d - 1) / 2 + e][r], t[e][r], y, 0, 0, 0);
         dn_settle(y);
-        const iu8_v4f f = *(const iu8_v4f *)&s_a[16 * i + n][16 * i + 4 * g];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) z = __builtin_amdgcn_mfma_f32_16x16x4f32(f[r], y[r], z, 0, 0, 0);
+        for (int r = 0; r < 4; ++r) z = __builtin_amdgcn_mfma_f32_16x16x4f32(of[d - 1][r], y[r], z, 0, 0, 0);
         dn_settle(z);
-        t[d] = -z;
+        z = -z;
+        if (d < 3) t[d < 3 ? d : 0] = z;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s_a[16 * wave + 4 * g + r][16 * i + n] = z[r];
       }
     }
+    // the inner matrix, row block `wave`
+    auto inner = [&](int jb) { return jb < 3 && jb < wave ? qk[jb < 3 ? jb : 0] * rq * w[jb < 3 ? jb : 0] : jb == wave ? across * rq * wd : none; };
+    give(inner(0), inner(1), wave < 2 ? wave : 2 * wave - 2, mine + DN_INNER, false);
+    if (wave >= 2) give(inner(2), inner(3), 2 * wave - 1, mine + DN_INNER, false);
+    if (wave == 3) {
+      const int i = lane;
+      const double end = s_sum[DN_CHUNK - 1];
+      float *f = (float *)(mine + DN_FACTORS);
+      const float eg = __builtin_amdgcn_exp2f((float)s_sum[i]);
+      const float k1 = s_rk[i] * dn_power(s_unit[i] & 0xFFFF), q1 = s_rq[i] * dn_power(s_unit[i] >> 16);
+      f[i] = eg * k1, f[64 + i] = eg * q1, f[128 + i] = __builtin_amdgcn_exp2f((float)(end - s_sum[i])) * k1;
+      if (i == 0) f[192] = __builtin_amdgcn_exp2f((float)end);
+    }
     __syncthreads();
-#pragma unroll
-    for (int d = 1; d < 4; ++d)
-      if (wave + d < 4) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) s_a[16 * (wave + d) + 4 * g + r][16 * wave + n] = t[d][r];
-      }
-    __syncthreads();
-    for (int f = wave; f < DN_FRAGS; f += 4) give(s_a, f, mine + DN_T, s_beta, true, true);
+    for (int f = wave; f < DN_FRAGS; f += 4) {
+      const int i = dn_frag_block(f), j = 2 * dn_frag_half(f);
+      auto block = [&](int b) { return *(const iu8_v4f *)(i == b ? &s_a[16 * i + n][16 * i + 4 * g] : &s_a[16 * b + n][16 * i + 4 * g]); };
+      const iu8_v4f y = block(j) * *(const iu8_v4f *)(s_beta + 16 * j + 4 * g);
+      const iu8_v4f z = j < i ? block(j + 1) * *(const iu8_v4f *)(s_beta + 16 * j + 16 + 4 * g) : none;
+      give(y, z, f, mine + DN_T, true);
+    }
   }
 }
 
@@ -280,7 +313,7 @@ static __device__ __forceinline__ iu8_v2u dn_transposed(const unsigned char *fro
 // the chain (K S, V - .., U, the next S), the other does what hangs from it, the rows' answers, with the operands that the first leaves in LDS, and asks for K, Q,
 // T, the inner matrix, the factors and V two chunks ahead, which come straight from memory into one of two LDS stages as soon as it has been read. O is
 // taken the other way round (the operands exchanged), so that a lane has four neighbouring values of one row to store. Two meetings a chunk: behind U, where the
-// stage is free, and behind the next S. W pairs a workgroup share a stage. A chunk takes 1.8 us (8,192 rows of 48 heads 225 us; the chain with the
+// stage is free, and behind the next S. W pairs a workgroup share a stage. A chunk takes 1.7 us (8,192 rows of 48 heads 222 us; the chain with the
 // stages' loads alone 204).
 template <int W>
 static __device__ __forceinline__ void delta_scan_body(const unsigned short *__restrict__ v, const unsigned char *__restrict__ keys,
@@ -296,18 +329,21 @@ static __device__ __forceinline__ void delta_scan_body(const unsigned short *__r
   const int lane = threadIdx.x & 63, wave = at_uniform(threadIdx.x >> 6), pair = wave % W, n = lane & 15, g = lane >> 4;
   int s = item / heads;
   const int h = item - s * heads, hk = h / group;
-  // The longest walks first, where a lane a sequence can tell (prompts of 2100, 777, 1859, 903 and 1173 rows, 48 heads: 115 us; in the sequences'
+  // The longest walks first, where a lane a sequence can tell (prompts of 2100, 777, 1859, 903 and 1173 rows, 48 heads: 114 us; in the sequences'
   // order, an eighth of the whole to each XCD, 158).
+  dn_rows x;
   if (seqs <= 64) {
-    const int length = lane < seqs ? cu[lane + 1] - cu[lane] : 0;
+    const int i = min(lane, seqs - 1), from = cu[i], end = cu[i + 1], to = slot ? slot[i] : i, length = end - from;
     int place = 0;
     for (int i = 0; i < seqs; ++i) {
       const int other = __builtin_amdgcn_readlane(length, i);
       place += other > length || (other == length && i < lane);
     }
     s = __builtin_ctzll(__ballot(lane < seqs && place == s));
+    x = dn_rows_of(s, __builtin_amdgcn_readlane(from, s), __builtin_amdgcn_readlane(end, s), __builtin_amdgcn_readlane(to, s), tokens, slots);
+  } else {
+    x = dn_sequence(cu, slot, s, tokens, slots);
   }
-  const dn_rows x = dn_sequence(cu, slot, s, tokens, slots);
   if (x.n <= 0) return;
   const int chunks = (x.n + DN_CHUNK - 1) / DN_CHUNK, column = 16 * (W * part + pair);
   const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) unsigned char *)smem;

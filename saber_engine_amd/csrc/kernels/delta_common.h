@@ -17,14 +17,15 @@ struct dn_rows {
 };
 
 // Sequence s of packed rows (cu), or row s alone; n <= 0 where there is nothing to do.
-static __device__ __forceinline__ dn_rows dn_sequence(const int *__restrict__ cu, const int *__restrict__ slot, int s, int tokens, int slots) {
+static __device__ __forceinline__ dn_rows dn_rows_of(int s, int t0, int end, int place, int tokens, int slots) {
   dn_rows x;
-  x.s = s;
-  x.t0 = cu ? cu[s] : s;
-  x.n = (cu ? min(cu[s + 1], tokens) : min(s + 1, tokens)) - x.t0;
-  x.slot = slot ? slot[s] : s;
-  if (x.t0 < 0 || (unsigned)x.slot >= (unsigned)slots) x.n = 0;
+  x.s = s, x.t0 = t0, x.slot = place;
+  x.n = min(end, tokens) - t0;
+  if (t0 < 0 || (unsigned)place >= (unsigned)slots) x.n = 0;
   return x;
+}
+static __device__ __forceinline__ dn_rows dn_sequence(const int *__restrict__ cu, const int *__restrict__ slot, int s, int tokens, int slots) {
+  return dn_rows_of(s, cu ? cu[s] : s, cu ? cu[s + 1] : s + 1, slot ? slot[s] : s, tokens, slots);
 }
 
 // The logarithm of a row's decay, and its beta.

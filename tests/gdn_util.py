@@ -32,7 +32,7 @@ def rule(q, k, v, a, b, a_log, dt_bias, state, eps, scale, chunked=False):
     The tolerances: a column's error goes through each row's update as the column does, by decay (1 - beta k^ k^T), which lengthens nothing, and each row
     adds ROW roundings of the column's length and its value. An answer has the column's error (|q^| = 1), the same roundings of its own sum,
     in the chunked form f16 factors beside the state in front of the chunk and its updates, and is rounded once. (In chunks: a row's update is
-    a sum of at most 64 inputs with weights of at most 1, each factor of a product that is f32 taken to 2^-22, four roundings of f32, or to 2^-25 of the column's
+    a sum of at most 64 inputs with weights of at most 1, made with ten roundings of f32 at most, each factor of a product that is f32 taken to 2^-22, four roundings more, or to 2^-25 of the column's
     unit, at most eight times its largest value: 64 roundings of the column's length once over the keys. Their 64-fold is less than what the chunk's rows add up to.)"""
     n, heads = v.shape[:2]
     of = np.arange(heads) // (heads // k.shape[1])

@@ -185,9 +185,8 @@ def test_descriptors_of_the_kernels_are_refused(kernel):
         iu8.Context.launch(type("C", (), {"_h": ctypes.c_void_p()})(), d, {})
 
 
-def test_matrix_results_are_read_no_earlier_than_they_are_there(tmp_path):
-    """The wait states that the compiler owes between a matrix instruction and the first lane instruction that reads its result, over every path from it (8 of the bf16 form,
-    10 of the f32 one, counted in instructions and the idle cycles of s_nop): tests/test_attn_host.py has why."""
+def listing(tmp_path):
+    """The delta kernels' instructions, as llvm-objdump prints them: (name, text) each."""
     tool = "/opt/rocm/llvm/bin/llvm-objdump"
     if not os.path.exists(tool):
         tool = shutil.which("llvm-objdump")
@@ -196,8 +195,14 @@ def test_matrix_results_are_read_no_earlier_than_they_are_there(tmp_path):
     bundle = open(os.path.join(iu8.PREBUILT, "delta_net.hsaco"), "rb").read()
     (tmp_path / "object").write_bytes(bundle[bundle.index(b"\x7fELF"):])
     text = subprocess.run([tool, "-d", "--no-show-raw-insn", str(tmp_path / "object")], capture_output=True, text=True, check=True).stdout
+    return re.findall(r"^[0-9a-f]+ <(delta_\w+)>:\n(.*?)(?=^[0-9a-f]+ <|\Z)", text, flags=re.S | re.M)
+
+
+def test_matrix_results_are_read_no_earlier_than_they_are_there(tmp_path):
+    """The wait states that the compiler owes between a matrix instruction and the first lane instruction that reads its result, over every path from it (8 of the bf16 form,
+    10 of the f32 one, counted in instructions and the idle cycles of s_nop): tests/test_attn_host.py has why."""
     checked = 0
-    for name, body in re.findall(r"^[0-9a-f]+ <(delta_\w+)>:\n(.*?)(?=^[0-9a-f]+ <|\Z)", text, flags=re.S | re.M):
+    for name, body in listing(tmp_path):
         code, place = [], {}
         for line in body.split("\n"):
             m = re.match(r"\s+(\S.*?)\s*// ([0-9A-F]+):?(.*)$", line)
@@ -240,3 +245,21 @@ def test_matrix_results_are_read_no_earlier_than_they_are_there(tmp_path):
                 idle = int(arg) + 1 if op == "s_nop" else 1
                 ways += [(n, waited + idle) for n in after(k)]
     assert checked > 250
+
+
+def test_lanes_are_read_no_earlier_than_they_are_there(tmp_path):
+    """A lane operation that reads other lanes' registers (DPP) comes two wait states behind the one that wrote them; in asm the compiler does not see to it."""
+    checked = 0
+    for name, body in listing(tmp_path):
+        code = [m.group(1) for m in re.finditer(r"^\s+(\S.*?)\s*// [0-9A-F]+", body, flags=re.M)]
+        for i, ins in enumerate(code):
+            if not ins.startswith("v_fmac_f32_dpp"):
+                continue
+            source, waited, k = registers(ins.split(",")[1].strip().lstrip("-").split()[0]), 0, i
+            checked += 1
+            while waited < 2 and k:
+                k -= 1
+                op, arg = (code[k].split(None, 1) + [""])[:2]
+                assert not (op.startswith("v_") and registers(arg.split(",")[0].strip()) & source), (name, code[k], ins)
+                waited += int(arg) + 1 if op == "s_nop" else 1
+    assert checked >= 100
