@@ -313,7 +313,7 @@ static __device__ __forceinline__ iu8_v2u dn_transposed(const unsigned char *fro
 // the chain (K S, V - .., U, the next S), the other does what hangs from it, the rows' answers, with the operands that the first leaves in LDS, and asks for K, Q,
 // T, the inner matrix, the factors and V two chunks ahead, which come straight from memory into one of two LDS stages as soon as it has been read. O is
 // taken the other way round (the operands exchanged), so that a lane has four neighbouring values of one row to store. Two meetings a chunk: behind U, where the
-// stage is free, and behind the next S. W pairs a workgroup share a stage. A chunk takes 1.7 us (8,192 rows of 48 heads 222 us; the chain with the
+// stage is free, and behind the next S. W pairs a workgroup share a stage. A chunk takes 1.7 us (8,192 rows of 48 heads 215 us; the chain with the
 // stages' loads alone 204).
 template <int W>
 static __device__ __forceinline__ void delta_scan_body(const unsigned short *__restrict__ v, const unsigned char *__restrict__ keys,
@@ -402,13 +402,27 @@ static __device__ __forceinline__ void delta_scan_body(const unsigned short *__r
 #pragma unroll
         for (int e = 0; e < 2; ++e) tf[f][e] = *(const iu8_v4u *)(wk + DN_T + (e * DN_FRAGS + f) * DN_FRAG + lane * 16);
       const float whole = factor[192];
+      // what the next state needs; where a wave has 512 registers, all the way ahead
+      auto ask_turned = [&]() {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int b = 0; b < 8; ++b) {
+            const unsigned char *from = at + K_AT + (4 * g + (n >> 2)) * 256 + (((n & 3) ^ g) << 4) + (((b >> 1) ^ (n >> 2)) << 6) + (b & 1) * 8;
+            const iu8_v2u lo = dn_transposed(from + 2 * i * 4096), hi = dn_transposed(from + (2 * i + 1) * 4096);
+            kt[b][i] = iu8_v4u{lo[0], lo[1], hi[0], hi[1]};
+          }
+#pragma unroll
+        for (int rb = 0; rb < 4; ++rb) ew[rb] = *(const iu8_v4f *)(factor + 128 + 16 * rb + 4 * g);
+      };
+      if constexpr (W == 2) ask_turned();
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
         for (int e = 1; e >= 0; --e)
 #pragma unroll
           for (int rb = 0; rb < 4; ++rb) p[rb] = dn_mfma(kf[ks][rb], sw[ks][e], p[rb]);
-      dn_step<32, 0, 1, 8, 29>();
+      dn_step<32, 0, W == 2 ? 2 : 1, 8, W == 2 ? 64 : 29>();
       // V - exp(G) / |k| K S
       float top = most;
 #pragma unroll
@@ -434,16 +448,7 @@ static __device__ __forceinline__ void delta_scan_body(const unsigned short *__r
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i) dn_operand<2>(p[2 * i], p[2 * i + 1], rt[i]);
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int b = 0; b < 8; ++b) {
-          const unsigned char *from = at + K_AT + (4 * g + (n >> 2)) * 256 + (((n & 3) ^ g) << 4) + (((b >> 1) ^ (n >> 2)) << 6) + (b & 1) * 8;
-          const iu8_v2u lo = dn_transposed(from + 2 * i * 4096), hi = dn_transposed(from + (2 * i + 1) * 4096);
-          kt[b][i] = iu8_v4u{lo[0], lo[1], hi[0], hi[1]};
-        }
-#pragma unroll
-      for (int rb = 0; rb < 4; ++rb) ew[rb] = *(const iu8_v4f *)(factor + 128 + 16 * rb + 4 * g);
+      if constexpr (W > 2) ask_turned();
       // U, the smallest products first
 #pragma unroll
       for (int i = 0; i < 2; ++i)
