@@ -17,11 +17,12 @@
 #pragma once
 #include "delta_step.h"
 
-// The workspace: of a chunk and key head K and Q, f16, 16 KiB each, row t's 16-byte pieces exchanged (piece ^ (t % 4 * 4 + t / 4 % 4)) as the walk keeps them in
-// LDS, where neither four neighbouring pieces of four neighbouring rows nor one piece of 16 rows share a bank; of a chunk and value head T diag(beta) in two
-// terms, the inner matrix in one, the factors. Operands are kept as fragments, 64 lanes x 16 bytes: lane (l % 16, g = l / 16) has row l % 16 of 16 and the
+// The workspace: of a chunk and key head K and Q, f16, 16 KiB each, piece p (16 bytes) of row t where dn_turned(p) ^ (t % 4 * 4 + t / 4 % 4) says, as the walk keeps
+// them in LDS: the 16 lanes that a wide read serves at once (of a quarter's fours 0 and 3, of the next one's 1 and 2) meet on no bank. Of a chunk and value
+// head T diag(beta) in two terms, the inner matrix in one, the factors. Operands are kept as fragments, 64 lanes x 16 bytes: lane (l % 16, g = l / 16) has row l % 16 of 16 and the
 // columns 4 g .. 4 g + 3 of the first and of the second 16 of 32, which is how a product's result lies (dn_operand).
 // Fragment f of a lower triangle: row blocks 0, 1 of the first 32 columns; row blocks 2, 3 of the first and of the last.
+static __host__ __device__ constexpr int dn_turned(int p) { return (p & ~3) | (-p & 3); }
 constexpr int DN_KEYS = 32768, DN_FRAGS = 6, DN_FRAG = 1024;
 static __host__ __device__ constexpr int dn_frag_block(int f) { return f < 2 ? f : 2 + (f - 2) / 2; }
 static __host__ __device__ constexpr int dn_frag_half(int f) { return f < 2 ? 0 : (f - 2) & 1; }
@@ -117,7 +118,7 @@ static __device__ __forceinline__ void delta_prep_body(const unsigned short *__r
     // decays from the first of its 16 rows to it, from it to the last
     s_in[wave][i] = __builtin_amdgcn_exp2f((float)(sum - dn_shared<0>(sum))), s_past[wave][i] = __builtin_amdgcn_exp2f((float)(dn_shared<15>(sum) - sum));
   }
-  const int turned = (n ^ (g << 2)) << 4;  // piece n of row 16 wave + 4 i + g, ^ 16 i
+  const int turned = (dn_turned(n) ^ (g << 2)) << 4;  // piece n of row 16 wave + 4 i + g, ^ 16 i
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int at = (16 * wave + 4 * i + g) * 256 + (turned ^ (i << 4));
@@ -125,7 +126,7 @@ static __device__ __forceinline__ void delta_prep_body(const unsigned short *__r
   }
   __syncthreads();
   // the products of the rows, row block `wave` with those up to it, and Q's with themselves; row i = 16 wave + n, rows j = 16 jb + 4 g + r in place r
-  const int row_piece = n * 256 + ((g ^ (n >> 2)) << 4);
+  const int row_piece = n * 256 + ((dn_turned(g) ^ (n >> 2)) << 4);
   auto fragment = [&](const unsigned char *from, int rb, int ks) { return *(const iu8_v4u *)(from + rb * 4096 + row_piece + ((ks ^ (n & 3)) << 6)); };
   iu8_v4f kk[3], qk[3], own = {0.f, 0.f, 0.f, 0.f}, qq = own, across = own;  // own, across: block `wave` itself
   {
@@ -349,7 +350,7 @@ static __device__ __forceinline__ void delta_scan_body(const unsigned short *__r
   const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) unsigned char *)smem;
   unsigned char *given = smem + 2 * STAGE + pair * GIVEN;  // 1 KiB each: S's four steps, U's row blocks; the state's unit over U's, U's
   float *units = (float *)(given + 8192);
-  const int row_piece = n * 256 + ((g ^ (n >> 2)) << 4);  // of K's and Q's row n; ^ 4 (ks ^ n % 4) pieces
+  const int row_piece = n * 256 + ((dn_turned(g) ^ (n >> 2)) << 4);  // of K's and Q's row n; ^ 4 (ks ^ n % 4) pieces
   auto meet = []() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
 
   if (wave < W) {  // ---- the chain
@@ -408,7 +409,7 @@ static __device__ __forceinline__ void delta_scan_body(const unsigned short *__r
         for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int b = 0; b < 8; ++b) {
-            const unsigned char *from = at + K_AT + (4 * g + (n >> 2)) * 256 + (((n & 3) ^ g) << 4) + (((b >> 1) ^ (n >> 2)) << 6) + (b & 1) * 8;
+            const unsigned char *from = at + K_AT + (4 * g + (n >> 2)) * 256 + ((dn_turned(n & 3) ^ g) << 4) + (((b >> 1) ^ (n >> 2)) << 6) + (b & 1) * 8;
             const iu8_v2u lo = dn_transposed(from + 2 * i * 4096), hi = dn_transposed(from + (2 * i + 1) * 4096);
             kt[b][i] = iu8_v4u{lo[0], lo[1], hi[0], hi[1]};
           }
