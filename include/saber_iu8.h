@@ -655,8 +655,8 @@ int saber_iu8_gdn_conv(saber_iu8_ctx *ctx, const void *x, uint32_t x_row, const 
  *   k^ = k / sqrt(|k|^2 + eps), q^ = q / sqrt(|q|^2 + eps), decay = exp(-exp(a_log[h]) softplus(a + dt_bias[h])), beta = sigmoid(b)
  *   S <- decay S + k^ (beta (v - (decay S)^T k^))^T,   out[t, h] = scale S^T q^
  * q, k, v rows `row` elements apart, heads 128 apart; a, b rows `ab_row` apart, a value a head; a_log, dt_bias f32 [heads]; out bf16 [tokens, heads, 128], which
- * must not overlap the rows, or NULL: the states alone (q may then be NULL). A decay below exp(-120) is zero. Values, states and gates are numbers: one that is not
- * spoils its head's rows from its chunk of 64 on, and the state.
+ * must not overlap the rows, or NULL: the states alone (q may then be NULL). A decay below exp(-120) is zero. Values, states and gates are numbers, and
+ * |q|^2 and |k|^2 numbers of f32: one that is not spoils its heads' rows from its chunk of 64 on, and their states.
  * max_q: the most new rows of a sequence, for the choice of the kernel alone. Long rows are taken in chunks of 64, with the workspace of saber_iu8_gdn_workspace (made
  * for (tokens, seqs, max_q), it holds every call of the same heads with at most these; calls that share it must not overlap in time), the rest, and whatever has no
  * workspace, kept, or no out, a row at a time: the same rule, other roundings. States, norms and sums in f32 (the chunks' matrix products hold 22 bits of
