@@ -314,7 +314,7 @@ static __device__ __forceinline__ iu8_v2u dn_transposed(const unsigned char *fro
 // the chain (K S, V - .., U, the next S), the other does what hangs from it, the rows' answers, with the operands that the first leaves in LDS, and asks for K, Q,
 // T, the inner matrix, the factors and V two chunks ahead, which come straight from memory into one of two LDS stages as soon as it has been read. O is
 // taken the other way round (the operands exchanged), so that a lane has four neighbouring values of one row to store. Two meetings a chunk: behind U, where the
-// stage is free, and behind the next S. W pairs a workgroup share a stage. A chunk takes 1.7 us (8,192 rows of 48 heads 215 us; the chain with the
+// stage is free, and behind the next S. W pairs a workgroup share a stage. A chunk takes 1.7 us (8,192 rows of 48 heads 210 us; the chain with the
 // stages' loads alone 204).
 template <int W>
 static __device__ __forceinline__ void delta_scan_body(const unsigned short *__restrict__ v, const unsigned char *__restrict__ keys,

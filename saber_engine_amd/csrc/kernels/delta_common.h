@@ -38,18 +38,23 @@ static __device__ __forceinline__ float dn_beta(float b) { return 1.f / (1.f + e
 typedef _Float16 dn_v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 dn_v2h __attribute__((ext_vector_type(2)));
 
-// f32 as a sum of f16: the first N terms, 11 bits each, of a pair of values (what two terms leave is 2^-22 of a value, and no less than half of f16's last
-// step, 2^-25; the matrix instructions keep values below 2^-14). What a term leaves is exact; v_fma_mix takes the f16 as it is, where conversion and
-// subtraction are two. (It is asm because the compiler makes those two of it. The conversion to f16 has read x and y in front of it, so a matrix result is there.)
+// f32 as a sum of f16: the first N terms (1 or 2), 11 bits each, of a pair of values (what two terms leave is 2^-22 of a value, and no less than half of f16's last
+// step, 2^-25; the matrix instructions keep values below 2^-14). What the first leaves is exact, and rounded once: by the mixed multiply-adds, which take f16 and f32
+// as they are and write a half, where conversion, subtraction and conversion are three. (-1 is hidden, so that a multiply-add stays; the first terms as well, so that
+// they stay a pair.)
+static __device__ __forceinline__ dn_v2h dn_pair(dn_v2h h) {
+  unsigned w = __builtin_bit_cast(unsigned, h);
+  asm("" : "+v"(w));
+  return __builtin_bit_cast(dn_v2h, w);
+}
+static __device__ __forceinline__ unsigned dn_rounded(float x, float y) { return __builtin_bit_cast(unsigned, dn_v2h{(_Float16)x, (_Float16)y}); }
 template <int N>
 static __device__ __forceinline__ void dn_split(float x, float y, unsigned (&t)[N]) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const dn_v2h h = __builtin_convertvector(iu8_v2f{x, y}, dn_v2h);
-    t[i] = __builtin_bit_cast(unsigned, h);
-    if (i + 1 < N)
-      asm("v_fma_mix_f32 %0, %2, -1.0, %0 op_sel_hi:[1,0,0]\n\tv_fma_mix_f32 %1, %2, -1.0, %1 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "+v"(x), "+v"(y) : "v"(t[i]));
-  }
+  float less;
+  asm("s_mov_b32 %0, -1.0" : "=s"(less));
+  const dn_v2h h = dn_pair(__builtin_convertvector(iu8_v2f{x, y}, dn_v2h));
+  t[0] = __builtin_bit_cast(unsigned, h);
+  if constexpr (N > 1) t[1] = dn_rounded(fmaf((float)h[0], less, x), fmaf((float)h[1], less, y));
 }
 // Two result blocks of a 16 x 16 product, rows 4 g + r of each, as the N terms of the next product's operand: its eight places
 // are the first block's rows 4 g .. 4 g + 3, then the second's.
