@@ -13,7 +13,7 @@
 // of two (its largest value brought to 1 .. 2); its norm's and decay's factors are moved to the other side of the product; the other side is split
 // into two f16 terms, 22 bits (dn_split), in a column's own unit, a power of two that follows the column's largest value. What goes only into the rows' bf16 answers takes
 // one term, 11 bits. (Three bf16 terms, which need no units, are half as many products again and twice the lane arithmetic: the walk of 8,192 rows of 48
-// heads 304 us, with f16 225.) G is summed, and its differences taken, in f64: after a strong decay the later rows' differences would be left with the sum's digits.
+// heads 304 us, with f16 208.) G is summed, and its differences taken, in f64: after a strong decay the later rows' differences would be left with the sum's digits.
 #pragma once
 #include "delta_step.h"
 
@@ -314,7 +314,7 @@ static __device__ __forceinline__ iu8_v2u dn_transposed(const unsigned char *fro
 // the chain (K S, V - .., U, the next S), the other does what hangs from it, the rows' answers, with the operands that the first leaves in LDS, and asks for K, Q,
 // T, the inner matrix, the factors and V two chunks ahead, which come straight from memory into one of two LDS stages as soon as it has been read. O is
 // taken the other way round (the operands exchanged), so that a lane has four neighbouring values of one row to store. Two meetings a chunk: behind U, where the
-// stage is free, and behind the next S. W pairs a workgroup share a stage. A chunk takes 1.7 us (8,192 rows of 48 heads 210 us; the chain with the
+// stage is free, and behind the next S. W pairs a workgroup share a stage. A chunk takes 1.6 us (8,192 rows of 48 heads 208 us; the chain with the
 // stages' loads alone 204).
 template <int W>
 static __device__ __forceinline__ void delta_scan_body(const unsigned short *__restrict__ v, const unsigned char *__restrict__ keys,
@@ -330,7 +330,7 @@ static __device__ __forceinline__ void delta_scan_body(const unsigned short *__r
   const int lane = threadIdx.x & 63, wave = at_uniform(threadIdx.x >> 6), pair = wave % W, n = lane & 15, g = lane >> 4;
   int s = item / heads;
   const int h = item - s * heads, hk = h / group;
-  // The longest walks first, where a lane a sequence can tell (prompts of 2100, 777, 1859, 903 and 1173 rows, 48 heads: 114 us; in the sequences'
+  // The longest walks first, where a lane a sequence can tell (prompts of 2100, 777, 1859, 903 and 1173 rows, 48 heads: 113 us; in the sequences'
   // order, an eighth of the whole to each XCD, 158).
   dn_rows x;
   if (seqs <= 64) {
@@ -354,8 +354,8 @@ static __device__ __forceinline__ void delta_scan_body(const unsigned short *__r
   auto meet = []() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
 
   if (wave < W) {  // ---- the chain
-    float *mine = state + ((size_t)x.slot * heads + h) * (DN * DN) + column + n;
-    auto channel = [&](int b, int r) { return 32 * (b >> 1) + 8 * g + 4 * (b & 1) + r; };
+    float *mine = state + ((size_t)x.slot * heads + h) * (DN * DN) + (8 * g) * DN + column + n;
+    auto channel = [](int b, int r) { return 32 * (b >> 1) + 4 * (b & 1) + r; };  // beside 8 g
     iu8_v4f st[8];  // in units of `unit`
     float unit, per_unit, most = 0.f;  // most: the column's largest value, in units
     iu8_v4u sw[4][2];
