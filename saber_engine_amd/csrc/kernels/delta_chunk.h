@@ -314,8 +314,8 @@ static __device__ __forceinline__ iu8_v2u dn_transposed(const unsigned char *fro
 // the chain (K S, V - .., U, the next S), the other does what hangs from it, the rows' answers, with the operands that the first leaves in LDS, and asks for K, Q,
 // T, the inner matrix, the factors and V two chunks ahead, which come straight from memory into one of two LDS stages as soon as it has been read. O is
 // taken the other way round (the operands exchanged), so that a lane has four neighbouring values of one row to store. Two meetings a chunk: behind U, where the
-// stage is free, and behind the next S. W pairs a workgroup share a stage. A chunk takes 1.6 us (8,192 rows of 48 heads 208 us; the chain with the
-// stages' loads alone 204).
+// stage is free, and behind the next S. W pairs a workgroup share a stage. A chunk takes 1.6 us with two pairs
+// (8,192 rows of 48 heads 208 us), 2.2 with four.
 template <int W>
 static __device__ __forceinline__ void delta_scan_body(const unsigned short *__restrict__ v, const unsigned char *__restrict__ keys,
                                                        const unsigned char *__restrict__ work, float *__restrict__ state, const int *__restrict__ slot,
