@@ -14,7 +14,7 @@ namespace {
 
 constexpr uint32_t DIM = 128, CHUNK = 64, I32_MAX = 0x7FFFFFFFu, GRID_MAX = 0xFFFFFFu;  // workgroups of 256 whose threads a launch counts in 32 bits
 constexpr uint64_t KEYS = 32768, PART = 19456;  // a chunk and key head's, a chunk and value head's bytes of the workspace (delta_chunk.h)
-constexpr uint64_t PIECE = 16384;      // a workgroup's bytes of block_copy
+constexpr uint64_t PIECE = 8192;  // a workgroup's bytes of block_copy, of 512 threads
 // Chunks and key heads from which a workgroup of the preparation takes the value heads of a key head, up to four, whose rows' products they share:
 // without, the card is not full. Three heads against one a workgroup, microseconds: 272 chunks and key heads 17.0 against 15.5, 400 19.6
 // against 21.6, 528 20.5 against 26.0, 2064 59 against 76.
@@ -85,9 +85,9 @@ int copy(saber_iu8_ctx *ctx, const char *op, void *a, void *b, uint64_t a_bytes,
   if (!ctx) return fail(SABER_IU8_E_ARG, fmt("%s: null argument", op));
   if (!n) return 0;
   const uint64_t pieces = (a_bytes + PIECE - 1) / PIECE + (b_bytes + PIECE - 1) / PIECE;
-  if ((__int128)pieces * n > GRID_MAX) return fail(SABER_IU8_E_RULE, fmt("%s: %u copies of %llu bytes pass a launch's 32-bit sizes", op, n, (unsigned long long)(a_bytes + b_bytes)));
+  if ((__int128)pieces * n > GRID_MAX / 2) return fail(SABER_IU8_E_RULE, fmt("%s: %u copies of %llu bytes pass a launch's 32-bit sizes", op, n, (unsigned long long)(a_bytes + b_bytes)));
   CopyArgs x{a, b, src, dst, (int64_t)a_bytes, (int64_t)b_bytes, (int32_t)blocks};
-  return launch_image(ctx, "block_copy", (uint32_t)(pieces * n), 256, &x, sizeof x, stream);
+  return launch_image(ctx, "block_copy", (uint32_t)(pieces * n), 512, &x, sizeof x, stream);
 }
 
 }  // namespace

@@ -51,7 +51,7 @@ extern "C" __global__ __launch_bounds__(256, 4) void delta_prep(
 DELTA_SCAN(2)
 DELTA_SCAN(4)
 
-extern "C" __global__ __launch_bounds__(256) void block_copy(unsigned char *__restrict__ a, unsigned char *__restrict__ b, const int *__restrict__ src,
+extern "C" __global__ __launch_bounds__(BLOCK_THREADS) void block_copy(unsigned char *__restrict__ a, unsigned char *__restrict__ b, const int *__restrict__ src,
                                                              const int *__restrict__ dst, long long a_bytes, long long b_bytes, int blocks) {
   block_copy_body(a, b, src, dst, a_bytes, b_bytes, blocks);
 }
