@@ -3,7 +3,8 @@
 // in f32, rounded once. What lies in front of a sequence's first row is its tail, bf16 [slots][W - 1][channels], the oldest input first;
 // the last W - 1 inputs of its first `kept` rows (all, without a table) are the new tail.
 //
-// Bound by the bytes, rows in and out (6,812 rows of 10,240 channels: 53 us, 5.2 TB/s). A thread takes 8 channels of `run` rows, the inputs that a row shares with the next kept in
+// Bound by the bytes, rows in and out (6,812 rows of 10,240 channels: 53 us, 5.2 TB/s; stored past the caches a tenth less
+// by itself, but then the rule behind it waits for the rows: both together 240 us against 237). A thread takes 8 channels of `run` rows, the inputs that a row shares with the next kept in
 // registers, four rows on the way at once. A tail is read and written by one thread alone: rows that see it (a sequence's first W - 1) belong to
 // the run of the sequence's first row, also past that run's end.
 #pragma once
