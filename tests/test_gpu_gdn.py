@@ -163,6 +163,13 @@ def test_rule_in_chunks_of_many_sequences(ctx, seqs):
     rule_case(ctx, r, chunked=True)
 
 
+@pytest.mark.parametrize("kh,heads,seqs", [(8, 24, 45), (6, 30, 60), (7, 14, 50)])
+def test_rule_in_chunks_whose_preparation_shares_a_key_head(ctx, kh, heads, seqs):
+    """Two, three and five value heads on a key head, in workgroups of up to four of them."""
+    say(f"delta rule in chunks, {seqs} sequences of {heads} heads on {kh}")
+    rule_case(ctx, Rows(kh, heads, [33] + [3 + (5 * i) % 17 for i in range(seqs - 2)] + [66], seed=seqs), chunked=True)
+
+
 @pytest.mark.parametrize("lens,heads", [([10], 4), ([11, 3], 4), ([20, 9], 96), ([21, 2], 96)])
 def test_rule_by_its_longest_rows(ctx, lens, heads):
     """The recurrent kernel up to a length, the chunks past it, whatever a workspace was made for."""
@@ -376,3 +383,38 @@ def test_states_copied_and_offsets_past_32_bits(ctx):
     for _, t, p, (want, tol, states, tols) in r.want({1499: was[0]}, True):
         check(f64(r.out.float()), want, tol, "rows")
         check(f64(state[p]), states[-1], np.broadcast_to(tols[-1], states[-1].shape), "state")
+
+
+@pytest.mark.parametrize("chunked", [False, True])
+def test_states_past_32_bits_are_the_same_states(ctx, chunked):
+    """The last slots of a pool past 4 GiB answer and are left as the same ones of a small pool, byte for byte."""
+    say(f"delta rule on states past 4 GiB, chunked {chunked}")
+    small, large = (Rows(1, 1, [70, 3], slots=2, seed=21) for _ in range(2))
+    small.slot.copy_(torch.arange(2))
+    first = 70000 - 2
+    pool = torch.zeros((first + 2, 1, 128, 128), dtype=torch.float32, device="cuda")
+    pool[first:] = large.state
+    large.state, large.slots = pool, first + 2
+    large.slot.copy_(torch.arange(first, first + 2))
+    for r in (small, large):
+        r.call(ctx, workspace=workspace(r) if chunked else None)
+    torch.cuda.synchronize()
+    assert torch.equal(small.out, large.out) and torch.equal(small.state, pool[first:]) and not pool[:first].any()
+
+
+def test_tails_past_32_bits_are_the_same_tails(ctx):
+    say("convolution on tails past 4 GiB")
+    channels, width, first = 384, 4, 2_000_000
+    g = torch.Generator().manual_seed(22)
+    x, weight = torch.randn(9, channels, generator=g).bfloat16().cuda(), torch.randn(channels, width, generator=g).bfloat16().cuda()
+    small = torch.randn(2, width - 1, channels, generator=g).bfloat16().cuda()
+    large = torch.zeros((first + 2, width - 1, channels), dtype=torch.bfloat16, device="cuda")
+    large[first:] = small
+    outs, cu = [], ends([7, 2])
+    for tail, at in ((small, 0), (large, first)):
+        slot = torch.arange(at, at + 2, dtype=torch.int32, device="cuda")
+        outs.append(torch.zeros(9, channels, dtype=torch.bfloat16, device="cuda"))
+        ctx.gdn_conv(x.data_ptr(), channels, weight.data_ptr(), tail.data_ptr(), len(tail), outs[-1].data_ptr(), channels, 9, 2, channels, width,
+                     slot=slot.data_ptr(), cu_q=cu.data_ptr())
+        torch.cuda.synchronize()
+    assert torch.equal(*outs) and torch.equal(small, large[first:]) and not large[:first].any()
