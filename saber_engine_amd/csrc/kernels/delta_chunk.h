@@ -154,10 +154,8 @@ static __device__ __forceinline__ void delta_prep_body(const unsigned short *__r
   if (g == n >> 2) {
     const float ks = (n & 2) ? ((n & 1) ? own[3] : own[2]) : ((n & 1) ? own[1] : own[0]), qs = (n & 2) ? ((n & 1) ? qq[3] : qq[2]) : ((n & 1) ? qq[1] : qq[0]);
     const bool live = 16 * wave + n < m;
-    // half the exponent; v_rsq_f32 takes no subnormal
-    auto unit_of = [](float ss) { return max((dn_exponent(ss) + 127) >> 1, 64); };
-    auto inverse = [](float ss) { return ss < 0x1p-96f ? __builtin_amdgcn_rsqf(ss * 0x1p64f) * 0x1p32f : __builtin_amdgcn_rsqf(ss); };
-    s_rk[16 * wave + n] = live ? inverse(ks + eps) : 0.f, s_rq[16 * wave + n] = live ? inverse(qs + eps) : 0.f;
+    auto unit_of = [](float ss) { return max((dn_exponent(ss) + 127) >> 1, 64); };  // half the exponent
+    s_rk[16 * wave + n] = live ? dn_inverse_root(ks + eps) : 0.f, s_rq[16 * wave + n] = live ? dn_inverse_root(qs + eps) : 0.f;
     s_unit[16 * wave + n] = unit_of(ks) | unit_of(qs) << 16;
   }
   __syncthreads();

@@ -35,6 +35,11 @@ static __device__ __forceinline__ float dn_log_decay(float a, float a_log, float
 }
 static __device__ __forceinline__ float dn_beta(float b) { return 1.f / (1.f + expf(-b)); }
 
+// 1 / sqrt(x) within a unit; v_rsq_f32 takes no subnormal.
+static __device__ __forceinline__ float dn_inverse_root(float x) {
+  return x < 0x1p-96f ? __builtin_amdgcn_rsqf(x * 0x1p64f) * 0x1p32f : __builtin_amdgcn_rsqf(x);
+}
+
 typedef _Float16 dn_v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 dn_v2h __attribute__((ext_vector_type(2)));
 

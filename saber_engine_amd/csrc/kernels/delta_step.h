@@ -4,7 +4,7 @@
 // key's channels 256 / C j + dg, so that its loads are rows of 4 C bytes. Both sums of a row are taken of the
 // state before it, so that they share the exchanges:
 //   past = decay S, u = beta (v - decay S^T k^), o = scale (decay S^T q^ + (k^ . q^) u), S <- past + k^ u^T
-// Rows are taken eight at a time, one or two a wave, normed, into LDS; the first eight are asked for before the state. Bound by the state, read and written
+// Rows are taken eight at a time, one or two a wave, normed, into LDS, their gates by the last wave; the first eight are asked for before the state. Bound by the state, read and written
 // once (64 sequences of a row, 48 heads: 76 us, 5.3 TB/s in and out), and with few sequences by a row's chain, about a microsecond.
 //
 // kept: the state behind the first kept[s] rows is the one that is stored (no table: behind all; 0: none); the rows behind them are still
@@ -52,7 +52,7 @@ static __device__ __forceinline__ void delta_step_body(const unsigned short *__r
   __shared__ __attribute__((aligned(16))) unsigned s_v[BATCH][64];
 
   unsigned kk[MINE], qq[MINE], vv[MINE];
-  unsigned short aa[MINE], bb[MINE];
+  unsigned short aa = 0, bb = 0;  // the last wave's: a row's gates a lane
   auto fetch = [&](int base) {
 #pragma unroll
     for (int y = 0; y < MINE; ++y) {
@@ -60,7 +60,10 @@ static __device__ __forceinline__ void delta_step_body(const unsigned short *__r
       kk[y] = *(const unsigned *)(k + t * row + hk * DN + 2 * lane);
       qq[y] = out ? *(const unsigned *)(q + t * row + hk * DN + 2 * lane) : 0u;
       vv[y] = *(const unsigned *)(v + t * row + h * DN + 2 * lane);
-      aa[y] = a[t * ab_row + h], bb[y] = b[t * ab_row + h];
+    }
+    if (wave == WAVES - 1) {
+      const size_t t = x.t0 + min(base + (lane & (BATCH - 1)), x.n - 1);
+      aa = a[t * ab_row + h], bb = b[t * ab_row + h];
     }
   };
   fetch(0);
@@ -81,19 +84,17 @@ static __device__ __forceinline__ void delta_step_body(const unsigned short *__r
 #pragma unroll
     for (int y = 0; y < MINE; ++y) {
       const int i = y * WAVES + wave;
+      if (i >= count) break;
       const float k0 = __uint_as_float(kk[y] << 16), k1 = __uint_as_float(kk[y] & 0xFFFF0000u), q0 = __uint_as_float(qq[y] << 16), q1 = __uint_as_float(qq[y] & 0xFFFF0000u);
-      const float rk = 1.f / sqrtf(dn_sum64(fmaf(k0, k0, k1 * k1)) + eps), rq = scale / sqrtf(dn_sum64(fmaf(q0, q0, q1 * q1)) + eps);
+      const float rk = dn_inverse_root(dn_sum64(fmaf(k0, k0, k1 * k1)) + eps), rq = scale * dn_inverse_root(dn_sum64(fmaf(q0, q0, q1 * q1)) + eps);
       const float kq = dn_sum64(fmaf(k0, q0, k1 * q1));
       s_v[i][lane] = vv[y];
       const int c = 2 * lane;  // channel DG j + dg lies at [dg][j]
       s_k[i][c % DG][c / DG] = k0 * rk, s_k[i][c % DG + 1][c / DG] = k1 * rk;
       s_q[i][c % DG][c / DG] = q0 * rq, s_q[i][c % DG + 1][c / DG] = q1 * rq;
-      if (lane == 0) {
-        s_g[i] = expf(dn_log_decay(iu8_bf16_f32(aa[y]), al, dt));
-        s_b[i] = dn_beta(iu8_bf16_f32(bb[y]));
-        s_kq[i] = kq * rk * rq;
-      }
+      if (lane == 0) s_kq[i] = kq * rk * rq;
     }
+    if (wave == WAVES - 1 && lane < BATCH) s_g[lane] = expf(dn_log_decay(iu8_bf16_f32(aa), al, dt)), s_b[lane] = dn_beta(iu8_bf16_f32(bb));
     __syncthreads();
     for (int i = 0; i < count; ++i) {
       const iu8_v2u now = *(const iu8_v2u *)&s_v[i][column / 2];
