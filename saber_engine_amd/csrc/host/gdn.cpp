@@ -23,12 +23,11 @@ constexpr uint64_t PREP_FULL = 384;
 // microseconds: 48 items 6.7 / 9.8 / 12.0 on 16 columns, 8.3 / 10.6 / 12.9 on 32; 432 items 15.2 / 16.9 / 21.0 and 10.5 / 15.2 / 17.9.
 constexpr uint64_t STEP_NARROW = 256;
 constexpr uint32_t ROW_MAX = 1u << 24;  // elements of a row: a chunk's bytes are counted in 32 bits
-// Rows of a sequence up to which the recurrent kernel runs though a workspace is given: STEP_FEW where its workgroups (sequences and heads) are
-// few, STEP_MANY from STEP_ITEMS of them. Measured, microseconds of a call, recurrent against chunks: 1 sequence of 48 heads, 8 / 12 / 16 rows
-// 12.2 / 17.6 / 21.1 against 14.8 / 14.5 / 14.6; 16 of 8 heads 12.9 / 17.2 / 20.5 against 17.3 / 17.0 / 17.0; 4 of 48 heads, 12 / 16 / 24 rows
-// 17.9 / 21.0 / 28.7 against 20.7 / 23.0 / 21.8; 64 of 48 heads, 16 / 24 / 32 rows 131 / 179 / 230 against 174 / 174 / 179.
-constexpr uint32_t STEP_FEW = 10, STEP_MANY = 20;
-constexpr uint64_t STEP_ITEMS = 192;
+// Rows of a sequence up to which the recurrent kernel runs though a workspace is given: 8 and one more for each 32 of its workgroups (sequences
+// and heads), from STEP_FEW to STEP_MANY. Measured, microseconds of a call, recurrent against chunks: 1 sequence of 48 heads, 8 / 12 / 16 rows
+// 11.0 / 15.2 / 17.9 against 13.5 / 13.7 / 13.3; 16 of 8 heads 12.7 / 17.0 / 19.6 against 15.5 / 15.4 / 15.7; 4 of 48 heads, 12 / 16 / 24 rows
+// 17.1 / 20.9 / 27.2 against 22.1; 64 of 8 heads, 16 / 24 / 32 rows 28 / 37 / 47 against 40 / 41 / 42; 64 of 48 heads 129 / 176 / 224 against 176 / 182 / 190.
+constexpr uint64_t STEP_FEW = 10, STEP_MANY = 24;
 
 // The kernels' arguments as abi.cpp declares them (natural alignment: the order says it all).
 struct ConvArgs {
@@ -139,7 +138,7 @@ int saber_iu8_gdn(saber_iu8_ctx *ctx, const void *q, const void *k, const void *
   if (!(eps >= 0.f && std::isfinite(eps)) || !std::isfinite(scale)) return fail(SABER_IU8_E_RULE, "gdn: eps must be a number from 0, the scale a number");
   const int32_t shape = (int32_t)(heads | key_heads << 16);
   const uint64_t items = (uint64_t)seqs * heads;
-  if (!workspace || kept || !out || !cu_q || max_q <= (items < STEP_ITEMS ? STEP_FEW : STEP_MANY)) {
+  if (!workspace || kept || !out || !cu_q || max_q <= std::min(std::max(8 + items / 32, STEP_FEW), STEP_MANY)) {
     if (items > GRID_MAX) return fail(SABER_IU8_E_RULE, fmt("gdn: %u sequences of %u heads pass a launch's 32-bit sizes", seqs, heads));
     StepArgs x{q, k, v, a, b, a_log, dt_bias, state, slot, cu_q, kept, out, (int32_t)row, (int32_t)ab_row, (int32_t)tokens, (int32_t)seqs, shape, (int32_t)slots, eps, scale};
     const bool narrow = items <= STEP_NARROW;

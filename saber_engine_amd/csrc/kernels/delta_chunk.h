@@ -328,17 +328,17 @@ static __device__ __forceinline__ void delta_scan_body(const unsigned short *__r
   const int lane = threadIdx.x & 63, wave = at_uniform(threadIdx.x >> 6), pair = wave % W, n = lane & 15, g = lane >> 4;
   int s = item / heads;
   const int h = item - s * heads, hk = h / group;
-  // The longest walks first, where a lane a sequence can tell (prompts of 2100, 777, 1859, 903 and 1173 rows, 48 heads: 113 us; in the sequences'
-  // order, an eighth of the whole to each XCD, 158).
+  // The longest walks first, where a lane a sequence can tell and walks are long enough to pay for it (prompts of 2100, 777, 1859, 903 and 1173 rows, 48
+  // heads: 113 us; in the sequences' order, an eighth of the whole to each XCD, 158).
   dn_rows x;
   if (seqs <= 64) {
-    const int i = min(lane, seqs - 1), from = cu[i], end = cu[i + 1], to = slot ? slot[i] : i, length = end - from;
-    int place = 0;
-    for (int i = 0; i < seqs; ++i) {
-      const int other = __builtin_amdgcn_readlane(length, i);
-      place += other > length || (other == length && i < lane);
+    const int i = min(lane, seqs - 1), from = cu[i], end = cu[i + 1], to = slot ? slot[i] : i, length = max((end - from + DN_CHUNK - 1) / DN_CHUNK, 0);
+    if (__any(length > 4)) {
+      const int key = length * 64 + 63 - lane;
+      int place = 0;
+      for (int i = 0; i < seqs; ++i) place += __builtin_amdgcn_readlane(key, i) > key;
+      s = __builtin_ctzll(__ballot(lane < seqs && place == s));
     }
-    s = __builtin_ctzll(__ballot(lane < seqs && place == s));
     x = dn_rows_of(s, __builtin_amdgcn_readlane(from, s), __builtin_amdgcn_readlane(end, s), __builtin_amdgcn_readlane(to, s), tokens, slots);
   } else {
     x = dn_sequence(cu, slot, s, tokens, slots);
