@@ -20,8 +20,9 @@ constexpr uint64_t PIECE = 8192;  // a workgroup's bytes of block_copy, of 512 t
 // against 21.6, 528 20.5 against 26.0, 2064 59 against 76.
 constexpr uint64_t PREP_FULL = 384;
 // Sequences and heads up to which the recurrent kernel's waves take 16 columns each (512 threads a workgroup), not 32 (256). 1 / 5 / 8 rows,
-// microseconds: 48 items 6.7 / 9.8 / 12.0 on 16 columns, 8.3 / 10.6 / 12.9 on 32; 432 items 15.2 / 16.9 / 21.0 and 10.5 / 15.2 / 17.9.
-constexpr uint64_t STEP_NARROW = 256;
+// microseconds: 48 items 5.4 / 8.5 / 10.9 on 16 columns, 5.7 / 8.8 / 11.2 on 32; 192 items 6.7 / 10.0 / 12.2 and 6.4 / 10.0 / 12.2; 432 items
+// 15.4 / 16.4 / 20.3 and 9.9 / 14.1 / 17.8.
+constexpr uint64_t STEP_NARROW = 128;
 constexpr uint32_t ROW_MAX = 1u << 24;  // elements of a row: a chunk's bytes are counted in 32 bits
 // Rows of a sequence up to which the recurrent kernel runs though a workspace is given: 8 and one more for each 32 of its workgroups (sequences
 // and heads), from STEP_FEW to STEP_MANY. Measured, microseconds of a call, recurrent against chunks: 1 sequence of 48 heads, 8 / 12 / 16 rows

@@ -140,6 +140,16 @@ def test_rule_few_rows(ctx, lens):
     rule_case(ctx, Rows(2, 4, lens, front=3, seed=sum(lens)), out=False)
 
 
+@pytest.mark.parametrize("kh,heads,lens", [(16, 48, [5, 0, 3, 1, 17]), (2, 4, [(3 * i) % 11 for i in range(60)]), (1, 3, [9] * 50)])
+def test_rule_few_rows_of_many_heads(ctx, kh, heads, lens):
+    """More sequences and heads than waves of 16 columns are taken for."""
+    say(f"delta rule a row at a time, {len(lens)} sequences of {heads} heads")
+    rule_case(ctx, Rows(kh, heads, lens, front=1, behind=2, seed=1))
+    rule_case(ctx, Rows(kh, heads, lens, more=8, seed=2), kept=[(3 * i + 2) % (n + 2) for i, n in enumerate(lens)])
+    rule_case(ctx, Rows(kh, heads, lens, seed=3), out=False)
+    rule_case(ctx, Rows(kh, heads, [1] * len(lens), seed=4), packed=False)
+
+
 @pytest.mark.parametrize("lens", [[33], [63], [64], [65], [128], [129], [200, 1, 0, 64, 70], [0, 90, 0], [300], [40, 40, 40, 40]])
 def test_rule_in_chunks(ctx, lens):
     say(f"delta rule in chunks, {lens}")
