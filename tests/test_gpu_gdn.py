@@ -329,6 +329,29 @@ def test_captured_calls_follow_rows_slots_and_kept(ctx):
             assert torch.equal(x.view(torch.int16), y.view(torch.int16)), (i, what)
 
 
+def test_calls_at_once_with_workspaces_of_their_own(ctx):
+    """Two batches on two streams, their launches alternating: the bytes of one after the other."""
+    say("delta rule, two calls at once")
+    def batch(i):
+        return Rows(2, 6, [150 + 40 * i, 3, 70], seed=30 + i)
+    want = []
+    for i in range(2):
+        r = batch(i)
+        for _ in range(4):
+            r.call(ctx, workspace=workspace(r))
+        torch.cuda.synchronize()
+        want.append((r.out, r.state))
+    both, streams = [batch(i) for i in range(2)], [torch.cuda.Stream() for _ in range(2)]
+    spaces = [workspace(r) for r in both]
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for r, ws, stream in zip(both, spaces, streams):
+            r.call(ctx, workspace=ws, stream=stream.cuda_stream)
+    torch.cuda.synchronize()
+    for r, (out, state) in zip(both, want):
+        assert torch.equal(r.out, out) and torch.equal(r.state, state)
+
+
 def test_calls_on_another_stream_follow_its_order(ctx):
     say("delta-net core on a side stream")
     r, side = Rows(2, 4, [200, 30], seed=20), torch.cuda.Stream()
