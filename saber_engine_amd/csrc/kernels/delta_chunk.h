@@ -369,9 +369,11 @@ static __device__ __forceinline__ void delta_scan_body(const unsigned short *__r
     }
 #pragma unroll
     for (int b = 0; b < 8; ++b) most = largest(most, st[b]);
-    most = at_both<32>(at_both<16>(most, at_max2), at_max2);
+    auto of_column = [](float m) { return at_both<32>(at_both<16>(m, at_max2), at_max2); };
+    auto exponent = [](float m) { return (int)(__float_as_uint(m) >> 23); };  // (of a number from 0)
+    most = of_column(most);
     {
-      const int e = most > 0.f ? max(dn_exponent(most) - 4, 7) : 127;
+      const int e = most > 0.f ? min(max(exponent(most) - 4, 7), 247) : 127;
       unit = dn_power(e), per_unit = dn_below(e), most *= per_unit;
     }
 #pragma unroll
@@ -432,18 +434,43 @@ static __device__ __forceinline__ void delta_scan_body(const unsigned short *__r
         for (int r = 0; r < 4; ++r) p[rb][r] = fmaf(vf[r], per_unit, -er[rb][r] * p[rb][r]);
         top = largest(top, p[rb]);
       }
-      top = at_both<32>(at_both<16>(top, at_max2), at_max2);
+      top = of_column(top);
       // The unit, in the beginning a 16th of the column's largest value, moves only when that has left 2 .. 256 of it: below, terms of f16 would lack bits; above,
-      // they could pass its range (inputs are at most 256 (1 + sqrt(128)), and 64 of them lengthen a column by no more than 8 of them).
-      float was = unit;
-      if (__any(top > 256.f || (top < 2.f && top > 0.f))) {
-        const int to = min(max(dn_exponent(unit) + (top > 0.f ? dn_exponent(top) - 131 : 0), 7), 247);
-        const float by = unit * dn_below(to);
+      // they could pass its range (inputs are at most 256 (1 + sqrt(128)), and 64 of them lengthen a column by no more than 8 of them). Where a column held nothing, or
+      // nothing beside inputs that pass f32's range in its unit, V alone says where it goes, and is taken again.
+      float by = 1.f;
+      if (__any(top > 256.f || top < 2.f)) {
+        auto inputs = [&](int rb) {
+          return iu8_v4f{__uint_as_float(vv[rb][0] << 16), __uint_as_float(vv[rb][0] & 0xFFFF0000u), __uint_as_float(vv[rb][1] << 16), __uint_as_float(vv[rb][1] & 0xFFFF0000u)};
+        };
+        const int was = dn_exponent(unit);
+        int to = was + exponent(top) - 131;
+        bool anew = false;
+        if (__any(!(top > 0x1p-60f && top < 0x1p60f))) {
+          float in = 0.f;
+#pragma unroll
+          for (int rb = 0; rb < 4; ++rb) in = largest(in, inputs(rb));
+          in = of_column(in);
+          const bool empty = of_column(most) == 0.f;
+          anew = empty || !(top < INFINITY);
+          if (anew) to = exponent(in) - 4;
+          to = (anew ? in : top) > 0.f ? max(to, empty ? 7 : was - 127) : was;
+        }
+        to = min(max(to, 7), 247);
+        by = dn_power(min(max(was - to + 127, 0), 254));  // (0: what the column held is nothing beside its inputs)
         unit = dn_power(to), per_unit = dn_below(to);
 #pragma unroll
         for (int b = 0; b < 8; ++b) st[b] *= by;
 #pragma unroll
         for (int rb = 0; rb < 4; ++rb) p[rb] *= by;
+        if (__any(anew)) {
+#pragma unroll
+          for (int rb = 0; rb < 4; ++rb) {
+            const iu8_v4f vf = inputs(rb) * per_unit;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) p[rb][r] = anew ? vf[r] : p[rb][r];
+          }
+        }
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i) dn_operand<2>(p[2 * i], p[2 * i + 1], rt[i]);
@@ -459,7 +486,7 @@ static __device__ __forceinline__ void delta_scan_body(const unsigned short *__r
       for (int b = 0; b < 8; ++b) st[b] *= whole;
 #pragma unroll
       for (int rb = 0; rb < 4; ++rb) *(iu8_v4f *)(given + (4 + rb) * 1024 + lane * 16) = u[rb];
-      if (g == 0) units[n] = was * per_unit, units[16 + n] = unit;
+      if (g == 0) units[n] = by, units[16 + n] = unit;
       meet();
       // the next state
 #pragma unroll
