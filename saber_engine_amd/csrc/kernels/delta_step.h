@@ -73,7 +73,8 @@ static __device__ __forceinline__ void delta_step_body(const unsigned short *__r
 #pragma unroll
   for (int j = 0; j < J; ++j) st[j] = __builtin_nontemporal_load((const iu8_v4f *)(mine + (DG * j + dg) * DN));
 
-  // The state is `kept_by` times what the registers hold: a row's decay is a factor of one number, not of 128, until that is small.
+  // The state is `kept_by` times what the registers hold: a row's decay is a factor of one number, not of 128, until that is small, or
+  // values come that 2^16 of would bring near f32's range.
   float kept_by = 1.f;
   for (int base = 0; base < x.n; base += BATCH) {
     const int count = min(BATCH, x.n - base);
@@ -121,7 +122,8 @@ static __device__ __forceinline__ void delta_step_body(const unsigned short *__r
       if (out && dg == 0)
         *(iu8_v2u *)(out + ((size_t)(x.t0 + base + i) * heads + h) * DN + column) = iu8_v2u{iu8_bf16_pack(o[0], o[1]), iu8_bf16_pack(o[2], o[3])};
       kept_by = at_uniform_f(g);
-      if (!(kept_by > 0x1p-16f) || base + i + 1 == hold) {
+      const bool large = __any(fmaxf(fmaxf(fabsf(vf[0]), fabsf(vf[1])), fmaxf(fabsf(vf[2]), fabsf(vf[3]))) > 0x1p96f);
+      if (!(kept_by > 0x1p-16f) || large || base + i + 1 == hold) {
 #pragma unroll
         for (int j = 0; j < J; ++j) st[j] *= kept_by;
         kept_by = 1.f;

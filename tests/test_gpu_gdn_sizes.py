@@ -88,3 +88,15 @@ def test_values_whose_sizes_have_nothing_in_common(ctx, chunked):
         r.call(ctx, workspace=workspace(r) if chunked else None)
         torch.cuda.synchronize()
         compare(r, was, chunked, 1.0)
+
+
+@pytest.mark.parametrize("chunked", [False, True])
+@pytest.mark.parametrize("state,sizes", [(1.0, [2.0 ** 118]), (0, [2.0 ** 112, 1.0]), (2.0 ** 118, [1.0, 2.0 ** 118])])
+def test_values_near_the_end_of_f32(ctx, state, sizes, chunked):
+    """Decays of a while together, of which a row's update may not be taken back out of f32's range."""
+    say(f"delta rule, states of {state}, values of {sizes}, chunked {chunked}")
+    r = sized(Rows(2, 4, [100, 30], a_at=-3.0, seed=56), sizes, state)
+    was = f64(r.state)
+    r.call(ctx, workspace=workspace(r) if chunked else None)
+    torch.cuda.synchronize()
+    compare(r, was, chunked, max([state] + sizes))
