@@ -28,9 +28,10 @@ static __device__ __forceinline__ dn_rows dn_sequence(const int *__restrict__ cu
   return dn_rows_of(s, cu ? cu[s] : s, cu ? cu[s + 1] : s + 1, slot ? slot[s] : s, tokens, slots);
 }
 
-// The logarithm of a row's decay, and its beta.
+// The logarithm of a row's decay, and its beta. (Far below 0 softplus is the exponential, and one exponential of the sum is taken: by themselves the factors may be
+// infinite and 0. An infinite sum of a and dt_bias stands for f32's largest number.)
 static __device__ __forceinline__ float dn_log_decay(float a, float a_log, float dt_bias) {
-  const float x = a + dt_bias, g = -expf(a_log) * (x > 20.f ? x : log1pf(expf(x)));
+  const float x = a + dt_bias, g = -expf(x < -20.f ? a_log + x : a_log) * (x < -20.f ? 1.f : x > 20.f ? (x < INFINITY ? x : 0x1.fffffep127f) : log1pf(expf(x)));
   return g < DN_LEAST ? DN_LEAST : g;
 }
 static __device__ __forceinline__ float dn_beta(float b) { return 1.f / (1.f + expf(-b)); }

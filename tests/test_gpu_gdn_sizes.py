@@ -100,3 +100,19 @@ def test_values_near_the_end_of_f32(ctx, state, sizes, chunked):
     r.call(ctx, workspace=workspace(r) if chunked else None)
     torch.cuda.synchronize()
     compare(r, was, chunked, max([state] + sizes))
+
+
+@pytest.mark.parametrize("chunked", [False, True])
+def test_gates_whose_factors_pass_f32(ctx, chunked):
+    """exp(a_log) that is no f32 times a softplus that is none, whose product is a decay like any other; sums of a and dt_bias past f32."""
+    say(f"delta rule, gates at the ends of f32, chunked {chunked}")
+    r = Rows(1, 6, [90, 20], seed=57)
+    r.a_log.copy_(torch.tensor([100.0, 95.0, -200.0, 90.0, -104.0, 30.0]))
+    r.dt_bias.copy_(torch.tensor([-105.0, 0.0, 3e38, -3e38, 3e38, -31.0]))
+    r.ab[:, 2], r.ab[:, 3] = 3e38, -3e38
+    for h, most in ((0, 2), (4, 0), (5, 3)):
+        r.ab[:, h] = torch.arange(r.tokens, device="cuda").remainder(most + 1).bfloat16()
+    was = f64(r.state)
+    r.call(ctx, workspace=workspace(r) if chunked else None)
+    torch.cuda.synchronize()
+    compare(r, was, chunked, 1.0)
