@@ -48,7 +48,8 @@ static __device__ __forceinline__ void delta_step_body(const unsigned short *__r
   if (!out) x.n = hold;
   if (x.n <= 0) return;
   __shared__ __attribute__((aligned(16))) float s_k[BATCH][DG][PAD], s_q[BATCH][DG][PAD];
-  __shared__ float s_g[BATCH], s_b[BATCH], s_kq[BATCH];
+  __shared__ float s_g[BATCH], s_b[BATCH];
+  __shared__ __attribute__((aligned(8))) iu8_v2f s_kq[BATCH];  // k^ . q^; what the decays held back may fall to
   __shared__ __attribute__((aligned(16))) unsigned s_v[BATCH][64];
 
   unsigned kk[MINE], qq[MINE], vv[MINE];
@@ -93,7 +94,8 @@ static __device__ __forceinline__ void delta_step_body(const unsigned short *__r
       const int c = 2 * lane;  // channel DG j + dg lies at [dg][j]
       s_k[i][c % DG][c / DG] = k0 * rk, s_k[i][c % DG + 1][c / DG] = k1 * rk;
       s_q[i][c % DG][c / DG] = q0 * rq, s_q[i][c % DG + 1][c / DG] = q1 * rq;
-      if (lane == 0) s_kq[i] = kq * rk * rq;
+      const bool large = __any((vv[y] & 0x7F80u) >= 0x7180u || (vv[y] & 0x7F800000u) >= 0x71800000u);  // (from 2^100 on)
+      if (lane == 0) s_kq[i] = iu8_v2f{kq * rk * rq, large ? 2.f : 0x1p-16f};
     }
     if (wave == WAVES - 1 && lane < BATCH) s_g[lane] = expf(dn_log_decay(iu8_bf16_f32(aa), al, dt)), s_b[lane] = dn_beta(iu8_bf16_f32(bb));
     __syncthreads();
@@ -111,7 +113,8 @@ static __device__ __forceinline__ void delta_step_body(const unsigned short *__r
           for (int cc = 0; cc < 4; ++cc) sk[cc] = fmaf(st[j + e][cc], y[e], sk[cc]), sq[cc] = fmaf(st[j + e][cc], z[e], sq[cc]);
         }
       }
-      const float g = kept_by * s_g[i], be = s_b[i], kq = s_kq[i];
+      const iu8_v2f and_least = s_kq[i];
+      const float g = kept_by * s_g[i], be = s_b[i], kq = and_least[0];
       const float vf[4] = {__uint_as_float(now[0] << 16), __uint_as_float(now[0] & 0xFFFF0000u), __uint_as_float(now[1] << 16), __uint_as_float(now[1] & 0xFFFF0000u)};
       float u[4], o[4];
 #pragma unroll
@@ -122,8 +125,7 @@ static __device__ __forceinline__ void delta_step_body(const unsigned short *__r
       if (out && dg == 0)
         *(iu8_v2u *)(out + ((size_t)(x.t0 + base + i) * heads + h) * DN + column) = iu8_v2u{iu8_bf16_pack(o[0], o[1]), iu8_bf16_pack(o[2], o[3])};
       kept_by = at_uniform_f(g);
-      const bool large = __any(fmaxf(fmaxf(fabsf(vf[0]), fabsf(vf[1])), fmaxf(fabsf(vf[2]), fabsf(vf[3]))) > 0x1p96f);
-      if (!(kept_by > 0x1p-16f) || large || base + i + 1 == hold) {
+      if (__any(!(g > and_least[1])) || base + i + 1 == hold) {
 #pragma unroll
         for (int j = 0; j < J; ++j) st[j] *= kept_by;
         kept_by = 1.f;
