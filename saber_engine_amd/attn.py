@@ -57,22 +57,26 @@ class PagedKvCache:
         if want - len(held) > len(self._free):
             raise iu8.IU8Error(iu8.E_RULE, f"{want - len(held)} more pages wanted, {len(self._free)} free")
         if want > len(held):
-            new = self._deal(want - len(held))
-            self.table[seq, len(held):want] = torch.tensor(new, dtype=torch.int32, device=self.table.device)
+            new = self._next(want - len(held))
+            self.table[seq, len(held):want] = device_numbers(new, self.table.device)
+            self._deal(new)
             held += new
 
     def release(self, seq):
         """The sequence's pages back (those that another sequence shares stay its), its count to zero."""
-        self._back(self._held[seq])
-        self._held[seq] = []
         self.table[seq] = -1
         self.kv_len[seq] = 0
+        self._back(self._held[seq])
+        self._held[seq] = []
 
-    def _deal(self, n):
-        new = [self._free.pop() for _ in range(n)]
-        for p in new:
+    # (What can fail, on the device, comes in front of the books: a call that raises has dealt nothing.)
+    def _next(self, n):  # the pages that _deal takes
+        return self._free[:-n - 1:-1]
+
+    def _deal(self, pages):
+        for p in pages:
+            self._free.pop()
             self._holders[p] = 1
-        return new
 
     def _back(self, pages):
         for p in reversed(pages):
@@ -93,16 +97,16 @@ class PagedKvCache:
             raise iu8.IU8Error(iu8.E_RULE, f"{tokens} tokens of sequence {src}'s {len(held)} pages to sequence {dst}, which has {len(self._held[dst])}")
         if more and not self._free:
             raise iu8.IU8Error(iu8.E_RULE, "a page more wanted, none free")
-        new = held[:whole]
-        for p in new:
-            self._holders[p] += 1
-        if more:
-            new = new + self._deal(1)
-            self._copy(ctx, [(held[whole], new[whole])])
+        own = self._next(more)
+        new = held[:whole] + own
+        self._copy(ctx, [(held[whole], p) for p in own])
         if new:
             self.table[dst, :len(new)] = device_numbers(new, self.table.device)
-        self._held[dst] = new
         self.kv_len[dst] = tokens
+        self._deal(own)
+        for p in held[:whole]:
+            self._holders[p] += 1
+        self._held[dst] = new
 
     def trim(self, ctx, seq, tokens):
         """The sequence's positions from `tokens` on back, as for drafted tokens that were not taken: pages behind them free, its count at most
@@ -113,17 +117,19 @@ class PagedKvCache:
         own = more and self._holders[held[whole]] > 1
         if own and not self._free and all(self._holders[p] > 1 for p in held[whole + 1:]):
             raise iu8.IU8Error(iu8.E_RULE, "a page more wanted, none free")
-        self._back(held[whole + more:])
-        last = held[whole:whole + more]
-        if own:
-            page = self._deal(1)
-            self._copy(ctx, [(last[0], page[0])])
-            self._back(last)
-            self.table[seq, whole] = page[0]
-            last = page
+        last, gone = held[whole:whole + more], held[whole + more:]
+        if own:  # (where one of the pages behind comes free, into that)
+            page = next((p for p in gone if self._holders[p] == 1), self._free[-1] if self._free else None)
+            self._copy(ctx, [(last[0], page)])
+            self.table[seq, whole] = page
         self.table[seq, whole + more:] = -1
-        self._held[seq] = held[:whole] + last
         self.kv_len[seq].clamp_(max=max(tokens, 0))
+        self._back(gone)
+        if own:
+            self._deal([page])
+            self._back(last)
+            last = [page]
+        self._held[seq] = held[:whole] + last
 
     def compact(self, ctx):
         """The pages in use to the front of the pool; returns how many they are. Those behind them can then be given up, or another pool's."""
@@ -132,12 +138,13 @@ class PagedKvCache:
         to = dict(zip([p for p in used if p >= n], [p for p in range(n) if not self._holders[p]]))
         self._copy(ctx, list(to.items()))
         if to:
+            moved = {seq: [to.get(p, p) for p in held] for seq, held in enumerate(self._held) if any(p in to for p in held)}
+            self.table[device_numbers(list(moved), self.table.device).long()] = device_numbers([h + [-1] * (self.table_stride - len(h)) for h in moved.values()],
+                                                                                              self.table.device)
             for old, new in to.items():
                 self._holders[new], self._holders[old] = self._holders[old], 0
-            for seq, held in enumerate(self._held):
-                if any(p in to for p in held):
-                    self._held[seq] = held = [to.get(p, p) for p in held]
-                    self.table[seq, :len(held)] = device_numbers(held, self.table.device)
+            for seq, held in moved.items():
+                self._held[seq] = held
             self._free = list(range(self.pages - 1, n - 1, -1))
         return n
 

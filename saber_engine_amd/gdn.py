@@ -26,26 +26,26 @@ class GdnState:
         self.slot = torch.full((seqs,), -1, dtype=torch.int32, device=device)
         self._free, self._held = list(range(self.slots - 1, -1, -1)), [None] * seqs
 
-    def _take(self, seq):
+    def _take(self, seq):  # (what can fail, on the device, in front of the books)
+        self.slot[seq] = self._free[-1]
+        self._held[seq] = self._free.pop()
+
+    def begin(self, seq):
+        """A slot for the sequence, its state and tail zeros."""
         if self._held[seq] is not None:
             raise iu8.IU8Error(iu8.E_RULE, f"sequence {seq} has a state already")
         if not self._free:
             raise iu8.IU8Error(iu8.E_RULE, f"a state more wanted, none of {self.slots} free")
-        self._held[seq] = slot = self._free.pop()
-        self.slot[seq] = slot
-        return slot
-
-    def begin(self, seq):
-        """A slot for the sequence, its state and tail zeros."""
-        slot = self._take(seq)
-        self.state[slot].zero_()
-        self.tail[slot].zero_()
+        self.state[self._free[-1]].zero_()
+        self.tail[self._free[-1]].zero_()
+        self._take(seq)
 
     def release(self, seq):
         """The sequence's slot back."""
         if self._held[seq] is not None:
+            self.slot[seq] = -1
             self._free.append(self._held[seq])
-            self._held[seq], self.slot[seq] = None, -1
+            self._held[seq] = None
 
     def fork(self, ctx, src, dsts):
         """Sequence src's memory to each of dsts, which have none yet."""
@@ -53,9 +53,11 @@ class GdnState:
             raise iu8.IU8Error(iu8.E_RULE, f"sequence {src} to {list(dsts)}: a source with a state, targets without, and {len(dsts)} of {len(self._free)} free slots")
         if dsts:
             device = self.state.device
-            of, to = device_numbers([self._held[src]] * len(dsts), device), device_numbers([self._take(d) for d in dsts], device)
+            of, to = device_numbers([self._held[src]] * len(dsts), device), device_numbers(self._free[:-len(dsts) - 1:-1], device)
             ctx.gdn_copy(self.state.data_ptr(), self.tail.data_ptr(), self.slots, self.heads, self.channels, self.width, of.data_ptr(), to.data_ptr(), len(dsts),
                          current_stream(device))
+            for d in dsts:
+                self._take(d)
 
 
 class GdnLayerIU8:
