@@ -26,7 +26,9 @@ class PagedKvCache:
     """The pages of one layer's sequences. The host deals pages (reserve, release); the table and the counts lie on the device, where
     the kernels read them, so that a captured step follows them; reserve, release, fork, trim and compact write there on torch's current stream. While a step
     runs they must stand still: where steps take another stream than torch's current one, order the two (make it current around reserve, release
-    and writes of kv_len, or wait for the step). A page that several sequences share (fork) is whole, and written by none of them."""
+    and writes of kv_len, or wait for the step). A page that several sequences share (fork) is whole, and written by none of them: the count of a sequence that has
+    been forked, or is a fork, goes back by trim alone, which gives it pages of its own to write in.
+    """
 
     def __init__(self, seqs, kv_heads, head_dim, max_kv, pages=None, page_tokens=64, kind=iu8.KV_BF16, k_scale=None, v_scale=None, device="cuda"):
         """max_kv: the most tokens a sequence may hold; pages: of all sequences together (None: enough for all at that length);
@@ -91,10 +93,13 @@ class PagedKvCache:
 
     def fork(self, ctx, src, dst, tokens):
         """Sequence dst, which has none, gets sequence src's first `tokens` positions: the pages that they fill are shared, the last one, where
-        they end inside it, is copied. dst's count becomes `tokens`."""
+        they end inside it, is copied. dst's count becomes `tokens`. More than src counts is refused (its next rows would be written in pages that are shared); a
+        count of 0 says nothing, as of pages that are filled before they are counted. The count is read here, which waits for torch's current stream."""
         held, whole, more = self._held[src], tokens // self.page_tokens, tokens % self.page_tokens > 0
         if self._held[dst] or src == dst or tokens < 0 or whole + more > len(held):
             raise iu8.IU8Error(iu8.E_RULE, f"{tokens} tokens of sequence {src}'s {len(held)} pages to sequence {dst}, which has {len(self._held[dst])}")
+        if 0 < int(self.kv_len[src]) < tokens:
+            raise iu8.IU8Error(iu8.E_RULE, f"{tokens} tokens of sequence {src}, which counts {int(self.kv_len[src])}")
         if more and not self._free:
             raise iu8.IU8Error(iu8.E_RULE, "a page more wanted, none free")
         own = self._next(more)

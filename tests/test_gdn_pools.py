@@ -58,3 +58,20 @@ def test_a_copy_that_fails_leaves_the_slots_as_they_were():
     s.fork(Copies(), 1, [0, 3])
     s.begin(2)
     assert sorted(s.slot.tolist()) == [0, 1, 2, 3] and s.slot.tolist() == s._held
+
+
+def test_positions_that_are_not_written_yet_are_not_shared():
+    """Pages reserved ahead of the count: shared, the source's next rows would be another sequence's too."""
+    c, ctx = attn.PagedKvCache(3, 1, 64, 200, pages=9, page_tokens=32, device="cpu"), Copies()
+    c.reserve(0, 96)
+    c.kv_len[0] = 70
+    was = books(c)
+    for tokens in (71, 96):
+        with pytest.raises(iu8.IU8Error, match="which counts 70"):
+            c.fork(ctx, 0, 1, tokens)
+        assert same(books(c), was) and not ctx.calls
+    c.fork(ctx, 0, 1, 70)
+    assert c._held[1][:2] == c._held[0][:2] and c._held[1][2] != c._held[0][2] and c._holders[c._held[0][2]] == 1
+    c.kv_len[0] = 96
+    c.fork(ctx, 0, 2, 96)
+    assert c._held[2] == c._held[0] and len(ctx.calls) == 1
