@@ -655,13 +655,13 @@ int saber_iu8_gdn_conv(saber_iu8_ctx *ctx, const void *x, uint32_t x_row, const 
  *   k^ = k / sqrt(|k|^2 + eps), q^ = q / sqrt(|q|^2 + eps), decay = exp(-exp(a_log[h]) softplus(a + dt_bias[h])), beta = sigmoid(b)
  *   S <- decay S + k^ (beta (v - (decay S)^T k^))^T,   out[t, h] = scale S^T q^
  * q, k, v rows `row` elements apart, heads 128 apart; a, b rows `ab_row` apart, a value a head; a_log, dt_bias f32 [heads]; out bf16 [tokens, heads, 128], which
- * must not overlap the rows, or NULL: the states alone (q may then be NULL). A decay below exp(-120) is zero. Values, states and gates are numbers, and
- * |q|^2 and |k|^2 numbers of f32: one that is not spoils its heads' rows from its chunk of 64 on, and their states.
+ * must not overlap the rows, or NULL: the states alone (q may then be NULL). A decay below exp(-120) is zero. Values, states and gates are numbers (of
+ * any size at which f32 holds what the rule makes of them), and |q|^2 and |k|^2 numbers of f32 (with an eps below 2^-100 of at least that): one that is not spoils its heads' rows from its chunk of 64 on, and their states.
  * max_q: the most new rows of a sequence, for the choice of the kernel alone. Long rows are taken in chunks of 64, with the workspace of saber_iu8_gdn_workspace (made
  * for (tokens, seqs, max_q), it holds every call of the same heads with at most these; calls that share it must not overlap in time), the rest, and whatever has no
  * workspace, kept, or no out, a row at a time: the same rule, other roundings. States, norms and sums in f32 (the chunks' matrix products hold 22 bits of
- * what enters the state, 11 of what goes into the rows' answers alone, and of both
- * nothing below 2^-26 of the largest value that its column has in the 64 rows), out rounded once; the same bytes on every run. */
+ * what enters the state, 11 of what goes into the rows' answers alone, and of both nothing below 2^-26 of the largest value that its column has in the 64 rows and the
+ * 64 before, values and state: what a decay leaves of a column while nothing as large comes in is better off a row at a time), out rounded once; the same bytes on every run. */
 int saber_iu8_gdn_workspace(uint32_t tokens, uint32_t seqs, uint32_t max_q, uint32_t key_heads, uint32_t heads, uint64_t *bytes);
 int saber_iu8_gdn(saber_iu8_ctx *ctx, const void *q, const void *k, const void *v, uint32_t row, const void *a, const void *b, uint32_t ab_row, const float *a_log,
                   const float *dt_bias, float *state, uint32_t slots, const int32_t *slot, const int32_t *cu_q, const int32_t *kept, void *out, uint32_t tokens,

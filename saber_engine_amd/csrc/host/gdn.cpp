@@ -28,6 +28,7 @@ constexpr uint32_t ROW_MAX = 1u << 24;  // elements of a row: a chunk's bytes ar
 // and heads), from STEP_FEW to STEP_MANY. Measured, microseconds of a call, recurrent against chunks: 1 sequence of 48 heads, 8 / 12 / 16 rows
 // 11.0 / 15.2 / 17.9 against 13.5 / 13.7 / 13.3; 16 of 8 heads 12.7 / 17.0 / 19.6 against 15.5 / 15.4 / 15.7; 4 of 48 heads, 12 / 16 / 24 rows
 // 17.1 / 20.9 / 27.2 against 22.1; 64 of 8 heads, 16 / 24 / 32 rows 28 / 37 / 47 against 40 / 41 / 42; 64 of 48 heads 129 / 176 / 224 against 176 / 182 / 190.
+// (A line through these, not each of them: 16 sequences of 8 heads stay recurrent up to 12 rows, where chunks are a tenth faster; 4 of 48 heads take chunks from 15, up to 16 a twentieth slower.)
 constexpr uint64_t STEP_FEW = 10, STEP_MANY = 24;
 
 // The kernels' arguments as abi.cpp declares them (natural alignment: the order says it all).

@@ -10,10 +10,10 @@
 // factors, and K and Q as the walk reads them; delta_scan walks a sequence's chunks in order.
 //
 // Precision: the state and all that enters it is f32, on the f16 matrix cores. A row of K or Q, bf16 as it comes, is an f16 row times a power
-// of two (its largest value brought to 1 .. 2); its norm's and decay's factors are moved to the other side of the product; the other side is split
+// of two (the one at or below its length, so that no value passes 2); its norm's and decay's factors are moved to the other side of the product; the other side is split
 // into two f16 terms, 22 bits (dn_split), in a column's own unit, a power of two that follows the column's largest value. What goes only into the rows' bf16 answers takes
-// one term, 11 bits. (Three bf16 terms, which need no units, are half as many products again and twice the lane arithmetic: the walk of 8,192 rows of 48
-// heads 304 us, with f16 208.) G is summed, and its differences taken, in f64: after a strong decay the later rows' differences would be left with the sum's digits.
+// one term, 11 bits. Units: nothing is kept below 2^-26 of the largest value that a column has in a chunk and the one before.
+// (Three bf16 terms, which need no units, are half as many products again and twice the lane arithmetic: the walk of 8,192 rows of 48 heads 304 us in a trace, with f16 221.) G is summed, and its differences taken, in f64: after a strong decay the later rows' differences would be left with the sum's digits.
 #pragma once
 #include "delta_step.h"
 
@@ -310,10 +310,10 @@ static __device__ __forceinline__ iu8_v2u dn_transposed(const unsigned char *fro
 //
 // The chunks' chain of products bounds a walk (a wave's lane arithmetic does not run under its own matrix instructions here), so its waves come in pairs: one walks
 // the chain (K S, V - .., U, the next S), the other does what hangs from it, the rows' answers, with the operands that the first leaves in LDS, and asks for K, Q,
-// T, the inner matrix, the factors and V two chunks ahead, which come straight from memory into one of two LDS stages as soon as it has been read. O is
+// T, the inner matrix, the factors and V of the next chunk, which come straight from memory into the LDS stage that the chunk before has left. O is
 // taken the other way round (the operands exchanged), so that a lane has four neighbouring values of one row to store. Two meetings a chunk: behind U, where the
-// stage is free, and behind the next S. W pairs a workgroup share a stage. A chunk takes 1.6 us with two pairs
-// (8,192 rows of 48 heads 208 us), 2.2 with four.
+// stage has been read, and behind the next S. W pairs a workgroup share a stage. A chunk takes 1.7 us with two pairs
+// (8,192 rows of 48 heads: 271 us with the preparation's 58; in a trace the walk has 216 to 222), 2.2 with four.
 template <int W>
 static __device__ __forceinline__ void delta_scan_body(const unsigned short *__restrict__ v, const unsigned char *__restrict__ keys,
                                                        const unsigned char *__restrict__ work, float *__restrict__ state, const int *__restrict__ slot,
