@@ -356,6 +356,7 @@ static __device__ __forceinline__ void delta_scan_body(const unsigned short *__r
     auto channel = [](int b, int r) { return 32 * (b >> 1) + 4 * (b & 1) + r; };  // beside 8 g
     iu8_v4f st[8];  // in units of `unit`
     float unit, per_unit, most = 0.f;  // most: the column's largest value, in units
+    float none = 0.f;                  // a `top` of no more has nothing to say; -1 where the unit is past 2^16, in which inputs may vanish
     iu8_v4u sw[4][2];
     auto largest = [](float m, iu8_v4f y) { return fmaxf(fmaxf(fmaxf(fmaxf(m, fabsf(y[0])), fabsf(y[1])), fabsf(y[2])), fabsf(y[3])); };
     auto give_state = [&](int ks) {
@@ -374,7 +375,7 @@ static __device__ __forceinline__ void delta_scan_body(const unsigned short *__r
     most = of_column(most);
     {
       const int e = most > 0.f ? min(max(exponent(most) - 4, 7), 247) : 127;
-      unit = dn_power(e), per_unit = dn_below(e), most *= per_unit;
+      unit = dn_power(e), per_unit = dn_below(e), none = e > 143 ? -1.f : 0.f, most *= per_unit;
     }
 #pragma unroll
     for (int b = 0; b < 8; ++b) st[b] *= per_unit;
@@ -439,7 +440,7 @@ static __device__ __forceinline__ void delta_scan_body(const unsigned short *__r
       // they could pass its range (inputs are at most 256 (1 + sqrt(128)), and 64 of them lengthen a column by no more than 8 of them). Where a column held nothing, or
       // nothing beside inputs that pass f32's range in its unit, V alone says where it goes, and is taken again.
       float by = 1.f;
-      if (__any(top > 256.f || top < 2.f)) {
+      if (__any(top > 256.f || (top < 2.f && top > none))) {
         auto inputs = [&](int rb) {
           return iu8_v4f{__uint_as_float(vv[rb][0] << 16), __uint_as_float(vv[rb][0] & 0xFFFF0000u), __uint_as_float(vv[rb][1] << 16), __uint_as_float(vv[rb][1] & 0xFFFF0000u)};
         };
@@ -454,11 +455,11 @@ static __device__ __forceinline__ void delta_scan_body(const unsigned short *__r
           const bool empty = of_column(most) == 0.f;
           anew = empty || !(top < INFINITY);
           if (anew) to = exponent(in) - 4;
-          to = (anew ? in : top) > 0.f ? max(to, empty ? 7 : was - 127) : was;
+          to = (anew ? in : top) > 0.f ? max(to, empty ? 7 : was - 127) : 127;
         }
         to = min(max(to, 7), 247);
         by = dn_power(min(max(was - to + 127, 0), 254));  // (0: what the column held is nothing beside its inputs)
-        unit = dn_power(to), per_unit = dn_below(to);
+        unit = dn_power(to), per_unit = dn_below(to), none = to > 143 ? -1.f : 0.f;
 #pragma unroll
         for (int b = 0; b < 8; ++b) st[b] *= by;
 #pragma unroll

@@ -116,3 +116,26 @@ def test_gates_whose_factors_pass_f32(ctx, chunked):
     r.call(ctx, workspace=workspace(r) if chunked else None)
     torch.cuda.synchronize()
     compare(r, was, chunked, 1.0)
+
+
+@pytest.mark.parametrize("chunked", [False, True])
+@pytest.mark.parametrize("before,behind", [(2.0 ** 60, 2.0 ** -100), (2.0 ** 20, 2.0 ** -120), (2.0 ** -110, 2.0 ** 90)])
+def test_columns_that_stay_empty_for_a_while(ctx, before, behind, chunked):
+    """Cleared, then a whole chunk without inputs, in some columns two, then values of another size; columns that never hold anything stay exactly that."""
+    say(f"delta rule, states of {before} cleared and left empty, then values of {behind}, chunked {chunked}")
+    r = sized(Rows(1, 3, [64 * 4 + 20], seed=58), [before, 0.0, behind], before)
+    v = r.rows[:, 2 * D:5 * D].view(-1, 3, D)
+    v[63] = 0
+    v[:192, :, 5::16] = 0
+    v[:, :, 7::32] = 0
+    r.state[:, :, :, 7::32] = 0
+    r.ab[63, :r.heads] = 20000.0
+    r.call(ctx, workspace=workspace(r) if chunked else None)
+    torch.cuda.synchronize()
+    x = parts(r, 64, 4 * 64 + 20 - 64)
+    x[2] = x[2] / behind
+    want, tol, states, tols = rule(*x, np.zeros((r.heads, D, D)), r.eps, r.scale, chunked)
+    # (bf16's steps below 2^-126 are 2^-133: an answer is rounded by as much as half of that, of values of 2^-120 that is 2^-14)
+    check(f64(r.out[64:].float()) / behind, want, tol + 2.0 ** -134 / behind, "rows behind")
+    check(f64(r.state[int(r.slot[0])]) / behind, states[-1], np.broadcast_to(tols[-1], states[-1].shape), "state")
+    assert (r.out[:, :, 7::32] == 0).all() and (r.state[int(r.slot[0]), :, :, 7::32] == 0).all()
